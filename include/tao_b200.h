@@ -458,6 +458,37 @@ int tao_qkv_split_norm_backward(const void* raw_q, const void* raw_k, const void
                                 const void* dv, const void* d_raw_q, const void* d_raw_k, long long rows,
                                 int heads, int width, float eps, void* d_projected, void* stream);
 
+/* Element types of the block operators below. */
+#define TAO_TYPE_BF16 0
+#define TAO_TYPE_FP16 1
+#define TAO_TYPE_FP32 2
+#define TAO_TYPE_E4M3 3
+
+/* Residual addition and root-mean-square norm of rows [rows][width] (bf16, fp16 or fp32;
+ * strides in elements, the last axis contiguous): s = x + residual rounded to the type
+ * (written to s [rows][width]; residual NULL: s is x and is not written),
+ * y = s * rsqrt(mean(s^2) + eps) * weight [width] (NULL: ones), in fp32, rounded once. */
+int tao_add_rms_norm(const void* x, long long x_stride, const void* residual, long long r_stride,
+                     const void* weight, long long rows, int width, int type, float eps, void* s,
+                     void* y, void* stream);
+
+/* The same with an e4m3 output: m = max(max|y|, 1e-30) over a row (group 0) or over 128
+ * channels (group 128), scale = m / 448 (fp32 [rows] or [rows][ceil(width / 128)]),
+ * q = e4m3(y * (448 / m)).  A NaN in a row makes its values and scales NaN. */
+int tao_add_rms_norm_fp8(const void* x, long long x_stride, const void* residual, long long r_stride,
+                         const void* weight, long long rows, int width, int type, float eps, int group,
+                         void* s, void* q, float* scale, void* stream);
+
+/* Gradient of tao_add_rms_norm from dy, the stream's own gradient ds (NULL: none) and s:
+ * with r = rsqrt(mean(s^2) + eps), n = s r: dx = ds + r (weight dy - n mean(weight dy n))
+ * (the gradient of x and of residual), dw = sum over rows of dy n (NULL: not wanted; the
+ * rows' order of summation is fixed).  workspace: tao_add_rms_norm_workspace_bytes. */
+size_t tao_add_rms_norm_workspace_bytes(long long rows, int width, int type);
+int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* ds, long long ds_stride,
+                              const void* s, long long s_stride, const void* weight, long long rows,
+                              int width, int type, float eps, void* dx, void* dw, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,6 +4,7 @@ The library is built in-tree by ``tao_memory_b200.build``.  There is no CPU or
 eager fallback: if the shared object is missing, every entry point raises.
 """
 
+import contextlib
 import ctypes
 import os
 
@@ -83,6 +84,11 @@ _SIGNATURES = {
     "tao_train_backward": (_I, [_VP] * 9 + [_I, _I, _I, _I, _VP, _VP, _VP, _VP]),
     "tao_qkv_split_norm": (_I, [_VP, _I64, _I, _I, _F, _VP, _VP, _VP, _VP, _VP, _VP]),
     "tao_qkv_split_norm_backward": (_I, [_VP] * 7 + [_I64, _I, _I, _F, _VP, _VP]),
+    "tao_add_rms_norm": (_I, [_VP, _I64, _VP, _I64, _VP, _I64, _I, _I, _F, _VP, _VP, _VP]),
+    "tao_add_rms_norm_fp8": (_I, [_VP, _I64, _VP, _I64, _VP, _I64, _I, _I, _F, _I, _VP, _VP, _VP, _VP]),
+    "tao_add_rms_norm_workspace_bytes": (_SZ, [_I64, _I, _I]),
+    "tao_add_rms_norm_backward": (_I, [_VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I, _I, _F, _VP, _VP, _VP, _SZ,
+                                       _VP]),
     "tao_feature_read_forward": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "tao_feature_read_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
     "tao_train_pairs": (_I, [_I]),
@@ -122,6 +128,15 @@ def check(rc):
     if rc in (TAO_ERR_ARG, TAO_ERR_POSITION, TAO_ERR_SEAL, TAO_ERR_CAPACITY):
         raise ValueError(msg)
     raise TaoError(msg)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device):
+    """Context in which ``device`` (a CUDA device with an index) is the current one."""
+    import torch
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def exported_symbols():

@@ -1,0 +1,533 @@
+// Root-mean-square norm with the residual's addition, the form between two halves of a
+// decoder block, with a 16/32-bit or an e4m3 output, and its gradient.
+//
+//   s = round(x + residual)          the stream the next block adds to (rounded to its type)
+//   n = s r,  r = rsqrt(mean(s^2) + eps)
+//   y = n w                          or q = e4m3(y * 448 / m), scale = m / 448,
+//                                    m = max(max|y|, 1e-30) over a row or 128 channels
+//   dx = ds + r (w dy - n mean(w dy n)),   dw = sum over rows of dy n
+//
+// The norm is taken of the rounded s, so that the forward and the gradient see the same
+// stream and the gradient needs no copy of x and residual.  All sums are in fp32.
+//
+// HBM-bound: each element is read and written once, a row lives in its threads' registers
+// between the sum and the scaling (V vectors of 16 bytes a thread).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/tao_b200.h"
+#include "common.cuh"
+
+void tao_set_last_error(const char* msg);
+
+namespace tao {
+namespace {
+
+constexpr float kE4m3Max = 448.f, kTiny = 1e-30f;
+
+template <class T> TAO_DEVI float to_f(T x);
+template <> TAO_DEVI float to_f<bf16>(bf16 x) { return __bfloat162float(x); }
+template <> TAO_DEVI float to_f<__half>(__half x) { return __half2float(x); }
+template <> TAO_DEVI float to_f<float>(float x) { return x; }
+template <class T> TAO_DEVI T from_f(float x);
+template <> TAO_DEVI bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
+template <> TAO_DEVI __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <> TAO_DEVI float from_f<float>(float x) { return x; }
+
+// One vector of 16 bytes of a row, as floats; elements beyond `width` read as zero and
+// are not written.  `wide` says that every row starts on 16 bytes and that the width
+// is whole vectors; otherwise the elements move one by one.
+template <class T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  union Bits {
+    uint4 u;
+    T e[N];
+    TAO_DEVI Bits() {}
+  };
+  static TAO_DEVI void load(const T* row, int at, int width, bool wide, float (&f)[N]) {
+    Bits b;
+    if (wide) {
+      b.u = *reinterpret_cast<const uint4*>(row + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) b.e[i] = at + i < width ? row[at + i] : from_f<T>(0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f<T>(b.e[i]);
+  }
+  static TAO_DEVI void store(T* row, int at, int width, bool wide, const float (&f)[N]) {
+    Bits b;
+#pragma unroll
+    for (int i = 0; i < N; ++i) b.e[i] = from_f<T>(f[i]);
+    if (wide) {
+      *reinterpret_cast<uint4*>(row + at) = b.u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at + i < width) row[at + i] = b.e[i];
+    }
+  }
+  static TAO_DEVI void store_e4m3(uint8_t* row, int at, int width, bool wide, const float (&f)[N]) {
+    __nv_fp8x2_storage_t p[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      p[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    if (wide) {
+      if constexpr (N == 8)
+        *reinterpret_cast<uint2*>(row + at) = make_uint2(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16);
+      else
+        *reinterpret_cast<uint32_t*>(row + at) = p[0] | (uint32_t)p[1] << 16;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at + i < width) row[at + i] = (uint8_t)(p[i / 2] >> (8 * (i & 1)));
+    }
+  }
+};
+
+// max that keeps a NaN, as the plain form's does: a row with a NaN has a NaN scale.
+TAO_DEVI float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sum (or maximum) over the threads of a row: blockDim.x of them; more than one warp only
+// where the block holds one row.  `red` has 32 floats for each value of the call's.
+template <int COUNT, bool MAX = false>
+TAO_DEVI void row_reduce(float (&v)[COUNT], float* red) {
+#pragma unroll
+  for (int c = 0; c < COUNT; ++c) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, v[c], o);
+      v[c] = MAX ? max_nan(v[c], other) : v[c] + other;
+    }
+  }
+  if (blockDim.x == 32) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  __syncthreads();  // the last call's reads of `red` are over
+  if (lane == 0) {
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c) red[c * 32 + warp] = v[c];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < COUNT; ++c) {
+    float t = lane < warps ? red[c * 32 + lane] : 0.f;  // maxima are of magnitudes
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, t, o);
+      t = MAX ? max_nan(t, other) : t + other;
+    }
+    v[c] = t;
+  }
+}
+
+struct NormArgs {
+  const void *x, *residual, *weight;
+  long long x_stride, r_stride, rows;
+  int width, group;  // group: 0 = one scale a row, 128 = one for 128 channels
+  float eps;
+  bool wide;
+  void *s, *y;
+  float* scale;
+};
+
+// MAXT: blocks of up to 256 threads are compiled with registers to spare for V vectors.
+template <class T, int V, bool FP8, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_kernel(const NormArgs a) {
+  using Ve = Vec<T>;
+  constexpr int N = Ve::N;
+  __shared__ float red[32];
+  const int width = a.width;
+  for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row < a.rows;
+       row += (long long)gridDim.x * blockDim.y) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    float v[V][N];
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = (threadIdx.x + i * blockDim.x) * N;
+      if (at < width) {
+        Ve::load(x, at, width, a.wide, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] = 0.f;
+      }
+    }
+    if (a.residual) {
+      const T* res = static_cast<const T*>(a.residual) + row * a.r_stride;
+      T* s = static_cast<T*>(a.s) + row * width;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int at = (threadIdx.x + i * blockDim.x) * N;
+        if (at < width) {
+          float r[N];
+          Ve::load(res, at, width, a.wide, r);
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[i][j] = to_f<T>(from_f<T>(v[i][j] + r[j]));
+          Ve::store(s, at, width, a.wide, v[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum[0] += v[i][j] * v[i][j];
+    row_reduce(sum, red);
+    const float r = rsqrtf(sum[0] / width + a.eps);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = (threadIdx.x + i * blockDim.x) * N;
+      float w[N];
+      if (a.weight && at < width) {
+        Ve::load(static_cast<const T*>(a.weight), at, width, a.wide, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i][j] = v[i][j] * r * w[j];
+      if constexpr (!FP8) {
+        if (at < width) Ve::store(static_cast<T*>(a.y) + row * width, at, width, a.wide, v[i]);
+      }
+    }
+    if constexpr (FP8) {
+      uint8_t* q = static_cast<uint8_t*>(a.y) + row * width;
+      float top[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        top[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) top[i] = max_nan(top[i], fabsf(v[i][j]));
+      }
+      if (a.group == 0) {
+        float m[1] = {top[0]};
+#pragma unroll
+        for (int i = 1; i < V; ++i) m[0] = max_nan(m[0], top[i]);
+        row_reduce<1, true>(m, red);
+#pragma unroll
+        for (int i = 0; i < V; ++i) top[i] = max_nan(m[0], kTiny);
+        if (threadIdx.x == 0) a.scale[row] = top[0] / kE4m3Max;
+      } else {
+        // 128 channels are 128 / N neighbouring threads of the same vector index
+        const int groups = (width + 127) / 128;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+          for (int o = 64 / N; o > 0; o >>= 1) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+          top[i] = max_nan(top[i], kTiny);
+          const int at = (threadIdx.x + i * blockDim.x) * N;
+          if (at < width && at % 128 == 0) a.scale[row * groups + at / 128] = top[i] / kE4m3Max;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int at = (threadIdx.x + i * blockDim.x) * N;
+        const float up = kE4m3Max / top[i];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] *= up;
+        if (at < width) Ve::store_e4m3(q, at, width, a.wide, v[i]);
+      }
+    }
+  }
+}
+
+struct NormGradArgs {
+  const void *dy, *ds, *s, *weight;
+  long long dy_stride, ds_stride, s_stride, rows;
+  int width;
+  float eps;
+  bool wide;
+  void* dx;
+  float* partial;  // [gridDim.x][width] sums of dy n over a block's rows, or null
+};
+
+// A block walks over rows with its columns' part of dw in registers.
+template <class T, int V, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_grad_kernel(const NormGradArgs a) {
+  using Ve = Vec<T>;
+  constexpr int N = Ve::N;
+  extern __shared__ float sh[];  // 64 floats, then (one-warp rows) [blockDim.y][width padded]
+  const int width = a.width;
+  float dw[V][N];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) dw[i][j] = 0.f;
+  for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row < a.rows;
+       row += (long long)gridDim.x * blockDim.y) {
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
+    const T* s = static_cast<const T*>(a.s) + row * a.s_stride;
+    float g[V][N], v[V][N];
+    float sum[2] = {0.f, 0.f};  // of s^2 and of w dy s
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = (threadIdx.x + i * blockDim.x) * N;
+      if (at < width) {
+        Ve::load(s, at, width, a.wide, v[i]);
+        Ve::load(dy, at, width, a.wide, g[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] = g[i][j] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = (threadIdx.x + i * blockDim.x) * N;
+      float w[N];
+      if (a.weight && at < width) {
+        Ve::load(static_cast<const T*>(a.weight), at, width, a.wide, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        sum[0] += v[i][j] * v[i][j];
+        sum[1] += w[j] * g[i][j] * v[i][j];
+      }
+    }
+    row_reduce(sum, sh);
+    const float r = rsqrtf(sum[0] / width + a.eps);
+    const float c = r * r * sum[1] / width;  // dx = ds + r (w dy - s c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = (threadIdx.x + i * blockDim.x) * N;
+      if (at >= width) continue;
+      float w[N], d[N];
+      if (a.weight) {
+        Ve::load(static_cast<const T*>(a.weight), at, width, a.wide, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = 1.f;
+      }
+      if (a.ds) {
+        Ve::load(static_cast<const T*>(a.ds) + row * a.ds_stride, at, width, a.wide, d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) d[j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        dw[i][j] += g[i][j] * (v[i][j] * r);
+        d[j] += r * (w[j] * g[i][j] - v[i][j] * c);
+      }
+      Ve::store(static_cast<T*>(a.dx) + row * width, at, width, a.wide, d);
+    }
+  }
+  if (!a.partial) return;
+  float* out = a.partial + (long long)blockIdx.x * width;
+  if (blockDim.y == 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int at = (threadIdx.x + i * blockDim.x) * N;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (at + j < width) out[at + j] = dw[i][j];
+    }
+    return;
+  }
+  // one warp a row: the warps' parts are added in order through shared memory
+  float* mine = sh + 64 + threadIdx.y * (V * 32 * N);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) mine[(threadIdx.x + i * 32) * N + j] = dw[i][j];
+  __syncthreads();
+  for (int c = threadIdx.y * 32 + threadIdx.x; c < width; c += 32 * blockDim.y) {
+    float t = 0.f;
+    for (int y = 0; y < blockDim.y; ++y) t += sh[64 + y * (V * 32 * N) + c];
+    out[c] = t;
+  }
+}
+
+// dw = sum of the blocks' parts: a column per lane, 32 warps share the parts.
+template <class T>
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float* partial, int parts, int width, T* dw) {
+  __shared__ float sh[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float t = 0.f;
+  if (c < width)
+    for (int p = threadIdx.y; p < parts; p += 32) t += partial[(long long)p * width + c];
+  sh[threadIdx.y][threadIdx.x] = t;
+  __syncthreads();
+  t = warp_sum(sh[threadIdx.x][threadIdx.y]);  // warp y adds column y's 32 sums
+  if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < width) dw[blockIdx.x * 32 + threadIdx.y] = from_f<T>(t);
+}
+
+// Threads a row, rows a block and vectors a thread.
+struct Shape {
+  int threads, rows, vectors;
+};
+
+Shape shape_of(long long rows, int width, int elements, bool grad) {
+  const int vectors = (width + elements - 1) / elements;
+  if (rows <= 1184 && vectors <= 1024 && !grad) return {(vectors + 31) / 32 * 32, 1, 1};
+  if (vectors <= 128) return {32, 8, (vectors + 31) / 32};
+  int threads = 128;
+  while (threads < 1024 && vectors > 4 * threads) threads *= 2;
+  const int v = (vectors + threads - 1) / threads;
+  return {threads, 1, v > 4 ? 8 : v};
+}
+
+int nfail(int code, const char* msg) {
+  tao_set_last_error(msg);
+  return code;
+}
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TAO_OK : nfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
+size_t size_of(int type) { return type == TAO_TYPE_FP32 ? 4 : 2; }
+
+// Whether rows of this base and stride start on 16 bytes (an absent operand does).
+bool wide_ok(const void* p, long long stride, size_t size) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (long long)size % 16 == 0);
+}
+
+int check(long long rows, int width, int type) {
+  if (type != TAO_TYPE_BF16 && type != TAO_TYPE_FP16 && type != TAO_TYPE_FP32)
+    return nfail(TAO_ERR_ARG, "the norm takes bf16, fp16 or fp32");
+  if (rows < 0 || width <= 0) return nfail(TAO_ERR_ARG, "rows must not be negative and the width must be positive");
+  if (width > (type == TAO_TYPE_FP32 ? 32768 : 65536))
+    return nfail(TAO_ERR_ARG, "the norm's width is limited to 65536 (32768 in fp32)");
+  return TAO_OK;
+}
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// f(vectors, most threads) as compile-time constants.
+template <class F>
+int by_shape(const Shape& sh, F f) {
+  if (sh.threads * sh.rows <= 256) {
+    switch (sh.vectors) {
+      case 1: return f(Int<1>(), Int<256>());
+      case 2: return f(Int<2>(), Int<256>());
+      case 3: return f(Int<3>(), Int<256>());
+      default: return f(Int<4>(), Int<256>());
+    }
+  }
+  switch (sh.vectors) {
+    case 1: return f(Int<1>(), Int<1024>());
+    case 2: return f(Int<2>(), Int<1024>());
+    case 3:
+    case 4: return f(Int<4>(), Int<1024>());
+    default: return f(Int<8>(), Int<1024>());
+  }
+}
+
+template <class F>
+int by_type(int type, F f) {
+  if (type == TAO_TYPE_BF16) return f(bf16());
+  if (type == TAO_TYPE_FP16) return f(__half());
+  return f(float());
+}
+
+constexpr int kMaxBlocks = 1 << 30;
+
+int forward(NormArgs a, int type, bool fp8, void* stream) {
+  const size_t size = size_of(type);
+  a.wide = a.width % (16 / size) == 0 && wide_ok(a.x, a.x_stride, size) && wide_ok(a.residual, a.r_stride, size) &&
+           wide_ok(a.weight, 0, size) && wide_ok(a.s, 0, size) && wide_ok(a.y, 0, size);
+  const Shape sh = shape_of(a.rows, a.width, (int)(16 / size), false);
+  const unsigned grid = (unsigned)std::min<long long>((a.rows + sh.rows - 1) / sh.rows, kMaxBlocks);
+  const dim3 block(sh.threads, sh.rows);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return by_type(type, [&](auto t) {
+    return by_shape(sh, [&](auto v, auto most) {
+      using T = decltype(t);
+      if (fp8)
+        norm_kernel<T, decltype(v)::value, true, decltype(most)::value><<<grid, block, 0, st>>>(a);
+      else
+        norm_kernel<T, decltype(v)::value, false, decltype(most)::value><<<grid, block, 0, st>>>(a);
+      return launched();
+    });
+  });
+}
+
+// Blocks of the gradient kernel: two of 256 threads an SM, as its registers allow.
+int grad_blocks(long long rows, const Shape& sh) {
+  const long long need = (rows + sh.rows - 1) / sh.rows;
+  const int resident = 148 * std::max(1, 512 / (sh.threads * sh.rows));
+  return (int)std::min<long long>(need, resident);
+}
+
+}  // namespace
+}  // namespace tao
+
+extern "C" {
+
+int tao_add_rms_norm(const void* x, long long x_stride, const void* residual, long long r_stride, const void* weight,
+                     long long rows, int width, int type, float eps, void* s, void* y, void* stream) {
+  using namespace tao;
+  if (int rc = check(rows, width, type)) return rc;
+  if (rows == 0) return TAO_OK;
+  if (!x || !y || (residual && !s)) return nfail(TAO_ERR_ARG, "null pointer");
+  return forward({x, residual, weight, x_stride, r_stride, rows, width, 0, eps, false, s, y, nullptr}, type, false,
+                 stream);
+}
+
+int tao_add_rms_norm_fp8(const void* x, long long x_stride, const void* residual, long long r_stride,
+                         const void* weight, long long rows, int width, int type, float eps, int group, void* s,
+                         void* q, float* scale, void* stream) {
+  using namespace tao;
+  if (int rc = check(rows, width, type)) return rc;
+  if (group != 0 && group != 128) return nfail(TAO_ERR_ARG, "8-bit scales are by row (0) or by 128 channels");
+  if (rows == 0) return TAO_OK;
+  if (!x || !q || !scale || (residual && !s)) return nfail(TAO_ERR_ARG, "null pointer");
+  return forward({x, residual, weight, x_stride, r_stride, rows, width, group, eps, false, s, q, scale}, type, true,
+                 stream);
+}
+
+size_t tao_add_rms_norm_workspace_bytes(long long rows, int width, int type) {
+  using namespace tao;
+  if (check(rows, width, type) != TAO_OK || rows == 0) return 0;
+  return (size_t)grad_blocks(rows, shape_of(rows, width, (int)(16 / size_of(type)), true)) * width * sizeof(float);
+}
+
+int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* ds, long long ds_stride, const void* s,
+                              long long s_stride, const void* weight, long long rows, int width, int type, float eps,
+                              void* dx, void* dw, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace tao;
+  if (int rc = check(rows, width, type)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t size = size_of(type);
+  if (rows == 0) {
+    if (dw && cudaMemsetAsync(dw, 0, width * size, st) != cudaSuccess) return launched();
+    return TAO_OK;
+  }
+  if (!dy || !s || !dx) return nfail(TAO_ERR_ARG, "null pointer");
+  if (dw && (!workspace || workspace_bytes < tao_add_rms_norm_workspace_bytes(rows, width, type)))
+    return nfail(TAO_ERR_ARG, "workspace too small for the norm's weight gradient");
+  NormGradArgs a = {dy, ds, s, weight, dy_stride, ds_stride, s_stride, rows, width, eps, false, dx,
+                    dw ? static_cast<float*>(workspace) : nullptr};
+  a.wide = width % (16 / size) == 0 && wide_ok(dy, dy_stride, size) && wide_ok(ds, ds_stride, size) &&
+           wide_ok(s, s_stride, size) && wide_ok(weight, 0, size) && wide_ok(dx, 0, size);
+  const Shape sh = shape_of(rows, width, (int)(16 / size), true);
+  const int grid = grad_blocks(rows, sh);
+  const dim3 block(sh.threads, sh.rows);
+  return by_type(type, [&](auto t) {
+    return by_shape(sh, [&](auto v, auto most) {
+      using T = decltype(t);
+      constexpr int V = decltype(v)::value;
+      const size_t smem = (64 + (sh.rows > 1 ? (size_t)sh.rows * V * 32 * Vec<T>::N : 0)) * sizeof(float);
+      norm_grad_kernel<T, V, decltype(most)::value><<<grid, block, smem, st>>>(a);
+      if (int rc = launched()) return rc;
+      if (dw) norm_dw_kernel<T><<<(width + 31) / 32, dim3(32, 32), 0, st>>>(a.partial, grid, width, static_cast<T*>(dw));
+      return launched();
+    });
+  });
+}
+
+}  // extern "C"

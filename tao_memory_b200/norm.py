@@ -1,0 +1,128 @@
+"""Root-mean-square norm with the residual's addition: what stands between two halves of
+a decoder block.  ``add_rms_norm`` (16 or 32 bits, differentiable) and
+``add_rms_norm_fp8`` (e4m3 with scales, for the products that take 8-bit activations).
+
+One library kernel forward; the gradient is one kernel and, for the weight, a second one
+that adds the blocks' parts in a fixed order.
+"""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# F.rms_norm's default eps: the epsilon of its fp32 compute type (also for 16-bit inputs)
+RMS_EPS = float(torch.finfo(torch.float32).eps)
+
+
+def _rows(t, width):
+    """``t`` as rows [n, width] with a contiguous last axis; copied only where its strides ask for it."""
+    t = t if t.dim() == 2 else t.reshape(-1, width)
+    return t if t.stride(1) == 1 or width == 1 else t.contiguous()
+
+
+def _check(x, weight, residual):
+    if x.dtype not in TYPES or not x.is_cuda:
+        raise ValueError("the norm takes a bf16, fp16 or fp32 CUDA tensor (no CPU fallback)")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("the norm needs a last axis to sum over")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
+                                 or residual.device != x.device):
+        raise ValueError("the residual must have x's shape, type and device")
+    if weight is not None and (weight.shape != x.shape[-1:] or weight.dtype != x.dtype or weight.device != x.device):
+        raise ValueError("the weight must be one value per channel, of x's type and device")
+
+
+def _forward(x, weight, residual, eps):
+    width = x.shape[-1]
+    rows = _rows(x, width)
+    res = None if residual is None else _rows(residual, width)
+    weight = None if weight is None else weight.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s = x if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _lib.on(x.device):
+        _lib.check(_lib.lib().tao_add_rms_norm(
+            rows.data_ptr(), rows.stride(0), None if res is None else res.data_ptr(),
+            0 if res is None else res.stride(0), None if weight is None else weight.data_ptr(), rows.shape[0], width,
+            TYPES[x.dtype], eps, None if res is None else s.data_ptr(), y.data_ptr(),
+            torch.cuda.current_stream(x.device).cuda_stream))
+    return y, s
+
+
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, s = _forward(x, weight, residual, eps)
+        ctx.save_for_backward(s, weight)
+        ctx.eps, ctx.added = eps, residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, s) if ctx.added else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, weight = ctx.saved_tensors
+        if dy is None:  # only the stream was used
+            return ds, None, ds if ctx.added else None, None
+        width = s.shape[-1]
+        rows, gy = _rows(s, width), _rows(dy, width)
+        gs = None if ds is None else _rows(ds, width)
+        w = None if weight is None else weight.contiguous()
+        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+        dw = torch.empty_like(w) if w is not None and ctx.needs_input_grad[1] else None
+        lib, code = _lib.lib(), TYPES[s.dtype]
+        ws = None
+        if dw is not None:
+            size = lib.tao_add_rms_norm_workspace_bytes(rows.shape[0], width, code)
+            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=s.device)
+        with _lib.on(s.device):
+            _lib.check(lib.tao_add_rms_norm_backward(
+                gy.data_ptr(), gy.stride(0), None if gs is None else gs.data_ptr(), 0 if gs is None else gs.stride(0),
+                rows.data_ptr(), rows.stride(0), None if w is None else w.data_ptr(), rows.shape[0], width, code,
+                ctx.eps, dx.data_ptr(), None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(),
+                0 if ws is None else ws.numel(), torch.cuda.current_stream(s.device).cuda_stream))
+        return dx, dw, dx if ctx.added else None, None
+
+
+def add_rms_norm(x, weight=None, residual=None, eps=RMS_EPS):
+    """(y, s): s = x + residual rounded to x's type (the stream the next block adds to; x
+    itself without a residual) and y = s * rsqrt(mean(s^2) + eps) * weight over the last axis,
+    in fp32, rounded once.  x, residual [..., width] bf16, fp16 or fp32; weight [width] of the
+    same type or None (ones).  Differentiable in x, residual and weight."""
+    _check(x, weight, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        if residual is None:
+            return _AddNorm.apply(x, weight, None, eps), x
+        return _AddNorm.apply(x, weight, residual, eps)
+    return _forward(x, weight, residual, eps)
+
+
+def add_rms_norm_fp8(x, weight=None, residual=None, eps=RMS_EPS, group=None):
+    """(q, scale, s): ``add_rms_norm`` with y in e4m3, y = q * scale: one fp32 scale a row
+    (``group=None``: scale [..., 1], as ``linear4`` and row-scaled products take it) or one for
+    128 channels (``group=128``: [..., ceil(width / 128)]).  Not differentiable."""
+    _check(x, weight, residual)
+    if group not in (None, 128):
+        raise ValueError("8-bit scales are by row (None) or by 128 channels")
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        raise ValueError("the 8-bit norm has no gradient: call it under torch.no_grad()")
+    width = x.shape[-1]
+    rows = _rows(x, width)
+    res = None if residual is None else _rows(residual, width)
+    weight = None if weight is None else weight.contiguous()
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(*x.shape[:-1], 1 if group is None else -(-width // 128), dtype=torch.float32, device=x.device)
+    s = x if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _lib.on(x.device):
+        _lib.check(_lib.lib().tao_add_rms_norm_fp8(
+            rows.data_ptr(), rows.stride(0), None if res is None else res.data_ptr(),
+            0 if res is None else res.stride(0), None if weight is None else weight.data_ptr(), rows.shape[0], width,
+            TYPES[x.dtype], eps, group or 0, None if res is None else s.data_ptr(), q.data_ptr(), scale.data_ptr(),
+            torch.cuda.current_stream(x.device).cuda_stream))
+    return q, scale, s
+
+
+__all__ = ["add_rms_norm", "add_rms_norm_fp8", "RMS_EPS"]
