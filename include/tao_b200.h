@@ -489,6 +489,20 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
                               int width, int type, float eps, void* dx, void* dw, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* y [rows][n] = x [rows][k] W^T + bias for a few rows of x and a 4-bit W [n][k]:
+ * W[n][k] = (code - zero) * scale, one scale (and zero point) for `group` (32, 64 or 128)
+ * consecutive k of a row, codes and zeros 0..15, zeros NULL: 8.  `type`: bf16 or fp16, the
+ * type of scales, bias and y.  x_type: the same, or TAO_TYPE_E4M3 with x_scale [rows] fp32 (NULL: ones).
+ * Products are summed in fp32 over a group, scaled, summed in fp32, rounded once.
+ * Layout (tiles = ceil(n / 16), blocks = ceil(k / 128), what lies beyond n or k has scale 0):
+ *   codes  [tiles][blocks][2][32][4] words: word j of lane 4g+t in half h holds, in nibble
+ *          i + 4p (i, p: 0..3, 0..1), the code of row 16 tile + g + 8 (i & 1) and
+ *          k = 128 block + 64h + 32 (j >> 1) + 8t + 4 (j & 1) + 2 (i >> 1) + p;
+ *   scales [tiles][blocks][128 / group][16], zeros the same in bytes; each on 16 bytes. */
+int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_scale, const void* codes,
+                const void* scales, const void* zeros, int group, int type, const void* bias,
+                long long rows, int n, int k, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

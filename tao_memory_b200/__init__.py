@@ -14,6 +14,7 @@ tokens arrive in and leave through page-locked host memory, and the serving call
 
 from .config import TaoConfig
 from .host_io import copy_to_device, copy_to_host
+from .linear4 import Weight4, linear4, quantize4
 from .norm import add_rms_norm, add_rms_norm_fp8
 from .operator import (new_state, tao_attention, tao_attention_decode,
                        tao_attention_decode_batch, tao_attention_prefill)
@@ -23,4 +24,5 @@ from .stream import DecodeSession, StreamCache
 __all__ = ["new_state", "tao_attention", "tao_attention_prefill",
            "tao_attention_decode", "tao_attention_decode_batch", "StreamCache",
            "TaoConfig", "copy_to_device", "copy_to_host", "DecodeSession", "RequestStates",
-           "DecodeScheduler", "save_snapshot", "load_snapshot", "add_rms_norm", "add_rms_norm_fp8"]
+           "DecodeScheduler", "save_snapshot", "load_snapshot", "add_rms_norm", "add_rms_norm_fp8",
+           "Weight4", "quantize4", "linear4"]

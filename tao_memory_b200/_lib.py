@@ -89,6 +89,7 @@ _SIGNATURES = {
     "tao_add_rms_norm_workspace_bytes": (_SZ, [_I64, _I, _I]),
     "tao_add_rms_norm_backward": (_I, [_VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I, _I, _F, _VP, _VP, _VP, _SZ,
                                        _VP]),
+    "tao_linear4": (_I, [_VP, _I64, _I, _VP, _VP, _VP, _VP, _I, _I, _VP, _I64, _I, _I, _VP, _VP]),
     "tao_feature_read_forward": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "tao_feature_read_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
     "tao_train_pairs": (_I, [_I]),

@@ -1,0 +1,174 @@
+"""Products of a few rows with 4-bit weights: the projections of a decode step, whose time
+is the time to read their weights.
+
+``quantize4`` makes a ``Weight4`` from a weight matrix, ``Weight4.from_codes`` from codes,
+scales and zero points quantised elsewhere; ``linear4`` is the product.  A ``Weight4`` holds
+the codes in the order in which the kernel's warps read them (laid out once, here).
+"""
+
+import torch
+
+from . import _lib
+from .norm import TYPES, _rows
+
+GROUPS = (32, 64, 128)
+_TILE, _BLOCK = 16, 128
+
+
+def _padded(t, n, k, value=0):
+    """``t`` [.., a, b] with its last axes filled up to n and k."""
+    if t.shape[-2:] == (n, k):
+        return t
+    return torch.nn.functional.pad(t, (0, k - t.shape[-1], 0, n - t.shape[-2]), value=value)
+
+
+class Weight4:
+    """4-bit weights [..., n, k]: W = (code - zero) * scale with one scale, and optionally one
+    zero point, for ``group`` consecutive k of a row.  Leading axes are matrices of a stack
+    (one for each expert)."""
+
+    def __init__(self, shape, group, codes, scales, zeros):
+        self.shape, self.group = tuple(shape), group
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+
+    @property
+    def dtype(self):
+        return self.scales.dtype
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def bytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
+
+    @classmethod
+    def from_codes(cls, codes, scales, zeros=None, group=128):
+        """codes uint8 [..., n, k] of 0..15, scales [..., n, ceil(k / group)] bf16 or fp16, zeros
+        uint8 like scales of 0..15 (None: 8 everywhere)."""
+        if group not in GROUPS:
+            raise ValueError("a group is 32, 64 or 128 weights")
+        if codes.dtype != torch.uint8 or codes.dim() < 2 or 0 in codes.shape:
+            raise ValueError("codes are a uint8 tensor [..., n, k]")
+        *lead, n, k = codes.shape
+        parts = -(-k // group)
+        if scales.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("4-bit scales are bf16 or fp16")
+        if zeros is not None and zeros.dtype != torch.uint8:
+            raise ValueError("zero points are uint8")
+        for t in (scales,) if zeros is None else (scales, zeros):
+            if tuple(t.shape) != (*lead, n, parts) or t.device != codes.device:
+                raise ValueError("scales and zeros have one value for each group of a row, on the codes' device")
+        if int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
+            raise ValueError("codes and zero points are 0..15")
+        tiles, blocks, per = -(-n // _TILE), -(-k // _BLOCK), _BLOCK // group
+        count = codes[..., 0, 0].numel()
+        laid = torch.empty(count, tiles, blocks, 1024, dtype=torch.uint8, device=codes.device)
+        flat = codes.reshape(count, n, k)
+        for i in range(count):  # matrix by matrix: the intermediate orders stay small
+            c = _padded(flat[i], tiles * _TILE, blocks * _BLOCK)
+            # n = (tile, row half, g), k = (block, half, j >> 1, t, j & 1, register pair, element)
+            c = c.view(tiles, 2, 8, blocks, 2, 2, 4, 2, 2, 2)
+            # -> tile, block, half, g, t, j >> 1, j & 1, then nibbles (element, register pair, row half)
+            c = c.permute(0, 3, 4, 2, 6, 5, 7, 9, 8, 1).reshape(tiles, blocks, 1024, 2)
+            laid[i] = c[..., 0] | c[..., 1] << 4
+
+        def by_tile(t):
+            t = _padded(t.reshape(count, n, parts), tiles * _TILE, blocks * per)
+            return t.view(count, tiles, _TILE, blocks, per).permute(0, 1, 3, 4, 2).contiguous()
+
+        return cls(codes.shape, group, laid, by_tile(scales), None if zeros is None else by_tile(zeros))
+
+    def to_codes(self):
+        """(codes, scales, zeros) as ``from_codes`` takes them."""
+        *lead, n, k = self.shape
+        count, tiles, blocks, _ = self.codes.shape
+        c = torch.stack((self.codes & 15, self.codes >> 4), -1).view(count, tiles, blocks, 2, 8, 4, 2, 2, 2, 2, 2)
+        c = c.permute(0, 1, 10, 4, 2, 3, 6, 5, 7, 9, 8).reshape(count, tiles * _TILE, blocks * _BLOCK)
+
+        def rows(t):
+            t = t.permute(0, 1, 4, 2, 3).reshape(count, tiles * _TILE, -1)
+            return t[:, :n, :-(-k // self.group)].reshape(*lead, n, -1)
+
+        return (c[:, :n, :k].reshape(*lead, n, k), rows(self.scales),
+                None if self.zeros is None else rows(self.zeros))
+
+    def dequantize(self):
+        """The weights in fp32 [..., n, k]."""
+        codes, scales, zeros = self.to_codes()
+        wide = lambda t: t.float().repeat_interleave(self.group, -1)[..., :codes.shape[-1]]
+        return (codes.float() - (8 if zeros is None else wide(zeros))) * wide(scales)
+
+
+def quantize4(weight, group=128, zeros=False):
+    """``Weight4`` of ``weight`` [..., n, k] (bf16 or fp16, or fp32 with bf16 scales), each group
+    rounded to the nearest of 16 evenly spaced values: from -8 to 7 scales around zero, or
+    (``zeros=True``) over the group's range, which zero is always part of."""
+    if group not in GROUPS:
+        raise ValueError("a group is 32, 64 or 128 weights")
+    if weight.dtype not in TYPES or weight.dim() < 2:
+        raise ValueError("quantize4 takes a bf16, fp16 or fp32 weight [..., n, k]")
+    dtype = torch.bfloat16 if weight.dtype == torch.float32 else weight.dtype
+    *lead, n, k = weight.shape
+    parts = -(-k // group)
+    w = _padded(weight.detach().float(), n, parts * group).view(*lead, n, parts, group)
+    if zeros:
+        low, high = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
+        scales = ((high - low) / 15).to(dtype)
+    else:
+        scales = torch.maximum(w.amax(-1) / 7, -w.amin(-1) / 8).to(dtype)
+    step = scales.float()
+    up = torch.where(step > 0, 1 / step, torch.zeros_like(step)).unsqueeze(-1)
+    if zeros:
+        zero = (-low * up.squeeze(-1)).round().clamp(0, 15)
+        codes = ((w * up).round() + zero.unsqueeze(-1)).clamp(0, 15)
+    else:
+        zero, codes = None, ((w * up).round() + 8).clamp(0, 15)
+    return Weight4.from_codes(codes.to(torch.uint8).view(*lead, n, parts * group)[..., :k], scales,
+                              None if zero is None else zero.to(torch.uint8), group)
+
+
+def linear4(x, weight, bias=None, x_scale=None, out=None):
+    """x W^T + bias: x [..., k] in the weight's type, or in e4m3 with one fp32 scale a row
+    (``x_scale`` [..., 1], as ``add_rms_norm_fp8`` gives them); returns [..., n] in the weight's type.
+
+    Made for few rows (a decode step's): the weight is read once for up to 16 rows, and again
+    for each 16 more.  No gradient."""
+    if not isinstance(weight, Weight4) or len(weight.shape) != 2:
+        raise ValueError("linear4 takes one Weight4 matrix")
+    n, k = weight.shape
+    if not x.is_cuda or x.device != weight.device:
+        raise ValueError("linear4 takes CUDA activations on the weight's device (no CPU fallback)")
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f"activations have {k} channels, as the weight")
+    fp8 = x.dtype == torch.float8_e4m3fn
+    if not fp8 and x.dtype != weight.dtype:
+        raise ValueError("activations have the type of the weight's scales, or are e4m3")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("linear4 has no gradient: call it under torch.no_grad()")
+    rows = _rows(x, k)
+    count = rows.shape[0]
+    if x_scale is not None:
+        if not fp8 or x_scale.dtype != torch.float32 or x_scale.numel() != count or x_scale.device != x.device:
+            raise ValueError("x_scale is one fp32 value a row of e4m3 activations, on their device")
+        x_scale = x_scale.contiguous()
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != weight.dtype or bias.device != x.device:
+            raise ValueError("the bias is one value per output, of the weight's type and device")
+        bias = bias.contiguous()
+    shape = (*x.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, dtype=weight.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != weight.dtype or out.device != x.device or not out.is_contiguous():
+        raise ValueError("out is a contiguous tensor of the result's shape, type and device")
+    with _lib.on(x.device):
+        _lib.check(_lib.lib().tao_linear4(
+            rows.data_ptr(), rows.stride(0), 3 if fp8 else TYPES[x.dtype],
+            None if x_scale is None else x_scale.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+            None if weight.zeros is None else weight.zeros.data_ptr(), weight.group, TYPES[weight.dtype],
+            None if bias is None else bias.data_ptr(), count, n, k, out.data_ptr(),
+            torch.cuda.current_stream(x.device).cuda_stream))
+    return out
+
+
+__all__ = ["Weight4", "quantize4", "linear4"]
