@@ -503,6 +503,31 @@ int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_sc
                 const void* scales, const void* zeros, int group, int type, const void* bias,
                 long long rows, int n, int k, void* y, void* stream);
 
+/* A mixture-of-experts layer: router [experts][width] bf16; gate and up [experts][inner][width] and
+ * down [experts][width][inner], bf16 (group 0: strides in elements between experts and rows, the last
+ * axis contiguous), or 4-bit in tao_linear4's layout with bf16 scales, expert after expert. */
+typedef struct TaoExperts {
+  const void* router;
+  const void *gate, *up, *down;
+  const void *gate_scales, *up_scales, *down_scales; /* 4-bit experts */
+  const void *gate_zeros, *up_zeros, *down_zeros;    /* all or none */
+  long long gate_expert, gate_row, up_expert, up_row, down_expert, down_row;
+  int width, inner, experts, top_k, group, renormalize;
+} TaoExperts;
+
+/* out [tokens][width] = sum over the top_k experts e of a token's softmax(x router^T) (ties to the
+ * lowest expert) of weight * down_e(silu(gate_e x) * (up_e x)), weight the softmax, divided by its sum
+ * over the chosen if `renormalize`.  x bf16, rows x_stride elements apart; sums in fp32 in a fixed
+ * order, out rounded once.  ids, id_weights [tokens][top_k]: the choice, or NULL.  One cooperative
+ * launch for 64 tokens.  workspace: tao_expert_workspace_bytes, zeroed before its first use, used
+ * by one launch at a time; its first word is an error word that tao_expert_check reads (and then
+ * zeroes the whole workspace).  width and inner: multiples of 8; up to 512 experts, top_k up to 16. */
+size_t tao_expert_workspace_bytes(const TaoExperts* layer, int tokens);
+int tao_expert_layer(const TaoExperts* layer, const void* x, long long x_stride, int tokens, void* out,
+                     int* ids, float* id_weights, void* workspace, size_t workspace_bytes,
+                     void* stream);
+int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

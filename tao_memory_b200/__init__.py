@@ -13,6 +13,7 @@ tokens arrive in and leave through page-locked host memory, and the serving call
 """
 
 from .config import TaoConfig
+from .experts import ExpertWeights, expert_layer
 from .host_io import copy_to_device, copy_to_host
 from .linear4 import Weight4, linear4, quantize4
 from .norm import add_rms_norm, add_rms_norm_fp8
@@ -25,4 +26,4 @@ __all__ = ["new_state", "tao_attention", "tao_attention_prefill",
            "tao_attention_decode", "tao_attention_decode_batch", "StreamCache",
            "TaoConfig", "copy_to_device", "copy_to_host", "DecodeSession", "RequestStates",
            "DecodeScheduler", "save_snapshot", "load_snapshot", "add_rms_norm", "add_rms_norm_fp8",
-           "Weight4", "quantize4", "linear4"]
+           "Weight4", "quantize4", "linear4", "ExpertWeights", "expert_layer"]

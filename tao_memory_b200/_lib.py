@@ -38,6 +38,14 @@ class TaoState(ctypes.Structure):
                 ("page_c", ctypes.c_void_p), ("coarse_w", ctypes.c_void_p)]
 
 
+class TaoExperts(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("router", "gate", "up", "down", "gate_scales", "up_scales",
+                                                "down_scales", "gate_zeros", "up_zeros", "down_zeros")]
+                + [(n, ctypes.c_longlong) for n in ("gate_expert", "gate_row", "up_expert", "up_row", "down_expert",
+                                                    "down_row")]
+                + [(n, ctypes.c_int) for n in ("width", "inner", "experts", "top_k", "group", "renormalize")])
+
+
 class TaoError(RuntimeError):
     """A CUDA or device-side failure reported by the library."""
 
@@ -90,6 +98,9 @@ _SIGNATURES = {
     "tao_add_rms_norm_backward": (_I, [_VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I, _I, _F, _VP, _VP, _VP, _SZ,
                                        _VP]),
     "tao_linear4": (_I, [_VP, _I64, _I, _VP, _VP, _VP, _VP, _I, _I, _VP, _I64, _I, _I, _VP, _VP]),
+    "tao_expert_workspace_bytes": (_SZ, [ctypes.POINTER(TaoExperts), _I]),
+    "tao_expert_layer": (_I, [ctypes.POINTER(TaoExperts), _VP, _I64, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "tao_expert_check": (_I, [_VP, _SZ, ctypes.POINTER(_I), _VP]),
     "tao_feature_read_forward": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "tao_feature_read_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
     "tao_train_pairs": (_I, [_I]),

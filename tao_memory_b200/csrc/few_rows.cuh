@@ -121,17 +121,19 @@ struct Four {
   const uint8_t* zeros;    // the same, or null: 8
 };
 
-// One 4-bit block against eight activation rows for each of NT column tiles.  `b(u, nt)`
-// gives the lane's 8 activations of 32-k part u as four operand registers;
-// `scale(j, row)` the scale of group j of the block.  The codes' products are summed in
-// fp32 over a group and scaled then, so no weight is ever rounded.
-template <class M, int GROUP, int NT, class B, class S>
-TAO_DEVI void four_block(float (&acc)[NT][4], uint32_t codes, uint32_t zeros, bool has_zeros, int lane, B b, S scale) {
-  constexpr int PARTS = GROUP / 32;  // 32-k parts of a group
+// KB (64 or 128) k of a 4-bit block against eight activation rows for each of NT column
+// tiles, those that hold some of the `cols` rows.  `b(u, n)` gives the lane's 8 activations
+// of 32-k part u as four operand registers; `scale(j, row)` the scale of group j.  The
+// codes' products are summed in fp32 over a group (or the KB k of it) and scaled then, so
+// no weight is ever rounded.
+template <class M, int GROUP, int KB, int NT, class B, class S>
+TAO_DEVI void four_block(float (&acc)[NT][4], uint32_t codes, uint32_t zeros, bool has_zeros, int lane, int cols, B b,
+                         S scale) {
+  constexpr int SPAN = GROUP < KB ? GROUP : KB, PARTS = SPAN / 32;  // k, and 32-k parts, under one scale
   const int g = lane >> 2;
   uint4 w = lds16(codes + lane * 16);
 #pragma unroll
-  for (int j = 0; j < 128 / GROUP; ++j) {
+  for (int j = 0; j < KB / SPAN; ++j) {
     uint32_t z0 = 8, z1 = 8;
     if (has_zeros) {
       z0 = lds_u8(zeros + j * 16 + g);
@@ -155,6 +157,7 @@ TAO_DEVI void four_block(float (&acc)[NT][4], uint32_t codes, uint32_t zeros, bo
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if (n && n * 8 >= cols) break;
         const uint4 x = b(u, n);
         M::mma(t[n], a[0][0], a[0][1], a[0][2], a[0][3], x.x, x.y);
         M::mma(t[n], a[1][0], a[1][1], a[1][2], a[1][3], x.z, x.w);

@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_kernel(const Linear4Args 
       }
     };
     auto scale = [&](int j, int row) { return scale_f(lds_u16(at + 1024 + (j * 16 + row) * 2), a.bf16_out); };
-    four_block<M, GROUP, NT>(acc, at, at + zoff, has_zeros, lane, b, scale);
+    four_block<M, GROUP, 128, NT>(acc, at, at + zoff, has_zeros, lane, rows, b, scale);
   }
   cp_wait<0>();
   __syncthreads();  // the rings become the warps' sums [warp][column][16 rows]

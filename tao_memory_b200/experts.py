@@ -1,0 +1,142 @@
+"""Mixture-of-experts layer for the few tokens of a decode step: routing, the chosen experts'
+gate, up and down products and their weighted sum in one kernel, whose time is the time to
+read the chosen experts.  Weights in bf16 or 4 bits (``Weight4`` stacks).
+"""
+
+import ctypes
+import weakref
+
+import torch
+
+from . import _lib
+from .linear4 import Weight4
+from .norm import _rows
+
+_BF16 = torch.bfloat16
+_TOKENS = 64  # of one launch
+
+
+class ExpertWeights:
+    """One layer's router and experts: router [experts, width] bf16; gate, up [experts, inner,
+    width] and down [experts, width, inner], all bf16 tensors (views of a fused tensor are taken
+    as they are where their rows start on 16 bytes) or all ``Weight4`` stacks of one group and
+    kind.  ``renormalize``: the chosen experts' softmax weights are divided by their sum."""
+
+    def __init__(self, router, gate, up, down, top_k, renormalize=True):
+        four = [isinstance(w, Weight4) for w in (gate, up, down)]
+        if any(four) and not all(four):
+            raise ValueError("gate, up and down are all bf16 tensors or all Weight4 stacks")
+        if router.dim() != 2 or len(gate.shape) != 3:
+            raise ValueError("the router is [experts, width] and experts are stacked [experts, ...]")
+        experts, width = router.shape
+        inner = gate.shape[1]
+        if (tuple(gate.shape) != (experts, inner, width) or tuple(up.shape) != (experts, inner, width)
+                or tuple(down.shape) != (experts, width, inner)):
+            raise ValueError("gate and up are [experts, inner, width], down [experts, width, inner]")
+        if any(t.dtype != _BF16 for t in (router, gate, up, down)):
+            raise ValueError("the expert layer takes bf16 weights (4-bit: bf16 scales)")
+        if not router.is_cuda or any(t.device != router.device for t in (gate, up, down)):
+            raise ValueError("the expert layer's weights are on one CUDA device (no CPU fallback)")
+        if all(four) and (len({w.group for w in (gate, up, down)}) > 1
+                          or len({w.zeros is None for w in (gate, up, down)}) > 1):
+            raise ValueError("4-bit experts share one group size, and have zero points all or none")
+        if not 1 <= top_k <= experts:
+            raise ValueError("top_k is 1 to 16 and at most the number of experts")
+        self.width, self.inner, self.experts, self.top_k = width, inner, experts, top_k
+        self.renormalize, self.device = bool(renormalize), router.device
+        self.router = _aligned(router)
+        if all(four):
+            self.gate, self.up, self.down = gate, up, down
+            data = [[w.codes, w.scales, w.zeros] for w in (gate, up, down)]
+            strides, group = [0] * 6, gate.group
+        else:
+            self.gate, self.up, self.down = (_aligned(w) for w in (gate, up, down))
+            data = [[w, None, None] for w in (self.gate, self.up, self.down)]
+            strides, group = [s for w in (self.gate, self.up, self.down) for s in w.stride()[:2]], 0
+        at = lambda t: None if t is None else t.data_ptr()
+        if self.router.stride(0) != width:
+            self.router = self.router.contiguous()
+        self._layer = _lib.TaoExperts(at(self.router), *(at(d[i]) for i in range(3) for d in data), *strides, width,
+                                      inner, experts, top_k, group, int(self.renormalize))
+        lib = _lib.lib()
+        one, most = (lib.tao_expert_workspace_bytes(ctypes.byref(self._layer), n) for n in (1, _TOKENS))
+        if one == 0:
+            _lib.check(_lib.TAO_ERR_ARG)
+        self._workspace_bytes = most
+
+
+def _aligned(t):
+    """``t`` with a contiguous last axis and rows that start on 16 bytes."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+class _Room:
+    """Workspaces of the expert layer: zeroed once, one for a device and stream, so calls on
+    two streams do not meet in one; a captured call gets one of its own, zeroed by its graph."""
+
+    cache = {}
+    captured = {}
+
+    @classmethod
+    def get(cls, device, stream, nbytes):
+        if torch.cuda.is_current_stream_capturing():
+            buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            cls.captured.setdefault(device, weakref.WeakSet()).add(buf)
+            return buf
+        buf = cls.cache.get((device, stream))
+        if buf is None or buf.numel() < nbytes:
+            buf = cls.cache[(device, stream)] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        return buf
+
+    @classmethod
+    def on_device(cls, device):
+        return [b for (d, _), b in list(cls.cache.items()) if d == device] + list(cls.captured.get(device, ()))
+
+
+def expert_layer(x, weights, out=None, return_routing=False):
+    """sum over the ``top_k`` experts of a token of weight * down(silu(gate x) * (up x)): x
+    [..., width] bf16 -> [..., width] bf16.  With ``return_routing`` also the chosen experts
+    [..., top_k] int32 (most probable first, ties to the lowest) and their weights in fp32.
+
+    One launch for 64 tokens; made for the few tokens of a decode step, it reads the chosen
+    experts again for each 64 more.  No gradient."""
+    if not isinstance(weights, ExpertWeights):
+        raise ValueError("expert_layer takes ExpertWeights")
+    if x.dtype != _BF16 or not x.is_cuda or x.device != weights.device:
+        raise ValueError("expert_layer takes bf16 CUDA activations on the weights' device (no CPU fallback)")
+    if x.dim() == 0 or x.shape[-1] != weights.width:
+        raise ValueError(f"activations have {weights.width} channels, as the layer")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("expert_layer has no gradient: call it under torch.no_grad()")
+    rows = _rows(x, weights.width)
+    if rows.data_ptr() % 16 or rows.stride(0) % 8:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    tokens = rows.shape[0]
+    if out is None:
+        out = torch.empty(x.shape, dtype=_BF16, device=x.device)
+    elif out.shape != x.shape or out.dtype != _BF16 or out.device != x.device or not out.is_contiguous():
+        raise ValueError("out is a contiguous tensor of x's shape, type and device")
+    ids = route = None
+    if return_routing:
+        ids = torch.empty(*x.shape[:-1], weights.top_k, dtype=torch.int32, device=x.device)
+        route = torch.empty(ids.shape, dtype=torch.float32, device=x.device)
+    with _lib.on(x.device):
+        stream = torch.cuda.current_stream(x.device).cuda_stream
+        ws = _Room.get(x.device, stream, weights._workspace_bytes)
+        _lib.check(_lib.lib().tao_expert_layer(
+            ctypes.byref(weights._layer), rows.data_ptr(), rows.stride(0), tokens, out.data_ptr(),
+            None if ids is None else ids.data_ptr(), None if ids is None else route.data_ptr(), ws.data_ptr(),
+            ws.numel(), stream))
+    return (out, ids, route) if return_routing else out
+
+
+def check_workspaces(device):
+    """Raise if an expert layer on ``device`` reported an error since the last check (part of
+    ``stream.check_device``; the device is synchronised)."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    for ws in _Room.on_device(device):
+        _lib.check(_lib.lib().tao_expert_check(ws.data_ptr(), ws.numel(), None, stream))
+
+
+__all__ = ["ExpertWeights", "expert_layer"]

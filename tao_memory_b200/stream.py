@@ -840,6 +840,8 @@ def check_device(device=None):
     for ws in [buf for _, buf in _Workspace.on_device(dev)] + list(_GRAPH_WORKSPACES.get(dev, ())):
         _lib.check(_lib.lib().tao_stream_check(ws.data_ptr(), ctypes.byref(flags), current))
         total |= flags.value
+    from .experts import check_workspaces
+    check_workspaces(dev)
     return total
 
 
