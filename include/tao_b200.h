@@ -495,10 +495,11 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
  * type of scales, bias and y.  x_type: the same, or TAO_TYPE_E4M3 with x_scale [rows] fp32 (NULL: ones).
  * Products are summed in fp32 over a group, scaled, summed in fp32, rounded once.
  * Layout (tiles = ceil(n / 16), blocks = ceil(k / 128), what lies beyond n or k has scale 0):
- *   codes  [tiles][blocks][2][32][4] words: word j of lane 4g+t in half h holds, in nibble
- *          i + 4p (i, p: 0..3, 0..1), the code of row 16 tile + g + 8 (i & 1) and
- *          k = 128 block + 64h + 32 (j >> 1) + 8t + 4 (j & 1) + 2 (i >> 1) + p;
- *   scales [tiles][blocks][128 / group][16], zeros the same in bytes; each on 16 bytes. */
+ *   codes  [tiles][blocks][2][32][16] bytes: byte 8i + 4f + e of lane 4g + t of half h holds the codes of
+ *          k = 128 block + 64h + 32i + 8t + 4f + (0, 2, 1, 3)[e], of row 16 tile + g in its low nibble and
+ *          of row 16 tile + g + 8 in the high one;
+ *   scales [tiles][blocks][8][128 / group][2]: rows g and g + 8 of a tile, group by group; zeros the
+ *          same in bytes; each of the three on 16 bytes.  k up to 65536. */
 int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_scale, const void* codes,
                 const void* scales, const void* zeros, int group, int type, const void* bias,
                 long long rows, int n, int k, void* y, void* stream);

@@ -41,6 +41,13 @@ TAO_DEVI float warp_max(float v) {
   return v;
 }
 
+// Maximum that keeps a NaN (fmaxf drops it).
+TAO_DEVI float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Products of two bf16 pairs rounded to bf16, lane by lane.  The product of two
 // bf16 values is exact in fp32, so this equals rb(a * b) for each lane.
 TAO_DEVI uint32_t hmul2u(uint32_t a, uint32_t b) {

@@ -9,10 +9,12 @@
 //   2. every block picks the top_k itself (the same arithmetic in all of them) and sorts the
 //      (token, expert) pairs by expert; then 16 inner channels of one expert's gate and up at a
 //      time, h = silu(gate) up;
-//   3. 32 outputs of one expert's down at a time, a row of sums for each pair; the block that
-//      completes 32 outputs adds the tokens' pairs in the order of their choice.
-// Parts 1 to 3 are the same product of a few rows (few_rows.cuh): the eight warps split k, each
-// streams its blocks through a ring that runs on from one unit of work to the next.
+//   3. 32 outputs of one expert's down at a time, a row of sums for each pair; and after a last
+//      barrier a token's pairs are added in the order of their choice.
+// Parts 1 to 3 are the same product of a few rows (few_rows.cuh).  One block an SM takes a run of
+// neighbouring units of work, so that its rows' activations stay in L1; its 16 warps are WT x WK, WT
+// units at a time, each one's k dealt to WK warps in runs, each warp's weights through a ring of its own
+// that runs on from unit to unit (part 3's starts before the barrier).
 // h is kept as the sum of two bf16 (16 mantissa bits), which are two columns of one mma: with bf16
 // alone its rounding would add as much to the error as the output's own.  Every sum's order is fixed.
 #include <cuda_runtime.h>
@@ -28,12 +30,12 @@ void tao_set_last_error(const char* msg);
 namespace tao {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kTokens = 64;    // of a launch: a bit each of an expert's mask
 constexpr int kExperts = 512;  // most experts, and
 constexpr int kTop = 16;       // most of them for a token
 constexpr int kCols = 8;       // tokens of an entry: (expert, up to 8 of its tokens)
-constexpr int kHeader = 256;   // workspace: error word, barrier word; then the outputs' counters
+constexpr int kHeader = 256;   // workspace: error word and barrier word
 
 struct Matrix16 {  // bf16 [experts][rows][k], the last axis contiguous
   const bf16* at;
@@ -52,81 +54,67 @@ struct ExpertArgs {
   float* id_weights;
   int* error;
   unsigned* barrier;
-  int* counters;     // [ceil(width / 32)], zero between launches
   float* logits;     // [tokens][experts]
   bf16* h;           // [2][pairs][inner]: rounded, and what the rounding left
   float* pair_out;   // [pairs][width]
 };
 
-// 16-bit weights: blocks of 16 rows x 32 k.
+// A run of blocks of a row tile of 16-bit weights, 16 rows x 32 k each, straight from the matrix' rows.
 struct W16 {
-  static constexpr int KB = 32, BYTES = 1024;
-  struct Ref {
-    const bf16 *r0, *r1;
-  };
-  static TAO_DEVI Ref ref(const Matrix16& m, int rows, int e, int tile, int lane) {
-    const int r = tile * 16 + (lane >> 2);  // rows beyond the matrix repeat its last one
-    const bf16* at = m.at + e * m.expert + (lane & 3) * 8;
-    return {at + min(r, rows - 1) * m.row, at + min(r + 8, rows - 1) * m.row};
+  static constexpr int KB = 32, BYTES = 1024, DEPTH = 4;
+  using Matrix = Matrix16;
+  const bf16 *r0, *r1, *any;
+  int left;  // of k from this lane's next chunk on
+
+  // From block `kb` on; rows beyond the matrix repeat its last one.
+  TAO_DEVI void start(const Matrix& m, int rows, int k, int e, int tile, int kb, int lane) {
+    const int r = tile * 16 + (lane >> 2), at = kb * KB + (lane & 3) * 8;
+    any = m.at + e * m.expert;
+    r0 = any + min(r, rows - 1) * m.row + at;
+    r1 = any + min(r + 8, rows - 1) * m.row + at;
+    left = k - at;
   }
-  static TAO_DEVI void issue(uint32_t to, const Ref& w, int kb, int k, int lane) {
-    const bool in = kb * 32 + (lane & 3) * 8 < k;
-    const int at = in ? kb * 32 : 0;
-    cp_async16(to + lane * 16, in ? w.r0 + at : w.r0 - (lane & 3) * 8, in);
-    cp_async16(to + 512 + lane * 16, in ? w.r1 + at : w.r1 - (lane & 3) * 8, in);
+  TAO_DEVI void issue(uint32_t to, int lane) {
+    cp_async16(to + lane * 16, left > 0 ? r0 : any, left > 0);
+    cp_async16(to + 512 + lane * 16, left > 0 ? r1 : any, left > 0);
+    r0 += KB;
+    r1 += KB;
+    left -= KB;
   }
   template <int NT, class B>
-  static TAO_DEVI void compute(float (&acc)[NT][4], uint32_t at, bool, int lane, int cols, B b) {
-    const uint4 w0 = lds16(at + lane * 16), w1 = lds16(at + 512 + lane * 16);
+  static TAO_DEVI void product(float (&acc)[NT][4], const uint8_t* from, bool, int lane, int cols, B b) {
+    const uint4 w0 = *reinterpret_cast<const uint4*>(from + lane * 16);
+    const uint4 w1 = *reinterpret_cast<const uint4*>(from + 512 + lane * 16);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (n && n * 8 >= cols) break;
       const uint4 x = b(0, n);
-      MmaBf16::mma(acc[n], w0.x, w1.x, w0.y, w1.y, x.x, x.y);
-      MmaBf16::mma(acc[n], w0.z, w1.z, w0.w, w1.w, x.z, x.w);
+      mma_bf16(acc[n], w0.x, w1.x, w0.y, w1.y, x.x, x.y);
+      mma_bf16(acc[n], w0.z, w1.z, w0.w, w1.w, x.z, x.w);
     }
   }
 };
 
-// 4-bit weights: blocks of 16 rows x 128 k, or halves of them where the rows' part of a
-// ring's stage would leave no room for two.
-template <int GROUP, int KBLOCK>
+// The same of 4-bit weights, 16 rows x 128 k each.
+template <int GROUP>
 struct W4 {
-  static constexpr int KB = KBLOCK, CODES = KB * 8, SCALES = (KB > GROUP ? KB / GROUP : 1) * 32;
-  static constexpr int BYTES = CODES + SCALES + SCALES / 2;
-  static constexpr int SHARED = KB < GROUP ? GROUP / KB : 1;  // blocks under one scale
-  struct Ref {
-    const uint8_t *codes, *scales, *zeros;
-  };
-  static TAO_DEVI Ref ref(const Four& m, int rows, int k, int e, int tile, int lane) {
-    const int tiles = (rows + 15) / 16, blocks = (k + 127) / 128;
-    const long long at = ((long long)e * tiles + min(tile, tiles - 1)) * blocks;
-    constexpr int ALL = 128 / GROUP * 32;
-    return {m.codes + at * 1024 + lane * 16, reinterpret_cast<const uint8_t*>(m.scales) + at * ALL + lane * 16,
-            m.zeros ? m.zeros + at * (ALL / 2) + (lane - 16) * 16 : nullptr};
-  }
-  static TAO_DEVI void issue(uint32_t to, const Ref& w, int kb, int, int lane) {
-#pragma unroll
-    for (int i = 0; i < CODES / 512; ++i)
-      cp_async16(to + i * 512 + lane * 16, w.codes + kb * (long long)CODES + i * 512, true);
-    if (lane < SCALES / 16)
-      cp_async16(to + CODES + lane * 16, w.scales + kb / SHARED * (long long)SCALES, true);
-    else if (w.zeros && lane >= 16 && lane < 16 + SCALES / 32)
-      cp_async16(to + CODES + SCALES + (lane - 16) * 16, w.zeros + kb / SHARED * (long long)(SCALES / 2), true);
-  }
-  template <int NT, class B>
-  static TAO_DEVI void compute(float (&acc)[NT][4], uint32_t at, bool zeros, int lane, int cols, B b) {
-    auto scale = [&](int j, int row) { return __uint_as_float(lds_u16(at + CODES + (j * 16 + row) * 2) << 16); };
-    four_block<MmaBf16, GROUP, KB, NT>(acc, at, at + CODES + SCALES, zeros, lane, cols, b, scale);
-  }
-};
+  static constexpr int KB = 128, BYTES = Block4<GROUP>::BYTES, DEPTH = 4;
+  using Matrix = Four;
+  const Four* m;
+  uint32_t block;
 
-// One unit of a part: R weight tiles against `cols` rows.
-template <class W, int R, int NT>
-struct Unit {
-  typename W::Ref w[R];
-  const bf16* x[NT];  // this lane's column of each column tile, or null
-  int cols;
+  TAO_DEVI void start(const Matrix& matrix, int rows, int k, int e, int tile, int kb, int) {
+    const uint32_t tiles = (rows + 15) / 16, blocks = (k + 127) / 128;
+    m = &matrix;
+    block = (e * tiles + min((uint32_t)tile, tiles - 1)) * blocks + kb;
+  }
+  TAO_DEVI void issue(uint32_t to, int lane) { Block4<GROUP>::issue(to, *m, block++, lane); }
+  template <int NT, class B>
+  static TAO_DEVI void product(float (&acc)[NT][4], const uint8_t* from, bool zeros, int lane, int cols, B b) {
+    Block4<GROUP> block;
+    block.load(from, zeros, lane);
+    block.template product16<MmaBf16, true, NT>(acc, cols, b);
+  }
 };
 
 struct Shared {
@@ -136,118 +124,140 @@ struct Shared {
   uint16_t id[kTokens * kTop], row[kTokens * kTop];   // of a token's choices: expert, row of its pair
   float weight[kTokens * kTop];
   uint8_t token[kTokens * kTop];                      // of a pair's row
-  int entries, last;
+  int entries;
   bool ok;
 };
 
-template <int N>
-TAO_DEVI void wait_open() { cp_wait<N>(); }
-TAO_DEVI void wait_open(int n) {
-  switch (n) {
-    case 0: cp_wait<0>(); break;
-    case 1: cp_wait<1>(); break;
-    case 2: cp_wait<2>(); break;
-    case 3: cp_wait<3>(); break;
-    case 4: cp_wait<4>(); break;
-    case 5: cp_wait<5>(); break;
-    default: cp_wait<6>(); break;
+constexpr int kSlot = 2 * 8 * 16;             // floats of a warp's sums of a unit
+constexpr int kSums = 2 * kWarps * kSlot;     // of the unit at hand and the one before
+
+// Warps of a unit: the fewest blocks on the longest warp's way, then the fewest warps.
+TAO_DEVI int pick_wk(int units, int kblocks) {
+  const int n = (units + gridDim.x - 1) / gridDim.x;
+  int best = 0, least = 1 << 30;
+#pragma unroll
+  for (int shift = 0; 1 << shift <= kWarps; ++shift) {
+    const int groups = kWarps >> shift, cost = (n + groups - 1) / groups * ((kblocks + (1 << shift) - 1) >> shift);
+    if (cost < least && 1 << shift <= kblocks) {
+      least = cost;
+      best = shift;
+    }
   }
+  return best;
 }
 
-// The units blockIdx.x, blockIdx.x + gridDim.x, ... of a part.  `unit(u)` gives a unit; `sink(u,
-// sum)` takes its sums, sum(r, column, row), where the columns of a PAIR are added in twos.
-// `red` holds 8 * R * (PAIR ? 4 : 8) * NT * 16 floats.
-template <class W, int R, int NT, bool PAIR, class UnitOf, class Sink>
-TAO_DEVI void run_part(int units, int k, int cols_max, bool zeros, uint32_t ring, int ring_bytes, float* red,
-                       UnitOf unit_of, Sink sink) {
-  constexpr int COLS = PAIR ? 4 * NT : 8 * NT;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kblocks = (k + W::KB - 1) / W::KB, per = (kblocks + kWarps - 1) / kWarps;
-  const int stage = R * W::BYTES + cols_max * W::KB * 2, depth = min(8, ring_bytes / stage);
-  const int mine = units > (int)blockIdx.x ? (units - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
-  const int total = mine * per;
+// A part's units, a run of neighbours for each block: unit u is row tiles R (u % tiles) ... of entry
+// u / tiles.  `weights(w, r, entry, tile, kb)` starts run w at block kb of unit (entry, tile)'s matrix r;
+// `rows(entry, c)` gives the row of column c or null; `cols(entry)` their number; `meet()` is called when
+// the first weights are on their way and before the first row is read; `sink(entry, tile, column, row,
+// sum)` takes sum(r) of each column and row, where the columns of a PAIR are added in twos.
+template <class W, int R, int NT, bool PAIR, class Weights, class Rows, class Cols, class Meet, class Sink>
+TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings, float* sums, Weights weights,
+                       Rows rows, Cols cols, Meet meet, Sink sink) {
+  constexpr int STAGE = R * W::BYTES;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int kblocks = (k + W::KB - 1) / W::KB, units = entries * tiles;
+  const int wks = pick_wk(units, kblocks), groups = kWarps >> wks;
+  const int wt = warp >> wks, wk = warp & ((1 << wks) - 1);
+  const int kw = kblocks * wk >> wks, per = (kblocks * (wk + 1) >> wks) - kw;
+  const int lo = (int)((long long)units * blockIdx.x / gridDim.x);
+  const int hi = (int)((long long)units * (blockIdx.x + 1) / gridDim.x);
+  const int mine = lo + wt < hi ? (hi - lo - wt + groups - 1) / groups : 0;
+  uint8_t* const ring = rings + warp * (W::DEPTH * STAGE);
+  const uint32_t ring_at = smem_u32(ring);
 
-  int iu = blockIdx.x, ib = 0, islot = 0, iat = 0;  // what is issued next
-  Unit<W, R, NT> next;
+  int entry = (lo + wt) / tiles, tile = lo + wt - entry * tiles;
+  int le = entry, lt = tile, lk = 0, left = mine * per, to_slot = 0;  // what is copied next
+  W w[R];
   auto issue = [&]() {
-    if (iat < total) {
-      if (ib == 0) next = unit_of(iu);
-      const int kb = ib * kWarps + warp;
-      if (kb < kblocks) {
-        const uint32_t to = ring + islot * stage;
+    if (left > 0) {
+      --left;
+      if (lk == 0) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) W::issue(to + r * W::BYTES, next.w[r], kb, k, lane);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (next.x[n]) {
-#pragma unroll
-            for (int u = 0; u < W::KB / 32; ++u) {
-              const int at = kb * W::KB + u * 32 + t * 8;
-              cp_async16(to + R * W::BYTES + ((u * cols_max + n * 8 + g) * 4 + t) * 16,
-                         at < k ? next.x[n] + at : next.x[n], at < k);
-            }
-          }
-        }
+        for (int r = 0; r < R; ++r) weights(w[r], r, le, lt, kw);
       }
-      ++iat;
-      if (++ib == per) {
-        ib = 0;
-        iu += gridDim.x;
+#pragma unroll
+      for (int r = 0; r < R; ++r) w[r].issue(ring_at + to_slot + r * W::BYTES, lane);
+      to_slot = to_slot == (W::DEPTH - 1) * STAGE ? 0 : to_slot + STAGE;
+      if (++lk == per) {
+        lk = 0;
+        for (lt += groups; lt >= tiles; lt -= tiles) ++le;
       }
-      if (++islot == depth) islot = 0;
     }
     cp_commit();
   };
+#pragma unroll 1
+  for (int d = 0; d < W::DEPTH - 1; ++d) issue();
+  if (!meet()) {
+    cp_wait<0>();
+    return false;
+  }
 
-  float acc[R][NT][4];
-  int slot = 0;
-  for (int i = 0; i < depth - 1; ++i) issue();
-  for (int ui = 0, u = blockIdx.x; ui < mine; ++ui, u += gridDim.x) {
-    const int cols = unit_of(u).cols;
+  int slot = 0, parity = 0;
+#pragma unroll 1
+  for (int u = 0; u < mine; ++u) {
+    const int n_cols = cols(entry);
+    const bf16* x[NT];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.f;
+    for (int n = 0; n < NT; ++n) x[n] = n * 8 + g < n_cols ? rows(entry, n * 8 + g) + t * 8 : nullptr;
+    float acc[R][NT][4] = {};
+#pragma unroll 1
     for (int i = 0; i < per; ++i) {
-      wait_open(depth - 2);
-      __syncwarp();  // the block is there for every lane, and every lane is done with the one before
-      issue();
-      const uint32_t at = ring + slot * stage;
-      if (++slot == depth) slot = 0;
-      if (i * kWarps + warp >= kblocks) continue;
-      auto b = [&](int uu, int n) {
-        const int m = min(n * 8 + g, cols - 1);  // columns without a row repeat one; nothing reads them
-        return lds16(at + R * W::BYTES + ((uu * cols_max + m) * 4 + t) * 16);
-      };
+      const int k0 = (kw + i) * W::KB;
+      uint4 v[W::KB / 32][NT];
 #pragma unroll
-      for (int r = 0; r < R; ++r) W::template compute<NT>(acc[r], at + r * W::BYTES, zeros, lane, cols, b);
+      for (int p = 0; p < W::KB / 32; ++p)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          v[p][n] = make_uint4(0, 0, 0, 0);
+          if (x[n] && k0 + p * 32 + t * 8 < k) v[p][n] = *reinterpret_cast<const uint4*>(x[n] + k0 + p * 32);
+        }
+      cp_wait<W::DEPTH - 2>();
+      __syncwarp();  // the stage is there for every lane, and every lane is done with the one before
+      issue();
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        W::template product<NT>(acc[r], ring + slot + r * W::BYTES, zeros, lane, n_cols,
+                                [&](int p, int n) { return v[p][n]; });
+      slot = slot == (W::DEPTH - 1) * STAGE ? 0 : slot + STAGE;
     }
+    float* to = sums + (parity * kWarps + warp) * kSlot;  // [R][column][16 rows]
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if constexpr (PAIR) {
-          float* to = red + ((warp * R + r) * COLS + n * 4 + t) * 16 + g;
-          to[0] = acc[r][n][0] + acc[r][n][1];
-          to[8] = acc[r][n][2] + acc[r][n][3];
+          float* c = to + (r * 8 + n * 4 + t) * 16 + g;
+          c[0] = acc[r][n][0] + acc[r][n][1];
+          c[8] = acc[r][n][2] + acc[r][n][3];
         } else {
-          float* to = red + ((warp * R + r) * COLS + n * 8 + 2 * t) * 16 + g;
-          to[0] = acc[r][n][0];
-          to[16] = acc[r][n][1];
-          to[8] = acc[r][n][2];
-          to[24] = acc[r][n][3];
+          float* c = to + (r * 8 + n * 8 + 2 * t) * 16 + g;
+          c[0] = acc[r][n][0];
+          c[16] = acc[r][n][1];
+          c[8] = acc[r][n][2];
+          c[24] = acc[r][n][3];
         }
       }
-    __syncthreads();
-    sink(u, [&](int r, int col, int row) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) s += red[((w * R + r) * COLS + col) * 16 + row];
-      return s;
-    });
-    __syncthreads();
+    // the unit's warps meet; the sums before the last ones are free again
+    if (wks == 0)
+      __syncwarp();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(32 << wks) : "memory");
+    const float* from = sums + (parity * kWarps + (wt << wks)) * kSlot;
+    const int outs = (PAIR ? n_cols / 2 : n_cols) * 16;
+    for (int i = wk * 32 + lane; i < outs; i += 32 << wks)
+      sink(entry, tile, i / 16, i % 16, [&](int r) {
+        float s = 0.f;
+        for (int q = 0; q < 1 << wks; ++q) s += from[q * kSlot + r * 128 + i];
+        return s;
+      });
+    parity ^= 1;
+    for (tile += groups; tile >= tiles; tile -= tiles) ++entry;
   }
   cp_wait<0>();
+  __syncthreads();
+  return true;
 }
 
 // All blocks of the launch meet.  The word's top bit flips when the last one arrives (block 0
@@ -384,161 +394,101 @@ TAO_DEVI void sort_pairs(const ExpertArgs& a, Shared& s) {
   __syncthreads();
 }
 
-// The experts' matrices in the layer's format; In and Down: the forms of parts 2 and 3.
+// The experts' matrices in the layer's format.
 struct Layer16 {
-  using In = W16;
-  using Down = W16;
-  static TAO_DEVI W16::Ref gate(const ExpertArgs& a, int e, int tile, int lane) {
-    return W16::ref(a.gate16, a.inner, e, tile, lane);
-  }
-  static TAO_DEVI W16::Ref up(const ExpertArgs& a, int e, int tile, int lane) {
-    return W16::ref(a.up16, a.inner, e, tile, lane);
-  }
-  static TAO_DEVI W16::Ref down(const ExpertArgs& a, int e, int tile, int lane) {
-    return W16::ref(a.down16, a.width, e, tile, lane);
-  }
-  static TAO_DEVI bool zeros(const ExpertArgs&) { return false; }
+  using W = W16;
+  static TAO_DEVI const Matrix16& gate(const ExpertArgs& a) { return a.gate16; }
+  static TAO_DEVI const Matrix16& up(const ExpertArgs& a) { return a.up16; }
+  static TAO_DEVI const Matrix16& down(const ExpertArgs& a) { return a.down16; }
 };
 template <int GROUP>
 struct Layer4 {
-  using In = W4<GROUP, 128>;
-  using Down = W4<GROUP, 64>;
-  static TAO_DEVI typename In::Ref gate(const ExpertArgs& a, int e, int tile, int lane) {
-    return In::ref(a.gate4, a.inner, a.width, e, tile, lane);
-  }
-  static TAO_DEVI typename In::Ref up(const ExpertArgs& a, int e, int tile, int lane) {
-    return In::ref(a.up4, a.inner, a.width, e, tile, lane);
-  }
-  static TAO_DEVI typename Down::Ref down(const ExpertArgs& a, int e, int tile, int lane) {
-    return Down::ref(a.down4, a.width, a.inner, e, tile, lane);
-  }
-  static TAO_DEVI bool zeros(const ExpertArgs& a) { return a.gate4.zeros != nullptr; }
+  using W = W4<GROUP>;
+  static TAO_DEVI const Four& gate(const ExpertArgs& a) { return a.gate4; }
+  static TAO_DEVI const Four& up(const ExpertArgs& a) { return a.up4; }
+  static TAO_DEVI const Four& down(const ExpertArgs& a) { return a.down4; }
 };
 
-constexpr int kRed = kWarps * 2 * 8 * 16;  // floats of the warps' sums, in every part
-// Two blocks an SM: half of its shared memory, less what the driver keeps of it for each.
-constexpr int kFixed = kRed * 4 + (int)sizeof(Shared);
-constexpr int kRing = (113 * 1024 - kFixed) / kWarps / 16 * 16;
-// Every part's ring holds two stages at least, with all of an entry's columns.
-static_assert(kRing >= 2 * (2 * W4<32, 128>::BYTES + 8 * 256), "");
-static_assert(kRing >= 2 * (2 * W4<32, 64>::BYTES + 16 * 128), "");
-static_assert(kRing >= 2 * (2 * W16::BYTES + 16 * 64), "");
+template <class W>
+constexpr int kRings = kWarps * (W::DEPTH * 2 * W::BYTES > W16::DEPTH * W16::BYTES ? W::DEPTH * 2 * W::BYTES
+                                                                                  : W16::DEPTH * W16::BYTES);
+template <class W>
+constexpr int kSmem = kRings<W> + kSums * 4 + (int)sizeof(Shared);
+static_assert(kSmem<W16> <= 227 * 1024 && kSmem<W4<32>> <= 227 * 1024, "");
 
 template <class L>
-__global__ void __launch_bounds__(kThreads, 2) experts_kernel(const ExpertArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) experts_kernel(const __grid_constant__ ExpertArgs a) {
+  using W = typename L::W;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem);
-  const uint32_t ring = smem_u32(smem + kRed * 4) + (threadIdx.x >> 5) * kRing;
-  Shared& s = *reinterpret_cast<Shared*>(smem + kRed * 4 + kWarps * kRing);
-  const int lane = threadIdx.x & 31, g = lane >> 2, warp = threadIdx.x >> 5;
-  const bool zeros = L::zeros(a);
+  float* sums = reinterpret_cast<float*>(smem + kRings<W>);
+  Shared& s = *reinterpret_cast<Shared*>(smem + kRings<W> + kSums * 4);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const auto now = [] { return true; };
 
-  {  // 1. logits
-    const int tiles = (a.experts + 15) / 16, cols_max = min(a.tokens, 8);
-    run_part<W16, 1, 1, false>(
-        tiles * ((a.tokens + 7) / 8), a.width, cols_max, false, ring, kRing, red,
-        [&](int u) {
-          Unit<W16, 1, 1> r;
-          const int m = u / tiles * 8 + g;
-          r.w[0] = W16::ref(a.router, a.experts, 0, u % tiles, lane);
-          r.x[0] = m < a.tokens ? a.x + m * a.x_stride : nullptr;
-          r.cols = min(8, a.tokens - u / tiles * 8);
-          return r;
-        },
-        [&](int u, auto sum) {
-          const int cols = min(8, a.tokens - u / tiles * 8);
-          for (int i = threadIdx.x; i < cols * 16; i += kThreads) {
-            const int e = u % tiles * 16 + i % 16;
-            if (e < a.experts) a.logits[(u / tiles * 8 + i / 16) * a.experts + e] = sum(0, i / 16, i % 16);
-          }
-        });
-  }
+  // 1. logits: an entry is 8 tokens
+  run_part<W16, 1, 1, false>(
+      (a.tokens + 7) / 8, (a.experts + 15) / 16, a.width, false, smem, sums,
+      [&](W16& w, int, int, int tile, int kb) { w.start(a.router, a.experts, a.width, 0, tile, kb, lane); },
+      [&](int entry, int c) { return a.x + (entry * 8 + c) * a.x_stride; },
+      [&](int entry) { return min(8, a.tokens - entry * 8); }, now,
+      [&](int entry, int tile, int col, int row, auto sum) {
+        const int e = tile * 16 + row;
+        if (e < a.experts) a.logits[(entry * 8 + col) * a.experts + e] = sum(0);
+      });
   if (!grid_meet(a, s)) return;
   for (int t = warp; t < a.tokens; t += kWarps) choose(a, s, t, lane);
   __syncthreads();
   sort_pairs(a, s);
 
   const int pairs = a.tokens * a.top_k;
-  {  // 2. h
-    const int tiles = (a.inner + 15) / 16;
-    using W = typename L::In;
-    run_part<W, 2, 1, false>(
-        s.entries * tiles, a.width, min(a.tokens, 8), zeros, ring, kRing, red,
-        [&](int u) {
-          Unit<W, 2, 1> r;
-          const uint32_t en = s.entry[u / tiles];
-          const int e = en >> 16, first = en >> 4 & 0xfff;
-          r.w[0] = L::gate(a, e, u % tiles, lane);
-          r.w[1] = L::up(a, e, u % tiles, lane);
-          r.cols = en & 15;
-          r.x[0] = g < r.cols ? a.x + s.token[first + g] * a.x_stride : nullptr;
-          return r;
-        },
-        [&](int u, auto sum) {
-          const uint32_t en = s.entry[u / tiles];
-          const int cols = en & 15, first = en >> 4 & 0xfff;
-          for (int i = threadIdx.x; i < cols * 16; i += kThreads) {
-            const int c = u % tiles * 16 + i % 16;
-            if (c >= a.inner) continue;
-            const float gate = sum(0, i / 16, i % 16), up = sum(1, i / 16, i % 16);
-            const float h = gate / (1.f + expf(-gate)) * up;
-            const long long at = (long long)(first + i / 16) * a.inner + c;
-            const bf16 high = tobf(h);
-            a.h[at] = high;
-            // an infinite h leaves nothing: infinity minus itself would be no number
-            a.h[at + (long long)pairs * a.inner] = isinf(bf(high)) ? tobf(0.f) : tobf(h - bf(high));
-          }
-        });
-  }
-  if (!grid_meet(a, s)) return;
-  {  // 3. the pairs' outputs, and the tokens'
-    const int tiles = (a.width + 31) / 32;
-    using W = typename L::Down;
-    run_part<W, 2, 2, true>(
-        s.entries * tiles, a.inner, min(2 * a.tokens, 16), zeros, ring, kRing, red,
-        [&](int u) {
-          Unit<W, 2, 2> r;
-          const uint32_t en = s.entry[u / tiles];
-          const int e = en >> 16, first = en >> 4 & 0xfff;
-          r.w[0] = L::down(a, e, u % tiles * 2, lane);
-          r.w[1] = L::down(a, e, u % tiles * 2 + 1, lane);
-          r.cols = 2 * (en & 15);
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int c = n * 8 + g;  // column: token c / 2, its high or its low part
-            r.x[n] = c < r.cols ? a.h + ((long long)(c & 1) * pairs + first + c / 2) * a.inner : nullptr;
-          }
-          return r;
-        },
-        [&](int u, auto sum) {
-          const uint32_t en = s.entry[u / tiles];
-          const int cols = en & 15, first = en >> 4 & 0xfff, tile = u % tiles;
-          for (int i = threadIdx.x; i < cols * 32; i += kThreads) {
-            const int n = tile * 32 + i % 32;
-            if (n < a.width) a.pair_out[(long long)(first + i / 32) * a.width + n] = sum(i % 32 / 16, i / 32, i % 16);
-          }
-          __syncthreads();
-          if (threadIdx.x == 0) {
-            const int done = atomic_add_release(a.counters + tile, 1) + 1;
-            s.last = done == s.entries;
-            if (s.last) {
-              fence_acquire();
-              a.counters[tile] = 0;
-            }
-          }
-          __syncthreads();
-          if (!s.last) return;
-          for (int i = threadIdx.x; i < a.tokens * 32; i += kThreads) {
-            const int t = i / 32, n = tile * 32 + i % 32;
-            if (n >= a.width) continue;
-            float o = 0.f;
-            for (int j = 0; j < a.top_k; ++j) {
-              const int p = t * a.top_k + j;
-              o += s.weight[p] * __ldcg(a.pair_out + (long long)s.row[p] * a.width + n);
-            }
-            a.out[(long long)t * a.width + n] = tobf(o);
-          }
-        });
+  const bool zeros = a.gate4.zeros != nullptr;
+  const auto expert = [&](int entry) { return (int)(s.entry[entry] >> 16); };
+  const auto first = [&](int entry) { return (int)(s.entry[entry] >> 4 & 0xfff); };
+  const auto count = [&](int entry) { return (int)(s.entry[entry] & 15); };
+  // 2. h
+  run_part<W, 2, 1, false>(
+      s.entries, (a.inner + 15) / 16, a.width, zeros, smem, sums,
+      [&](W& w, int r, int entry, int tile, int kb) {
+        w.start(r ? L::up(a) : L::gate(a), a.inner, a.width, expert(entry), tile, kb, lane);
+      },
+      [&](int entry, int c) { return a.x + s.token[first(entry) + c] * a.x_stride; }, count, now,
+      [&](int entry, int tile, int col, int row, auto sum) {
+        const int c = tile * 16 + row;
+        if (c >= a.inner) return;
+        const float gate = sum(0), up = sum(1);
+        const float h = gate / (1.f + expf(-gate)) * up;
+        const long long at = (long long)(first(entry) + col) * a.inner + c;
+        const bf16 high = tobf(h);
+        a.h[at] = high;
+        // an infinite h leaves nothing: infinity minus itself would be no number
+        a.h[at + (long long)pairs * a.inner] = isinf(bf(high)) ? tobf(0.f) : tobf(h - bf(high));
+      });
+  // 3. the pairs' outputs: two columns a token, its h's high and low parts; and the tokens'
+  const bool met = run_part<W, 2, 2, true>(
+      s.entries, (a.width + 31) / 32, a.inner, zeros, smem, sums,
+      [&](W& w, int r, int entry, int tile, int kb) {
+        w.start(L::down(a), a.width, a.inner, expert(entry), tile * 2 + r, kb, lane);
+      },
+      [&](int entry, int c) { return a.h + ((long long)(c & 1) * pairs + first(entry) + c / 2) * a.inner; },
+      [&](int entry) { return 2 * count(entry); }, [&] { return grid_meet(a, s); },
+      [&](int entry, int tile, int col, int row, auto sum) {
+        float* to = a.pair_out + (long long)(first(entry) + col) * a.width;
+        const int n = tile * 32 + row;
+        if (n < a.width) to[n] = sum(0);
+        if (n + 16 < a.width) to[n + 16] = sum(1);
+      });
+  if (!met || !grid_meet(a, s)) return;
+  const int quads = a.width / 4;
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < a.tokens * quads; i += gridDim.x * kThreads) {
+    const int t = i / quads, n = i % quads * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < a.top_k; ++j) {
+      const int p = t * a.top_k + j;
+      const float w = s.weight[p];
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.pair_out + (long long)s.row[p] * a.width + n));
+      o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+    }
+    *reinterpret_cast<uint2*>(a.out + (long long)t * a.width + n) = make_uint2(bf16x2(o.x, o.y), bf16x2(o.z, o.w));
   }
 }
 
@@ -550,14 +500,13 @@ int efail(int code, const char* msg) {
 size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Room {
-  size_t counters, logits, h, pair_out, total;
+  size_t logits, h, pair_out, total;
 };
 
 Room room_of(int tokens, int width, int inner, int experts, int top_k) {
   const size_t t = std::min(tokens, kTokens), pairs = t * top_k;
   Room r;
-  r.counters = kHeader;
-  r.logits = r.counters + round_up((size_t)(width + 31) / 32 * 4);
+  r.logits = kHeader;
   r.h = r.logits + round_up(t * experts * 4);
   r.pair_out = r.h + round_up(2 * pairs * inner * 2);
   r.total = r.pair_out + round_up(pairs * width * 4);
@@ -579,7 +528,7 @@ int check(const TaoExperts* p, int tokens) {
 
 template <class L>
 int launch(ExpertArgs a, cudaStream_t s) {
-  const int smem = kFixed + kWarps * kRing;
+  const int smem = kSmem<typename L::W>;
   auto kernel = experts_kernel<L>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   int device = 0, sms = 0, per = 0;
@@ -625,7 +574,7 @@ int tao_expert_layer(const TaoExperts* p, const void* x, long long x_stride, int
   if (workspace_bytes < tao_expert_workspace_bytes(p, tokens)) return efail(TAO_ERR_ARG, "workspace too small");
   auto M = [](const void* at, long long e, long long r) { return Matrix16{static_cast<const bf16*>(at), e, r}; };
   auto F = [](const void* c, const void* s, const void* z) {
-    return Four{static_cast<const uint8_t*>(c), static_cast<const uint16_t*>(s), static_cast<const uint8_t*>(z)};
+    return Four{static_cast<const uint8_t*>(c), static_cast<const uint8_t*>(s), static_cast<const uint8_t*>(z)};
   };
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const Room room = room_of(tokens, p->width, p->inner, p->experts, p->top_k);
@@ -655,7 +604,6 @@ int tao_expert_layer(const TaoExperts* p, const void* x, long long x_stride, int
     a.id_weights = ids ? id_weights + (long long)at * p->top_k : nullptr;
     a.error = reinterpret_cast<int*>(ws);
     a.barrier = reinterpret_cast<unsigned*>(ws + 128);
-    a.counters = reinterpret_cast<int*>(ws + room.counters);
     a.logits = reinterpret_cast<float*>(ws + room.logits);
     a.h = reinterpret_cast<bf16*>(ws + room.h);
     a.pair_out = reinterpret_cast<float*>(ws + room.pair_out);
@@ -676,7 +624,7 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemcpyAsync(&host, workspace, sizeof(int), cudaMemcpyDeviceToHost, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  // a wait that ran out leaves the barrier and the counters anywhere: all of it starts again
+  // a wait that ran out leaves the barrier anywhere: all of it starts again
   if (e == cudaSuccess && host) e = cudaMemsetAsync(workspace, 0, workspace_bytes, s);
   if (e != cudaSuccess) return efail(TAO_ERR_CUDA, cudaGetErrorString(e));
   if (flags) *flags = host;

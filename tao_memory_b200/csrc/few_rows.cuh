@@ -3,20 +3,24 @@
 //
 //   D[n][m] += sum over k of W[n][k] x[m][k]
 //
-// The weights are the 16-row operand of mma.m16n8k16 and eight activation rows its
-// columns, so a weight is used once per eight rows with no conversion to fp32; with one
-// row the other seven columns compute values that nothing reads.  The work is bound by
-// the weights' bytes, far from where tcgen05 tiles (128 rows, operands through shared
-// memory, where 4-bit weights would first have to be written as 16 bits) would pay.
+// The weights are the 16-row operand of a warp's mma and eight activation columns the other, so a
+// weight is used once per eight columns.  The work is bound by the weights' bytes, far from where
+// tcgen05 tiles (128 rows, operands through shared memory, where 4-bit weights would first have to be
+// written unpacked) would pay; what is left to save is the instructions per weight.
 //
-// The order of k inside a product is free, as long as both operands use the same:  of
-// every 32 k lane (g, t) = (lane / 4, lane % 4) takes 8t..8t+7, the first four in one
-// mma and the last four in the next.  So a lane reads 16 contiguous bytes of an
-// activation row (and of a 16-bit weight row).  A 4-bit block of 16 rows x 128 k is
-// laid out so that a lane's 64 codes are two 16-byte words:  word j of half h is the mma
-// step 4h + j, and its nibble i + 4p holds element p (low, high) of operand register i.
+// A few rows (product8): the codes 0..15 go as bytes into the integer mma.m16n8k32, three
+// instructions for eight of them.  The activations become sums of signed bytes under a power of
+// two s for each row and 128 k,  x = s (p0 + p1 / 2^7 + p2 / 2^14)  up to 2^-21 of the 128's largest
+// magnitude, a column of the mma for each piece (and an empty fourth).  Over a group
+//   sum of (q - zero) x = s 2^-7 (sum of q P - zero sum of P) + s 2^-14 (the same of p2),  P = 2^7 p0 + p1,
+// whole numbers below 2^31, so a group's product is exact; fp32 sums over the groups.
+// More rows (product16): codes become 16-bit floats with their zero point subtracted, exactly, for
+// mma.m16n8k16: eleven instructions for eight, but one column a row.
 //
-// Each warp streams its blocks through a ring in shared memory filled by cp.async.
+// The order of k inside a product is free, as long as both operands use the same: of every 32 k lane
+// (g, t) = (lane / 4, lane % 4) takes 8t..8t+7.  A 4-bit block of 16 rows x 128 k is laid out so that a
+// lane's 64 codes are two 16-byte words: byte 8i + 4f + e of half h is k = 64h + 32i + 8t + 4f + (0, 2, 1, 3)[e],
+// of row g in the low nibble and of row g + 8 in the high one; nibbles 16 bits apart are neighbouring k.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,150 +32,236 @@
 
 namespace tao {
 
-TAO_DEVI void cp_async16(uint32_t dst, const void* src, bool in) {
-  const int n = in ? 16 : 0;  // the rest is filled with zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-// Through L1: activations that other warps of the SM read too.
-TAO_DEVI void cp_async16_l1(uint32_t dst, const void* src, bool in) {
-  const int n = in ? 16 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-TAO_DEVI void cp_async8_l1(uint32_t dst, const void* src, bool in) {
-  const int n = in ? 8 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// Asynchronous copy of 16 bytes to shared memory; zeros where `in` is false.
+TAO_DEVI void cp_async16(uint32_t to, const void* from, bool in = true) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
 }
 TAO_DEVI void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
+template <int OPEN>
 TAO_DEVI void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  asm volatile("cp.async.wait_group %0;" ::"n"(OPEN) : "memory");
 }
-TAO_DEVI uint4 lds16(uint32_t at) {
+// 16-bit weights: read once, kept out of L1.
+TAO_DEVI uint4 ldg16(const void* p) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-TAO_DEVI uint2 lds8(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-  return v;
-}
-TAO_DEVI uint32_t lds_u16(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
-  return v;
-}
-TAO_DEVI uint32_t lds_u8(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
   return v;
 }
 
-// The 16-bit type of the mma: what an operand register pair means, and 4-bit codes in it.
+TAO_DEVI void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+TAO_DEVI void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The 16-bit type of product16's mma: 4-bit codes in it.
 struct MmaBf16 {
-  // 0x4300 | q is 128 + q exactly (7 mantissa bits); one subtraction leaves q - zero exactly.
+  // 0x4300 | q is 128 + q exactly (7 mantissa bits); adding -(128 + zero) leaves q - zero exactly.
   static constexpr uint32_t kMagic = 0x43004300u;
-  static TAO_DEVI uint32_t sub(uint32_t a, uint32_t b) {
-    __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<uint32_t*>(&r);
+  static TAO_DEVI uint32_t add(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x3f803f80u), "r"(b));
+    return r;
   }
-  static TAO_DEVI void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                           uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  static TAO_DEVI void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_bf16(d, a[0], a[1], a[2], a[3], b0, b1);
   }
 };
 struct MmaF16 {
   static constexpr uint32_t kMagic = 0x64006400u;  // 1024 + q
-  static TAO_DEVI uint32_t sub(uint32_t a, uint32_t b) {
-    __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<uint32_t*>(&r);
+  static TAO_DEVI uint32_t add(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
   }
-  static TAO_DEVI void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                           uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  static TAO_DEVI void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 
-// Two codes (nibbles i and i + 4 of w) as a pair of magic + q.
-template <class M>
-TAO_DEVI uint32_t codes_at(uint32_t w, int i) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(r) : "r"(w >> (4 * i)), "r"(M::kMagic));
-  return r;
+// 2^14 / s and s / 2^7 of a 128's largest magnitude: x / s is below 64.  A magnitude that is no finite
+// number makes both no numbers.
+TAO_DEVI void units_of(float most, float& up, float& unit) {
+  const uint32_t e = __float_as_uint(most) >> 23;  // of a magnitude: no sign
+  const uint32_t f = e > 22 ? e - 5 : 17u;         // the exponent of s; 2^14 / s and s / 2^14 are normal numbers
+  up = __uint_as_float(e == 255 ? 0x7fc00000u : (254 + 14 - f) << 23);
+  unit = __uint_as_float(e == 255 ? 0x7fc00000u : (f - 7) << 23);
 }
 
-// Four e4m3 in 32 bits as two pairs of fp16 (exact).
-TAO_DEVI void e4m3_to_f16(uint32_t v, uint32_t& lo, uint32_t& hi) {
-  const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffff), __NV_E4M3);
-  const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> 16), __NV_E4M3);
-  lo = a.x | (uint32_t)a.y << 16;
-  hi = b.x | (uint32_t)b.y << 16;
+// Eight 2^14 x / s (below 2^20 in magnitude), rounded to whole numbers, as three pieces of 8 signed
+// bytes each in the order of the codes (digits of -64..63, the first up to 64), and the sums of P = 2^7 p0 + p1 and of p2.
+TAO_DEVI void split8(const float (&x)[8], uint2 (&p)[3], int& sum, int& sum2) {
+  uint32_t w[3][2] = {};
+  int all = 0;
+  sum2 = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // the addition rounds to a whole number and leaves it in the low bits (conversions are slow)
+    const int v = __float_as_int(x[i] + 12582912.f) - 0x4b400000;
+    const int v1 = (v + 64) >> 7, p2 = v - (v1 << 7);
+    const int v0 = (v1 + 64) >> 7, p1 = v1 - (v0 << 7);
+    const int q[3] = {v0, p1, p2};
+#pragma unroll
+    for (int j = 0; j < 3; ++j) w[j][i / 4] |= (uint32_t)(q[j] & 0xff) << (8 * (i % 4 * 2 % 3 + i % 4 / 3 * 3));
+    all += v1;
+    sum2 += p2;
+  }
+  sum = all;
+#pragma unroll
+  for (int j = 0; j < 3; ++j) p[j] = make_uint2(w[j][0], w[j][1]);
 }
 
 // A 4-bit matrix laid out in blocks of 16 rows x 128 k, row tiles outermost.
 struct Four {
-  const uint8_t* codes;    // [tiles][blocks][1024]
-  const uint16_t* scales;  // [tiles][blocks][128 / group][16]
-  const uint8_t* zeros;    // the same, or null: 8
+  const uint8_t* codes;   // [tiles][blocks][1024]
+  const uint8_t* scales;  // [tiles][blocks][8][128 / group][2] 16-bit: rows g and g + 8 of the tile
+  const uint8_t* zeros;   // the same in bytes, or null: 8
 };
 
-// KB (64 or 128) k of a 4-bit block against eight activation rows for each of NT column
-// tiles, those that hold some of the `cols` rows.  `b(u, n)` gives the lane's 8 activations
-// of 32-k part u as four operand registers; `scale(j, row)` the scale of group j.  The
-// codes' products are summed in fp32 over a group (or the KB k of it) and scaled then, so
-// no weight is ever rounded.
-template <class M, int GROUP, int KB, int NT, class B, class S>
-TAO_DEVI void four_block(float (&acc)[NT][4], uint32_t codes, uint32_t zeros, bool has_zeros, int lane, int cols, B b,
-                         S scale) {
-  constexpr int SPAN = GROUP < KB ? GROUP : KB, PARTS = SPAN / 32;  // k, and 32-k parts, under one scale
-  const int g = lane >> 2;
-  uint4 w = lds16(codes + lane * 16);
+// A block in registers: this lane's codes, and the scales and zero points of its rows g, g + 8.
+template <int GROUP>
+struct Block4 {
+  static constexpr int GROUPS = 128 / GROUP, PARTS = GROUP / 32;  // groups of a block, 32-k parts of a group
+  uint4 c[2];
+  uint32_t s[GROUPS], z[(GROUPS + 1) / 2];
+
+  // A block in a ring in shared memory: codes, scales, zero points.
+  static constexpr int SCALES = 32 * GROUPS, ZEROS = 16 * GROUPS, BYTES = 1024 + SCALES + ZEROS;
+
+  // Starts the copy of block `block` of the matrix by the warp.
+  static TAO_DEVI void issue(uint32_t to, const Four& w, uint32_t block, int lane) {
+    const uint8_t* codes = w.codes + lane * 16 + (uint64_t)block * 1024u;
+    cp_async16(to + lane * 16, codes);
+    cp_async16(to + 512 + lane * 16, codes + 512);
+    if (lane < SCALES / 16)
+      cp_async16(to + 1024 + lane * 16, w.scales + lane * 16 + (uint64_t)block * (uint32_t)SCALES);
+    else if (w.zeros && lane >= 16 && lane < 16 + ZEROS / 16)
+      cp_async16(to + 1024 + SCALES + (lane - 16) * 16, w.zeros + (lane - 16) * 16 + (uint64_t)block * (uint32_t)ZEROS);
+  }
+  // From the ring, when the copy is over and the warp has met since.
+  TAO_DEVI void load(const uint8_t* from, bool has_zeros, int lane) {
+    c[0] = *reinterpret_cast<const uint4*>(from + lane * 16);
+    c[1] = *reinterpret_cast<const uint4*>(from + 512 + lane * 16);
+    const uint32_t* sp = reinterpret_cast<const uint32_t*>(from + 1024) + (lane >> 2) * GROUPS;
 #pragma unroll
-  for (int j = 0; j < KB / SPAN; ++j) {
-    uint32_t z0 = 8, z1 = 8;
-    if (has_zeros) {
-      z0 = lds_u8(zeros + j * 16 + g);
-      z1 = lds_u8(zeros + j * 16 + g + 8);
-    }
-    z0 = M::kMagic | z0 | z0 << 16;
-    z1 = M::kMagic | z1 | z1 << 16;
-    float t[NT][4];
+    for (int i = 0; i < GROUPS; ++i) s[i] = sp[i];
+    const uint16_t* zp = reinterpret_cast<const uint16_t*>(from + 1024 + SCALES) + (lane >> 2) * GROUPS;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) t[n][0] = t[n][1] = t[n][2] = t[n][3] = 0.f;
+    for (int i = 0; i < (GROUPS + 1) / 2; ++i)
+      z[i] = !has_zeros ? 0x08080808u : GROUPS == 1 ? zp[0] : reinterpret_cast<const uint32_t*>(zp)[i];
+  }
+  TAO_DEVI uint32_t zeros(int j) const { return z[j / 2] >> (16 * (j & 1)); }  // of rows g, g + 8, a byte each
+  template <bool BF16_SCALES>
+  TAO_DEVI float2 scales(int j) const {
+    if constexpr (BF16_SCALES) return make_float2(lo_f(s[j]), hi_f(s[j]));
+    return __half22float2(*reinterpret_cast<const __half2*>(&s[j]));
+  }
+  TAO_DEVI uint32_t word(int u, int i) const {
+    const uint4& w = c[u / 2];
+    return u & 1 ? (i ? w.w : w.z) : (i ? w.y : w.x);
+  }
+
+  // Adds to acc[n][0..1] rows g and g + 8 of the block's product with the row of x whose pieces 0 and 1
+  // (t even) or 2 (t odd) are columns 2t, 2t + 1 of column tile n; the row's whole product is the sum over
+  // the two lanes.  `b(h, n)`: the lane's 16 bytes of half h; `xsum(j, n)`: the sum over group j of P (t odd:
+  // of p2); `unit(n)`: s / 2^7 (t odd: s / 2^14).
+  template <bool BF16_SCALES, int NT, class B, class X, class U>
+  TAO_DEVI void product8(float (&acc)[NT][2], bool odd, B b, X xsum, U unit) const {
+    constexpr uint32_t MASK = 0x0f0f0f0fu;
+    uint32_t a[4][4];
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-      const int u = j * PARTS + p;
-      if (u == 2) w = lds16(codes + 512 + lane * 16);
-      const uint32_t w0 = u & 1 ? w.z : w.x, w1 = u & 1 ? w.w : w.y;
-      uint32_t a[2][4];
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[0][i] = M::sub(codes_at<M>(w0, i), i & 1 ? z1 : z0);
-        a[1][i] = M::sub(codes_at<M>(w1, i), i & 1 ? z1 : z0);
+      for (int i = 0; i < 2; ++i) {
+        a[u][2 * i] = word(u, i) & MASK;
+        a[u][2 * i + 1] = word(u, i) >> 4 & MASK;
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (n && n * 8 >= cols) break;
-        const uint4 x = b(u, n);
-        M::mma(t[n], a[0][0], a[0][1], a[0][2], a[0][3], x.x, x.y);
-        M::mma(t[n], a[1][0], a[1][1], a[1][2], a[1][3], x.z, x.w);
-      }
-    }
-    const float s0 = scale(j, g), s1 = scale(j, g + 8);
+    const int m0 = odd ? 1 : 128, m1 = odd ? 0 : 1;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      acc[n][0] += s0 * t[n][0];
-      acc[n][1] += s0 * t[n][1];
-      acc[n][2] += s1 * t[n][2];
-      acc[n][3] += s1 * t[n][3];
+      const uint4 x0 = b(0, n), x1 = b(1, n);
+      const uint32_t bs[4][2] = {{x0.x, x0.y}, {x0.z, x0.w}, {x1.x, x1.y}, {x1.z, x1.w}};
+      const float un = unit(n);
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        int d[4] = {0, 0, 0, 0}, d2[4] = {0, 0, 0, 0};  // two chains of dependent products
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          const int u = j * PARTS + p;
+          mma_u8s8(p & 1 ? d2 : d, a[u][0], a[u][1], a[u][2], a[u][3], bs[u][0], bs[u][1]);
+        }
+        if constexpr (PARTS > 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] += d2[i];
+        }
+        const int z0 = zeros(j) & 0xff, z1 = zeros(j) >> 8 & 0xff;
+        const int xs = xsum(j, n);
+        const float2 sc = scales<BF16_SCALES>(j);
+        acc[n][0] += sc.x * un * (float)(d[0] * m0 + d[1] * m1 - z0 * xs);
+        acc[n][1] += sc.y * un * (float)(d[2] * m0 + d[3] * m1 - z1 * xs);
+      }
     }
   }
-}
+
+  // Adds D of the block's product with eight rows of x for each of NT column tiles, those that hold some
+  // of the `cols` rows.  `b(u, n)`: the lane's 8 activations of 32-k part u.
+  template <class M, bool BF16_SCALES, int NT, class B>
+  TAO_DEVI void product16(float (&acc)[NT][4], int cols, B b) const {
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      // -(magic + zero) in both halves: the zero's byte below the magic's with its sign
+      const uint32_t zz = zeros(j);
+      const uint32_t z0 = __byte_perm(zz, M::kMagic >> 24 | 0x80, 0x4040);
+      const uint32_t z1 = __byte_perm(zz, M::kMagic >> 24 | 0x80, 0x4141);
+      // two chains of dependent products, or as many as there are column tiles
+      constexpr int CHAINS = NT == 1 ? 2 : 1;
+      float d[NT * CHAINS][4];
+#pragma unroll
+      for (int n = 0; n < NT * CHAINS; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        const int u = j * PARTS + p;
+        uint32_t a[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // register r: row half r & 1, elements (0, 1) or (2, 3)
+            uint32_t v;
+            asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(v) : "r"(word(u, i) >> (4 * r)), "r"(M::kMagic));
+            a[i][r] = M::add(v, r & 1 ? z1 : z0);
+          }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (n && n * 8 >= cols) break;
+          const uint4 x = b(u, n);
+          M::mma(d[n], a[0], x.x, x.y);
+          M::mma(d[n + CHAINS - 1], a[1], x.z, x.w);
+        }
+      }
+      if constexpr (CHAINS == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[0][i] += d[1][i];
+      }
+      const float2 sc = scales<BF16_SCALES>(j);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc[n][0] += sc.x * d[n][0];
+        acc[n][1] += sc.x * d[n][1];
+        acc[n][2] += sc.y * d[n][2];
+        acc[n][3] += sc.y * d[n][3];
+      }
+    }
+  }
+};
 
 }  // namespace tao

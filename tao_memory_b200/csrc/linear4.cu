@@ -2,13 +2,14 @@
 //
 //   W[n][k] = (code[n][k] - zero[n][k / group]) scale[n][k / group],  codes 0..15
 //
-// x in bf16 or fp16, or in e4m3 with one fp32 scale a row (read as fp16, exactly); y in
-// the type of the weight's scales.  Products of codes are summed in fp32 over a group,
-// scaled, and summed in fp32 over the groups; y is rounded once.
+// x in bf16 or fp16, or in e4m3 with one fp32 scale a row; y in the type of the weight's scales.
+// How the product is formed: few_rows.cuh.  Sums are in fp32, y is rounded once.
 //
-// Bound by the codes' bytes: half a byte a weight.  A block owns 16 output rows; its
-// warps take the 128-k blocks in turn, each through a ring of its own, and add their sums
-// in order through shared memory.
+// Bound by the codes' bytes, half a byte a weight.  One block an SM.  x, or a cluster's block's part of its
+// k, is laid out in shared memory once, in the order of the mma's operands.  The warps are WT x WK: WT row
+// tiles at a time, each one's 128-k blocks dealt to WK warps in runs, each warp's through a ring of its own
+// (registers would do, but a warp's few scoreboards make a load wait for later ones).  A warp leaves its sums of a tile in shared memory; these are added at the end, a cluster's blocks' through
+// distributed shared memory, in a fixed order.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -22,7 +23,9 @@ void tao_set_last_error(const char* msg);
 namespace tao {
 namespace {
 
-enum Act { kBf16 = 0, kF16 = 1, kE4m3 = 3 };
+constexpr int kSmem = 226 * 1024;
+constexpr int kXBytes = 96 * 1024;   // most of it that x takes
+constexpr int kMaxK = 65536;         // two rows' pieces of a cluster of 8's part fit kXBytes
 
 struct Linear4Args {
   Four w;
@@ -32,144 +35,299 @@ struct Linear4Args {
   const void* bias;
   void* y;
   int rows, n, k;
-  int kblocks, stages;
-  bool wide;      // rows of x start on 16 (e4m3: 8) bytes and k is whole chunks of 8
-  bool bf16_out;  // the type of scales, bias and y
+  int tiles, kblocks;
+  int shift, wk_shift;  // log2 of a cluster's blocks, of a tile's warps
+  int ring, sums;   // where the rings and the sums start in shared memory
+  int steps;        // row tiles of a warp
+  int x_type;
+  bool wide;        // rows of x start on 16 (e4m3: 8) bytes and k is whole chunks of 8
 };
 
-TAO_DEVI float scale_f(uint32_t bits, bool is_bf16) {
-  if (is_bf16) return __uint_as_float(bits << 16);
-  return __half2float(__ushort_as_half((unsigned short)bits));
+TAO_DEVI uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+TAO_DEVI void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+TAO_DEVI float4 ld_cluster(uint32_t at, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n .reg .u32 p;\n mapa.shared::cluster.u32 p, %4, %5;\n ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [p];\n}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(at), "r"(rank)
+      : "memory");
+  return v;
 }
 
-constexpr int kWarps = 8;
-
-// Bytes of one stage of a warp's ring: codes, scales, zeros, activations of `rows` rows.
-__host__ __device__ constexpr int meta_bytes(int group, bool zeros) { return 128 / group * 16 * (zeros ? 3 : 2); }
-__host__ __device__ constexpr int stage_bytes(int group, bool zeros, int rows, int act) {
-  return 1024 + meta_bytes(group, zeros) + rows * 128 * (act == kE4m3 ? 1 : 2);
-}
-
-template <int ACT, int GROUP, int NT>
-__global__ void __launch_bounds__(kWarps * 32) linear4_kernel(const Linear4Args a) {
-  using M = std::conditional_t<ACT == kBf16, MmaBf16, MmaF16>;
-  constexpr int XB = ACT == kE4m3 ? 1 : 2;  // bytes of an activation
-  constexpr int CHUNK = 8 * XB;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.x, m0 = blockIdx.y * (8 * NT), rows = min(a.rows - m0, 8 * NT);
-  const bool has_zeros = a.w.zeros != nullptr;
-  constexpr int SCALES = 128 / GROUP * 32;
-  const int zoff = 1024 + SCALES, xoff = 1024 + meta_bytes(GROUP, has_zeros);
-  const int xrows = min(a.rows, 8 * NT);  // the ring's room, equal for all blocks
-  const int stage = stage_bytes(GROUP, has_zeros, xrows, ACT);
-  const uint32_t ring = smem_u32(smem) + warp * a.stages * stage;
-  const int mine = a.kblocks > warp ? (a.kblocks - warp + kWarps - 1) / kWarps : 0;
-  const uint8_t* x = static_cast<const uint8_t*>(a.x) + (long long)m0 * a.x_stride * XB;
-
-  auto issue = [&](int i) {
-    if (i < mine) {
-      const int kb = warp + i * kWarps;
-      const long long block = (long long)tile * a.kblocks + kb;
-      const uint32_t to = ring + (i % a.stages) * stage;
-      const uint8_t* src = a.w.codes + block * 1024 + lane * 16;
-      cp_async16(to + lane * 16, src, true);
-      cp_async16(to + 512 + lane * 16, src + 512, true);
-      if (lane < SCALES / 16)
-        cp_async16(to + 1024 + lane * 16, reinterpret_cast<const uint8_t*>(a.w.scales) + block * SCALES + lane * 16,
-                   true);
-      else if (has_zeros && lane >= 16 && lane < 16 + SCALES / 32)
-        cp_async16(to + zoff + (lane - 16) * 16, a.w.zeros + block * (SCALES / 2) + (lane - 16) * 16, true);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int m = n * 8 + g;
-        if (m < rows) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int k = kb * 128 + u * 32 + t * 8;
-            const uint32_t dst = to + xoff + ((u * xrows + m) * 4 + t) * CHUNK;
-            const uint8_t* from = x + ((long long)m * a.x_stride + k) * XB;
-            if (a.wide) {
-              if constexpr (XB == 2)
-                cp_async16_l1(dst, k < a.k ? from : x, k < a.k);
-              else
-                cp_async8_l1(dst, k < a.k ? from : x, k < a.k);
-            } else {
-              uint32_t v[CHUNK / 4] = {};
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                if (k + e < a.k) {
-                  if constexpr (XB == 2)
-                    v[e / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(from)[e] << (16 * (e & 1));
-                  else
-                    v[e / 4] |= (uint32_t)from[e] << (8 * (e & 3));
-                }
-              }
-#pragma unroll
-              for (int e = 0; e < CHUNK / 4; ++e)
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 4 * e), "r"(v[e]) : "memory");
-            }
-          }
-        }
+// Eight activations of a row from k on (e4m3: in the first two words); zeros beyond its end.
+TAO_DEVI uint4 chunk_of(const Linear4Args& a, long long m, int k) {
+  const long long at = m * a.x_stride + k;
+  uint32_t w[4] = {};
+  if (a.x_type == TAO_TYPE_E4M3) {
+    const uint8_t* p = static_cast<const uint8_t*>(a.x) + at;
+    if (a.wide) {
+      if (k < a.k) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x, w[1] = v.y;
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < a.k) w[i / 4] |= (uint32_t)__ldg(p + i) << (8 * (i & 3));
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
+    if (a.wide) {
+      if (k < a.k) return __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < a.k) w[i / 2] |= (uint32_t)__ldg(p + i) << (16 * (i & 1));
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// ... as pairs of fp16 (from e4m3).
+TAO_DEVI uint4 widen_e4m3(uint4 v) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t q = (i < 2 ? v.x : v.y) >> (16 * (i & 1)) & 0xffff;
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q, __NV_E4M3);
+    h[i] = r.x | (uint32_t)r.y << 16;
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
+// The two forms of the product: signed bytes (4 columns a row), or the 16-bit type M (one).
+struct Bytes {};
+
+// COLS: columns of the mma for a row; WARPS: of a block; DEPTH: blocks of a warp's ring.  Shared memory of a block's 128 k of x: bytes have a row's three pieces as [half][3 row + piece][t] 16 bytes, a lane's
+// operands in the order of the lanes, then [row] s / 2^7, then [group][row] the sums (P, p2); 16 bits have
+// [32-k part][row][t] 16 bytes.
+template <class M, int GROUP, int NT>
+struct Form {
+  static constexpr bool BYTES = std::is_same<M, Bytes>::value;
+  static constexpr int COLS = BYTES ? 4 : 1, ROWS = 8 * NT / COLS, GROUPS = 128 / GROUP;
+  static constexpr int WARPS = 16, DEPTH = 6;
+  static constexpr int UNITS = ROWS * 384, SUMS = UNITS + ROWS * 4 + ROWS * 4 % 8;
+  static constexpr int XBLOCK = BYTES ? (SUMS + GROUPS * ROWS * 8 + 15) / 16 * 16 : ROWS * 256;
+};
+
+// M: the form.  BF16: the type of scales, bias and y.  NT: column tiles of 8 columns of the mma.
+template <class M, bool BF16, int GROUP, int NT>
+__global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_kernel(const Linear4Args a) {
+  using F = Form<M, GROUP, NT>;
+  using B4 = Block4<GROUP>;
+  constexpr bool BYTES = F::BYTES;
+  constexpr int ROWS = F::ROWS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), warps = blockDim.x / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int m0 = blockIdx.y * ROWS, rows = min(a.rows - m0, ROWS);
+  const int rank = a.shift ? (int)cluster_rank() : 0;
+  const int id = blockIdx.x >> a.shift, clusters = gridDim.x >> a.shift;
+  const int k0 = a.kblocks * rank >> a.shift, nb = (a.kblocks * (rank + 1) >> a.shift) - k0;
+  // a warp's row tiles are first, first + stride, ...; of each the `per` blocks from k0 + kw on
+  const int wks = a.wk_shift, groups = warps >> wks, stride = clusters * groups;
+  const int wt = warp >> wks, wk = warp & ((1 << wks) - 1), first = id * groups + wt;
+  const int kw = nb * wk >> wks, per = (nb * (wk + 1) >> wks) - kw;
+
+  // x before the weights, whose many copies in flight the others' come behind
+  const int l = lane & 15;
+  const bool copied = !BYTES && a.wide && a.x_type != TAO_TYPE_E4M3;
+  if (copied) {
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + m0 * a.x_stride;
+    for (int m = warp; m < rows; m += warps)
+      for (int c = lane; c < nb * 16; c += 32) {
+        const int k = k0 * 128 + c * 8;
+        const uint32_t to = smem_u32(smem) + (c >> 4) * F::XBLOCK + (((c >> 2 & 3) * ROWS + m) * 4 + (c & 3)) * 16;
+        cp_async16(to, k < a.k ? x + m * a.x_stride + k : x, k < a.k);
+      }
+  }
+
+  const int mine = first < a.tiles ? min(a.steps, (a.tiles - first + stride - 1) / stride) : 0, total = mine * per;
+  const uint8_t* const ring = smem + a.ring + warp * (F::DEPTH * B4::BYTES);
+  const uint32_t ring_at = smem_u32(ring);
+  uint32_t next = first * a.kblocks + k0 + kw;  // block to copy
+  int left = total, lk = per, to_slot = 0;
+  auto issue = [&]() {
+    if (left > 0) {
+      --left;
+      B4::issue(ring_at + to_slot, a.w, next++, lane);
+      if (--lk == 0) {
+        lk = per;
+        next += stride * a.kblocks - per;
+      }
+      to_slot = to_slot == (F::DEPTH - 1) * B4::BYTES ? 0 : to_slot + B4::BYTES;
     }
     cp_commit();
   };
-
-  float acc[NT][4] = {};
-  for (int i = 0; i < a.stages - 1; ++i) issue(i);
-  for (int i = 0; i < mine; ++i) {
-    // stages - 2 younger groups may be open; the ring's depth is 2, 4 or 8
-    if (a.stages == 2)
-      cp_wait<0>();
-    else if (a.stages == 4)
-      cp_wait<2>();
-    else
-      cp_wait<6>();
-    __syncwarp();  // block i is there for every lane, and every lane is done with block i - 1
-    issue(i + a.stages - 1);
-    const uint32_t at = ring + (i % a.stages) * stage;
-    auto b = [&](int u, int n) {
-      const int m = min(n * 8 + g, xrows - 1);  // columns without a row repeat one; nothing reads them
-      const uint32_t from = at + xoff + ((u * xrows + m) * 4 + t) * CHUNK;
-      if constexpr (XB == 2) {
-        return lds16(from);
-      } else {
-        const uint2 v = lds8(from);
-        uint4 r;
-        e4m3_to_f16(v.x, r.x, r.y);
-        e4m3_to_f16(v.y, r.z, r.w);
-        return r;
+  const int items = copied ? 0 : rows * nb, each = warps * 2;  // 16 lanes: a row's 128 k
+  auto chunk = [&](int i) {
+    const int kb = rows == 1 ? i : i / rows;
+    return i < items ? chunk_of(a, m0 + i - kb * rows, (k0 + kb) * 128 + l * 8) : make_uint4(0, 0, 0, 0);
+  };
+  const int item0 = warp * 2 + (lane >> 4);
+  uint4 ahead = chunk(item0);
+  cp_commit();  // x's copies
+#pragma unroll 1
+  for (int d = 0; d < F::DEPTH - 1; ++d) issue();
+  if (copied) {
+    cp_wait<F::DEPTH - 1>();
+  } else {
+    for (int i = item0; i - (lane >> 4) < items; i += each) {
+      const int kb = rows == 1 ? i : i / rows, m = i - kb * rows;
+      const bool in = i < items;
+      uint4 v = ahead;
+      ahead = chunk(i + each);
+      uint8_t* to = smem + kb * F::XBLOCK;
+      if (a.x_type == TAO_TYPE_E4M3) v = widen_e4m3(v);
+      if constexpr (BYTES) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        float f[8], most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+          f[2 * e] = a.x_type == TAO_TYPE_BF16 ? lo_f(w[e]) : h.x;
+          f[2 * e + 1] = a.x_type == TAO_TYPE_BF16 ? hi_f(w[e]) : h.y;
+          most = max_nan(most, max_nan(fabsf(f[2 * e]), fabsf(f[2 * e + 1])));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float up, unit;
+        units_of(most, up, unit);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= up;
+        uint2 p[3];
+        int2 sum;
+        split8(f, p, sum.x, sum.y);
+#pragma unroll
+        for (int o = 1; o < GROUP / 8; o <<= 1) {
+          sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+          sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+        }
+        if (in) {
+          if (l == 0) reinterpret_cast<float*>(to + F::UNITS)[m] = unit;
+          if (l % (GROUP / 8) == 0) reinterpret_cast<int2*>(to + F::SUMS)[l / (GROUP / 8) * ROWS + m] = sum;
+#pragma unroll
+          for (int c = 0; c < 3; ++c)
+            *reinterpret_cast<uint2*>(to + ((l / 8 * ROWS * 3 + m * 3 + c) * 4 + l % 4) * 16 + l / 4 % 2 * 8) = p[c];
+        }
+      } else if (in) {
+        *reinterpret_cast<uint4*>(to + ((l / 4 * ROWS + m) * 4 + l % 4) * 16) = v;
       }
-    };
-    auto scale = [&](int j, int row) { return scale_f(lds_u16(at + 1024 + (j * 16 + row) * 2), a.bf16_out); };
-    four_block<M, GROUP, 128, NT>(acc, at, at + zoff, has_zeros, lane, rows, b, scale);
-  }
-  cp_wait<0>();
-  __syncthreads();  // the rings become the warps' sums [warp][column][16 rows]
-  float* red = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      red[(warp * 8 * NT + n * 8 + 2 * t + (c & 1)) * 16 + g + 8 * (c >> 1)] = acc[n][c];
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * 16; i += kWarps * 32) {
-    const int m = i / 16, n = tile * 16 + i % 16;
-    if (n >= a.n) continue;
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += red[(w * 8 * NT + m) * 16 + i % 16];
-    if (a.x_scale) s *= a.x_scale[m0 + m];
-    const long long at = (long long)(m0 + m) * a.n + n;
-    if (a.bf16_out) {
-      if (a.bias) s += bf(static_cast<const bf16*>(a.bias)[n]);
-      static_cast<bf16*>(a.y)[at] = tobf(s);
-    } else {
-      if (a.bias) s += __half2float(static_cast<const __half*>(a.bias)[n]);
-      static_cast<__half*>(a.y)[at] = __float2half_rn(s);
     }
   }
+  __syncthreads();
+
+  // What this lane reads of a block of x.  Columns without a row hold anything, a row's empty fourth
+  // reads another piece; nothing uses what they give.
+  constexpr int OUTS = BYTES ? 2 : 4;
+  constexpr int NEXT = BYTES ? 2 * 3 * 64 : 8 * 64;  // bytes to the next column tile
+  const uint8_t* const xfirst = smem + kw * F::XBLOCK;
+  const uint8_t* xblock = xfirst;
+  const int xlane = ((BYTES ? g / 4 * 3 + min(g % 4, 2) : g) * 4 + t) * 16;
+  const int ulane = F::UNITS + t / 2 * 4, slane = F::SUMS + t / 2 * 8 + (t & 1) * 4;
+  const float part = t & 1 ? 1.f / 128.f : 1.f;
+  const int slot = rows * 16;  // floats of a warp's sums of a tile
+  float* const sums = reinterpret_cast<float*>(smem + a.sums);  // [step][warp][row][16]
+  float* to = sums + warp * slot;
+  float acc[NT][OUTS] = {};
+  int kb = per;
+  auto product = [&](const B4& b) {
+    if constexpr (BYTES) {
+      b.template product8<BF16, NT>(
+          acc, t & 1,
+          [&](int h, int n) { return *reinterpret_cast<const uint4*>(xblock + xlane + n * NEXT + h * ROWS * 192); },
+          [&](int j, int n) { return *reinterpret_cast<const int*>(xblock + slane + (j * ROWS + n * 2) * 8); },
+          [&](int n) { return *reinterpret_cast<const float*>(xblock + ulane + n * 8) * part; });
+    } else {
+      b.template product16<M, BF16, NT>(acc, rows, [&](int u, int n) {
+        return *reinterpret_cast<const uint4*>(xblock + xlane + n * NEXT + u * ROWS * 64);
+      });
+    }
+    xblock += F::XBLOCK;
+    if (--kb == 0) {
+      kb = per;
+      xblock = xfirst;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (BYTES) {
+          const int m = n * 2 + t / 2;
+          acc[n][0] += __shfl_xor_sync(0xffffffffu, acc[n][0], 1);
+          acc[n][1] += __shfl_xor_sync(0xffffffffu, acc[n][1], 1);
+          if (m < rows) to[m * 16 + g + 8 * (t & 1)] = t & 1 ? acc[n][1] : acc[n][0];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int m = n * 8 + 2 * t + (c & 1);
+            if (m < rows) to[m * 16 + g + 8 * (c >> 1)] = acc[n][c];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < OUTS; ++c) acc[n][c] = 0.f;
+      }
+      to += warps * slot;
+    }
+  };
+
+  const bool has_zeros = a.w.zeros != nullptr;
+  int slot_at = 0;
+#pragma unroll 1
+  for (int i = 0; i < total; ++i) {
+    cp_wait<F::DEPTH - 2>();
+    __syncwarp();  // the block is there for every lane, and every lane is done with the one before
+    issue();
+    B4 b;
+    b.load(ring + slot_at, has_zeros, lane);
+    slot_at = slot_at == (F::DEPTH - 1) * B4::BYTES ? 0 : slot_at + B4::BYTES;
+    product(b);
+  }
+
+  // The sums added, four rows of W a thread.
+  if (a.shift)
+    cluster_sync();
+  else
+    __syncthreads();
+  const int quads = a.steps * groups * rows * 4;
+  for (int i = (((warp << a.shift) + rank) << 5) + lane; i < quads; i += (warps << a.shift) << 5) {
+    const int mg = i / 4, gs = rows == 1 ? mg : mg / rows, m = mg - gs * rows;
+    const int step = gs / groups, grp = gs - step * groups;
+    const int n = (id * groups + grp + step * stride) * 16 + i % 4 * 4;
+    if (n >= a.n) continue;
+    const float* at = sums + (step * warps + (grp << wks)) * slot + m * 16 + i % 4 * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!a.shift) {
+#pragma unroll 4
+      for (int w = 0; w < 1 << wks; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(at + w * slot);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+    } else {
+#pragma unroll 8
+      for (int w = 0; w < 1 << (wks + a.shift); ++w) {
+        const float4 v = ld_cluster(smem_u32(at + (w >> a.shift) * slot), w & ((1 << a.shift) - 1));
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+    }
+    const float xs = a.x_scale ? a.x_scale[m0 + m] : 1.f;
+    const float out[4] = {s.x * xs, s.y * xs, s.z * xs, s.w * xs};
+    using T = std::conditional_t<BF16, bf16, __half>;
+    const T* bias = static_cast<const T*>(a.bias);
+    T* y = static_cast<T*>(a.y) + (long long)(m0 + m) * a.n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (n + e >= a.n) break;
+      if constexpr (BF16)
+        y[n + e] = tobf(out[e] + (bias ? bf(bias[n + e]) : 0.f));
+      else
+        y[n + e] = __float2half_rn(out[e] + (bias ? __half2float(bias[n + e]) : 0.f));
+    }
+  }
+  if (a.shift) cluster_sync();  // the others' reads of these sums are over
 }
 
 int lfail(int code, const char* msg) {
@@ -177,36 +335,92 @@ int lfail(int code, const char* msg) {
   return code;
 }
 
-template <int ACT, int GROUP, int NT>
-int launch(const Linear4Args& a, cudaStream_t s) {
-  const int xrows = std::min(a.rows, 8 * NT);
-  const int smem = std::max(kWarps * a.stages * stage_bytes(GROUP, a.w.zeros != nullptr, xrows, ACT),
-                            kWarps * 8 * NT * 16 * 4);
-  auto kernel = linear4_kernel<ACT, GROUP, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+struct Plan {
+  int shift, wk_shift, warps, blocks, steps, ring, sums, smem;
+};
+
+// The split with the least time by a rough measure, in us: what the longest warp's blocks of 128 k
+// take one after the other, or all of an SM's; x on its way; the additions.  `xblock`, `wring`: bytes of
+// a block of x, and of a warp's ring.
+Plan plan_of(int tiles, int kblocks, int rows, int xblock, int wring, int max_warps) {
+  Plan best = {};
+  double least = 1e30;
+  for (int shift = 0; shift <= 3; ++shift) {
+    const int cluster = 1 << shift, kb = (kblocks + cluster - 1) / cluster, x = (kb * xblock + 127) / 128 * 128;
+    if (x > kXBytes || cluster > kblocks) continue;
+    // clusters that the device holds at once, with one block an SM
+    const int clusters = shift == 0 ? 148 : shift == 1 ? 74 : shift == 2 ? 33 : 15;
+    for (int warps = 4; warps <= max_warps; warps *= 2) {
+      const int slot = warps * rows * 16 * 4;  // bytes of the warps' sums of a tile each
+      const int ring = warps * wring, most = (kSmem - x - ring) / slot;
+      // every warp of a block has some of its k
+      for (int wks = 0; 1 << wks <= std::min(warps, kblocks / cluster); ++wks) {
+        const int groups = warps >> wks, sets = (tiles + groups - 1) / groups;
+        const int all = (sets + clusters - 1) / clusters, waves = (all + most - 1) / std::max(most, 1);
+        if (most < 1) continue;
+        const int steps = (all + waves - 1) / waves, used = (sets + steps - 1) / steps;
+        const int per = (kb + (1 << wks) - 1) >> wks;
+        const double cost = waves * (std::max(steps * per * 0.20, (double)steps * groups * kb * 0.024) + x * 4e-5 +
+                                     (shift ? 0.7 : 0.) + steps * 0.05 + warps * 0.01);
+        if (cost >= least) continue;
+        least = cost;
+        best = {shift, wks, warps, used * cluster, steps, x, x + ring, x + ring + steps * slot};
+      }
+    }
+  }
+  return best;
+}
+
+template <class M, bool BF16, int GROUP, int NT>
+int launch(Linear4Args a, cudaStream_t s) {
+  using F = Form<M, GROUP, NT>;
+  const Plan p = plan_of(a.tiles, a.kblocks, std::min(a.rows, F::ROWS), F::XBLOCK, F::DEPTH * Block4<GROUP>::BYTES, F::WARPS);
+  if (p.steps < 1) return lfail(TAO_ERR_CAPACITY, "no split of this product fits the device");
+  a.shift = p.shift;
+  a.wk_shift = p.wk_shift;
+  a.steps = p.steps;
+  a.ring = p.ring;
+  a.sums = p.sums;
+  auto kernel = linear4_kernel<M, BF16, GROUP, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e == cudaSuccess) {
-    const dim3 grid((a.n + 15) / 16, (a.rows + 8 * NT - 1) / (8 * NT));
-    kernel<<<grid, kWarps * 32, smem, s>>>(a);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(p.blocks, (a.rows + F::ROWS - 1) / F::ROWS);
+    c.blockDim = dim3(p.warps * 32);
+    c.dynamicSmemBytes = p.smem;
+    c.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1 << p.shift;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    c.attrs = attr;
+    c.numAttrs = p.shift ? 1 : 0;
+    e = cudaLaunchKernelEx(&c, kernel, a);
   }
   return e == cudaSuccess ? TAO_OK : lfail(TAO_ERR_CUDA, cudaGetErrorString(e));
 }
 
-template <int ACT, int GROUP>
-int by_rows(Linear4Args a, cudaStream_t s) {
-  if (a.rows <= 8) {
-    a.stages = 4;
-    return launch<ACT, GROUP, 1>(a, s);
-  }
-  a.stages = 2;
-  return launch<ACT, GROUP, 2>(a, s);
+template <class F>
+bool fits(const Linear4Args& a) {
+  return (a.kblocks + 7) / 8 * F::XBLOCK <= kXBytes;
 }
 
-template <int ACT>
+template <class M, bool BF16, int GROUP>
+int by_rows(const Linear4Args& a, cudaStream_t s) {
+  // The bytes' form costs four columns a row and little else, the 16-bit one eight more instructions for
+  // eight weights.  A form serves as many rows as a cluster of 8 blocks can hold.
+  if (a.rows <= 2 || !fits<Form<Bytes, GROUP, 2>>(a)) return launch<Bytes, BF16, GROUP, 1>(a, s);
+  if (a.rows <= 4 || !fits<Form<M, GROUP, 1>>(a)) return launch<Bytes, BF16, GROUP, 2>(a, s);
+  if (a.rows <= 8 || !fits<Form<M, GROUP, 2>>(a)) return launch<M, BF16, GROUP, 1>(a, s);
+  if (a.rows <= 16 || !fits<Form<M, GROUP, 4>>(a)) return launch<M, BF16, GROUP, 2>(a, s);
+  return launch<M, BF16, GROUP, 4>(a, s);
+}
+
+template <class M, bool BF16>
 int by_group(const Linear4Args& a, int group, cudaStream_t s) {
-  if (group == 32) return by_rows<ACT, 32>(a, s);
-  if (group == 64) return by_rows<ACT, 64>(a, s);
-  return by_rows<ACT, 128>(a, s);
+  if (group == 32) return by_rows<M, BF16, 32>(a, s);
+  if (group == 64) return by_rows<M, BF16, 64>(a, s);
+  return by_rows<M, BF16, 128>(a, s);
 }
 
 }  // namespace
@@ -223,32 +437,33 @@ int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_sc
     return lfail(TAO_ERR_ARG, "activations are of the scales' type, or e4m3");
   if (group != 32 && group != 64 && group != 128) return lfail(TAO_ERR_ARG, "a group is 32, 64 or 128 weights");
   if (rows < 0 || n <= 0 || k <= 0) return lfail(TAO_ERR_ARG, "rows must not be negative, n and k must be positive");
-  if (n > (1 << 24) || k > (1 << 24)) return lfail(TAO_ERR_ARG, "n and k are limited to 2^24");
+  if (n > (1 << 24) || k > kMaxK) return lfail(TAO_ERR_ARG, "n is limited to 2^24 and k to 65536");
   if (rows == 0) return TAO_OK;
   if (!x || !codes || !scales || !y) return lfail(TAO_ERR_ARG, "null pointer");
   for (const void* p : {codes, scales, zeros})
     if (reinterpret_cast<uintptr_t>(p) % 16) return lfail(TAO_ERR_ARG, "a laid-out weight starts on 16 bytes");
   const int size = x_type == TAO_TYPE_E4M3 ? 1 : 2;
-  constexpr long long kMost = 1 << 19;  // rows of a launch: 65536 blocks of 8 in the grid's second axis, less one
-  for (long long at = 0; at < rows; at += kMost - 16) {
+  constexpr long long kMost = 1 << 16;  // rows of a launch: the grid's second axis has at most 65535 blocks
+  for (long long at = 0; at < rows; at += kMost) {
     Linear4Args a = {};
-    a.w = {static_cast<const uint8_t*>(codes), static_cast<const uint16_t*>(scales),
+    a.w = {static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
            static_cast<const uint8_t*>(zeros)};
     a.x = static_cast<const uint8_t*>(x) + at * x_stride * size;
     a.x_stride = x_stride;
     a.x_scale = x_scale ? x_scale + at : nullptr;
     a.bias = bias;
     a.y = static_cast<uint8_t*>(y) + at * n * 2;
-    a.rows = (int)std::min(rows - at, kMost - 16);
+    a.rows = (int)std::min(rows - at, kMost);
     a.n = n;
     a.k = k;
+    a.tiles = (n + 15) / 16;
     a.kblocks = (k + 127) / 128;
-    a.bf16_out = type == TAO_TYPE_BF16;
     a.wide = k % 8 == 0 && reinterpret_cast<uintptr_t>(a.x) % (8 * size) == 0 && x_stride % 8 == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int rc = x_type == TAO_TYPE_E4M3 ? by_group<kE4m3>(a, group, s)
-                   : x_type == TAO_TYPE_BF16 ? by_group<kBf16>(a, group, s)
-                                             : by_group<kF16>(a, group, s);
+    a.x_type = x_type;
+    const int rc = x_type == TAO_TYPE_BF16 ? by_group<MmaBf16, true>(a, group, s)
+                   : type == TAO_TYPE_BF16 ? by_group<MmaF16, true>(a, group, s)
+                                           : by_group<MmaF16, false>(a, group, s);
     if (rc) return rc;
   }
   return TAO_OK;

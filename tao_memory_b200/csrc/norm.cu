@@ -91,13 +91,6 @@ struct Vec {
   }
 };
 
-// max that keeps a NaN, as the plain form's does: a row with a NaN has a NaN scale.
-TAO_DEVI float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Sum (or maximum) over the threads of a row: blockDim.x of them; more than one warp only
 // where the block holds one row.  `red` has 32 floats for each value of the call's.
 template <int COUNT, bool MAX = false>

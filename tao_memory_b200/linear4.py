@@ -67,15 +67,16 @@ class Weight4:
         flat = codes.reshape(count, n, k)
         for i in range(count):  # matrix by matrix: the intermediate orders stay small
             c = _padded(flat[i], tiles * _TILE, blocks * _BLOCK)
-            # n = (tile, row half, g), k = (block, half, j >> 1, t, j & 1, register pair, element)
+            # n = (tile, row half, g), k = (block, half, i, t, f, e high, e low)
             c = c.view(tiles, 2, 8, blocks, 2, 2, 4, 2, 2, 2)
-            # -> tile, block, half, g, t, j >> 1, j & 1, then nibbles (element, register pair, row half)
+            # -> tile, block, half, g, t, i, f, e low, e high, then the byte's nibbles: rows g, g + 8
             c = c.permute(0, 3, 4, 2, 6, 5, 7, 9, 8, 1).reshape(tiles, blocks, 1024, 2)
             laid[i] = c[..., 0] | c[..., 1] << 4
 
         def by_tile(t):
             t = _padded(t.reshape(count, n, parts), tiles * _TILE, blocks * per)
-            return t.view(count, tiles, _TILE, blocks, per).permute(0, 1, 3, 4, 2).contiguous()
+            # a lane's rows g and g + 8 next to each other, the groups of a block within them
+            return t.view(count, tiles, 2, 8, blocks, per).permute(0, 1, 4, 3, 5, 2).contiguous()
 
         return cls(codes.shape, group, laid, by_tile(scales), None if zeros is None else by_tile(zeros))
 
@@ -87,7 +88,7 @@ class Weight4:
         c = c.permute(0, 1, 10, 4, 2, 3, 6, 5, 7, 9, 8).reshape(count, tiles * _TILE, blocks * _BLOCK)
 
         def rows(t):
-            t = t.permute(0, 1, 4, 2, 3).reshape(count, tiles * _TILE, -1)
+            t = t.permute(0, 1, 5, 3, 2, 4).reshape(count, tiles * _TILE, -1)
             return t[:, :n, :-(-k // self.group)].reshape(*lead, n, -1)
 
         return (c[:, :n, :k].reshape(*lead, n, k), rows(self.scales),
