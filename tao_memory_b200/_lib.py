@@ -4,9 +4,10 @@ The library is built in-tree by ``tao_memory_b200.build``.  There is no CPU or
 eager fallback: if the shared object is missing, every entry point raises.
 """
 
-import contextlib
 import ctypes
 import os
+
+import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtao_b200.so")
@@ -142,13 +143,14 @@ def check(rc):
     raise TaoError(msg)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def on(device):
-    """Context in which ``device`` (a CUDA device with an index) is the current one."""
-    import torch
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def on_device(device_index, fn, *args):
+    """``fn(*args, stream)`` checked, with the device current and its current stream's handle."""
+    if device_index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device_index):
+            return check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)))
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(device_index))
+    if rc:
+        check(rc)
 
 
 def exported_symbols():

@@ -3,23 +3,25 @@
 //   p = softmax(x R^T), the top_k largest of a row (ties to the lowest expert), their weights
 //   p or p / sum of the chosen;  out = sum over them of weight * down_e(silu(gate_e x) * (up_e x))
 //
-// Bound by the bytes of the chosen experts.  One cooperative launch, its blocks all resident, in
-// three parts with a grid barrier between them:
-//   1. logits [token][expert], 16 experts x 8 tokens to a block;
+// Bound by the bytes of the chosen experts; with a token or two by what lies between the reads, so the
+// code is short (it comes from memory too) and the blocks meet seldom.  One cooperative launch, a block
+// an SM, in three parts with a grid barrier between them:
+//   1. logits, one expert's to a block;
 //   2. every block picks the top_k itself (the same arithmetic in all of them) and sorts the
 //      (token, expert) pairs by expert; then 16 inner channels of one expert's gate and up at a
 //      time, h = silu(gate) up;
 //   3. 32 outputs of one expert's down at a time, a row of sums for each pair; and after a last
 //      barrier a token's pairs are added in the order of their choice.
-// Parts 1 to 3 are the same product of a few rows (few_rows.cuh).  One block an SM takes a run of
-// neighbouring units of work, so that its rows' activations stay in L1; its 16 warps are WT x WK, WT
-// units at a time, each one's k dealt to WK warps in runs, each warp's weights through a ring of its own
-// that runs on from unit to unit (part 3's starts before the barrier).
+// Parts 2 and 3 are the same product of a few rows (few_rows.cuh).  A block takes a run of neighbouring
+// units of work, so that its rows' activations stay in L1; its 16 warps are WT x WK, WT units at a time,
+// each one's k dealt to WK warps in runs, each warp's weights through a ring of its own that runs on from
+// unit to unit (part 3's starts before the barrier).
 // h is kept as the sum of two bf16 (16 mantissa bits), which are two columns of one mma: with bf16
 // alone its rounding would add as much to the error as the output's own.  Every sum's order is fixed.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/tao_b200.h"
@@ -31,10 +33,11 @@ namespace tao {
 namespace {
 
 constexpr int kWarps = 16, kThreads = kWarps * 32;
-constexpr int kTokens = 64;    // of a launch: a bit each of an expert's mask
+constexpr int kBlocks = 148;   // one an SM
+constexpr int kTokens = 64;    // of a launch: a bit each of an expert's mask, four a warp
 constexpr int kExperts = 512;  // most experts, and
 constexpr int kTop = 16;       // most of them for a token
-constexpr int kCols = 8;       // tokens of an entry: (expert, up to 8 of its tokens)
+constexpr int kCols = 4;       // tokens of an entry (an expert and some of its tokens) for each column tile
 constexpr int kHeader = 256;   // workspace: error word and barrier word
 
 struct Matrix16 {  // bf16 [experts][rows][k], the last axis contiguous
@@ -61,7 +64,7 @@ struct ExpertArgs {
 
 // A run of blocks of a row tile of 16-bit weights, 16 rows x 32 k each, straight from the matrix' rows.
 struct W16 {
-  static constexpr int KB = 32, BYTES = 1024, DEPTH = 4;
+  static constexpr int KB = 32, BYTES = 1024;
   using Matrix = Matrix16;
   const bf16 *r0, *r1, *any;
   int left;  // of k from this lane's next chunk on
@@ -98,7 +101,7 @@ struct W16 {
 // The same of 4-bit weights, 16 rows x 128 k each.
 template <int GROUP>
 struct W4 {
-  static constexpr int KB = 128, BYTES = Block4<GROUP>::BYTES, DEPTH = 4;
+  static constexpr int KB = 128, BYTES = Block4<GROUP>::BYTES;
   using Matrix = Four;
   const Four* m;
   uint32_t block;
@@ -120,24 +123,253 @@ struct W4 {
 struct Shared {
   unsigned long long mask[kExperts];
   int base[kExperts];
-  uint32_t entry[kExperts + kTokens * kTop / kCols];  // expert << 16 | first row << 4 | tokens
+  uint32_t entry[kExperts + kTokens * kTop / kCols];  // expert << 16 | first row << 5 | tokens
   uint16_t id[kTokens * kTop], row[kTokens * kTop];   // of a token's choices: expert, row of its pair
   float weight[kTokens * kTop];
   uint8_t token[kTokens * kTop];                      // of a pair's row
+  uint32_t parts[kWarps];                             // of the sort: a warp's pairs and entries
   int entries;
   bool ok;
 };
 
-constexpr int kSlot = 2 * 8 * 16;             // floats of a warp's sums of a unit
-constexpr int kSums = 2 * kWarps * kSlot;     // of the unit at hand and the one before
+// All blocks of the launch meet.  The word's top bit flips when the last one arrives (block 0
+// adds what the others leave to 2^31), so it needs no reset and any grid may use it next.  `bit` is
+// thread 0's, the bit before.
+TAO_DEVI bool grid_meet(const ExpertArgs& a, Shared& s, uint32_t& bit) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t add = blockIdx.x == 0 ? 0x80000000u - (gridDim.x - 1) : 1u;
+    asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(a.barrier), "r"(add) : "memory");
+    bool ok = false;
+    for (int i = 0; i < (1 << 22) && !ok; ++i) {  // seconds; every block is resident, so none is expected to be late
+      uint32_t now;
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(a.barrier) : "memory");
+      ok = ((now ^ bit) & 0x80000000u) != 0;
+    }
+    bit ^= 0x80000000u;
+    if (!ok) atomicOr(a.error, kErrWaitTimeout);
+    s.ok = ok;
+  }
+  __syncthreads();
+  return s.ok;
+}
 
-// Warps of a unit: the fewest blocks on the longest warp's way, then the fewest warps.
-TAO_DEVI int pick_wk(int units, int kblocks) {
-  const int n = (units + gridDim.x - 1) / gridDim.x;
+// Part 1: a block takes an expert, its warps 128 channels at a time, 16 lanes the even tokens and 16 the
+// odd ones, eight of them at once.  `sums`: [token][warp].
+TAO_DEVI void logits(const ExpertArgs& a, float* sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k0 = warp * 128 + (lane & 15) * 8;
+  for (int e = blockIdx.x; e < a.experts; e += gridDim.x) {
+    const bf16* r = a.router.at + e * a.router.row;
+#pragma unroll 1
+    for (int first = 0; first < a.tokens; first += 8) {  // all lanes' trips: they meet in the sums
+      const int t0 = first + (lane >> 4);
+      float sum[4] = {};
+#pragma unroll 1
+      for (int k = k0; k < a.width; k += kWarps * 128) {
+        const uint4 r8 = __ldg(reinterpret_cast<const uint4*>(r + k));
+        uint4 x8[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // a token beyond the last repeats it
+          x8[j] = __ldg(reinterpret_cast<const uint4*>(a.x + min(t0 + 2 * j, a.tokens - 1) * a.x_stride + k));
+        float w[8], v[8];
+        unpack8(r8, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          unpack8(x8[j], v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[j] += w[i] * v[i];
+        }
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+      if ((lane & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t0 + 2 * j < a.tokens) sums[(t0 + 2 * j) * kWarps + warp] = sum[j];
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < a.tokens) {
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) l += sums[threadIdx.x * kWarps + i];
+      a.logits[threadIdx.x * a.experts + e] = l;
+    }
+    __syncthreads();
+  }
+}
+
+// A float's order as an unsigned's; 0 and 1 are below every number (taken, and not a number).
+TAO_DEVI uint32_t order_of(float v) {
+  if (v != v) return 1u;
+  const uint32_t u = __float_as_uint(v + 0.f);  // -0 is 0
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// The top_k of TOK tokens (token, token + kWarps, ...) by one warp: ids and weights to shared memory.
+// Lane l has the experts l EACH .. l EACH + EACH - 1; the best of all is the lowest lane's with the most.
+// A token's choices come one after the other, several tokens' side by side.
+template <int EACH, int TOK>
+TAO_DEVI void choose(const ExpertArgs& a, Shared& s, int token, int lane) {
+  float v[TOK][EACH];
+  uint32_t key[TOK][EACH];
+  float mine[TOK], top[TOK];
+  int my_id[TOK];
+#pragma unroll
+  for (int q = 0; q < TOK; ++q) {
+    const int t = min(token + q * kWarps, a.tokens - 1);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int e = lane * EACH + i;
+      v[q][i] = e < a.experts ? __ldcg(a.logits + t * a.experts + e) : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < TOK; ++q)
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) key[q][i] = lane * EACH + i < a.experts ? order_of(v[q][i]) : 0u;
+#pragma unroll 1
+  for (int j = 0; j < a.top_k; ++j) {
+#pragma unroll
+    for (int q = 0; q < TOK; ++q) {
+      uint32_t best = key[q][0];
+      int at = 0;
+      float bv = v[q][0];
+#pragma unroll
+      for (int i = 1; i < EACH; ++i) {
+        if (key[q][i] > best) {
+          best = key[q][i];
+          at = i;
+          bv = v[q][i];
+        }
+      }
+      const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+      const int who = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
+      const float chosen = __shfl_sync(0xffffffffu, bv, who);
+      const int id = __shfl_sync(0xffffffffu, lane * EACH + at, who);
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        if (lane == who && i == at) key[q][i] = 0;
+      if (j == 0) top[q] = chosen;
+      if (lane == j) {
+        mine[q] = chosen;
+        my_id[q] = id;
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < TOK; ++q) {
+    const int t = token + q * kWarps;
+    bool nan = false;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      nan |= v[q][i] != v[q][i];
+      if (!a.renormalize) sum += lane * EACH + i < a.experts ? expf(v[q][i] - top[q]) : 0.f;
+    }
+    if (a.renormalize) sum = lane < a.top_k ? expf(mine[q] - top[q]) : 0.f;
+    sum = warp_sum(sum);
+    nan = __any_sync(0xffffffffu, nan);
+    if (lane < a.top_k && t < a.tokens) {
+      const float w = nan ? NAN : expf(mine[q] - top[q]) / sum;
+      s.id[t * a.top_k + lane] = (uint16_t)my_id[q];
+      s.weight[t * a.top_k + lane] = w;
+      if (blockIdx.x == 0 && a.ids) {
+        a.ids[t * a.top_k + lane] = my_id[q];
+        a.id_weights[t * a.top_k + lane] = w;
+      }
+    }
+  }
+}
+
+// Up to 32 pairs, by one warp: entries of up to `cols` tokens in the order of the experts' first pairs.
+TAO_DEVI void group_few_pairs(const ExpertArgs& a, Shared& s, int cols, int lane) {
+  const int pairs = a.tokens * a.top_k;
+  const bool in = lane < pairs;
+  const int id = in ? s.id[lane] : -1;
+  const uint32_t same = __match_any_sync(0xffffffffu, id), below = (1u << lane) - 1;
+  const int count = __popc(same), parts = (count + cols - 1) / cols;
+  const bool leads = in && (same & below) == 0;
+  const uint32_t own = leads ? (uint32_t)count << 16 | parts : 0u;
+  uint32_t run = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t before = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += before;
+  }
+  const int first = (int)((run - own) >> 16), at = (int)((run - own) & 0xffff);
+  if (leads)
+    for (int i = 0; i < parts; ++i)
+      s.entry[at + i] = (uint32_t)id << 16 | (uint32_t)(first + i * cols) << 5 | min(cols, count - i * cols);
+  const int row = __shfl_sync(0xffffffffu, first, __ffs(same) - 1) + __popc(same & below);
+  if (in) {
+    s.row[lane] = (uint16_t)row;
+    s.token[row] = (uint8_t)(lane / a.top_k);
+  }
+  if (lane == 31) s.entries = (int)(run & 0xffff);
+}
+
+// Pairs sorted by expert, then token; entries of up to `cols` tokens.  Thread e has expert e.
+TAO_DEVI void sort_pairs(const ExpertArgs& a, Shared& s, int cols) {
+  static_assert(kThreads >= kExperts, "");
+  const int pairs = a.tokens * a.top_k, e = threadIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  s.mask[e] = 0;
+  __syncthreads();
+  for (int p = threadIdx.x; p < pairs; p += kThreads) atomicOr(&s.mask[s.id[p]], 1ull << (p / a.top_k));
+  __syncthreads();
+  const int count = __popcll(s.mask[e]), parts = (count + cols - 1) / cols;
+  uint32_t run = (uint32_t)count << 16 | parts;  // sums over the experts up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t before = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += before;
+  }
+  if (lane == 31) s.parts[warp] = run;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) run += s.parts[w];
+  }
+  const int first = (int)(run >> 16) - count, at = (int)(run & 0xffff) - parts;
+  s.base[e] = first;
+  for (int i = 0; i < parts; ++i)
+    s.entry[at + i] = (uint32_t)e << 16 | (uint32_t)(first + i * cols) << 5 | min(cols, count - i * cols);
+  if (e == kThreads - 1) s.entries = (int)(run & 0xffff);
+  __syncthreads();
+  for (int p = threadIdx.x; p < pairs; p += kThreads) {
+    const int t = p / a.top_k, x = s.id[p], row = s.base[x] + __popcll(s.mask[x] & ((1ull << t) - 1));
+    s.row[p] = (uint16_t)row;
+    s.token[row] = (uint8_t)t;
+  }
+  __syncthreads();
+}
+
+// The experts' matrices in the layer's format.
+struct Layer16 {
+  using W = W16;
+  static TAO_DEVI const Matrix16& of(const ExpertArgs& a, int part, int r) {
+    return part ? a.down16 : r ? a.up16 : a.gate16;
+  }
+};
+template <int GROUP>
+struct Layer4 {
+  using W = W4<GROUP>;
+  static TAO_DEVI const Four& of(const ExpertArgs& a, int part, int r) { return part ? a.down4 : r ? a.up4 : a.gate4; }
+};
+
+template <int NT>
+constexpr int kDepth = NT == 4 ? 3 : 4;  // stages of a warp's ring, as shared memory allows
+template <int NT>
+constexpr int kSlot = 2 * kCols * NT * 16;  // floats of a warp's sums of a unit: [matrix][token][16 rows]
+
+// log2 of a unit's warps: the fewest blocks on the longest warp's way, then the fewest warps.
+TAO_DEVI int pick_wk(int units_of_block, int kblocks) {
   int best = 0, least = 1 << 30;
 #pragma unroll
   for (int shift = 0; 1 << shift <= kWarps; ++shift) {
-    const int groups = kWarps >> shift, cost = (n + groups - 1) / groups * ((kblocks + (1 << shift) - 1) >> shift);
+    const int groups = kWarps >> shift;
+    const int cost = (units_of_block + groups - 1) / groups * ((kblocks + (1 << shift) - 1) >> shift);
     if (cost < least && 1 << shift <= kblocks) {
       least = cost;
       best = shift;
@@ -146,40 +378,42 @@ TAO_DEVI int pick_wk(int units, int kblocks) {
   return best;
 }
 
-// A part's units, a run of neighbours for each block: unit u is row tiles R (u % tiles) ... of entry
-// u / tiles.  `weights(w, r, entry, tile, kb)` starts run w at block kb of unit (entry, tile)'s matrix r;
-// `rows(entry, c)` gives the row of column c or null; `cols(entry)` their number; `meet()` is called when
-// the first weights are on their way and before the first row is read; `sink(entry, tile, column, row,
-// sum)` takes sum(r) of each column and row, where the columns of a PAIR are added in twos.
-template <class W, int R, int NT, bool PAIR, class Weights, class Rows, class Cols, class Meet, class Sink>
-TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings, float* sums, Weights weights,
-                       Rows rows, Cols cols, Meet meet, Sink sink) {
-  constexpr int STAGE = R * W::BYTES;
+// Parts 2 (`part` 0) and 3 (1).  A unit is an entry's 16 inner channels or 32 outputs, two row tiles in
+// both; a column of the mma a token's x or (in turn) the two parts of its h.
+template <class L, int NT>
+TAO_DEVI bool run_part(const ExpertArgs& a, Shared& s, uint8_t* rings, float* sums, int part, uint32_t& bit) {
+  using W = typename L::W;
+  constexpr int STAGE = 2 * W::BYTES, SLOT = kSlot<NT>, DEPTH = kDepth<NT>;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kblocks = (k + W::KB - 1) / W::KB, units = entries * tiles;
-  const int wks = pick_wk(units, kblocks), groups = kWarps >> wks;
+  const int k = part ? a.inner : a.width, rows = part ? a.width : a.inner, pairs = a.tokens * a.top_k;
+  const int tiles = part ? (a.width + 31) / 32 : (a.inner + 15) / 16;
+  const int kblocks = (k + W::KB - 1) / W::KB, units = s.entries * tiles;
+  // a run of neighbouring units for each block
+  const int each = units / gridDim.x, more = units - each * gridDim.x, b = blockIdx.x;
+  const int lo = each * b + min(b, more), hi = lo + each + (b < more);
+  const int wks = pick_wk(each + (more > 0), kblocks), groups = kWarps >> wks;
   const int wt = warp >> wks, wk = warp & ((1 << wks) - 1);
   const int kw = kblocks * wk >> wks, per = (kblocks * (wk + 1) >> wks) - kw;
-  const int lo = (int)((long long)units * blockIdx.x / gridDim.x);
-  const int hi = (int)((long long)units * (blockIdx.x + 1) / gridDim.x);
-  const int mine = lo + wt < hi ? (hi - lo - wt + groups - 1) / groups : 0;
-  uint8_t* const ring = rings + warp * (W::DEPTH * STAGE);
+  const int mine = lo + wt < hi ? (hi - lo - wt + groups - 1) >> (4 - wks) : 0;
+  uint8_t* const ring = rings + warp * (DEPTH * STAGE);
   const uint32_t ring_at = smem_u32(ring);
+  const bool zeros = a.gate4.zeros != nullptr;
 
   int entry = (lo + wt) / tiles, tile = lo + wt - entry * tiles;
   int le = entry, lt = tile, lk = 0, left = mine * per, to_slot = 0;  // what is copied next
-  W w[R];
+  W w[2];
   auto issue = [&]() {
     if (left > 0) {
       --left;
       if (lk == 0) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) weights(w[r], r, le, lt, kw);
+        for (int r = 0; r < 2; ++r)
+          w[r].start(L::of(a, part, r), rows, k, s.entry[le] >> 16, part ? lt * 2 + r : lt, kw, lane);
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) w[r].issue(ring_at + to_slot + r * W::BYTES, lane);
-      to_slot = to_slot == (W::DEPTH - 1) * STAGE ? 0 : to_slot + STAGE;
+      for (int r = 0; r < 2; ++r) w[r].issue(ring_at + to_slot + r * W::BYTES, lane);
+      to_slot = to_slot == (DEPTH - 1) * STAGE ? 0 : to_slot + STAGE;
       if (++lk == per) {
         lk = 0;
         for (lt += groups; lt >= tiles; lt -= tiles) ++le;
@@ -188,8 +422,8 @@ TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings
     cp_commit();
   };
 #pragma unroll 1
-  for (int d = 0; d < W::DEPTH - 1; ++d) issue();
-  if (!meet()) {
+  for (int d = 0; d < DEPTH - 1; ++d) issue();
+  if (part && !grid_meet(a, s, bit)) {
     cp_wait<0>();
     return false;
   }
@@ -197,11 +431,17 @@ TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings
   int slot = 0, parity = 0;
 #pragma unroll 1
   for (int u = 0; u < mine; ++u) {
-    const int n_cols = cols(entry);
+    const uint32_t en = s.entry[entry];
+    const int first = en >> 5 & 0x7ff, tokens = en & 31, cols = tokens << part;
     const bf16* x[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) x[n] = n * 8 + g < n_cols ? rows(entry, n * 8 + g) + t * 8 : nullptr;
-    float acc[R][NT][4] = {};
+    for (int n = 0; n < NT; ++n) {
+      const int c = n * 8 + g;
+      x[n] = c >= cols ? nullptr
+             : part    ? a.h + ((long long)(c & 1) * pairs + first + c / 2) * a.inner + t * 8
+                       : a.x + s.token[first + c] * a.x_stride + t * 8;
+    }
+    float acc[2][NT][4] = {};
 #pragma unroll 1
     for (int i = 0; i < per; ++i) {
       const int k0 = (kw + i) * W::KB;
@@ -213,26 +453,27 @@ TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings
           v[p][n] = make_uint4(0, 0, 0, 0);
           if (x[n] && k0 + p * 32 + t * 8 < k) v[p][n] = *reinterpret_cast<const uint4*>(x[n] + k0 + p * 32);
         }
-      cp_wait<W::DEPTH - 2>();
+      cp_wait<DEPTH - 2>();
       __syncwarp();  // the stage is there for every lane, and every lane is done with the one before
       issue();
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        W::template product<NT>(acc[r], ring + slot + r * W::BYTES, zeros, lane, n_cols,
+      for (int r = 0; r < 2; ++r)
+        W::template product<NT>(acc[r], ring + slot + r * W::BYTES, zeros, lane, cols,
                                 [&](int p, int n) { return v[p][n]; });
-      slot = slot == (W::DEPTH - 1) * STAGE ? 0 : slot + STAGE;
+      slot = slot == (DEPTH - 1) * STAGE ? 0 : slot + STAGE;
     }
-    float* to = sums + (parity * kWarps + warp) * kSlot;  // [R][column][16 rows]
+    float* to = sums + (parity * kWarps + warp) * SLOT + g;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        if constexpr (PAIR) {
-          float* c = to + (r * 8 + n * 4 + t) * 16 + g;
+        float* c = to + r * (SLOT / 2) + n * 8 * 16;
+        if (part) {  // a token's two columns
+          c = to + r * (SLOT / 2) + (n * 4 + t) * 16;
           c[0] = acc[r][n][0] + acc[r][n][1];
           c[8] = acc[r][n][2] + acc[r][n][3];
-        } else {
-          float* c = to + (r * 8 + n * 8 + 2 * t) * 16 + g;
+        } else if (n * 8 + 2 * t < kCols * NT) {  // two tokens
+          c += 2 * t * 16;
           c[0] = acc[r][n][0];
           c[16] = acc[r][n][1];
           c[8] = acc[r][n][2];
@@ -244,14 +485,31 @@ TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings
       __syncwarp();
     else
       asm volatile("bar.sync %0, %1;" ::"r"(1 + wt), "r"(32 << wks) : "memory");
-    const float* from = sums + (parity * kWarps + (wt << wks)) * kSlot;
-    const int outs = (PAIR ? n_cols / 2 : n_cols) * 16;
-    for (int i = wk * 32 + lane; i < outs; i += 32 << wks)
-      sink(entry, tile, i / 16, i % 16, [&](int r) {
-        float s = 0.f;
-        for (int q = 0; q < 1 << wks; ++q) s += from[q * kSlot + r * 128 + i];
-        return s;
-      });
+    const float* from = sums + (parity * kWarps + (wt << wks)) * SLOT;
+    for (int i = wk * 32 + lane; i < tokens * 16; i += 32 << wks) {
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+      for (int q = 0; q < 1 << wks; ++q) {
+        s0 += from[q * SLOT + i];
+        s1 += from[q * SLOT + SLOT / 2 + i];
+      }
+      const long long pair = first + i / 16;
+      if (part) {
+        const int n = tile * 32 + i % 16;
+        float* out = a.pair_out + pair * a.width + n;
+        if (n < a.width) out[0] = s0;
+        if (n + 16 < a.width) out[16] = s1;
+      } else {
+        const int c = tile * 16 + i % 16;
+        if (c < a.inner) {
+          const float h = s0 / (1.f + expf(-s0)) * s1;
+          const bf16 high = tobf(h);
+          a.h[pair * a.inner + c] = high;
+          // an infinite h leaves nothing: infinity minus itself would be no number
+          a.h[(pair + pairs) * a.inner + c] = isinf(bf(high)) ? tobf(0.f) : tobf(h - bf(high));
+        }
+      }
+    }
     parity ^= 1;
     for (tile += groups; tile >= tiles; tile -= tiles) ++entry;
   }
@@ -260,228 +518,50 @@ TAO_DEVI bool run_part(int entries, int tiles, int k, bool zeros, uint8_t* rings
   return true;
 }
 
-// All blocks of the launch meet.  The word's top bit flips when the last one arrives (block 0
-// adds what the others leave to 2^31), so it needs no reset and any grid may use it next.
-TAO_DEVI bool grid_meet(const ExpertArgs& a, Shared& s) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const unsigned add = blockIdx.x == 0 ? 0x80000000u - (gridDim.x - 1) : 1u;
-    const unsigned old = (unsigned)atomic_add_release(reinterpret_cast<int*>(a.barrier), (int)add);
-    bool ok = false;
-    for (int i = 0; i < (1 << 22) && !ok; ++i) {  // seconds; every block is resident, so none is expected to be late
-      unsigned now;
-      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(a.barrier) : "memory");
-      ok = ((now ^ old) & 0x80000000u) != 0;
-    }
-    fence_acquire();
-    if (!ok) atomicOr(a.error, kErrWaitTimeout);
-    s.ok = ok;
-  }
-  __syncthreads();
-  return s.ok;
-}
+template <class W, int NT>
+constexpr int kRings = kWarps * kDepth<NT> * 2 * W::BYTES;
+template <class W, int NT>  // the sums of the unit at hand and of the one before
+constexpr int kSmem = kRings<W, NT> + 2 * kWarps * kSlot<NT> * 4 + (int)sizeof(Shared);
+static_assert(kSmem<W16, 4> <= 227 * 1024 && kSmem<W4<32>, 4> <= 227 * 1024, "");
+static_assert(kSlot<1> * 2 * kWarps >= kTokens * kWarps, "part 1's sums fit too");
 
-// A float's order as an unsigned's; 0 and 1 are below every number (taken, and not a number).
-TAO_DEVI uint32_t order_of(float v) {
-  if (v != v) return 1u;
-  const uint32_t u = __float_as_uint(v + 0.f);  // -0 is 0
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-// The top_k of one token by one warp: ids and weights to shared memory.
-TAO_DEVI void choose(const ExpertArgs& a, Shared& s, int token, int lane) {
-  constexpr int N = kExperts / 32;
-  float v[N];
-  uint32_t key[N];
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * 32 + lane;
-    key[i] = 0;
-    if (i * 32 < a.experts && e < a.experts) {
-      v[i] = __ldcg(a.logits + token * a.experts + e);
-      key[i] = order_of(v[i]);
-      nan |= v[i] != v[i];
-    } else {
-      v[i] = -INFINITY;
-    }
-  }
-  nan = __any_sync(0xffffffffu, nan);
-  float top = 0.f, sum = 0.f, mine = 0.f;
-  int my_id = 0;
-  for (int j = 0; j < a.top_k; ++j) {
-    uint32_t best = 0;
-    float bv = 0.f;
-    int bi = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (i * 32 < a.experts && key[i] > best) {
-        best = key[i];
-        bi = i;
-        bv = v[i];
-      }
-    }
-    const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == most ? (uint32_t)(bi * 32 + lane) : 0xffffffffu);
-    const float chosen = __shfl_sync(0xffffffffu, bv, e & 31);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * 32 + lane == e) key[i] = 0;
-    if (j == 0) {
-      top = chosen;
-      if (!a.renormalize) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += i * 32 + lane < a.experts ? expf(v[i] - top) : 0.f;
-        sum = warp_sum(sum);
-      }
-    }
-    const float p = expf(chosen - top);
-    if (a.renormalize) sum += p;
-    if (lane == j) {
-      mine = p;
-      my_id = e;
-    }
-  }
-  if (lane < a.top_k) {
-    const float w = nan ? NAN : mine / sum;
-    s.id[token * a.top_k + lane] = (uint16_t)my_id;
-    s.weight[token * a.top_k + lane] = w;
-    if (blockIdx.x == 0 && a.ids) {
-      a.ids[token * a.top_k + lane] = my_id;
-      a.id_weights[token * a.top_k + lane] = w;
-    }
-  }
-}
-
-// Pairs sorted by expert, then token; entries of up to kCols tokens.
-TAO_DEVI void sort_pairs(const ExpertArgs& a, Shared& s) {
-  const int pairs = a.tokens * a.top_k;
-  for (int e = threadIdx.x; e < a.experts; e += kThreads) s.mask[e] = 0;
-  __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += kThreads) atomicOr(&s.mask[s.id[p]], 1ull << (p / a.top_k));
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    int rows = 0, entries = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int e = e0 + threadIdx.x;
-      const int count = e < a.experts ? __popcll(s.mask[e]) : 0, parts = (count + kCols - 1) / kCols;
-      int r = count, n = parts;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int r2 = __shfl_up_sync(0xffffffffu, r, o), n2 = __shfl_up_sync(0xffffffffu, n, o);
-        if ((int)threadIdx.x >= o) {
-          r += r2;
-          n += n2;
-        }
-      }
-      const int first = rows + r - count;
-      if (e < a.experts) s.base[e] = first;
-      for (int i = 0; i < parts; ++i)
-        s.entry[entries + n - parts + i] =
-            (uint32_t)e << 16 | (uint32_t)(first + i * kCols) << 4 | min(kCols, count - i * kCols);
-      rows += __shfl_sync(0xffffffffu, r, 31);
-      entries += __shfl_sync(0xffffffffu, n, 31);
-    }
-    if (threadIdx.x == 0) s.entries = entries;
-  }
-  __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += kThreads) {
-    const int t = p / a.top_k, e = s.id[p];
-    const int row = s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1));
-    s.row[p] = (uint16_t)row;
-    s.token[row] = (uint8_t)t;
-  }
-  __syncthreads();
-}
-
-// The experts' matrices in the layer's format.
-struct Layer16 {
-  using W = W16;
-  static TAO_DEVI const Matrix16& gate(const ExpertArgs& a) { return a.gate16; }
-  static TAO_DEVI const Matrix16& up(const ExpertArgs& a) { return a.up16; }
-  static TAO_DEVI const Matrix16& down(const ExpertArgs& a) { return a.down16; }
-};
-template <int GROUP>
-struct Layer4 {
-  using W = W4<GROUP>;
-  static TAO_DEVI const Four& gate(const ExpertArgs& a) { return a.gate4; }
-  static TAO_DEVI const Four& up(const ExpertArgs& a) { return a.up4; }
-  static TAO_DEVI const Four& down(const ExpertArgs& a) { return a.down4; }
-};
-
-template <class W>
-constexpr int kRings = kWarps * (W::DEPTH * 2 * W::BYTES > W16::DEPTH * W16::BYTES ? W::DEPTH * 2 * W::BYTES
-                                                                                  : W16::DEPTH * W16::BYTES);
-template <class W>
-constexpr int kSmem = kRings<W> + kSums * 4 + (int)sizeof(Shared);
-static_assert(kSmem<W16> <= 227 * 1024 && kSmem<W4<32>> <= 227 * 1024, "");
-
-template <class L>
+// NT: column tiles of an entry in part 3.
+template <class L, int NT>
 __global__ void __launch_bounds__(kThreads, 1) experts_kernel(const __grid_constant__ ExpertArgs a) {
   using W = typename L::W;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* sums = reinterpret_cast<float*>(smem + kRings<W>);
-  Shared& s = *reinterpret_cast<Shared*>(smem + kRings<W> + kSums * 4);
+  float* sums = reinterpret_cast<float*>(smem + kRings<W, NT>);
+  Shared& s = *reinterpret_cast<Shared*>(smem + kRings<W, NT> + 2 * kWarps * kSlot<NT> * 4);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const auto now = [] { return true; };
+  uint32_t bit = threadIdx.x == 0 ? *reinterpret_cast<volatile unsigned*>(a.barrier) : 0;
 
-  // 1. logits: an entry is 8 tokens
-  run_part<W16, 1, 1, false>(
-      (a.tokens + 7) / 8, (a.experts + 15) / 16, a.width, false, smem, sums,
-      [&](W16& w, int, int, int tile, int kb) { w.start(a.router, a.experts, a.width, 0, tile, kb, lane); },
-      [&](int entry, int c) { return a.x + (entry * 8 + c) * a.x_stride; },
-      [&](int entry) { return min(8, a.tokens - entry * 8); }, now,
-      [&](int entry, int tile, int col, int row, auto sum) {
-        const int e = tile * 16 + row;
-        if (e < a.experts) a.logits[(entry * 8 + col) * a.experts + e] = sum(0);
-      });
-  if (!grid_meet(a, s)) return;
-  for (int t = warp; t < a.tokens; t += kWarps) choose(a, s, t, lane);
+  logits(a, sums);
+  if (!grid_meet(a, s, bit)) return;
+  if (a.experts <= 128) {
+    if (a.tokens <= kWarps) {
+      if (warp < a.tokens) choose<4, 1>(a, s, warp, lane);
+    } else {
+      choose<4, 4>(a, s, warp, lane);
+    }
+  } else {
+    for (int t = warp; t < a.tokens; t += kWarps) choose<16, 1>(a, s, t, lane);
+  }
   __syncthreads();
-  sort_pairs(a, s);
-
-  const int pairs = a.tokens * a.top_k;
-  const bool zeros = a.gate4.zeros != nullptr;
-  const auto expert = [&](int entry) { return (int)(s.entry[entry] >> 16); };
-  const auto first = [&](int entry) { return (int)(s.entry[entry] >> 4 & 0xfff); };
-  const auto count = [&](int entry) { return (int)(s.entry[entry] & 15); };
-  // 2. h
-  run_part<W, 2, 1, false>(
-      s.entries, (a.inner + 15) / 16, a.width, zeros, smem, sums,
-      [&](W& w, int r, int entry, int tile, int kb) {
-        w.start(r ? L::up(a) : L::gate(a), a.inner, a.width, expert(entry), tile, kb, lane);
-      },
-      [&](int entry, int c) { return a.x + s.token[first(entry) + c] * a.x_stride; }, count, now,
-      [&](int entry, int tile, int col, int row, auto sum) {
-        const int c = tile * 16 + row;
-        if (c >= a.inner) return;
-        const float gate = sum(0), up = sum(1);
-        const float h = gate / (1.f + expf(-gate)) * up;
-        const long long at = (long long)(first(entry) + col) * a.inner + c;
-        const bf16 high = tobf(h);
-        a.h[at] = high;
-        // an infinite h leaves nothing: infinity minus itself would be no number
-        a.h[at + (long long)pairs * a.inner] = isinf(bf(high)) ? tobf(0.f) : tobf(h - bf(high));
-      });
-  // 3. the pairs' outputs: two columns a token, its h's high and low parts; and the tokens'
-  const bool met = run_part<W, 2, 2, true>(
-      s.entries, (a.width + 31) / 32, a.inner, zeros, smem, sums,
-      [&](W& w, int r, int entry, int tile, int kb) {
-        w.start(L::down(a), a.width, a.inner, expert(entry), tile * 2 + r, kb, lane);
-      },
-      [&](int entry, int c) { return a.h + ((long long)(c & 1) * pairs + first(entry) + c / 2) * a.inner; },
-      [&](int entry) { return 2 * count(entry); }, [&] { return grid_meet(a, s); },
-      [&](int entry, int tile, int col, int row, auto sum) {
-        float* to = a.pair_out + (long long)(first(entry) + col) * a.width;
-        const int n = tile * 32 + row;
-        if (n < a.width) to[n] = sum(0);
-        if (n + 16 < a.width) to[n + 16] = sum(1);
-      });
-  if (!met || !grid_meet(a, s)) return;
+  if (a.tokens * a.top_k <= 32) {
+    if (warp == 0) group_few_pairs(a, s, kCols * NT, lane);
+    __syncthreads();
+  } else {
+    sort_pairs(a, s, kCols * NT);
+  }
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part)
+    if (!run_part<L, NT>(a, s, smem, sums, part, bit)) return;
+  if (!grid_meet(a, s, bit)) return;
   const int quads = a.width / 4;
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < a.tokens * quads; i += gridDim.x * kThreads) {
-    const int t = i / quads, n = i % quads * 4;
+    const int t = i / quads, n = (i - t * quads) * 4;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int j = 0; j < a.top_k; ++j) {
       const int p = t * a.top_k + j;
       const float w = s.weight[p];
@@ -526,20 +606,33 @@ int check(const TaoExperts* p, int tokens) {
   return TAO_OK;
 }
 
-template <class L>
-int launch(ExpertArgs a, cudaStream_t s) {
-  const int smem = kSmem<typename L::W>;
-  auto kernel = experts_kernel<L>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  int device = 0, sms = 0, per = 0;
-  if (e == cudaSuccess) e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, smem);
+template <class L, int NT>
+int launch_as(ExpertArgs a, cudaStream_t s) {
+  const int smem = kSmem<typename L::W, NT>;
+  auto kernel = experts_kernel<L, NT>;
+  static std::atomic<uint64_t> ready{0};  // devices (the first 64) on which the kernel may use its shared memory
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t mark = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & mark)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) ready |= mark;
+  }
   if (e == cudaSuccess) {
     void* args[] = {&a};
-    e = cudaLaunchCooperativeKernel((const void*)kernel, dim3(sms * per), dim3(kThreads), args, smem, s);
+    e = cudaLaunchCooperativeKernel((const void*)kernel, dim3(kBlocks), dim3(kThreads), args, smem, s);
   }
   return e == cudaSuccess ? TAO_OK : efail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
+// An entry's weights come once for its 4, 8 or 16 tokens, and from L2 for each further entry of the
+// expert; columns that few entries fill cost instructions.  So by the mean tokens of an expert.
+template <class L>
+int launch(const ExpertArgs& a, cudaStream_t s) {
+  const int pairs = a.tokens * a.top_k;
+  if (pairs <= 2 * a.experts) return launch_as<L, 1>(a, s);
+  if (pairs <= 8 * a.experts) return launch_as<L, 2>(a, s);
+  return launch_as<L, 4>(a, s);
 }
 
 }  // namespace

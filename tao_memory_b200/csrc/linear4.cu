@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/tao_b200.h"
@@ -382,7 +383,14 @@ int launch(Linear4Args a, cudaStream_t s) {
   a.ring = p.ring;
   a.sums = p.sums;
   auto kernel = linear4_kernel<M, BF16, GROUP, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> ready{0};  // devices (the first 64) on which the kernel may use its shared memory
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t mark = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & mark)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) ready |= mark;
+  }
   if (e == cudaSuccess) {
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(p.blocks, (a.rows + F::ROWS - 1) / F::ROWS);

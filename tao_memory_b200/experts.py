@@ -62,7 +62,7 @@ class ExpertWeights:
         one, most = (lib.tao_expert_workspace_bytes(ctypes.byref(self._layer), n) for n in (1, _TOKENS))
         if one == 0:
             _lib.check(_lib.TAO_ERR_ARG)
-        self._workspace_bytes = most
+        self._workspace_bytes, self._at = most, ctypes.byref(self._layer)
 
 
 def _aligned(t):
@@ -112,22 +112,19 @@ def expert_layer(x, weights, out=None, return_routing=False):
     rows = _rows(x, weights.width)
     if rows.data_ptr() % 16 or rows.stride(0) % 8:
         rows = rows.clone(memory_format=torch.contiguous_format)
-    tokens = rows.shape[0]
     if out is None:
-        out = torch.empty(x.shape, dtype=_BF16, device=x.device)
+        out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != _BF16 or out.device != x.device or not out.is_contiguous():
         raise ValueError("out is a contiguous tensor of x's shape, type and device")
-    ids = route = None
+    ids = route = ids_at = route_at = None
     if return_routing:
-        ids = torch.empty(*x.shape[:-1], weights.top_k, dtype=torch.int32, device=x.device)
-        route = torch.empty(ids.shape, dtype=torch.float32, device=x.device)
-    with _lib.on(x.device):
-        stream = torch.cuda.current_stream(x.device).cuda_stream
-        ws = _Room.get(x.device, stream, weights._workspace_bytes)
-        _lib.check(_lib.lib().tao_expert_layer(
-            ctypes.byref(weights._layer), rows.data_ptr(), rows.stride(0), tokens, out.data_ptr(),
-            None if ids is None else ids.data_ptr(), None if ids is None else route.data_ptr(), ws.data_ptr(),
-            ws.numel(), stream))
+        ids = x.new_empty((*x.shape[:-1], weights.top_k), dtype=torch.int32)
+        route = x.new_empty(ids.shape, dtype=torch.float32)
+        ids_at, route_at = ids.data_ptr(), route.data_ptr()
+    device = x.device.index
+    ws = _Room.get(x.device, torch._C._cuda_getCurrentRawStream(device), weights._workspace_bytes)
+    _lib.on_device(device, _lib.lib().tao_expert_layer, weights._at, rows.data_ptr(), rows.stride(0), rows.shape[0],
+                   out.data_ptr(), ids_at, route_at, ws.data_ptr(), ws.numel())
     return (out, ids, route) if return_routing else out
 
 

@@ -12,6 +12,7 @@ from . import _lib
 from .norm import TYPES, _rows
 
 GROUPS = (32, 64, 128)
+E4M3 = 3  # the library's code of the type, beside TYPES
 _TILE, _BLOCK = 16, 128
 
 
@@ -30,14 +31,10 @@ class Weight4:
     def __init__(self, shape, group, codes, scales, zeros):
         self.shape, self.group = tuple(shape), group
         self.codes, self.scales, self.zeros = codes, scales, zeros
-
-    @property
-    def dtype(self):
-        return self.scales.dtype
-
-    @property
-    def device(self):
-        return self.codes.device
+        self.dtype, self.device = scales.dtype, codes.device
+        # what tao_linear4 takes of it
+        self.args = (codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
+                     TYPES[scales.dtype])
 
     def bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
@@ -133,42 +130,43 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
     """x W^T + bias: x [..., k] in the weight's type, or in e4m3 with one fp32 scale a row
     (``x_scale`` [..., 1], as ``add_rms_norm_fp8`` gives them); returns [..., n] in the weight's type.
 
-    Made for few rows (a decode step's): the weight is read once for up to 16 rows, and again
-    for each 16 more.  No gradient."""
+    Made for few rows (a decode step's): the weight is read once for up to 32 rows, and from L2
+    for each 32 more.  No gradient."""
     if not isinstance(weight, Weight4) or len(weight.shape) != 2:
         raise ValueError("linear4 takes one Weight4 matrix")
     n, k = weight.shape
-    if not x.is_cuda or x.device != weight.device:
+    device, dtype = weight.device, weight.dtype
+    if x.device != device or device.type != "cuda":
         raise ValueError("linear4 takes CUDA activations on the weight's device (no CPU fallback)")
     if x.dim() == 0 or x.shape[-1] != k:
         raise ValueError(f"activations have {k} channels, as the weight")
-    fp8 = x.dtype == torch.float8_e4m3fn
-    if not fp8 and x.dtype != weight.dtype:
+    code = TYPES.get(x.dtype)
+    if x.dtype == torch.float8_e4m3fn:
+        code = E4M3
+    elif x.dtype != dtype:
         raise ValueError("activations have the type of the weight's scales, or are e4m3")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("linear4 has no gradient: call it under torch.no_grad()")
     rows = _rows(x, k)
     count = rows.shape[0]
+    scale_at = bias_at = None
     if x_scale is not None:
-        if not fp8 or x_scale.dtype != torch.float32 or x_scale.numel() != count or x_scale.device != x.device:
+        if code != E4M3 or x_scale.dtype != torch.float32 or x_scale.numel() != count or x_scale.device != device:
             raise ValueError("x_scale is one fp32 value a row of e4m3 activations, on their device")
         x_scale = x_scale.contiguous()
+        scale_at = x_scale.data_ptr()
     if bias is not None:
-        if bias.shape != (n,) or bias.dtype != weight.dtype or bias.device != x.device:
+        if bias.shape != (n,) or bias.dtype != dtype or bias.device != device:
             raise ValueError("the bias is one value per output, of the weight's type and device")
         bias = bias.contiguous()
+        bias_at = bias.data_ptr()
     shape = (*x.shape[:-1], n)
     if out is None:
-        out = torch.empty(shape, dtype=weight.dtype, device=x.device)
-    elif out.shape != shape or out.dtype != weight.dtype or out.device != x.device or not out.is_contiguous():
+        out = x.new_empty(shape, dtype=dtype)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError("out is a contiguous tensor of the result's shape, type and device")
-    with _lib.on(x.device):
-        _lib.check(_lib.lib().tao_linear4(
-            rows.data_ptr(), rows.stride(0), 3 if fp8 else TYPES[x.dtype],
-            None if x_scale is None else x_scale.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-            None if weight.zeros is None else weight.zeros.data_ptr(), weight.group, TYPES[weight.dtype],
-            None if bias is None else bias.data_ptr(), count, n, k, out.data_ptr(),
-            torch.cuda.current_stream(x.device).cuda_stream))
+    _lib.on_device(device.index, _lib.lib().tao_linear4, rows.data_ptr(), rows.stride(0), code, scale_at,
+                   *weight.args, bias_at, count, n, k, out.data_ptr())
     return out
 
 

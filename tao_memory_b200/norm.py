@@ -18,7 +18,8 @@ RMS_EPS = float(torch.finfo(torch.float32).eps)
 
 def _rows(t, width):
     """``t`` as rows [n, width] with a contiguous last axis; copied only where its strides ask for it."""
-    t = t if t.dim() == 2 else t.reshape(-1, width)
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
     return t if t.stride(1) == 1 or width == 1 else t.contiguous()
 
 
@@ -34,19 +35,23 @@ def _check(x, weight, residual):
         raise ValueError("the weight must be one value per channel, of x's type and device")
 
 
+def _new(x, dtype=None):
+    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _forward(x, weight, residual, eps):
     width = x.shape[-1]
     rows = _rows(x, width)
-    res = None if residual is None else _rows(residual, width)
-    weight = None if weight is None else weight.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = x if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _lib.on(x.device):
-        _lib.check(_lib.lib().tao_add_rms_norm(
-            rows.data_ptr(), rows.stride(0), None if res is None else res.data_ptr(),
-            0 if res is None else res.stride(0), None if weight is None else weight.data_ptr(), rows.shape[0], width,
-            TYPES[x.dtype], eps, None if res is None else s.data_ptr(), y.data_ptr(),
-            torch.cuda.current_stream(x.device).cuda_stream))
+    y = _new(x)
+    res, stride, s = None, 0, x
+    if residual is not None:
+        residual = _rows(residual, width)
+        res, stride, s = residual.data_ptr(), residual.stride(0), _new(x)
+    if weight is not None:
+        weight = weight.contiguous()
+    _lib.on_device(x.device.index, _lib.lib().tao_add_rms_norm, rows.data_ptr(), rows.stride(0), res, stride,
+                   None if weight is None else weight.data_ptr(), rows.shape[0], width, TYPES[x.dtype], eps,
+                   None if res is None else s.data_ptr(), y.data_ptr())
     return y, s
 
 
@@ -65,23 +70,23 @@ class _AddNorm(torch.autograd.Function):
         s, weight = ctx.saved_tensors
         if dy is None:  # only the stream was used
             return ds, None, ds if ctx.added else None, None
-        width = s.shape[-1]
-        rows, gy = _rows(s, width), _rows(dy, width)
-        gs = None if ds is None else _rows(ds, width)
-        w = None if weight is None else weight.contiguous()
-        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
-        dw = torch.empty_like(w) if w is not None and ctx.needs_input_grad[1] else None
-        lib, code = _lib.lib(), TYPES[s.dtype]
-        ws = None
-        if dw is not None:
+        width, code, lib = s.shape[-1], TYPES[s.dtype], _lib.lib()
+        rows, dy = _rows(s, width), _rows(dy, width)
+        if ds is not None:
+            ds = _rows(ds, width)
+        if weight is not None:
+            weight = weight.contiguous()
+        dx = _new(s)
+        dw = ws = None
+        size = 0
+        if weight is not None and ctx.needs_input_grad[1]:
+            dw = torch.empty_like(weight)
             size = lib.tao_add_rms_norm_workspace_bytes(rows.shape[0], width, code)
-            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=s.device)
-        with _lib.on(s.device):
-            _lib.check(lib.tao_add_rms_norm_backward(
-                gy.data_ptr(), gy.stride(0), None if gs is None else gs.data_ptr(), 0 if gs is None else gs.stride(0),
-                rows.data_ptr(), rows.stride(0), None if w is None else w.data_ptr(), rows.shape[0], width, code,
-                ctx.eps, dx.data_ptr(), None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(),
-                0 if ws is None else ws.numel(), torch.cuda.current_stream(s.device).cuda_stream))
+            ws = dy.new_empty(max(size, 1), dtype=torch.uint8)
+        at = lambda t: None if t is None else t.data_ptr()
+        _lib.on_device(s.device.index, lib.tao_add_rms_norm_backward, dy.data_ptr(), dy.stride(0), at(ds),
+                       0 if ds is None else ds.stride(0), rows.data_ptr(), rows.stride(0), at(weight), rows.shape[0],
+                       width, code, ctx.eps, dx.data_ptr(), at(dw), at(ws), size)
         return dx, dw, dx if ctx.added else None, None
 
 
@@ -111,17 +116,17 @@ def add_rms_norm_fp8(x, weight=None, residual=None, eps=RMS_EPS, group=None):
         raise ValueError("the 8-bit norm has no gradient: call it under torch.no_grad()")
     width = x.shape[-1]
     rows = _rows(x, width)
-    res = None if residual is None else _rows(residual, width)
-    weight = None if weight is None else weight.contiguous()
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(*x.shape[:-1], 1 if group is None else -(-width // 128), dtype=torch.float32, device=x.device)
-    s = x if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _lib.on(x.device):
-        _lib.check(_lib.lib().tao_add_rms_norm_fp8(
-            rows.data_ptr(), rows.stride(0), None if res is None else res.data_ptr(),
-            0 if res is None else res.stride(0), None if weight is None else weight.data_ptr(), rows.shape[0], width,
-            TYPES[x.dtype], eps, group or 0, None if res is None else s.data_ptr(), q.data_ptr(), scale.data_ptr(),
-            torch.cuda.current_stream(x.device).cuda_stream))
+    q = _new(x, torch.float8_e4m3fn)
+    scale = x.new_empty((*x.shape[:-1], 1 if group is None else -(-width // 128)), dtype=torch.float32)
+    res, stride, s = None, 0, x
+    if residual is not None:
+        residual = _rows(residual, width)
+        res, stride, s = residual.data_ptr(), residual.stride(0), _new(x)
+    if weight is not None:
+        weight = weight.contiguous()
+    _lib.on_device(x.device.index, _lib.lib().tao_add_rms_norm_fp8, rows.data_ptr(), rows.stride(0), res, stride,
+                   None if weight is None else weight.data_ptr(), rows.shape[0], width, TYPES[x.dtype], eps,
+                   group or 0, None if res is None else s.data_ptr(), q.data_ptr(), scale.data_ptr())
     return q, scale, s
 
 
