@@ -7,7 +7,6 @@ that adds the blocks' parts in a fixed order.
 """
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -55,6 +54,23 @@ def _forward(x, weight, residual, eps):
     return y, s
 
 
+class _Room:
+    """The weight gradient's scratch: one buffer for a device and stream, whose calls run in
+    order; a captured call gets one of its own."""
+
+    cache = {}
+
+    @classmethod
+    def get(cls, device, size):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(size, dtype=torch.uint8, device=device)
+        key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
+        buf = cls.cache.get(key)
+        if buf is None or buf.numel() < size:
+            buf = cls.cache[key] = torch.empty(max(size, 1 << 20), dtype=torch.uint8, device=device)
+        return buf
+
+
 class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
@@ -65,8 +81,9 @@ class _AddNorm(torch.autograd.Function):
         return (y, s) if ctx.added else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, ds=None):
+        if torch.is_grad_enabled():
+            raise RuntimeError("add_rms_norm is differentiable once (its gradient has none)")
         s, weight = ctx.saved_tensors
         if dy is None:  # only the stream was used
             return ds, None, ds if ctx.added else None, None
@@ -82,7 +99,7 @@ class _AddNorm(torch.autograd.Function):
         if weight is not None and ctx.needs_input_grad[1]:
             dw = torch.empty_like(weight)
             size = lib.tao_add_rms_norm_workspace_bytes(rows.shape[0], width, code)
-            ws = dy.new_empty(max(size, 1), dtype=torch.uint8)
+            ws = _Room.get(s.device, size)
         at = lambda t: None if t is None else t.data_ptr()
         _lib.on_device(s.device.index, lib.tao_add_rms_norm_backward, dy.data_ptr(), dy.stride(0), at(ds),
                        0 if ds is None else ds.stride(0), rows.data_ptr(), rows.stride(0), at(weight), rows.shape[0],

@@ -200,6 +200,37 @@ def test_same_result_on_another_stream_and_again():
         assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
 
 
+def test_gradient_has_no_gradient():
+    from tao_memory_b200 import add_rms_norm
+    x, _, w, _, _ = _inputs(3, 64, torch.float32, residual=False)
+    y, _ = add_rms_norm(x.requires_grad_(True), w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_captured_training_step():
+    from tao_memory_b200 import add_rms_norm
+    x, res, w, dy, ds = _inputs(300, 256, torch.bfloat16, seed=6)
+    leaves = [t.requires_grad_(True) for t in (x, w, res)]
+
+    def step():
+        y, s = add_rms_norm(*leaves, eps=EPS)
+        return (y, s) + torch.autograd.grad((y, s), leaves, (dy, ds))
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    with torch.no_grad():
+        x.mul_(1.5)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(outs, step()))
+
+
 def test_refusals():
     from tao_memory_b200 import add_rms_norm, add_rms_norm_fp8
     x = torch.randn(4, 64, device="cuda", dtype=torch.bfloat16)
