@@ -141,7 +141,7 @@ TAO_DEVI bool grid_meet(const ExpertArgs& a, Shared& s, uint32_t& bit) {
     const uint32_t add = blockIdx.x == 0 ? 0x80000000u - (gridDim.x - 1) : 1u;
     asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(a.barrier), "r"(add) : "memory");
     bool ok = false;
-    for (int i = 0; i < (1 << 22) && !ok; ++i) {  // seconds; every block is resident, so none is expected to be late
+    for (int i = 0; i < (1 << 21) && !ok; ++i) {  // a second or two; every block is resident, so none is expected to be late
       uint32_t now;
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(a.barrier) : "memory");
       ok = ((now ^ bit) & 0x80000000u) != 0;

@@ -163,6 +163,22 @@ def test_layers_of_different_size_share_a_workspace():
             _run(x, layer, router, wide)
 
 
+def test_an_error_word_is_reported_once():
+    """The host's side of an expired wait: the word is set here by hand."""
+    from tao_memory_b200 import _lib, expert_layer
+    from tao_memory_b200.experts import _Room
+    from tao_memory_b200.stream import check_device
+    layer, router, wide = _layer(64, 32, 4, 2)
+    x = torch.randn(2, 64, device="cuda").bfloat16()
+    out = expert_layer(x, layer)
+    room = _Room.get(x.device, torch.cuda.current_stream().cuda_stream, 1)
+    room[:4] = torch.tensor([1, 0, 0, 0], dtype=torch.uint8)
+    with pytest.raises(_lib.TaoError):
+        check_device()
+    assert check_device() == 0 and (room == 0).all()
+    assert torch.equal(expert_layer(x, layer), out)
+
+
 def test_refusals():
     from tao_memory_b200 import ExpertWeights, expert_layer, quantize4
     layer, router, wide = _layer(64, 32, 4, 2)
