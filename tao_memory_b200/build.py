@@ -23,7 +23,7 @@ def sources():
 
 def build(verbose=False, extra=()):
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
+    cmd = [nvcc, *ARCH, "--threads", "0", "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
            "-I", os.path.join(ROOT, "include"), "-o", LIB, *sources(), "-lcudart", *extra]
     if verbose:
         print(" ".join(cmd), flush=True)
