@@ -25,8 +25,7 @@ namespace tao {
 namespace {
 
 constexpr int kSmem = 226 * 1024;
-constexpr int kXBytes = 96 * 1024;   // most of it that x takes
-constexpr int kMaxK = 65536;         // two rows' pieces of a cluster of 8's part fit kXBytes
+constexpr int kMaxK = 65536;  // two rows' pieces of a cluster of 8's part fit beside the rings
 
 struct Linear4Args {
   Four w;
@@ -112,7 +111,7 @@ template <class M, int GROUP, int NT>
 struct Form {
   static constexpr bool BYTES = std::is_same<M, Bytes>::value;
   static constexpr int COLS = BYTES ? 4 : 1, ROWS = 8 * NT / COLS, GROUPS = 128 / GROUP;
-  static constexpr int WARPS = 16, DEPTH = 6;
+  static constexpr int WARPS = 16, DEPTH = NT == 8 ? 3 : 6;
   static constexpr int UNITS = ROWS * 384, SUMS = UNITS + ROWS * 4 + ROWS * 4 % 8;
   static constexpr int XBLOCK = BYTES ? (SUMS + GROUPS * ROWS * 8 + 15) / 16 * 16 : ROWS * 256;
 };
@@ -348,12 +347,12 @@ Plan plan_of(int tiles, int kblocks, int rows, int xblock, int wring, int max_wa
   double least = 1e30;
   for (int shift = 0; shift <= 3; ++shift) {
     const int cluster = 1 << shift, kb = (kblocks + cluster - 1) / cluster, x = (kb * xblock + 127) / 128 * 128;
-    if (x > kXBytes || cluster > kblocks) continue;
+    if (cluster > kblocks) continue;
     // clusters that the device holds at once, with one block an SM
     const int clusters = shift == 0 ? 148 : shift == 1 ? 74 : shift == 2 ? 33 : 15;
     for (int warps = 4; warps <= max_warps; warps *= 2) {
       const int slot = warps * rows * 16 * 4;  // bytes of the warps' sums of a tile each
-      const int ring = warps * wring, most = (kSmem - x - ring) / slot;
+      const int ring = warps * wring, most = std::max(0, kSmem - x - ring) / slot;
       // every warp of a block has some of its k
       for (int wks = 0; 1 << wks <= std::min(warps, kblocks / cluster); ++wks) {
         const int groups = warps >> wks, sets = (tiles + groups - 1) / groups;
@@ -408,20 +407,19 @@ int launch(Linear4Args a, cudaStream_t s) {
   return e == cudaSuccess ? TAO_OK : lfail(TAO_ERR_CUDA, cudaGetErrorString(e));
 }
 
-template <class F>
-bool fits(const Linear4Args& a) {
-  return (a.kblocks + 7) / 8 * F::XBLOCK <= kXBytes;
-}
-
+// The bytes' form costs four columns a row and little else, the 16-bit one eight more instructions for
+// eight weights.  A form whose x does not fit a cluster of 8 blocks' shared memory leaves the product to the
+// next smaller one, which reads the weights again (from L2) for each of its row tiles.
 template <class M, bool BF16, int GROUP>
 int by_rows(const Linear4Args& a, cudaStream_t s) {
-  // The bytes' form costs four columns a row and little else, the 16-bit one eight more instructions for
-  // eight weights.  A form serves as many rows as a cluster of 8 blocks can hold.
-  if (a.rows <= 2 || !fits<Form<Bytes, GROUP, 2>>(a)) return launch<Bytes, BF16, GROUP, 1>(a, s);
-  if (a.rows <= 4 || !fits<Form<M, GROUP, 1>>(a)) return launch<Bytes, BF16, GROUP, 2>(a, s);
-  if (a.rows <= 8 || !fits<Form<M, GROUP, 2>>(a)) return launch<M, BF16, GROUP, 1>(a, s);
-  if (a.rows <= 16 || !fits<Form<M, GROUP, 4>>(a)) return launch<M, BF16, GROUP, 2>(a, s);
-  return launch<M, BF16, GROUP, 4>(a, s);
+  int rc = TAO_ERR_CAPACITY;
+  if (a.rows > 32) rc = launch<M, BF16, GROUP, 8>(a, s);
+  if (a.rows > 16 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 4>(a, s);
+  if (a.rows > 8 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 2>(a, s);
+  if (a.rows > 4 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 1>(a, s);
+  if (a.rows > 2 && rc == TAO_ERR_CAPACITY) rc = launch<Bytes, BF16, GROUP, 2>(a, s);
+  if (rc == TAO_ERR_CAPACITY) rc = launch<Bytes, BF16, GROUP, 1>(a, s);
+  return rc;
 }
 
 template <class M, bool BF16>

@@ -130,8 +130,8 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
     """x W^T + bias: x [..., k] in the weight's type, or in e4m3 with one fp32 scale a row
     (``x_scale`` [..., 1], as ``add_rms_norm_fp8`` gives them); returns [..., n] in the weight's type.
 
-    Made for few rows (a decode step's): the weight is read once for up to 32 rows, and from L2
-    for each 32 more.  No gradient."""
+    Made for few rows (a decode step's): the weight is read once for up to 64 rows, and from L2
+    for each 64 more.  No gradient."""
     if not isinstance(weight, Weight4) or len(weight.shape) != 2:
         raise ValueError("linear4 takes one Weight4 matrix")
     n, k = weight.shape

@@ -76,7 +76,8 @@ class _AddNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         y, s = _forward(x, weight, residual, eps)
         ctx.save_for_backward(s, weight)
-        ctx.eps, ctx.added = eps, residual is not None
+        ctx.added = residual is not None
+        ctx.fixed = x.shape[-1], TYPES[x.dtype], eps, x.device
         ctx.set_materialize_grads(False)
         return (y, s) if ctx.added else y
 
@@ -87,23 +88,27 @@ class _AddNorm(torch.autograd.Function):
         s, weight = ctx.saved_tensors
         if dy is None:  # only the stream was used
             return ds, None, ds if ctx.added else None, None
-        width, code, lib = s.shape[-1], TYPES[s.dtype], _lib.lib()
+        width, code, eps, device = ctx.fixed
+        lib = _lib.lib()
         rows, dy = _rows(s, width), _rows(dy, width)
+        count = rows.shape[0]
+        dx = _new(s)
+        ds_at = w_at = dw = dw_at = ws_at = None
+        ds_stride = size = 0
         if ds is not None:
             ds = _rows(ds, width)
+            ds_at, ds_stride = ds.data_ptr(), ds.stride(0)
         if weight is not None:
             weight = weight.contiguous()
-        dx = _new(s)
-        dw = ws = None
-        size = 0
-        if weight is not None and ctx.needs_input_grad[1]:
-            dw = torch.empty_like(weight)
-            size = lib.tao_add_rms_norm_workspace_bytes(rows.shape[0], width, code)
-            ws = _Room.get(s.device, size)
-        at = lambda t: None if t is None else t.data_ptr()
-        _lib.on_device(s.device.index, lib.tao_add_rms_norm_backward, dy.data_ptr(), dy.stride(0), at(ds),
-                       0 if ds is None else ds.stride(0), rows.data_ptr(), rows.stride(0), at(weight), rows.shape[0],
-                       width, code, ctx.eps, dx.data_ptr(), at(dw), at(ws), size)
+            w_at = weight.data_ptr()
+            if ctx.needs_input_grad[1]:
+                dw = torch.empty_like(weight)
+                size = lib.tao_add_rms_norm_workspace_bytes(count, width, code)
+                room = _Room.get(device, size)  # held until the launch
+                dw_at, ws_at = dw.data_ptr(), room.data_ptr()
+        _lib.on_device(device.index, lib.tao_add_rms_norm_backward, dy.data_ptr(), dy.stride(0), ds_at, ds_stride,
+                       rows.data_ptr(), rows.stride(0), w_at, count, width, code, eps, dx.data_ptr(), dw_at, ws_at,
+                       size)
         return dx, dw, dx if ctx.added else None, None
 
 
