@@ -503,6 +503,8 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
 int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_scale, const void* codes,
                 const void* scales, const void* zeros, int group, int type, const void* bias,
                 long long rows, int n, int k, void* y, void* stream);
+/* The current device's error word of tao_linear4 (a wait that ran out; more than 16 rows), read and cleared. */
+int tao_linear4_check(int* flags, void* stream);
 
 /* A mixture-of-experts layer: router [experts][width] bf16; gate and up [experts][inner][width] and
  * down [experts][width][inner], bf16 (group 0: strides in elements between experts and rows, the last

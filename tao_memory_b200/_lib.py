@@ -99,6 +99,7 @@ _SIGNATURES = {
     "tao_add_rms_norm_backward": (_I, [_VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I, _I, _F, _VP, _VP, _VP, _SZ,
                                        _VP]),
     "tao_linear4": (_I, [_VP, _I64, _I, _VP, _VP, _VP, _VP, _I, _I, _VP, _I64, _I, _I, _VP, _VP]),
+    "tao_linear4_check": (_I, [ctypes.POINTER(_I), _VP]),
     "tao_expert_workspace_bytes": (_SZ, [ctypes.POINTER(TaoExperts), _I]),
     "tao_expert_layer": (_I, [ctypes.POINTER(TaoExperts), _VP, _I64, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "tao_expert_check": (_I, [_VP, _SZ, ctypes.POINTER(_I), _VP]),

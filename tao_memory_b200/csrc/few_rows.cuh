@@ -212,16 +212,30 @@ struct Block4 {
     }
   }
 
+  // Operand registers of 32-k part u as 16-bit floats, code - zero: of the first four k of a lane's eight
+  // and of the last four; register r is row half r & 1, elements (0, 1) or (2, 3).
+  template <class M>
+  TAO_DEVI void operands16(int u, uint32_t (&a)[2][4]) const {
+    // -(magic + zero) in both halves: the zero's byte below the magic's with its sign
+    const uint32_t zz = zeros(u / PARTS);
+    const uint32_t z0 = __byte_perm(zz, M::kMagic >> 24 | 0x80, 0x4040);
+    const uint32_t z1 = __byte_perm(zz, M::kMagic >> 24 | 0x80, 0x4141);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        uint32_t v;
+        asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(v) : "r"(word(u, i) >> (4 * r)), "r"(M::kMagic));
+        a[i][r] = M::add(v, r & 1 ? z1 : z0);
+      }
+  }
+
   // Adds D of the block's product with eight rows of x for each of NT column tiles, those that hold some
   // of the `cols` rows.  `b(u, n)`: the lane's 8 activations of 32-k part u.
   template <class M, bool BF16_SCALES, int NT, class B>
   TAO_DEVI void product16(float (&acc)[NT][4], int cols, B b) const {
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) {
-      // -(magic + zero) in both halves: the zero's byte below the magic's with its sign
-      const uint32_t zz = zeros(j);
-      const uint32_t z0 = __byte_perm(zz, M::kMagic >> 24 | 0x80, 0x4040);
-      const uint32_t z1 = __byte_perm(zz, M::kMagic >> 24 | 0x80, 0x4141);
       // two chains of dependent products, or as many as there are column tiles
       constexpr int CHAINS = NT == 1 ? 2 : 1;
       float d[NT * CHAINS][4];
@@ -231,15 +245,7 @@ struct Block4 {
       for (int p = 0; p < PARTS; ++p) {
         const int u = j * PARTS + p;
         uint32_t a[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            // register r: row half r & 1, elements (0, 1) or (2, 3)
-            uint32_t v;
-            asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(v) : "r"(word(u, i) >> (4 * r)), "r"(M::kMagic));
-            a[i][r] = M::add(v, r & 1 ? z1 : z0);
-          }
+        operands16<M>(u, a);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (n && n * 8 >= cols) break;

@@ -3,7 +3,8 @@
 //   W[n][k] = (code[n][k] - zero[n][k / group]) scale[n][k / group],  codes 0..15
 //
 // x in bf16 or fp16, or in e4m3 with one fp32 scale a row; y in the type of the weight's scales.
-// How the product is formed: few_rows.cuh.  Sums are in fp32, y is rounded once.
+// How the product is formed: few_rows.cuh for up to 16 rows, which this file is about; linear4_tc.cuh for
+// more.  Sums are in fp32, y is rounded once.
 //
 // Bound by the codes' bytes, half a byte a weight.  One block an SM.  x, or a cluster's block's part of its
 // k, is laid out in shared memory once, in the order of the mma's operands.  The warps are WT x WK: WT row
@@ -17,7 +18,7 @@
 #include <type_traits>
 
 #include "../../include/tao_b200.h"
-#include "few_rows.cuh"
+#include "linear4_tc.cuh"
 
 void tao_set_last_error(const char* msg);
 
@@ -26,80 +27,6 @@ namespace {
 
 constexpr int kSmem = 226 * 1024;
 constexpr int kMaxK = 65536;  // two rows' pieces of a cluster of 8's part fit beside the rings
-
-struct Linear4Args {
-  Four w;
-  const void* x;
-  long long x_stride;
-  const float* x_scale;  // one a row, or null
-  const void* bias;
-  void* y;
-  int rows, n, k;
-  int tiles, kblocks;
-  int shift, wk_shift;  // log2 of a cluster's blocks, of a tile's warps
-  int ring, sums;   // where the rings and the sums start in shared memory
-  int steps;        // row tiles of a warp
-  int x_type;
-  bool wide;        // rows of x start on 16 (e4m3: 8) bytes and k is whole chunks of 8
-};
-
-TAO_DEVI uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-TAO_DEVI void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-TAO_DEVI float4 ld_cluster(uint32_t at, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n .reg .u32 p;\n mapa.shared::cluster.u32 p, %4, %5;\n ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [p];\n}"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(at), "r"(rank)
-      : "memory");
-  return v;
-}
-
-// Eight activations of a row from k on (e4m3: in the first two words); zeros beyond its end.
-TAO_DEVI uint4 chunk_of(const Linear4Args& a, long long m, int k) {
-  const long long at = m * a.x_stride + k;
-  uint32_t w[4] = {};
-  if (a.x_type == TAO_TYPE_E4M3) {
-    const uint8_t* p = static_cast<const uint8_t*>(a.x) + at;
-    if (a.wide) {
-      if (k < a.k) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x, w[1] = v.y;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < a.k) w[i / 4] |= (uint32_t)__ldg(p + i) << (8 * (i & 3));
-    }
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
-    if (a.wide) {
-      if (k < a.k) return __ldg(reinterpret_cast<const uint4*>(p));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < a.k) w[i / 2] |= (uint32_t)__ldg(p + i) << (16 * (i & 1));
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// ... as pairs of fp16 (from e4m3).
-TAO_DEVI uint4 widen_e4m3(uint4 v) {
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t q = (i < 2 ? v.x : v.y) >> (16 * (i & 1)) & 0xffff;
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q, __NV_E4M3);
-    h[i] = r.x | (uint32_t)r.y << 16;
-  }
-  return make_uint4(h[0], h[1], h[2], h[3]);
-}
 
 // The two forms of the product: signed bytes (4 columns a row), or the 16-bit type M (one).
 struct Bytes {};
@@ -111,7 +38,7 @@ template <class M, int GROUP, int NT>
 struct Form {
   static constexpr bool BYTES = std::is_same<M, Bytes>::value;
   static constexpr int COLS = BYTES ? 4 : 1, ROWS = 8 * NT / COLS, GROUPS = 128 / GROUP;
-  static constexpr int WARPS = 16, DEPTH = NT == 8 ? 3 : 6;
+  static constexpr int WARPS = 16, DEPTH = 6;
   static constexpr int UNITS = ROWS * 384, SUMS = UNITS + ROWS * 4 + ROWS * 4 % 8;
   static constexpr int XBLOCK = BYTES ? (SUMS + GROUPS * ROWS * 8 + 15) / 16 * 16 : ROWS * 256;
 };
@@ -371,6 +298,35 @@ Plan plan_of(int tiles, int kblocks, int rows, int xblock, int wring, int max_wa
   return best;
 }
 
+// Launches KERNEL in clusters of 2^a.shift blocks; what it may use of shared memory is set once for each of
+// the first 64 devices.
+template <void (*KERNEL)(Linear4Args)>
+int start(const Linear4Args& a, dim3 grid, int threads, int smem, int most_smem, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t mark = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & mark)) {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem);
+    if (e == cudaSuccess) ready |= mark;
+  }
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1 << a.shift;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    c.attrs = attr;
+    c.numAttrs = a.shift ? 1 : 0;
+    e = cudaLaunchKernelEx(&c, KERNEL, a);
+  }
+  return e == cudaSuccess ? TAO_OK : lfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
 template <class M, bool BF16, int GROUP, int NT>
 int launch(Linear4Args a, cudaStream_t s) {
   using F = Form<M, GROUP, NT>;
@@ -381,30 +337,26 @@ int launch(Linear4Args a, cudaStream_t s) {
   a.steps = p.steps;
   a.ring = p.ring;
   a.sums = p.sums;
-  auto kernel = linear4_kernel<M, BF16, GROUP, NT>;
-  static std::atomic<uint64_t> ready{0};  // devices (the first 64) on which the kernel may use its shared memory
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  const uint64_t mark = device < 64 ? 1ull << device : 0;
-  if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & mark)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (e == cudaSuccess) ready |= mark;
+  return start<linear4_kernel<M, BF16, GROUP, NT>>(a, dim3(p.blocks, (a.rows + F::ROWS - 1) / F::ROWS), p.warps * 32,
+                                                   p.smem, kSmem, s);
+}
+
+// Blocks of 128 rows of W, a cluster of them for as many parts of k as the device has room for.
+template <class M, bool BF16, int GROUP>
+int launch_tc(Linear4Args a, cudaStream_t s) {
+  using C = Linear4Tc<GROUP>;
+  const int sets = (a.tiles + 7) / 8, passes = (a.rows + C::COLS - 1) / C::COLS;
+  double least = 1e30;
+  for (int shift = 0; shift <= 3 && 1 << shift <= a.kblocks; ++shift) {
+    const int clusters = shift == 0 ? 148 : shift == 1 ? 74 : shift == 2 ? 33 : 15;
+    const int waves = (sets * passes + clusters - 1) / clusters, kb = (a.kblocks + (1 << shift) - 1) >> shift;
+    const double cost = waves * (kb * 0.25 + 2. + (shift ? 1. : 0.));  // us, roughly
+    if (cost < least) {
+      least = cost;
+      a.shift = shift;
+    }
   }
-  if (e == cudaSuccess) {
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(p.blocks, (a.rows + F::ROWS - 1) / F::ROWS);
-    c.blockDim = dim3(p.warps * 32);
-    c.dynamicSmemBytes = p.smem;
-    c.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1 << p.shift;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    c.attrs = attr;
-    c.numAttrs = p.shift ? 1 : 0;
-    e = cudaLaunchKernelEx(&c, kernel, a);
-  }
-  return e == cudaSuccess ? TAO_OK : lfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+  return start<linear4_tc_kernel<M, BF16, GROUP>>(a, dim3(sets << a.shift, passes), C::THREADS, C::SMEM, C::SMEM, s);
 }
 
 // The bytes' form costs four columns a row and little else, the 16-bit one eight more instructions for
@@ -412,10 +364,9 @@ int launch(Linear4Args a, cudaStream_t s) {
 // next smaller one, which reads the weights again (from L2) for each of its row tiles.
 template <class M, bool BF16, int GROUP>
 int by_rows(const Linear4Args& a, cudaStream_t s) {
+  if (a.rows > 16) return launch_tc<M, BF16, GROUP>(a, s);
   int rc = TAO_ERR_CAPACITY;
-  if (a.rows > 32) rc = launch<M, BF16, GROUP, 8>(a, s);
-  if (a.rows > 16 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 4>(a, s);
-  if (a.rows > 8 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 2>(a, s);
+  if (a.rows > 8) rc = launch<M, BF16, GROUP, 2>(a, s);
   if (a.rows > 4 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 1>(a, s);
   if (a.rows > 2 && rc == TAO_ERR_CAPACITY) rc = launch<Bytes, BF16, GROUP, 2>(a, s);
   if (rc == TAO_ERR_CAPACITY) rc = launch<Bytes, BF16, GROUP, 1>(a, s);
@@ -473,6 +424,22 @@ int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_sc
     if (rc) return rc;
   }
   return TAO_OK;
+}
+
+int tao_linear4_check(int* flags, void* stream) {
+  using namespace tao;
+  int host = 0;
+  const int none = 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&host, g_linear4_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && host) {
+    e = cudaMemcpyToSymbolAsync(g_linear4_error, &none, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  if (e != cudaSuccess) return lfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+  if (flags) *flags = host;
+  return host ? lfail(TAO_ERR_DEVICE, "a 4-bit product waited too long for the tensor cores") : TAO_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,211 @@
+// The 4-bit product of more than a few rows (up to 64 at a time) on tcgen05: with 17 rows and more the
+// legacy mma and its operand loads take several times as long as the weights' bytes.
+//
+// A block computes 128 rows of W (8 row tiles, one a warp) against 64 rows of x over its k, a cluster's
+// blocks a part of k each.  Per 128 k:  a warp makes 16-bit floats (code - zero, exact) of its tile's codes
+// and writes them to the A operand (K-major, 128-byte swizzle, two buffers); one thread issues the
+// 8 products of 16 k into TMEM, an accumulator of its own for each scale group (two sets); and while those
+// run, the block before's accumulators are read, scaled and added in fp32 registers, row and column half
+// a thread.  So no weight is rounded and every sum's order is fixed.  x comes by cp.async into five slots of
+// the B operand, codes into eight of a ring: both are a block's whole latency ahead.
+#pragma once
+#include "linear4.cuh"
+#include "tcgen05.cuh"
+
+namespace tao {
+
+static __device__ int g_linear4_error;  // an expired wait, until tao_linear4_check
+
+template <int GROUP>
+struct Linear4Tc {
+  static constexpr int THREADS = 256, COLS = 64, GROUPS = 128 / GROUP;
+  static constexpr int A = 128 * 256, X = COLS * 256, XSLOTS = 5, CODES = 8 * Block4<GROUP>::BYTES, CSLOTS = 8;
+  static constexpr int TMEM = 2 * GROUPS * COLS;
+  static constexpr int SMEM = 1024 + 2 * A + XSLOTS * X + CSLOTS * CODES + 64;
+  static_assert(SMEM <= 227 * 1024, "");
+};
+
+// M: the operands' type.  BF16: the type of scales, bias and y.
+template <class M, bool BF16, int GROUP>
+__global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a) {
+  using namespace tc;
+  using C = Linear4Tc<GROUP>;
+  using B4 = Block4<GROUP>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  uint8_t *const sA = sm, *const sX = sm + 2 * C::A, *const sC = sX + C::XSLOTS * C::X;
+  uint64_t* const bar = reinterpret_cast<uint64_t*>(sC + C::CSLOTS * C::CODES);  // of each set of accumulators
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bar + 2);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int m0 = blockIdx.y * C::COLS, rows = min(a.rows - m0, C::COLS);
+  const int rank = a.shift ? (int)cluster_rank() : 0, tile0 = (blockIdx.x >> a.shift) * 8;
+  const int k0 = a.kblocks * rank >> a.shift, nb = (a.kblocks * (rank + 1) >> a.shift) - k0;
+  const bool has_zeros = a.w.zeros != nullptr;
+  const bool copied = a.wide && a.x_type != TAO_TYPE_E4M3;
+
+  // this warp's row tile (one beyond the matrix repeats the last), and the row whose sums this thread adds
+  const uint32_t first = (uint32_t)min(tile0 + warp, a.tiles - 1) * a.kblocks + k0;
+  uint8_t* const my_codes = sC + warp * B4::BYTES;
+  const int r = (warp & 3) * 32 + lane, half = warp >> 2;
+  const uint16_t* scale_at = reinterpret_cast<const uint16_t*>(a.w.scales) +
+                             ((uint64_t)min(tile0 + r / 16, a.tiles - 1) * a.kblocks + k0) * (16 * C::GROUPS) +
+                             (r & 7) * (2 * C::GROUPS) + (r >> 3 & 1);
+
+  // chunk c of 8 k of x row m of block kb: its place in a slot
+  auto place = [&](int m, int c) { return (c >> 3) * (C::COLS * 128) + m * 128 + (((c & 7) ^ (m & 7)) << 4); };
+  auto copy = [&](int codes_kb, int x_kb) {
+    if (codes_kb < nb) B4::issue(smem_u32(my_codes + codes_kb % C::CSLOTS * C::CODES), a.w, first + codes_kb, lane);
+    if (copied && x_kb >= 0 && x_kb < nb) {
+      const uint16_t* x = static_cast<const uint16_t*>(a.x) + (long long)m0 * a.x_stride;
+      const uint32_t to = smem_u32(sX + x_kb % C::XSLOTS * C::X);
+      for (int i = tid; i < rows * 16; i += C::THREADS) {
+        const int m = i >> 4, c = i & 15, k = (k0 + x_kb) * 128 + c * 8;
+        cp_async16(to + place(m, c), k < a.k ? x + m * a.x_stride + k : x, k < a.k);
+      }
+    }
+    cp_commit();
+  };
+  uint4 ahead[4];  // x that needs work on its way, a block ahead
+  auto fetch = [&](int kb) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid + j * C::THREADS;
+      if (!copied && kb < nb && i < rows * 16) ahead[j] = chunk_of(a, m0 + (i >> 4), (k0 + kb) * 128 + (i & 15) * 8);
+    }
+  };
+  for (int j = -7; j < 0; ++j) copy(j + 7, j + 4);
+  fetch(0);
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 0) {
+    mbar_init(&bar[0], 1);
+    mbar_init(&bar[1], 1);
+    fence_mbar_init();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tbase = *tmem_slot;
+
+  float acc[32] = {};
+  float scale[C::GROUPS], scale_before[C::GROUPS];
+  bool ok = true;  // after a wait that ran out nothing more is waited for
+  // adds block kb's accumulators
+  auto add = [&](int kb) {
+    if (ok) ok = mbar_wait(&bar[kb & 1], kb >> 1 & 1, &g_linear4_error);
+    __syncwarp();
+    fence_after();
+#pragma unroll
+    for (int j = 0; j < C::GROUPS; ++j) {
+      float v[32];
+      tmem_ld32(tbase + ((uint32_t)((warp & 3) * 32) << 16) + ((kb & 1) * C::GROUPS + j) * C::COLS + half * 32, v);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[i] += scale_before[j] * v[i];
+    }
+    fence_before();
+  };
+
+#pragma unroll 1
+  for (int kb = 0; kb < nb; ++kb) {
+    cp_wait<3>();  // this block's codes and x; younger groups may be open
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < C::GROUPS; ++j) {
+      scale_before[j] = scale[j];
+      const uint32_t bits = __ldg(scale_at + (uint64_t)kb * (16 * C::GROUPS) + j * 2);
+      scale[j] = BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
+    }
+    // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k
+    B4 b;
+    b.load(my_codes + kb % C::CSLOTS * C::CODES, has_zeros, lane);
+    uint8_t* const to = sA + (kb & 1) * C::A + (warp * 16 + g) * 128;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t v[2][4];
+      b.template operands16<M>(u, v);
+      uint8_t* const at = to + (u >> 1) * (C::A / 2) + ((((u & 1) * 4 + t) ^ g) << 4);
+      *reinterpret_cast<uint4*>(at) = make_uint4(v[0][0], v[0][2], v[1][0], v[1][2]);
+      *reinterpret_cast<uint4*>(at + 8 * 128) = make_uint4(v[0][1], v[0][3], v[1][1], v[1][3]);
+    }
+    if (!copied) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = tid + j * C::THREADS;
+        if (i < rows * 16)
+          *reinterpret_cast<uint4*>(sX + kb % C::XSLOTS * C::X + place(i >> 4, i & 15)) =
+              a.x_type == TAO_TYPE_E4M3 ? widen_e4m3(ahead[j]) : ahead[j];
+      }
+      fetch(kb + 1);
+    }
+    fence_proxy_async();
+    fence_before();
+    __syncthreads();
+    if (tid == 0) {
+      fence_after();
+      constexpr uint32_t TYPE = std::is_same<M, MmaBf16>::value ? 1u << 7 | 1u << 10 : 0u;  // bf16, or fp16
+      constexpr uint32_t I = (idesc_bf16(128, C::COLS, 0, 0) & ~(1u << 7 | 1u << 10)) | TYPE;
+      const uint32_t pa = smem_u32(sA + (kb & 1) * C::A), px = smem_u32(sX + kb % C::XSLOTS * C::X);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        tc::mma(tbase + ((kb & 1) * C::GROUPS + k * 16 / GROUP) * C::COLS,
+                sdesc(pa + (k >> 2) * (C::A / 2) + (k & 3) * 32, 16, 1024),
+                sdesc(px + (k >> 2) * (C::X / 2) + (k & 3) * 32, 16, 1024), I, k * 16 % GROUP ? 1u : 0u);
+      commit(&bar[kb & 1]);
+    }
+    __syncwarp();
+    if (kb > 0) add(kb - 1);
+    copy(kb + 7, kb + 4);  // into the slots of block kb - 1, whose product is over
+  }
+#pragma unroll
+  for (int j = 0; j < C::GROUPS; ++j) scale_before[j] = scale[j];
+  add(nb - 1);
+  if (!ok) mbar_wait(&bar[(nb - 1) & 1], (nb - 1) >> 1 & 1, nullptr);  // what is in flight has its time before it ends
+  cp_wait<0>();
+  fence_before();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
+
+  using T = std::conditional_t<BF16, bf16, __half>;
+  const T* bias = static_cast<const T*>(a.bias);
+  auto put = [&](int m, int n, float o) {
+    if (a.x_scale) o *= a.x_scale[m0 + m];
+    T* y = static_cast<T*>(a.y) + (long long)(m0 + m) * a.n + n;
+    if constexpr (BF16)
+      *y = tobf(o + (bias ? bf(bias[n]) : 0.f));
+    else
+      *y = __float2half_rn(o + (bias ? __half2float(bias[n]) : 0.f));
+  };
+  const int n0 = tile0 * 16;
+  if (!a.shift) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (half * 32 + i < rows && n0 + r < a.n) put(half * 32 + i, n0 + r, acc[i]);
+    return;
+  }
+  float* sums = reinterpret_cast<float*>(sm);  // [column][128 rows], over the operands
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sums[(half * 32 + i) * 128 + r] = acc[i];
+  cluster_sync();
+  for (int i = (((warp << a.shift) + rank) << 5) + lane; i < rows * 32; i += C::THREADS << a.shift) {
+    const int m = i >> 5, n = n0 + (i & 31) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < 1 << a.shift; ++q) {
+      const float4 v = ld_cluster(smem_u32(sums + m * 128 + (i & 31) * 4), q);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float o[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.n) put(m, n + e, o[e]);
+  }
+  cluster_sync();  // the others' reads of these sums are over
+}
+
+}  // namespace tao

@@ -842,6 +842,8 @@ def check_device(device=None):
         total |= flags.value
     from .experts import check_workspaces
     check_workspaces(dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().tao_linear4_check(None, current))
     return total
 
 
