@@ -36,6 +36,9 @@ namespace tao {
 TAO_DEVI void cp_async16(uint32_t to, const void* from, bool in = true) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
 }
+TAO_DEVI void cp_async8(uint32_t to, const void* from, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(in ? 8 : 0) : "memory");
+}
 TAO_DEVI void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int OPEN>
 TAO_DEVI void cp_wait() {
@@ -158,6 +161,14 @@ struct Block4 {
 #pragma unroll
     for (int i = 0; i < (GROUPS + 1) / 2; ++i)
       z[i] = !has_zeros ? 0x08080808u : GROUPS == 1 ? zp[0] : reinterpret_cast<const uint32_t*>(zp)[i];
+  }
+  // Exchanges 32-k parts 0 and 1, 2 and 3, the zero points with them.
+  TAO_DEVI void swap_parts() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      c[i] = make_uint4(c[i].z, c[i].w, c[i].x, c[i].y);
+      if constexpr (GROUP == 32) z[i] = z[i] >> 16 | z[i] << 16;
+    }
   }
   TAO_DEVI uint32_t zeros(int j) const { return z[j / 2] >> (16 * (j & 1)); }  // of rows g, g + 8, a byte each
   template <bool BF16_SCALES>

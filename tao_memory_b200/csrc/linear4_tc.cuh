@@ -7,7 +7,8 @@
 // 8 products of 16 k into TMEM, an accumulator of its own for each scale group (two sets); and while those
 // run, the block before's accumulators are read, scaled and added in fp32 registers, row and column half
 // a thread.  So no weight is rounded and every sum's order is fixed.  x comes by cp.async into five slots of
-// the B operand, codes into eight of a ring: both are a block's whole latency ahead.
+// the B operand, codes and scales into eight of a ring: both are
+// a memory's whole latency ahead.
 #pragma once
 #include "linear4.cuh"
 #include "tcgen05.cuh"
@@ -20,6 +21,7 @@ template <int GROUP>
 struct Linear4Tc {
   static constexpr int THREADS = 256, COLS = 64, GROUPS = 128 / GROUP;
   static constexpr int A = 128 * 256, X = COLS * 256, XSLOTS = 5, CODES = 8 * Block4<GROUP>::BYTES, CSLOTS = 8;
+  static constexpr int RAW = 6;  // slots of x as e4m3
   static constexpr int TMEM = 2 * GROUPS * COLS;
   static constexpr int SMEM = 1024 + 2 * A + XSLOTS * X + CSLOTS * CODES + 64;
   static_assert(SMEM <= 227 * 1024, "");
@@ -42,40 +44,46 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
   const int rank = a.shift ? (int)cluster_rank() : 0, tile0 = (blockIdx.x >> a.shift) * 8;
   const int k0 = a.kblocks * rank >> a.shift, nb = (a.kblocks * (rank + 1) >> a.shift) - k0;
   const bool has_zeros = a.w.zeros != nullptr;
-  const bool copied = a.wide && a.x_type != TAO_TYPE_E4M3;
 
   // this warp's row tile (one beyond the matrix repeats the last), and the row whose sums this thread adds
   const uint32_t first = (uint32_t)min(tile0 + warp, a.tiles - 1) * a.kblocks + k0;
   uint8_t* const my_codes = sC + warp * B4::BYTES;
   const int r = (warp & 3) * 32 + lane, half = warp >> 2;
-  const uint16_t* scale_at = reinterpret_cast<const uint16_t*>(a.w.scales) +
-                             ((uint64_t)min(tile0 + r / 16, a.tiles - 1) * a.kblocks + k0) * (16 * C::GROUPS) +
-                             (r & 7) * (2 * C::GROUPS) + (r >> 3 & 1);
+  const uint8_t* const scales = sC + r / 16 * B4::BYTES + 1024 + (r & 7) * (4 * C::GROUPS) + (r >> 3 & 1) * 2;
 
-  // chunk c of 8 k of x row m of block kb: its place in a slot
-  auto place = [&](int m, int c) { return (c >> 3) * (C::COLS * 128) + m * 128 + (((c & 7) ^ (m & 7)) << 4); };
+  // This thread brings chunk c of 8 k of rows m, m + 16, m + 32, m + 48 of x to `place` and 16 rows on in a slot
+  // of the B operand.  e4m3 is widened on its way, from a ring of raw chunks in the last three slots' room.
+  const int m = tid >> 4, c = tid & 15;
+  const uint32_t place = (c >> 3) * (C::COLS * 128) + m * 128 + (((c & 7) ^ (m & 7)) << 4);
+  const bool copied = a.wide && a.x_type != TAO_TYPE_E4M3, staged = a.wide && a.x_type == TAO_TYPE_E4M3;
+  const long long x_at = (long long)(m0 + m) * a.x_stride + k0 * 128 + c * 8;
+  const uint8_t* const x = static_cast<const uint8_t*>(a.x) + (staged ? x_at : x_at * 2);
+  const long long x_step = (staged ? 16 : 32) * a.x_stride;  // of 16 rows, in bytes
+  uint8_t* const sRaw = sX + 2 * C::X + tid * 8;
+  auto x_slot = [&](int kb) { return sX + (copied ? kb % C::XSLOTS : kb & 1) * C::X; };
   auto copy = [&](int codes_kb, int x_kb) {
     if (codes_kb < nb) B4::issue(smem_u32(my_codes + codes_kb % C::CSLOTS * C::CODES), a.w, first + codes_kb, lane);
-    if (copied && x_kb >= 0 && x_kb < nb) {
-      const uint16_t* x = static_cast<const uint16_t*>(a.x) + (long long)m0 * a.x_stride;
-      const uint32_t to = smem_u32(sX + x_kb % C::XSLOTS * C::X);
-      for (int i = tid; i < rows * 16; i += C::THREADS) {
-        const int m = i >> 4, c = i & 15, k = (k0 + x_kb) * 128 + c * 8;
-        cp_async16(to + place(m, c), k < a.k ? x + m * a.x_stride + k : x, k < a.k);
+    if (x_kb >= 0 && x_kb < nb) {
+      const bool in = (k0 + x_kb) * 128 + c * 8 < a.k;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (m + 16 * j >= rows) break;
+        if (copied)
+          cp_async16(smem_u32(x_slot(x_kb) + place + j * 16 * 128), in ? x + x_kb * 256 + j * x_step : x, in);
+        else if (staged)
+          cp_async8(smem_u32(sRaw + x_kb % C::RAW * (C::X / 2) + j * 2048), in ? x + x_kb * 128 + j * x_step : x, in);
       }
     }
     cp_commit();
   };
-  uint4 ahead[4];  // x that needs work on its way, a block ahead
+  uint4 ahead[4];  // x off its alignment, a block ahead
   auto fetch = [&](int kb) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid + j * C::THREADS;
-      if (!copied && kb < nb && i < rows * 16) ahead[j] = chunk_of(a, m0 + (i >> 4), (k0 + kb) * 128 + (i & 15) * 8);
-    }
+    for (int j = 0; j < 4; ++j)
+      if (kb < nb && m + 16 * j < rows) ahead[j] = chunk_of(a, m0 + m + 16 * j, (k0 + kb) * 128 + c * 8);
   };
-  for (int j = -7; j < 0; ++j) copy(j + 7, j + 4);
-  fetch(0);
+  for (int j = -6; j < 0; ++j) copy(j + 6, j + 4);
+  if (!a.wide) fetch(0);
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -93,7 +101,6 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
   const uint32_t tbase = *tmem_slot;
 
   float acc[32] = {};
-  float scale[C::GROUPS], scale_before[C::GROUPS];
   bool ok = true;  // after a wait that ran out nothing more is waited for
   // adds block kb's accumulators
   auto add = [&](int kb) {
@@ -102,10 +109,12 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
     fence_after();
 #pragma unroll
     for (int j = 0; j < C::GROUPS; ++j) {
+      const uint16_t bits = *reinterpret_cast<const uint16_t*>(scales + kb % C::CSLOTS * C::CODES + j * 4);
+      const float s = BF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
       float v[32];
       tmem_ld32(tbase + ((uint32_t)((warp & 3) * 32) << 16) + ((kb & 1) * C::GROUPS + j) * C::COLS + half * 32, v);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) acc[i] += scale_before[j] * v[i];
+      for (int i = 0; i < 32; ++i) acc[i] += s * v[i];
     }
     fence_before();
   };
@@ -114,33 +123,33 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
   for (int kb = 0; kb < nb; ++kb) {
     cp_wait<3>();  // this block's codes and x; younger groups may be open
     __syncwarp();
-#pragma unroll
-    for (int j = 0; j < C::GROUPS; ++j) {
-      scale_before[j] = scale[j];
-      const uint32_t bits = __ldg(scale_at + (uint64_t)kb * (16 * C::GROUPS) + j * 2);
-      scale[j] = BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
-    }
-    // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k
+    // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k; odd rows' lanes take the parts of 64 k in the
+    // other order, so that 8 lanes write to all banks
     B4 b;
     b.load(my_codes + kb % C::CSLOTS * C::CODES, has_zeros, lane);
+    const int odd = g & 1;
+    if (odd) b.swap_parts();
     uint8_t* const to = sA + (kb & 1) * C::A + (warp * 16 + g) * 128;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       uint32_t v[2][4];
       b.template operands16<M>(u, v);
-      uint8_t* const at = to + (u >> 1) * (C::A / 2) + ((((u & 1) * 4 + t) ^ g) << 4);
+      uint8_t* const at = to + (u >> 1) * (C::A / 2) + (((((u & 1) ^ odd) * 4 + t) ^ g) << 4);
       *reinterpret_cast<uint4*>(at) = make_uint4(v[0][0], v[0][2], v[1][0], v[1][2]);
       *reinterpret_cast<uint4*>(at + 8 * 128) = make_uint4(v[0][1], v[0][3], v[1][1], v[1][3]);
     }
     if (!copied) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int i = tid + j * C::THREADS;
-        if (i < rows * 16)
-          *reinterpret_cast<uint4*>(sX + kb % C::XSLOTS * C::X + place(i >> 4, i & 15)) =
-              a.x_type == TAO_TYPE_E4M3 ? widen_e4m3(ahead[j]) : ahead[j];
+        if (m + 16 * j >= rows) break;
+        uint4 v = ahead[j];
+        if (staged) {
+          const uint2 raw = *reinterpret_cast<const uint2*>(sRaw + kb % C::RAW * (C::X / 2) + j * 2048);
+          v.x = raw.x, v.y = raw.y;
+        }
+        if (a.x_type == TAO_TYPE_E4M3) v = widen_e4m3(v);
+        *reinterpret_cast<uint4*>(x_slot(kb) + place + j * 16 * 128) = v;
       }
-      fetch(kb + 1);
     }
     fence_proxy_async();
     fence_before();
@@ -149,7 +158,7 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
       fence_after();
       constexpr uint32_t TYPE = std::is_same<M, MmaBf16>::value ? 1u << 7 | 1u << 10 : 0u;  // bf16, or fp16
       constexpr uint32_t I = (idesc_bf16(128, C::COLS, 0, 0) & ~(1u << 7 | 1u << 10)) | TYPE;
-      const uint32_t pa = smem_u32(sA + (kb & 1) * C::A), px = smem_u32(sX + kb % C::XSLOTS * C::X);
+      const uint32_t pa = smem_u32(sA + (kb & 1) * C::A), px = smem_u32(x_slot(kb));
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         tc::mma(tbase + ((kb & 1) * C::GROUPS + k * 16 / GROUP) * C::COLS,
@@ -158,11 +167,10 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
       commit(&bar[kb & 1]);
     }
     __syncwarp();
+    if (!a.wide) fetch(kb + 1);
     if (kb > 0) add(kb - 1);
-    copy(kb + 7, kb + 4);  // into the slots of block kb - 1, whose product is over
+    copy(kb + 6, kb + 4);  // into the slots of blocks kb - 2, whose scales are used, and kb - 1, whose product is over
   }
-#pragma unroll
-  for (int j = 0; j < C::GROUPS; ++j) scale_before[j] = scale[j];
   add(nb - 1);
   if (!ok) mbar_wait(&bar[(nb - 1) & 1], (nb - 1) >> 1 & 1, nullptr);  // what is in flight has its time before it ends
   cp_wait<0>();
