@@ -3,7 +3,7 @@
 //
 // A block computes 128 rows of W (8 row tiles, one a warp) against 64 rows of x over its k, a cluster's
 // blocks a part of k each.  Per 128 k:  a warp makes 16-bit floats (code - zero, exact) of its tile's codes
-// and writes them to the A operand (K-major, 128-byte swizzle, two buffers); one thread issues the
+// and writes them to the A operand (K-major, 128-byte swizzle, two buffers); a ninth issues the
 // 8 products of 16 k into TMEM, an accumulator of its own for each scale group (two sets); and while those
 // run, the block before's accumulators are read, scaled and added in fp32 registers, row and column half
 // a thread.  So no weight is rounded and every sum's order is fixed.  x comes by cp.async into five slots of
@@ -17,9 +17,16 @@ namespace tao {
 
 static __device__ int g_linear4_error;  // an expired wait, until tao_linear4_check
 
+// One lane of a warp that has met, the same for all that ask.
+TAO_DEVI bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
 template <int GROUP>
 struct Linear4Tc {
-  static constexpr int THREADS = 256, COLS = 64, GROUPS = 128 / GROUP;
+  static constexpr int WORKERS = 8, THREADS = 32 * (WORKERS + 1), COLS = 64, GROUPS = 128 / GROUP;
   static constexpr int A = 128 * 256, X = COLS * 256, XSLOTS = 5, CODES = 8 * Block4<GROUP>::BYTES, CSLOTS = 8;
   static constexpr int RAW = 6;  // slots of x as e4m3
   static constexpr int TMEM = 2 * GROUPS * COLS;
@@ -29,7 +36,7 @@ struct Linear4Tc {
 
 // M: the operands' type.  BF16: the type of scales, bias and y.
 template <class M, bool BF16, int GROUP>
-__global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a) {
+__global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kernel(const Linear4Args a) {
   using namespace tc;
   using C = Linear4Tc<GROUP>;
   using B4 = Block4<GROUP>;
@@ -82,8 +89,10 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
     for (int j = 0; j < 4; ++j)
       if (kb < nb && m + 16 * j < rows) ahead[j] = chunk_of(a, m0 + m + 16 * j, (k0 + kb) * 128 + c * 8);
   };
-  for (int j = -6; j < 0; ++j) copy(j + 6, j + 4);
-  if (!a.wide) fetch(0);
+  if (warp < C::WORKERS) {
+    for (int j = -6; j < 0; ++j) copy(j + 6, j + 4);
+    if (!a.wide) fetch(0);
+  }
 
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -119,60 +128,69 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
     fence_before();
   };
 
+  // one barrier a block: its operands are written, and what it overwrites has been read
+  if (warp == C::WORKERS) {
+    constexpr uint32_t TYPE = std::is_same<M, MmaBf16>::value ? 1u << 7 | 1u << 10 : 0u;  // bf16, or fp16
+    constexpr uint32_t I = (idesc_bf16(128, C::COLS, 0, 0) & ~(1u << 7 | 1u << 10)) | TYPE;
 #pragma unroll 1
-  for (int kb = 0; kb < nb; ++kb) {
-    cp_wait<3>();  // this block's codes and x; younger groups may be open
-    __syncwarp();
-    // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k; odd rows' lanes take the parts of 64 k in the
-    // other order, so that 8 lanes write to all banks
-    B4 b;
-    b.load(my_codes + kb % C::CSLOTS * C::CODES, has_zeros, lane);
-    const int odd = g & 1;
-    if (odd) b.swap_parts();
-    uint8_t* const to = sA + (kb & 1) * C::A + (warp * 16 + g) * 128;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint32_t v[2][4];
-      b.template operands16<M>(u, v);
-      uint8_t* const at = to + (u >> 1) * (C::A / 2) + (((((u & 1) ^ odd) * 4 + t) ^ g) << 4);
-      *reinterpret_cast<uint4*>(at) = make_uint4(v[0][0], v[0][2], v[1][0], v[1][2]);
-      *reinterpret_cast<uint4*>(at + 8 * 128) = make_uint4(v[0][1], v[0][3], v[1][1], v[1][3]);
-    }
-    if (!copied) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (m + 16 * j >= rows) break;
-        uint4 v = ahead[j];
-        if (staged) {
-          const uint2 raw = *reinterpret_cast<const uint2*>(sRaw + kb % C::RAW * (C::X / 2) + j * 2048);
-          v.x = raw.x, v.y = raw.y;
-        }
-        if (a.x_type == TAO_TYPE_E4M3) v = widen_e4m3(v);
-        *reinterpret_cast<uint4*>(x_slot(kb) + place + j * 16 * 128) = v;
-      }
-    }
-    fence_proxy_async();
-    fence_before();
-    __syncthreads();
-    if (tid == 0) {
+    for (int kb = 0; kb < nb; ++kb) {
+      const uint64_t pa = sdesc(smem_u32(sA + (kb & 1) * C::A), 16, 1024);
+      const uint64_t px = sdesc(smem_u32(x_slot(kb)), 16, 1024);  // addresses count 16 bytes
+      __syncthreads();
       fence_after();
-      constexpr uint32_t TYPE = std::is_same<M, MmaBf16>::value ? 1u << 7 | 1u << 10 : 0u;  // bf16, or fp16
-      constexpr uint32_t I = (idesc_bf16(128, C::COLS, 0, 0) & ~(1u << 7 | 1u << 10)) | TYPE;
-      const uint32_t pa = smem_u32(sA + (kb & 1) * C::A), px = smem_u32(x_slot(kb));
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        tc::mma(tbase + ((kb & 1) * C::GROUPS + k * 16 / GROUP) * C::COLS,
-                sdesc(pa + (k >> 2) * (C::A / 2) + (k & 3) * 32, 16, 1024),
-                sdesc(px + (k >> 2) * (C::X / 2) + (k & 3) * 32, 16, 1024), I, k * 16 % GROUP ? 1u : 0u);
-      commit(&bar[kb & 1]);
+        for (int k = 0; k < 8; ++k)
+          tc::mma(tbase + ((kb & 1) * C::GROUPS + k * 16 / GROUP) * C::COLS,
+                  pa + (((k >> 2) * (C::A / 2) + (k & 3) * 32) >> 4), px + (((k >> 2) * (C::X / 2) + (k & 3) * 32) >> 4),
+                  I, k * 16 % GROUP ? 1u : 0u);
+        commit(&bar[kb & 1]);
+      }
+      __syncwarp();
     }
-    __syncwarp();
-    if (!a.wide) fetch(kb + 1);
-    if (kb > 0) add(kb - 1);
-    copy(kb + 6, kb + 4);  // into the slots of blocks kb - 2, whose scales are used, and kb - 1, whose product is over
+  } else {
+#pragma unroll 1
+    for (int kb = 0; kb < nb; ++kb) {
+      cp_wait<3>();  // this block's codes and x; younger groups may be open
+      __syncwarp();
+      // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k; odd rows' lanes take the parts of 64 k in the
+      // other order, so that 8 lanes write to all banks
+      B4 b;
+      b.load(my_codes + kb % C::CSLOTS * C::CODES, has_zeros, lane);
+      const int odd = g & 1;
+      if (odd) b.swap_parts();
+      uint8_t* const to = sA + (kb & 1) * C::A + (warp * 16 + g) * 128;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t v[2][4];
+        b.template operands16<M>(u, v);
+        uint8_t* const at = to + (u >> 1) * (C::A / 2) + (((((u & 1) ^ odd) * 4 + t) ^ g) << 4);
+        *reinterpret_cast<uint4*>(at) = make_uint4(v[0][0], v[0][2], v[1][0], v[1][2]);
+        *reinterpret_cast<uint4*>(at + 8 * 128) = make_uint4(v[0][1], v[0][3], v[1][1], v[1][3]);
+      }
+      if (!copied) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (m + 16 * j >= rows) break;
+          uint4 v = ahead[j];
+          if (staged) {
+            const uint2 raw = *reinterpret_cast<const uint2*>(sRaw + kb % C::RAW * (C::X / 2) + j * 2048);
+            v.x = raw.x, v.y = raw.y;
+          }
+          if (a.x_type == TAO_TYPE_E4M3) v = widen_e4m3(v);
+          *reinterpret_cast<uint4*>(x_slot(kb) + place + j * 16 * 128) = v;
+        }
+      }
+      fence_proxy_async();
+      fence_before();
+      __syncthreads();
+      if (!a.wide) fetch(kb + 1);
+      if (kb > 0) add(kb - 1);
+      copy(kb + 6, kb + 4);  // into the slots of blocks kb - 2, whose scales are used, and kb - 1, whose product is over
+    }
+    add(nb - 1);
+    if (!ok) mbar_wait(&bar[(nb - 1) & 1], (nb - 1) >> 1 & 1, nullptr);  // what is in flight has its time before it ends
   }
-  add(nb - 1);
-  if (!ok) mbar_wait(&bar[(nb - 1) & 1], (nb - 1) >> 1 & 1, nullptr);  // what is in flight has its time before it ends
   cp_wait<0>();
   fence_before();
   __syncthreads();
@@ -193,12 +211,13 @@ __global__ void __launch_bounds__(256, 1) linear4_tc_kernel(const Linear4Args a)
   if (!a.shift) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (half * 32 + i < rows && n0 + r < a.n) put(half * 32 + i, n0 + r, acc[i]);
+      if (warp < C::WORKERS && half * 32 + i < rows && n0 + r < a.n) put(half * 32 + i, n0 + r, acc[i]);
     return;
   }
   float* sums = reinterpret_cast<float*>(sm);  // [column][128 rows], over the operands
 #pragma unroll
-  for (int i = 0; i < 32; ++i) sums[(half * 32 + i) * 128 + r] = acc[i];
+  for (int i = 0; i < 32; ++i)
+    if (warp < C::WORKERS) sums[(half * 32 + i) * 128 + r] = acc[i];
   cluster_sync();
   for (int i = (((warp << a.shift) + rank) << 5) + lane; i < rows * 32; i += C::THREADS << a.shift) {
     const int m = i >> 5, n = n0 + (i & 31) * 4;
