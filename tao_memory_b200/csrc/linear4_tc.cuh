@@ -26,7 +26,7 @@ TAO_DEVI bool elect_one() {
 
 template <int GROUP>
 struct Linear4Tc {
-  static constexpr int WORKERS = 8, THREADS = 32 * (WORKERS + 1), COLS = 64, GROUPS = 128 / GROUP;
+  static constexpr int WORKERS = 8, LOADERS = 8, THREADS = 32 * (WORKERS + 1 + LOADERS), COLS = 64, GROUPS = 128 / GROUP;
   static constexpr int A = 128 * 256, X = COLS * 256, XSLOTS = 5, CODES = 8 * Block4<GROUP>::BYTES, CSLOTS = 8;
   static constexpr int RAW = 6;  // slots of x as e4m3
   static constexpr int TMEM = 2 * GROUPS * COLS;
@@ -58,28 +58,29 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
   const int r = (warp & 3) * 32 + lane, half = warp >> 2;
   const uint8_t* const scales = sC + r / 16 * B4::BYTES + 1024 + (r & 7) * (4 * C::GROUPS) + (r >> 3 & 1) * 2;
 
-  // This thread brings chunk c of 8 k of rows m, m + 16, m + 32, m + 48 of x to `place` and 16 rows on in a slot
+  // A loader brings chunk c of 8 k of rows m, m + 16, m + 32, m + 48 of x to `place` and 16 rows on in a slot
   // of the B operand.  e4m3 is widened on its way, from a ring of raw chunks in the last three slots' room.
-  const int m = tid >> 4, c = tid & 15;
+  const int loader = tid - 32 * (C::WORKERS + 1), m = loader >> 4, c = loader & 15;
   const uint32_t place = (c >> 3) * (C::COLS * 128) + m * 128 + (((c & 7) ^ (m & 7)) << 4);
   const bool copied = a.wide && a.x_type != TAO_TYPE_E4M3, staged = a.wide && a.x_type == TAO_TYPE_E4M3;
   const long long x_at = (long long)(m0 + m) * a.x_stride + k0 * 128 + c * 8;
   const uint8_t* const x = static_cast<const uint8_t*>(a.x) + (staged ? x_at : x_at * 2);
   const long long x_step = (staged ? 16 : 32) * a.x_stride;  // of 16 rows, in bytes
-  uint8_t* const sRaw = sX + 2 * C::X + tid * 8;
+  uint8_t* const sRaw = sX + 2 * C::X + loader * 8;
   auto x_slot = [&](int kb) { return sX + (copied ? kb % C::XSLOTS : kb & 1) * C::X; };
-  auto copy = [&](int codes_kb, int x_kb) {
-    if (codes_kb < nb) B4::issue(smem_u32(my_codes + codes_kb % C::CSLOTS * C::CODES), a.w, first + codes_kb, lane);
-    if (x_kb >= 0 && x_kb < nb) {
-      const bool in = (k0 + x_kb) * 128 + c * 8 < a.k;
+  auto copy_codes = [&](int kb) {
+    if (kb < nb) B4::issue(smem_u32(my_codes + kb % C::CSLOTS * C::CODES), a.w, first + kb, lane);
+    cp_commit();
+  };
+  auto copy_x = [&](int kb) {
+    const bool in = (k0 + kb) * 128 + c * 8 < a.k;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (m + 16 * j >= rows) break;
-        if (copied)
-          cp_async16(smem_u32(x_slot(x_kb) + place + j * 16 * 128), in ? x + x_kb * 256 + j * x_step : x, in);
-        else if (staged)
-          cp_async8(smem_u32(sRaw + x_kb % C::RAW * (C::X / 2) + j * 2048), in ? x + x_kb * 128 + j * x_step : x, in);
-      }
+    for (int j = 0; j < 4; ++j) {
+      if (kb >= nb || m + 16 * j >= rows) break;
+      if (copied)
+        cp_async16(smem_u32(x_slot(kb) + place + j * 16 * 128), in ? x + kb * 256 + j * x_step : x, in);
+      else if (staged)
+        cp_async8(smem_u32(sRaw + kb % C::RAW * (C::X / 2) + j * 2048), in ? x + kb * 128 + j * x_step : x, in);
     }
     cp_commit();
   };
@@ -90,7 +91,9 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
       if (kb < nb && m + 16 * j < rows) ahead[j] = chunk_of(a, m0 + m + 16 * j, (k0 + kb) * 128 + c * 8);
   };
   if (warp < C::WORKERS) {
-    for (int j = -6; j < 0; ++j) copy(j + 6, j + 4);
+    for (int kb = 0; kb < 6; ++kb) copy_codes(kb);
+  } else if (warp > C::WORKERS) {
+    for (int kb = 0; kb < 4; ++kb) copy_x(kb);
     if (!a.wide) fetch(0);
   }
 
@@ -111,10 +114,14 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
 
   float acc[32] = {};
   bool ok = true;  // after a wait that ran out nothing more is waited for
-  // adds block kb's accumulators
-  auto add = [&](int kb) {
+  // until block kb's products are over
+  auto done = [&](int kb) {
     if (ok) ok = mbar_wait(&bar[kb & 1], kb >> 1 & 1, &g_linear4_error);
     __syncwarp();
+  };
+  // adds block kb's accumulators
+  auto add = [&](int kb) {
+    done(kb);
     fence_after();
 #pragma unroll
     for (int j = 0; j < C::GROUPS; ++j) {
@@ -148,10 +155,10 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp < C::WORKERS) {
 #pragma unroll 1
     for (int kb = 0; kb < nb; ++kb) {
-      cp_wait<3>();  // this block's codes and x; younger groups may be open
+      cp_wait<5>();  // this block's codes; younger ones may be on their way
       __syncwarp();
       // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k; odd rows' lanes take the parts of 64 k in the
       // other order, so that 8 lanes write to all banks
@@ -168,6 +175,18 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
         *reinterpret_cast<uint4*>(at) = make_uint4(v[0][0], v[0][2], v[1][0], v[1][2]);
         *reinterpret_cast<uint4*>(at + 8 * 128) = make_uint4(v[0][1], v[0][3], v[1][1], v[1][3]);
       }
+      fence_proxy_async();
+      fence_before();
+      __syncthreads();
+      if (kb > 0) add(kb - 1);
+      copy_codes(kb + 6);  // into the slot of block kb - 2, whose scales all have used
+    }
+    add(nb - 1);
+    if (!ok) mbar_wait(&bar[(nb - 1) & 1], (nb - 1) >> 1 & 1, nullptr);  // what is in flight has its time before it ends
+  } else {
+#pragma unroll 1
+    for (int kb = 0; kb < nb; ++kb) {
+      cp_wait<3>();
       if (!copied) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -182,14 +201,11 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
         }
       }
       fence_proxy_async();
-      fence_before();
       __syncthreads();
       if (!a.wide) fetch(kb + 1);
-      if (kb > 0) add(kb - 1);
-      copy(kb + 6, kb + 4);  // into the slots of blocks kb - 2, whose scales are used, and kb - 1, whose product is over
+      if (kb > 0) done(kb - 1);
+      copy_x(kb + 4);  // into the slot of block kb - 1
     }
-    add(nb - 1);
-    if (!ok) mbar_wait(&bar[(nb - 1) & 1], (nb - 1) >> 1 & 1, nullptr);  // what is in flight has its time before it ends
   }
   cp_wait<0>();
   fence_before();
