@@ -24,11 +24,24 @@ TAO_DEVI bool elect_one() {
   return p != 0;
 }
 
+// 16 consecutive fp32 columns of this thread's TMEM lane.
+TAO_DEVI void tmem_ld16(uint32_t at, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 template <int GROUP>
 struct Linear4Tc {
   static constexpr int WORKERS = 8, LOADERS = 8, THREADS = 32 * (WORKERS + 1 + LOADERS), COLS = 64, GROUPS = 128 / GROUP;
   static constexpr int A = 128 * 256, X = COLS * 256, XSLOTS = 5, CODES = 8 * Block4<GROUP>::BYTES, CSLOTS = 8;
-  static constexpr int RAW = 6;  // slots of x as e4m3
+  static constexpr int RAW = 4;  // slots of x as e4m3
   static constexpr int TMEM = 2 * GROUPS * COLS;
   static constexpr int SMEM = 1024 + 2 * A + XSLOTS * X + CSLOTS * CODES + 64;
   static_assert(SMEM <= 227 * 1024, "");
@@ -58,42 +71,43 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
   const int r = (warp & 3) * 32 + lane, half = warp >> 2;
   const uint8_t* const scales = sC + r / 16 * B4::BYTES + 1024 + (r & 7) * (4 * C::GROUPS) + (r >> 3 & 1) * 2;
 
+  constexpr int LOADING = 32 * C::LOADERS, STEP = LOADING / 16, EACH = C::COLS / STEP;
   // A loader brings chunk c of 8 k of rows m, m + 16, m + 32, m + 48 of x to `place` and 16 rows on in a slot
-  // of the B operand.  e4m3 is widened on its way, from a ring of raw chunks in the last three slots' room.
+  // of the B operand.  e4m3 is widened on its way, from a ring of raw chunks in the last two slots' room.
   const int loader = tid - 32 * (C::WORKERS + 1), m = loader >> 4, c = loader & 15;
   const uint32_t place = (c >> 3) * (C::COLS * 128) + m * 128 + (((c & 7) ^ (m & 7)) << 4);
   const bool copied = a.wide && a.x_type != TAO_TYPE_E4M3, staged = a.wide && a.x_type == TAO_TYPE_E4M3;
   const long long x_at = (long long)(m0 + m) * a.x_stride + k0 * 128 + c * 8;
   const uint8_t* const x = static_cast<const uint8_t*>(a.x) + (staged ? x_at : x_at * 2);
-  const long long x_step = (staged ? 16 : 32) * a.x_stride;  // of 16 rows, in bytes
-  uint8_t* const sRaw = sX + 2 * C::X + loader * 8;
-  auto x_slot = [&](int kb) { return sX + (copied ? kb % C::XSLOTS : kb & 1) * C::X; };
+  const long long x_step = (staged ? STEP : 2 * STEP) * a.x_stride;  // of STEP rows, in bytes
+  uint8_t* const sRaw = sX + 3 * C::X + loader * 8;
+  auto x_slot = [&](int kb) { return sX + kb % (copied ? C::XSLOTS : 3) * C::X; };
   auto copy_codes = [&](int kb) {
-    if (kb < nb) B4::issue(smem_u32(my_codes + kb % C::CSLOTS * C::CODES), a.w, first + kb, lane);
+    if (kb < nb) B4::issue(smem_u32(my_codes + (kb & (C::CSLOTS - 1)) * C::CODES), a.w, first + kb, lane);
     cp_commit();
   };
   auto copy_x = [&](int kb) {
     const bool in = (k0 + kb) * 128 + c * 8 < a.k;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (kb >= nb || m + 16 * j >= rows) break;
+    for (int j = 0; j < EACH; ++j) {
+      if (kb >= nb || m + STEP * j >= rows) break;
       if (copied)
-        cp_async16(smem_u32(x_slot(kb) + place + j * 16 * 128), in ? x + kb * 256 + j * x_step : x, in);
+        cp_async16(smem_u32(x_slot(kb) + place + j * STEP * 128), in ? x + kb * 256 + j * x_step : x, in);
       else if (staged)
-        cp_async8(smem_u32(sRaw + kb % C::RAW * (C::X / 2) + j * 2048), in ? x + kb * 128 + j * x_step : x, in);
+        cp_async8(smem_u32(sRaw + (kb & (C::RAW - 1)) * (C::X / 2) + j * (LOADING * 8)), in ? x + kb * 128 + j * x_step : x, in);
     }
     cp_commit();
   };
-  uint4 ahead[4];  // x off its alignment, a block ahead
+  uint4 ahead[EACH];  // x off its alignment, a block ahead
   auto fetch = [&](int kb) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (kb < nb && m + 16 * j < rows) ahead[j] = chunk_of(a, m0 + m + 16 * j, (k0 + kb) * 128 + c * 8);
+    for (int j = 0; j < EACH; ++j)
+      if (kb < nb && m + STEP * j < rows) ahead[j] = chunk_of(a, m0 + m + STEP * j, (k0 + kb) * 128 + c * 8);
   };
   if (warp < C::WORKERS) {
     for (int kb = 0; kb < 6; ++kb) copy_codes(kb);
   } else if (warp > C::WORKERS) {
-    for (int kb = 0; kb < 4; ++kb) copy_x(kb);
+    for (int kb = 0; kb < 3; ++kb) copy_x(kb);
     if (!a.wide) fetch(0);
   }
 
@@ -114,23 +128,22 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
 
   float acc[32] = {};
   bool ok = true;  // after a wait that ran out nothing more is waited for
-  // until block kb's products are over
-  auto done = [&](int kb) {
-    if (ok) ok = mbar_wait(&bar[kb & 1], kb >> 1 & 1, &g_linear4_error);
-    __syncwarp();
-  };
   // adds block kb's accumulators
   auto add = [&](int kb) {
-    done(kb);
+    if (ok) ok = mbar_wait(&bar[kb & 1], kb >> 1 & 1, &g_linear4_error);
+    __syncwarp();
     fence_after();
 #pragma unroll
     for (int j = 0; j < C::GROUPS; ++j) {
-      const uint16_t bits = *reinterpret_cast<const uint16_t*>(scales + kb % C::CSLOTS * C::CODES + j * 4);
+      const uint16_t bits = *reinterpret_cast<const uint16_t*>(scales + (kb & (C::CSLOTS - 1)) * C::CODES + j * 4);
       const float s = BF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
-      float v[32];
-      tmem_ld32(tbase + ((uint32_t)((warp & 3) * 32) << 16) + ((kb & 1) * C::GROUPS + j) * C::COLS + half * 32, v);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) acc[i] += s * v[i];
+      for (int h = 0; h < 2; ++h) {
+        float v[16];
+        tmem_ld16(tbase + ((uint32_t)((warp & 3) * 32) << 16) + ((kb & 1) * C::GROUPS + j) * C::COLS + half * 32 + h * 16, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[h * 16 + i] += s * v[i];
+      }
     }
     fence_before();
   };
@@ -163,7 +176,7 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
       // A: two chunks of 16 bytes (rows g, g + 8) for each 32 k; odd rows' lanes take the parts of 64 k in the
       // other order, so that 8 lanes write to all banks
       B4 b;
-      b.load(my_codes + kb % C::CSLOTS * C::CODES, has_zeros, lane);
+      b.load(my_codes + (kb & (C::CSLOTS - 1)) * C::CODES, has_zeros, lane);
       const int odd = g & 1;
       if (odd) b.swap_parts();
       uint8_t* const to = sA + (kb & 1) * C::A + (warp * 16 + g) * 128;
@@ -186,25 +199,24 @@ __global__ void __launch_bounds__(Linear4Tc<GROUP>::THREADS, 1) linear4_tc_kerne
   } else {
 #pragma unroll 1
     for (int kb = 0; kb < nb; ++kb) {
-      cp_wait<3>();
+      cp_wait<2>();
       if (!copied) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (m + 16 * j >= rows) break;
+        for (int j = 0; j < EACH; ++j) {
+          if (m + STEP * j >= rows) break;
           uint4 v = ahead[j];
           if (staged) {
-            const uint2 raw = *reinterpret_cast<const uint2*>(sRaw + kb % C::RAW * (C::X / 2) + j * 2048);
+            const uint2 raw = *reinterpret_cast<const uint2*>(sRaw + (kb & (C::RAW - 1)) * (C::X / 2) + j * (LOADING * 8));
             v.x = raw.x, v.y = raw.y;
           }
           if (a.x_type == TAO_TYPE_E4M3) v = widen_e4m3(v);
-          *reinterpret_cast<uint4*>(x_slot(kb) + place + j * 16 * 128) = v;
+          *reinterpret_cast<uint4*>(x_slot(kb) + place + j * STEP * 128) = v;
         }
       }
       fence_proxy_async();
       __syncthreads();
       if (!a.wide) fetch(kb + 1);
-      if (kb > 0) done(kb - 1);
-      copy_x(kb + 4);  // into the slot of block kb - 1
+      copy_x(kb + 3);  // into the slot of block kb - 2: its sums were added before this barrier
     }
   }
   cp_wait<0>();
