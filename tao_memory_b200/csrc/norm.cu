@@ -384,10 +384,19 @@ struct Shape {
   int threads, rows, vectors;
 };
 
-Shape shape_of(long long rows, int width, int elements, bool grad) {
+// Measured in bf16 with a residual (us):
+//  - rows whose vectors all fit the device at once, half full: a thread a vector, for latency.  64x768 2.3 (a warp
+//    a row 3.5), 592x2048 3.2 (two vectors 3.4); above that 1184x8192 21.2 (14.1).
+//  - 65 to 128 vectors: a thread a vector.  32768x768 37.5 (a warp a row 41.5); below, 32768x384 21.8 (18.4).
+//    The e4m3 form needs the rows' largest values too, which a warp finds alone: 32768x768 49.3 (40.7).
+//  - more: two vectors a thread.  16384x2048 43.7 (one 50.5), 16384x8192 177.7 (one 283, four 229).
+//  - the gradient of 513 to 1024 vectors, whose two vectors a thread leave one block of 512 threads an SM:
+//    forward and backward of 4096x8192 118 (167); of 4096 elements 136 (109).
+Shape shape_of(long long rows, int width, int elements, bool fp8, bool grad) {
   const int vectors = (width + elements - 1) / elements;
-  // few rows: the widest block, whose latency counts
-  if (rows <= 1184 && vectors <= 1024 && !grad) return {(vectors + 31) / 32 * 32, 1, 1};
+  const bool fit = vectors <= 1024 && rows * vectors <= 148 * 1024;
+  if (grad ? vectors > 512 && vectors <= 1024 : fit || (!fp8 && vectors > 64 && vectors <= 128))
+    return {(vectors + 31) / 32 * 32, 1, 1};
   if (vectors <= 128) return {32, 8, (vectors + 31) / 32};
   int threads = 128;
   while (threads < 1024 && vectors > 2 * threads) threads *= 2;
@@ -473,7 +482,7 @@ int forward(const NormArgs& a, int type, bool fp8, void* stream) {
   const bool wide = a.width % (16 / size) == 0 && wide_ok(a.x, a.x_stride, size) &&
                     wide_ok(a.residual, a.r_stride, size) && wide_ok(a.weight, 0, size) && wide_ok(a.s, 0, size) &&
                     wide_ok(a.y, 0, size);
-  Shape sh = shape_of(a.rows, a.width, wide ? (int)(16 / size) : 1, false);
+  Shape sh = shape_of(a.rows, a.width, wide ? (int)(16 / size) : 1, fp8, false);
   // single elements: 128 channels are four whole warps of a block
   if (fp8 && a.group && !wide && sh.threads % 128) sh = {128, 1, (a.width + 127) / 128};
   if (!wide && sh.vectors > 4 && sh.threads < 256) sh = {256, 1, 4};
@@ -531,8 +540,8 @@ size_t tao_add_rms_norm_workspace_bytes(long long rows, int width, int type) {
   using namespace tao;
   if (check(rows, width, type) != TAO_OK || rows == 0) return 0;
   // of the shape with the more blocks
-  const int blocks = std::max(grad_blocks(rows, shape_of(rows, width, (int)(16 / size_of(type)), true)),
-                              grad_blocks(rows, shape_of(rows, width, 1, true)));
+  const int blocks = std::max(grad_blocks(rows, shape_of(rows, width, (int)(16 / size_of(type)), false, true)),
+                              grad_blocks(rows, shape_of(rows, width, 1, false, true)));
   return (size_t)blocks * width * sizeof(float);
 }
 
@@ -554,7 +563,7 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
                           dw ? static_cast<float*>(workspace) : nullptr};
   const bool wide = width % (16 / size) == 0 && wide_ok(dy, dy_stride, size) && wide_ok(ds, ds_stride, size) &&
                     wide_ok(s, s_stride, size) && wide_ok(weight, 0, size) && wide_ok(dx, 0, size);
-  const Shape sh = shape_of(rows, width, wide ? (int)(16 / size) : 1, true);
+  const Shape sh = shape_of(rows, width, wide ? (int)(16 / size) : 1, false, true);
   const int grid = grad_blocks(rows, sh);
   const dim3 block(sh.threads, sh.rows);
   return by_vector(type, wide, [&](auto t, auto n) {
