@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/tao_b200.h"
 #include "few_rows.cuh"
@@ -626,13 +627,21 @@ int launch_as(ExpertArgs a, cudaStream_t s) {
 }
 
 // An entry's weights come once for its 4, 8 or 16 tokens, and from L2 for each further entry of the
-// expert; columns that few entries fill cost instructions.  So by the mean tokens of an expert.
+// expert; columns that few entries fill cost instructions.  So by the mean tokens of an expert; us, of 64 experts
+// (2048, 1024) with 8 for a token and of 8 (4096, 2048) with 2:
+//   mean 2 (16 of 64):          bf16 137.9, 138.4, 140.7    4 bits 83.5, 87.4, 149.2
+//   mean 4 (32 of 64):          bf16 189.5, 172.3, 173.9    4 bits 125.8, 113.3, 171.1
+//   mean 8 (64 of 64, 32 of 8): bf16 197.1, 217.0, 190.7 and 121.5, 111.0, 107.9    4 bits 175.3, 154.0, 191.8
+//   mean 16 (64 of 8):          bf16 218.9, 175.1, 141.6    4 bits 162.7, 146.3, 158.5
+// Four tiles leave 4-bit weights, which need registers to be unpacked, too few.
 template <class L>
 int launch(const ExpertArgs& a, cudaStream_t s) {
   const int pairs = a.tokens * a.top_k;
   if (pairs <= 2 * a.experts) return launch_as<L, 1>(a, s);
-  if (pairs <= 8 * a.experts) return launch_as<L, 2>(a, s);
-  return launch_as<L, 4>(a, s);
+  if constexpr (std::is_same<L, Layer16>::value) {
+    if (pairs > 4 * a.experts) return launch_as<L, 4>(a, s);
+  }
+  return launch_as<L, 2>(a, s);
 }
 
 }  // namespace
