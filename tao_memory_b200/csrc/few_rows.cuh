@@ -4,9 +4,9 @@
 //   D[n][m] += sum over k of W[n][k] x[m][k]
 //
 // The weights are the 16-row operand of a warp's mma and eight activation columns the other, so a
-// weight is used once per eight columns.  The work is bound by the weights' bytes, far from where
-// tcgen05 tiles (128 rows, operands through shared memory, where 4-bit weights would first have to be
-// written unpacked) would pay; what is left to save is the instructions per weight.
+// weight is used once per eight columns.  Up to 16 rows the work is bound by the weights' bytes and the
+// instructions per weight; a tcgen05 tile has operands in shared memory, where 4-bit weights would first have
+// to be written unpacked, which pays from 17 rows on (linear4_tc.cuh).
 //
 // A few rows (product8): the codes 0..15 go as bytes into the integer mma.m16n8k32, three
 // instructions for eight of them.  The activations become sums of signed bytes under a power of

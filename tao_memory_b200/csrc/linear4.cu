@@ -9,8 +9,9 @@
 // Bound by the codes' bytes, half a byte a weight.  One block an SM.  x, or a cluster's block's part of its
 // k, is laid out in shared memory once, in the order of the mma's operands.  The warps are WT x WK: WT row
 // tiles at a time, each one's 128-k blocks dealt to WK warps in runs, each warp's through a ring of its own
-// (registers would do, but a warp's few scoreboards make a load wait for later ones).  A warp leaves its sums of a tile in shared memory; these are added at the end, a cluster's blocks' through
-// distributed shared memory, in a fixed order.
+// (registers would do, but a warp's few scoreboards make a load wait for later ones).  A warp leaves its sums
+// of a tile in shared memory; these are added at the end, a cluster's blocks' through distributed shared
+// memory, in a fixed order.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -350,7 +351,7 @@ int launch_tc(Linear4Args a, cudaStream_t s) {
   for (int shift = 0; shift <= 3 && 1 << shift <= a.kblocks; ++shift) {
     const int clusters = shift == 0 ? 148 : shift == 1 ? 74 : shift == 2 ? 33 : 15;
     const int waves = (sets * passes + clusters - 1) / clusters, kb = (a.kblocks + (1 << shift) - 1) >> shift;
-    const double cost = waves * (kb * 0.25 + 2. + (shift ? 1. : 0.));  // us, roughly
+    const double cost = waves * (kb * 0.8 + 2. + (shift ? 1. : 0.));  // us, measured
     if (cost < least) {
       least = cost;
       a.shift = shift;
@@ -360,15 +361,18 @@ int launch_tc(Linear4Args a, cudaStream_t s) {
 }
 
 // The bytes' form costs four columns a row and little else, the 16-bit one eight more instructions for
-// eight weights.  A form whose x does not fit a cluster of 8 blocks' shared memory leaves the product to the
-// next smaller one, which reads the weights again (from L2) for each of its row tiles.
+// eight weights: of k = n = 8192 one row takes 10.3 us (13.3 in 16 bits), two 11.3 (13.8), four 13.7 (14.2 as
+// bytes in two column tiles, a form that is not kept).  tcgen05 needs the weights in shared memory: 16 rows
+// 26.7 us (16.2 here), 17 26.9 (28.8), 64 29.5 (60.6); of k = 2048, n = 6144 17 rows 9.9 (8.7), 32 10.3 (10.7),
+// 64 11.1 (18.9).  A form whose x does not fit a cluster of 8 blocks'
+// shared memory leaves the product to the next smaller one, which reads the weights again (from L2) for each
+// of its row tiles.
 template <class M, bool BF16, int GROUP>
 int by_rows(const Linear4Args& a, cudaStream_t s) {
   if (a.rows > 16) return launch_tc<M, BF16, GROUP>(a, s);
   int rc = TAO_ERR_CAPACITY;
   if (a.rows > 8) rc = launch<M, BF16, GROUP, 2>(a, s);
-  if (a.rows > 4 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 1>(a, s);
-  if (a.rows > 2 && rc == TAO_ERR_CAPACITY) rc = launch<Bytes, BF16, GROUP, 2>(a, s);
+  if (a.rows > 2 && rc == TAO_ERR_CAPACITY) rc = launch<M, BF16, GROUP, 1>(a, s);
   if (rc == TAO_ERR_CAPACITY) rc = launch<Bytes, BF16, GROUP, 1>(a, s);
   return rc;
 }

@@ -1,14 +1,19 @@
 // The 4-bit product of more than a few rows (up to 64 at a time) on tcgen05: with 17 rows and more the
 // legacy mma and its operand loads take several times as long as the weights' bytes.
 //
-// A block computes 128 rows of W (8 row tiles, one a warp) against 64 rows of x over its k, a cluster's
-// blocks a part of k each.  Per 128 k:  a warp makes 16-bit floats (code - zero, exact) of its tile's codes
-// and writes them to the A operand (K-major, 128-byte swizzle, two buffers); a ninth issues the
-// 8 products of 16 k into TMEM, an accumulator of its own for each scale group (two sets); and while those
-// run, the block before's accumulators are read, scaled and added in fp32 registers, row and column half
-// a thread.  So no weight is rounded and every sum's order is fixed.  x comes by cp.async into five slots of
-// the B operand, codes and scales into eight of a ring: both are
-// a memory's whole latency ahead.
+// A block computes 128 rows of W (8 row tiles) against 64 rows of x over its k, a cluster's blocks a part of
+// k each.  Per 128 k:  eight warps make 16-bit floats (code - zero, exact) of a tile's codes each and write
+// them to the A operand (K-major, 128-byte swizzle, two buffers); a ninth issues the 8 products of 16 k into
+// TMEM, an accumulator of its own for each scale group (two sets); and while those run, the eight read the
+// block before's accumulators, scale them and add them in fp32 registers, row and column half a thread.  So no
+// weight is rounded and every sum's order is fixed.  Eight more warps bring x to five slots of the B operand;
+// codes and scales come to eight of a ring.  All copies have a memory's latency and more.
+//
+// 64x8192x8192 takes 28.9 us, 1.27 TB/s of its bytes and 0.30 PFLOP/s.  What bounds it is the eight warps'
+// chain of a block: unpacking and the operand's writes to shared memory, fence, barrier, and the sums (about
+// 1600 cycles where the products take 260 and the bytes 350).  It was 35.3 us while the eight brought x too,
+// 40.5 us while one of them issued the products, and sixteen warps with half a tile each took 32.5 us: the
+// same shared memory writes, and twice the warps at the barrier.
 #pragma once
 #include "linear4.cuh"
 #include "tcgen05.cuh"
