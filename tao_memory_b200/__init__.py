@@ -8,7 +8,9 @@ Drop-in for the reference package's public API (``tao_attention/__init__.py``):
 host memory, ``DecodeSession`` for a serving loop over a fixed batch whose
 tokens arrive in and leave through page-locked host memory, and the serving caller
 (``RequestStates``, ``DecodeScheduler``, ``save_snapshot`` / ``load_snapshot``);
-``tao_memory_b200.model`` holds the model-side neighbours (``ProjectedInputs``).  All compute runs in
+``tao_memory_b200.model`` holds the model-side neighbours (``ProjectedInputs``, ``ServedBlock``).
+Around the attention stand ``add_rms_norm`` / ``add_rms_norm_fp8``, ``linear4`` on 4-bit
+``Weight4`` (``quantize4``) and ``expert_layer`` on ``ExpertWeights``.  All compute runs in
 ``libtao_b200.so`` (hand-written CUDA for sm_100a) behind a C ABI.
 """
 
