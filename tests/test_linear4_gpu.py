@@ -3,8 +3,10 @@
 Bound: y is rounded once (unit roundoff u: 2^-8 bf16, 2^-11 fp16; half a subnormal step of
 fp16), and the fp32 sums before it lose at most D units of 2^-24 of the sum of the terms'
 magnitudes, D the depth of the additions: 16 in a group (8 matrix instructions, which may
-truncate), one a group of a warp's blocks (k / 1024 at group 128, four times that at 32),
-8 warps, and the scalings: D = 64 for the sizes here."""
+truncate), one a group of a warp's or block's run of k (at most 2304 / 128 at group 128, four
+times that at 32, and a part of it where several share k), 8 to 16 such sums, and the scalings:
+D = 64 for the sizes here.  One or two rows have exact group sums in whole numbers, of x to
+2^-21 of the largest magnitude of its 128: for normal x at most 5 times the mean, 40 units."""
 import pytest
 import torch
 
