@@ -12,6 +12,9 @@
 // (registers would do, but a warp's few scoreboards make a load wait for later ones).  A warp leaves its sums
 // of a tile in shared memory; these are added at the end, a cluster's blocks' through distributed shared
 // memory, in a fixed order.
+// With k = n = 8192 and groups of 128 one row takes 10.3 us (3.4 TB/s of its bytes), 8 rows 14.2, 16 rows 16.3: half of
+// the issue slots, the rest waits at the few meetings.  A single row of k = 2048, n = 6144 takes 4.4 us, of which
+// the bytes are 1: launch, x and the first weights follow one another.
 #include <cuda_runtime.h>
 
 #include <algorithm>
