@@ -35,7 +35,8 @@ constexpr int kMaxK = 65536;  // two rows' pieces of a cluster of 8's part fit b
 // The two forms of the product: signed bytes (4 columns a row), or the 16-bit type M (one).
 struct Bytes {};
 
-// COLS: columns of the mma for a row; WARPS: of a block; DEPTH: blocks of a warp's ring.  Shared memory of a block's 128 k of x: bytes have a row's three pieces as [half][3 row + piece][t] 16 bytes, a lane's
+// COLS: columns of the mma for a row; WARPS: of a block; DEPTH: blocks of a warp's ring.  Shared memory of a
+// block's 128 k of x: bytes have a row's three pieces as [half][3 row + piece][t] 16 bytes, a lane's
 // operands in the order of the lanes, then [row] s / 2^7, then [group][row] the sums (P, p2); 16 bits have
 // [32-k part][row][t] 16 bytes.
 template <class M, int GROUP, int NT>
