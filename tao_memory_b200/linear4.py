@@ -62,13 +62,14 @@ class Weight4:
         count = codes[..., 0, 0].numel()
         laid = torch.empty(count, tiles, blocks, 1024, dtype=torch.uint8, device=codes.device)
         flat = codes.reshape(count, n, k)
-        for i in range(count):  # matrix by matrix: the intermediate orders stay small
-            c = _padded(flat[i], tiles * _TILE, blocks * _BLOCK)
+        most = max(1, (1 << 25) // (tiles * blocks * _TILE * _BLOCK))
+        for i in range(0, count, most):  # a few matrices at a time: the intermediate orders stay small
+            c = _padded(flat[i:i + most], tiles * _TILE, blocks * _BLOCK)
             # n = (tile, row half, g), k = (block, half, i, t, f, e high, e low)
-            c = c.view(tiles, 2, 8, blocks, 2, 2, 4, 2, 2, 2)
+            c = c.view(-1, tiles, 2, 8, blocks, 2, 2, 4, 2, 2, 2)
             # -> tile, block, half, g, t, i, f, e low, e high, then the byte's nibbles: rows g, g + 8
-            c = c.permute(0, 3, 4, 2, 6, 5, 7, 9, 8, 1).reshape(tiles, blocks, 1024, 2)
-            laid[i] = c[..., 0] | c[..., 1] << 4
+            c = c.permute(0, 1, 4, 5, 3, 7, 6, 8, 10, 9, 2).reshape(-1, tiles, blocks, 1024, 2)
+            torch.bitwise_or(c[..., 0], c[..., 1] << 4, out=laid[i:i + most])
 
         def by_tile(t):
             t = _padded(t.reshape(count, n, parts), tiles * _TILE, blocks * per)
