@@ -68,6 +68,17 @@ def test_against_64_bits(rows, n, k, group, act):
         _check(y, xd, wide, b)
 
 
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16, "fp8"])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("rows,k", [(40, 1100), (64, 1152), (21, 1104)])
+def test_all_of_k_in_one_block(rows, k, group, act):
+    """More row tiles than the device takes at once: a block has nine runs of 128 k, more than its rings."""
+    from tao_memory_b200 import linear4
+    x, scale, xd = _x(rows, k, act)
+    w, wide = _weight(18960, k, group, True, act if act != "fp8" else torch.bfloat16)
+    _check(linear4(x, w, x_scale=scale), xd, wide)
+
+
 @pytest.mark.parametrize("rows", [1, 8, 24])
 def test_large(rows):
     from tao_memory_b200 import linear4

@@ -37,7 +37,7 @@ def _check(a, b, dtype, terms=None):
 
 
 SHAPES = [(1, 1), (1, 64), (3, 7), (8, 768), (5, 1001), (2, 1024), (1185, 96), (1300, 768), (1201, 2048), (1190, 4100),
-          (7, 8192), (1200, 8192), (3, 16384), (2, 65536)]
+          (7, 8192), (1200, 8192), (3, 16384), (2, 65536), (2600, 480), (600, 2048), (1700, 640)]
 
 
 @pytest.mark.parametrize("dtype", list(U))
@@ -135,7 +135,7 @@ def _check_fp8(q, scale, y, group):
 @pytest.mark.parametrize("group", [None, 128])
 @pytest.mark.parametrize("dtype", list(U))
 @pytest.mark.parametrize("rows,width", [(1, 1), (4, 130), (9, 768), (3, 1001), (1300, 768), (1190, 2048), (1200, 5000),
-                                        (2, 16384)])
+                                        (2, 16384), (1700, 640), (600, 2048)])
 def test_fp8(rows, width, dtype, group):
     from tao_memory_b200 import add_rms_norm_fp8
     x, res, w, _, _ = _inputs(rows, width, dtype, seed=4)
