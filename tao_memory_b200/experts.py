@@ -112,10 +112,13 @@ def expert_layer(x, weights, out=None, return_routing=False):
     rows = _rows(x, weights.width)
     if rows.data_ptr() % 16 or rows.stride(0) % 8:
         rows = rows.clone(memory_format=torch.contiguous_format)
+    result = out
     if out is None:
-        out = x.new_empty(x.shape)
+        out = result = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != _BF16 or out.device != x.device or not out.is_contiguous():
         raise ValueError("out is a contiguous tensor of x's shape, type and device")
+    elif out.data_ptr() % 8:  # the kernel stores 8 bytes at a time
+        result = x.new_empty(x.shape)
     ids = route = ids_at = route_at = None
     if return_routing:
         ids = x.new_empty((*x.shape[:-1], weights.top_k), dtype=torch.int32)
@@ -124,7 +127,9 @@ def expert_layer(x, weights, out=None, return_routing=False):
     device = x.device.index
     ws = _Room.get(x.device, torch._C._cuda_getCurrentRawStream(device), weights._workspace_bytes)
     _lib.on_device(device, _lib.lib().tao_expert_layer, weights._at, rows.data_ptr(), rows.stride(0), rows.shape[0],
-                   out.data_ptr(), ids_at, route_at, ws.data_ptr(), ws.numel())
+                   result.data_ptr(), ids_at, route_at, ws.data_ptr(), ws.numel())
+    if result is not out:
+        out.copy_(result)
     return (out, ids, route) if return_routing else out
 
 
