@@ -499,7 +499,8 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
  *          k = 128 block + 64h + 32i + 8t + 4f + (0, 2, 1, 3)[e], of row 16 tile + g in its low nibble and
  *          of row 16 tile + g + 8 in the high one;
  *   scales [tiles][blocks][8][128 / group][2]: rows g and g + 8 of a tile, group by group; zeros the
- *          same in bytes; each of the three on 16 bytes.  k up to 65536. */
+ *          same in bytes; each of the three on 16 bytes.  k up to 65536.
+ * y must not overlap x, x_scale or bias (TAO_ERR_ARG). */
 int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_scale, const void* codes,
                 const void* scales, const void* zeros, int group, int type, const void* bias,
                 long long rows, int n, int k, void* y, void* stream);

@@ -48,6 +48,19 @@ TAO_DEVI float max_nan(float a, float b) {
   return r;
 }
 
+// Whether rows of `bytes` bytes, `stride` bytes apart from x on, share any with the `size` bytes from y on.
+inline bool rows_overlap(const void* x, long long rows, long long stride, long long bytes, const void* y,
+                         long long size) {
+  long long at = reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x);
+  if (stride < 0) {  // from the last row on
+    stride = -stride;
+    at += (rows - 1) * stride;
+  }
+  // the first row that ends behind y's start
+  const long long first = at < bytes ? 0 : stride == 0 ? rows : (at - bytes) / stride + 1;
+  return first < rows && first * stride < at + size;
+}
+
 // Products of two bf16 pairs rounded to bf16, lane by lane.  The product of two
 // bf16 values is exact in fp32, so this equals rb(a * b) for each lane.
 TAO_DEVI uint32_t hmul2u(uint32_t a, uint32_t b) {

@@ -409,6 +409,11 @@ int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_sc
   for (const void* p : {codes, scales, zeros})
     if (reinterpret_cast<uintptr_t>(p) % 16) return lfail(TAO_ERR_ARG, "a laid-out weight starts on 16 bytes");
   const int size = x_type == TAO_TYPE_E4M3 ? 1 : 2;
+  // a block writes its part of y while others still read theirs of x
+  if (rows_overlap(x, rows, x_stride * size, (long long)k * size, y, rows * n * 2) ||
+      (x_scale && rows_overlap(x_scale, 1, 0, rows * 4, y, rows * n * 2)) ||
+      (bias && rows_overlap(bias, 1, 0, n * 2LL, y, rows * n * 2)))
+    return lfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   constexpr long long kMost = 1 << 16;  // rows of a launch: the grid's second axis has at most 65535 blocks
   for (long long at = 0; at < rows; at += kMost) {
     Linear4Args a = {};

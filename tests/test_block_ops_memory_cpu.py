@@ -12,12 +12,34 @@ def _layer(**k):
 
 
 def _experts(x, out, tokens=1, stride=8):
-    return _lib.lib().tao_expert_layer(ctypes.byref(_layer()), x, stride, tokens, out, None, None, 1 << 21, 1 << 20,
-                                       None)
+    # a workspace too small is refused last: no call here launches anything, whatever the machine
+    return _lib.lib().tao_expert_layer(ctypes.byref(_layer()), x, stride, tokens, out, None, None, 1 << 21, 16, None)
 
 
 def test_an_expert_layers_out_starts_on_8_bytes():
     # the sums' kernel stores 8 bytes at a time
     for offset in (1, 2, 4, 6, 10):
-        assert _experts(16, (1 << 22) + offset) == _lib.TAO_ERR_ARG, offset
+        assert _experts(16, (1 << 22) + offset) == _lib.TAO_ERR_ARG
         assert b"8 bytes" in _lib.lib().tao_last_error()
+
+
+def _overlaps(x, y, rows=4, stride=128, x_type=0, x_scale=None, bias=None):
+    """tao_linear4's refusal of a y [rows, 128] over its operands (only calls that it refuses are made here)."""
+    rc = _lib.lib().tao_linear4(x, stride, x_type, x_scale, 1 << 20, 1 << 21, None, 128, 0, bias, rows, 128, 128, y,
+                                None)
+    return rc == _lib.TAO_ERR_ARG and b"overlap" in _lib.lib().tao_last_error()
+
+
+def test_a_products_output_does_not_overlap_its_operands():
+    # blocks write their part of y while others still read x: any overlap is a race
+    x, size = 1 << 24, 4 * 128 * 2
+    for y in (x, x + 2, x - 2, x + size - 2, x - size + 2):
+        assert _overlaps(x, y), y - x
+    # rows apart
+    for off in (128 - 1, 2048 - 255, 2048, 2048 + 127):
+        assert _overlaps(x, x + off * 2, rows=2, stride=2048), off
+    assert _overlaps(x, x + 100, stride=0)  # one row for all
+    # e4m3 rows, their scales, and the bias
+    assert _overlaps(x, x + 4 * 128 - 2, x_type=3)
+    assert _overlaps(x, x + 4096, x_type=3, x_scale=x + 4096 + size - 4)
+    assert _overlaps(x, x + 4096, bias=x + 4096 + size - 2)

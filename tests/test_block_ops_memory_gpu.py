@@ -38,3 +38,34 @@ def test_a_products_out_may_be_any_contiguous_view(rows, offset):
     assert linear4(x, w, out=out) is out
     assert torch.equal(out, linear4(x, w))
     assert (room[:offset] == 7).all() and (room[offset + rows * 50:] == 7).all()
+
+
+def test_a_products_out_over_its_activations_is_refused():
+    from tao_memory_b200 import linear4, quantize4
+    w = quantize4(torch.randn(128, 128, device="cuda").bfloat16())
+    room = torch.randn(9, 128, device="cuda").bfloat16()
+    kept = room.clone()
+    for x, out in ((room[:4], room[:4]), (room[:4], room[3:7]), (room[2:6], room[:4]), (room[:8:2], room[1:5])):
+        with pytest.raises(ValueError, match="overlap"):
+            linear4(x, w, out=out)
+    assert torch.equal(room, kept)
+    assert torch.equal(linear4(room[:4], w, out=room[4:8]), linear4(kept[:4], w))
+
+
+def test_a_products_out_beside_its_activations():
+    """What lies next to x, and between rows that are apart, is free."""
+    from tao_memory_b200 import linear4, quantize4
+    w = quantize4(torch.randn(64, 128, device="cuda").bfloat16())
+    room = torch.randn(4096, device="cuda").bfloat16()
+    kept = room.clone()
+    rows = lambda t, stride: t.as_strided((2, 128), (stride, 1), 1024)
+    for stride, at in ((128, 1024 - 128), (128, 1024 + 256), (1024, 1024 + 128), (1024, 2048 - 128), (1024, 2048 + 128),
+                       (0, 1024 + 128), (0, 1024 - 128)):
+        room.copy_(kept)
+        out = room[at:at + 128].view(2, 64)
+        assert torch.equal(linear4(rows(room, stride), w, out=out), linear4(rows(kept, stride), w)), (stride, at)
+    room.copy_(kept)
+    x, bias = room[:256].view(2, 128), room[256:320]
+    assert torch.equal(linear4(x, w, bias=bias, out=room[320:448].view(2, 64)), linear4(x, w, bias=bias))
+    with pytest.raises(ValueError, match="overlap"):
+        linear4(x, w, bias=bias, out=room[300:428].view(2, 64))
