@@ -526,7 +526,8 @@ typedef struct TaoExperts {
  * launch for 64 tokens.  workspace: tao_expert_workspace_bytes, zeroed before its first use, used
  * by one launch at a time; its first word is an error word that tao_expert_check reads (and then
  * zeroes the whole workspace).  width and inner: multiples of 8; up to 512 experts, top_k up to 16.
- * Operands and the rows of x start on 16 bytes, out on 8. */
+ * Operands and the rows of x start on 16 bytes, out on 8.  out may be x itself; with more than 64 tokens it
+ * must not overlap x otherwise (TAO_ERR_ARG). */
 size_t tao_expert_workspace_bytes(const TaoExperts* layer, int tokens);
 int tao_expert_layer(const TaoExperts* layer, const void* x, long long x_stride, int tokens, void* out,
                      int* ids, float* id_weights, void* workspace, size_t workspace_bytes,

@@ -677,6 +677,11 @@ int tao_expert_layer(const TaoExperts* p, const void* x, long long x_stride, int
                                p->down_row};
   for (int i = 0; i < (p->group ? 1 : 7); ++i)
     if (strides[i] % 8) return efail(TAO_ERR_ARG, "the expert layer's rows start on 16 bytes");
+  // a launch writes after its last read of x; a later one's rows it may not write, unless it has read them itself
+  const long long row = p->width * 2LL;
+  if (tokens > kTokens && !(out == x && x_stride == p->width) &&
+      rows_overlap(x, tokens, x_stride * 2, row, out, tokens * row))
+    return efail(TAO_ERR_ARG, "the expert layer's output must not overlap a later launch's tokens");
   if (workspace_bytes < tao_expert_workspace_bytes(p, tokens)) return efail(TAO_ERR_ARG, "workspace too small");
   auto M = [](const void* at, long long e, long long r) { return Matrix16{static_cast<const bf16*>(at), e, r}; };
   auto F = [](const void* c, const void* s, const void* z) {

@@ -100,7 +100,8 @@ def expert_layer(x, weights, out=None, return_routing=False):
     [..., top_k] int32 (most probable first, ties to the lowest) and their weights in fp32.
 
     One launch for 64 tokens; made for the few tokens of a decode step, it reads the chosen
-    experts again for each 64 more.  No gradient."""
+    experts again for each 64 more.  ``out`` may be x itself; with more than 64 tokens it must not
+    overlap x otherwise.  No gradient."""
     if not isinstance(weights, ExpertWeights):
         raise ValueError("expert_layer takes ExpertWeights")
     if x.dtype != _BF16 or not x.is_cuda or x.device != weights.device:

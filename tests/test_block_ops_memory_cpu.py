@@ -43,3 +43,18 @@ def test_a_products_output_does_not_overlap_its_operands():
     assert _overlaps(x, x + 4 * 128 - 2, x_type=3)
     assert _overlaps(x, x + 4096, x_type=3, x_scale=x + 4096 + size - 4)
     assert _overlaps(x, x + 4096, bias=x + 4096 + size - 2)
+
+
+def test_an_expert_layers_output_does_not_overlap_a_later_launchs_tokens():
+    # 64 tokens a launch: rows of a later one would be read after this one wrote them
+    x, row = 1 << 24, 16
+
+    def refused(out, tokens, stride=8):
+        return _experts(x, out, tokens, stride) == _lib.TAO_ERR_ARG and b"overlap" in _lib.lib().tao_last_error()
+
+    for out in (x + row, x - row, x + 199 * row, x - 199 * row):
+        assert refused(out, 200), out - x
+    assert refused(x, 200, stride=16) and refused(x, 200, stride=0)  # rows over others' rows
+    # a launch writes after its last read of x; the same rows; rows next to each other
+    for out, tokens in ((x, 64), (x + row, 64), (x, 200), (x + 200 * row, 200), (x - 200 * row, 200)):
+        assert not refused(out, tokens), (out - x, tokens)

@@ -69,3 +69,23 @@ def test_a_products_out_beside_its_activations():
     assert torch.equal(linear4(x, w, bias=bias, out=room[320:448].view(2, 64)), linear4(x, w, bias=bias))
     with pytest.raises(ValueError, match="overlap"):
         linear4(x, w, bias=bias, out=room[300:428].view(2, 64))
+
+
+@pytest.mark.parametrize("tokens", [3, 64, 65, 200])
+def test_an_expert_layers_out_over_its_tokens(tokens):
+    from tao_memory_b200 import expert_layer
+    layer = _layer()
+    x = torch.randn(tokens, 64, device="cuda").bfloat16()
+    want = expert_layer(x, layer)
+    same = x.clone()
+    assert torch.equal(expert_layer(same, layer, out=same), want)
+    for shift, off in ((1, 1), (1, 0), (0, 1)):
+        room = torch.zeros(tokens + 2, 64, device="cuda", dtype=torch.bfloat16)
+        room[shift:shift + tokens] = x
+        out = room[off:off + tokens]
+        if shift == off or tokens <= 64:
+            assert torch.equal(expert_layer(room[shift:shift + tokens], layer, out=out), want)
+        else:
+            with pytest.raises(ValueError, match="overlap"):
+                expert_layer(room[shift:shift + tokens], layer, out=out)
+            assert torch.equal(room[shift:shift + tokens], x)
