@@ -26,15 +26,24 @@ def _padded(t, n, k, value=0):
 class Weight4:
     """4-bit weights [..., n, k]: W = (code - zero) * scale with one scale, and optionally one
     zero point, for ``group`` consecutive k of a row.  Leading axes are matrices of a stack
-    (one for each expert)."""
+    (one for each expert).  May be copied, saved and loaded; its tensors cannot be exchanged."""
 
     def __init__(self, shape, group, codes, scales, zeros):
         self.shape, self.group = tuple(shape), group
-        self.codes, self.scales, self.zeros = codes, scales, zeros
-        self.dtype, self.device = scales.dtype, codes.device
-        # what tao_linear4 takes of it
-        self.args = (codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
-                     TYPES[scales.dtype])
+        self._tensors = codes, scales, zeros
+
+    codes = property(lambda self: self._tensors[0])
+    scales = property(lambda self: self._tensors[1])
+    zeros = property(lambda self: self._tensors[2])
+    dtype = property(lambda self: self._tensors[1].dtype)
+    device = property(lambda self: self._tensors[0].device)
+
+    @property
+    def args(self):
+        """What tao_linear4 takes of it: of the tensors as they are now, which a copy or a file keeps apart."""
+        codes, scales, zeros = self._tensors
+        return (codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), self.group,
+                TYPES[scales.dtype])
 
     def bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)

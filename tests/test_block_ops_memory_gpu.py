@@ -89,3 +89,23 @@ def test_an_expert_layers_out_over_its_tokens(tokens):
             with pytest.raises(ValueError, match="overlap"):
                 expert_layer(room[shift:shift + tokens], layer, out=out)
             assert torch.equal(room[shift:shift + tokens], x)
+
+
+def test_a_copied_or_loaded_weight_outlives_its_original():
+    import copy
+    import io
+    from tao_memory_b200 import linear4, quantize4
+    w = quantize4(torch.randn(96, 256, device="cuda").bfloat16(), zeros=True)
+    x = torch.randn(3, 256, device="cuda").bfloat16()
+    want = linear4(x, w)
+    file = io.BytesIO()
+    torch.save(w, file)
+    file.seek(0)
+    others = [copy.deepcopy(w), torch.load(file, weights_only=False)]
+    for t in (w.codes, w.scales, w.zeros):
+        t.zero_()  # what the original's memory holds no longer matters
+    for other in others:
+        assert torch.equal(linear4(x, other), want)
+    file.seek(0)
+    with pytest.raises(ValueError):
+        linear4(x, torch.load(file, weights_only=False, map_location="cpu"))
