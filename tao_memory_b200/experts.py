@@ -20,7 +20,8 @@ class ExpertWeights:
     """One layer's router and experts: router [experts, width] bf16; gate, up [experts, inner,
     width] and down [experts, width, inner], all bf16 tensors (views of a fused tensor are taken
     as they are where their rows start on 16 bytes) or all ``Weight4`` stacks of one group and
-    kind.  ``renormalize``: the chosen experts' softmax weights are divided by their sum."""
+    kind.  ``renormalize``: the chosen experts' softmax weights are divided by their sum.  May be
+    copied, saved and loaded; its tensors cannot be exchanged."""
 
     def __init__(self, router, gate, up, down, top_k, renormalize=True):
         four = [isinstance(w, Weight4) for w in (gate, up, down)]
@@ -44,25 +45,43 @@ class ExpertWeights:
             raise ValueError("top_k is 1 to 16 and at most the number of experts")
         self.width, self.inner, self.experts, self.top_k = width, inner, experts, top_k
         self.renormalize, self.device = bool(renormalize), router.device
-        self.router = _aligned(router)
-        if all(four):
-            self.gate, self.up, self.down = gate, up, down
-            data = [[w.codes, w.scales, w.zeros] for w in (gate, up, down)]
-            strides, group = [0] * 6, gate.group
-        else:
-            self.gate, self.up, self.down = (_aligned(w) for w in (gate, up, down))
-            data = [[w, None, None] for w in (self.gate, self.up, self.down)]
-            strides, group = [s for w in (self.gate, self.up, self.down) for s in w.stride()[:2]], 0
-        at = lambda t: None if t is None else t.data_ptr()
-        if self.router.stride(0) != width:
-            self.router = self.router.contiguous()
-        self._layer = _lib.TaoExperts(at(self.router), *(at(d[i]) for i in range(3) for d in data), *strides, width,
-                                      inner, experts, top_k, group, int(self.renormalize))
+        if not all(four):
+            gate, up, down = (_aligned(w) for w in (gate, up, down))
+        router = _aligned(router)
+        if router.stride(0) != width:
+            router = router.contiguous()
+        self._weights = router, gate, up, down
+        self._four, self._layer_at = all(four), None
         lib = _lib.lib()
-        one, most = (lib.tao_expert_workspace_bytes(ctypes.byref(self._layer), n) for n in (1, _TOKENS))
-        if one == 0:
+        self._workspace_bytes = lib.tao_expert_workspace_bytes(self.layer(), _TOKENS)
+        if self._workspace_bytes == 0:
             _lib.check(_lib.TAO_ERR_ARG)
-        self._workspace_bytes, self._at = most, ctypes.byref(self._layer)
+
+    router = property(lambda self: self._weights[0])
+    gate = property(lambda self: self._weights[1])
+    up = property(lambda self: self._weights[2])
+    down = property(lambda self: self._weights[3])
+
+    def layer(self):
+        """What tao_expert_layer takes of it, of the tensors as they are now."""
+        router, *weights = self._weights
+        if self._four:
+            at = (router.data_ptr(), *(p for i in range(3) for p in (w.args[i] for w in weights)))
+        else:
+            at = (router.data_ptr(), *(w.data_ptr() for w in weights))
+        if at != self._layer_at:
+            strides = [0] * 6 if self._four else [s for w in weights for s in w.stride()[:2]]
+            self._layer = _lib.TaoExperts(*at, *(None,) * (10 - len(at)), *strides, self.width, self.inner,
+                                          self.experts, self.top_k, weights[0].group if self._four else 0,
+                                          int(self.renormalize))
+            self._layer_at = at
+        return ctypes.byref(self._layer)
+
+    def __getstate__(self):
+        return (*self._weights, self.top_k, self.renormalize)
+
+    def __setstate__(self, state):
+        self.__init__(*state)
 
 
 def _aligned(t):
@@ -127,7 +146,7 @@ def expert_layer(x, weights, out=None, return_routing=False):
         ids_at, route_at = ids.data_ptr(), route.data_ptr()
     device = x.device.index
     ws = _Room.get(x.device, torch._C._cuda_getCurrentRawStream(device), weights._workspace_bytes)
-    _lib.on_device(device, _lib.lib().tao_expert_layer, weights._at, rows.data_ptr(), rows.stride(0), rows.shape[0],
+    _lib.on_device(device, _lib.lib().tao_expert_layer, weights.layer(), rows.data_ptr(), rows.stride(0), rows.shape[0],
                    result.data_ptr(), ids_at, route_at, ws.data_ptr(), ws.numel())
     if result is not out:
         out.copy_(result)

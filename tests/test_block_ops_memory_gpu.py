@@ -109,3 +109,44 @@ def test_a_copied_or_loaded_weight_outlives_its_original():
     file.seek(0)
     with pytest.raises(ValueError):
         linear4(x, torch.load(file, weights_only=False, map_location="cpu"))
+
+
+@pytest.mark.parametrize("four", [False, True])
+def test_expert_weights_are_copied_and_loaded(four):
+    import copy
+    import io
+    from tao_memory_b200 import ExpertWeights, expert_layer, quantize4
+    layer = _layer()
+    if four:
+        layer = ExpertWeights(layer.router, *(quantize4(w, 32, zeros=True) for w in (layer.gate, layer.up, layer.down)),
+                              top_k=2, renormalize=False)
+    x = torch.randn(5, 64, device="cuda").bfloat16()
+    want = expert_layer(x, layer)
+    file = io.BytesIO()
+    torch.save(layer, file)
+    file.seek(0)
+    others = [copy.deepcopy(layer), torch.load(file, weights_only=False)]
+    tensors = [t for w in (layer.gate, layer.up, layer.down) for t in ((w.codes, w.scales, w.zeros) if four else (w,))]
+    for t in [layer.router, *tensors]:
+        t.zero_()
+    for other in others:
+        assert (other.top_k, other.renormalize) == (layer.top_k, layer.renormalize)
+        assert torch.equal(expert_layer(x, other), want)
+    file.seek(0)
+    with pytest.raises(ValueError):  # a layer is on a GPU
+        torch.load(file, weights_only=False, map_location="cpu")
+
+
+def test_expert_weights_follow_their_tensors():
+    """A tensor of a layer cannot be exchanged; one whose memory was (as modules do) is found there."""
+    from tao_memory_b200 import expert_layer
+    layer, other = _layer(seed=1), _layer(seed=2)
+    x = torch.randn(5, 64, device="cuda").bfloat16()
+    want, moved = expert_layer(x, other), expert_layer(x, layer)
+    for name in ("router", "gate", "up", "down"):
+        with pytest.raises(AttributeError):
+            setattr(layer, name, getattr(other, name))
+    assert torch.equal(expert_layer(x, layer), moved)
+    for name in ("router", "gate", "up", "down"):
+        getattr(layer, name).data = getattr(other, name).clone()
+    assert torch.equal(expert_layer(x, layer), want)
