@@ -517,15 +517,17 @@ typedef struct TaoExperts {
   const void *gate_zeros, *up_zeros, *down_zeros;    /* all or none */
   long long gate_expert, gate_row, up_expert, up_row, down_expert, down_row;
   int width, inner, experts, top_k, group, renormalize;
+  int* error; /* a word of the device that a wait that ran out sets beside the workspace's, or NULL: for
+                 workspaces that do not last, as a graph's */
 } TaoExperts;
 
 /* out [tokens][width] = sum over the top_k experts e of a token's softmax(x router^T) (ties to the
  * lowest expert) of weight * down_e(silu(gate_e x) * (up_e x)), weight the softmax, divided by its sum
  * over the chosen if `renormalize`.  x bf16, rows x_stride elements apart; sums in fp32 in a fixed
  * order, out rounded once.  ids, id_weights [tokens][top_k]: the choice, or NULL.  One cooperative
- * launch for 64 tokens.  workspace: tao_expert_workspace_bytes, zeroed before its first use, used
- * by one launch at a time; its first word is an error word that tao_expert_check reads (and then
- * zeroes the whole workspace).  width and inner: multiples of 8; up to 512 experts, top_k up to 16.
+ * launch for 64 tokens.  workspace: tao_expert_workspace_bytes, its first 256 bytes zeroed before its first
+ * use, used by one launch at a time; its first word is an error word that tao_expert_check reads (and
+ * then zeroes the whole workspace).  width and inner: multiples of 8; up to 512 experts, top_k up to 16.
  * Operands and the rows of x start on 16 bytes, out on 8.  out may be x itself; with more than 64 tokens it
  * must not overlap x otherwise (TAO_ERR_ARG). */
 size_t tao_expert_workspace_bytes(const TaoExperts* layer, int tokens);

@@ -44,7 +44,8 @@ class TaoExperts(ctypes.Structure):
                                                 "down_scales", "gate_zeros", "up_zeros", "down_zeros")]
                 + [(n, ctypes.c_longlong) for n in ("gate_expert", "gate_row", "up_expert", "up_row", "down_expert",
                                                     "down_row")]
-                + [(n, ctypes.c_int) for n in ("width", "inner", "experts", "top_k", "group", "renormalize")])
+                + [(n, ctypes.c_int) for n in ("width", "inner", "experts", "top_k", "group", "renormalize")]
+                + [("error", ctypes.c_void_p)])
 
 
 class TaoError(RuntimeError):

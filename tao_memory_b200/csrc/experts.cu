@@ -58,7 +58,7 @@ struct ExpertArgs {
   bf16* out;
   int* ids;          // [tokens][top_k] and their weights, or null
   float* id_weights;
-  int* error;
+  int *error, *device_error;  // the second may be null
   unsigned* barrier;
   float* logits;     // [tokens][experts]
   bf16* h;           // [2][pairs][inner]: rounded, and what the rounding left
@@ -150,7 +150,10 @@ TAO_DEVI bool grid_meet(const ExpertArgs& a, Shared& s, uint32_t& bit) {
       ok = ((now ^ bit) & 0x80000000u) != 0;
     }
     bit ^= 0x80000000u;
-    if (!ok) atomicOr(a.error, kErrWaitTimeout);
+    if (!ok) {
+      atomicOr(a.error, kErrWaitTimeout);
+      if (a.device_error) atomicOr(a.device_error, kErrWaitTimeout);
+    }
     s.ok = ok;
   }
   __syncthreads();
@@ -714,6 +717,7 @@ int tao_expert_layer(const TaoExperts* p, const void* x, long long x_stride, int
     a.ids = ids ? ids + (long long)at * p->top_k : nullptr;
     a.id_weights = ids ? id_weights + (long long)at * p->top_k : nullptr;
     a.error = reinterpret_cast<int*>(ws);
+    a.device_error = p->error;
     a.barrier = reinterpret_cast<unsigned*>(ws + 128);
     a.logits = reinterpret_cast<float*>(ws + room.logits);
     a.h = reinterpret_cast<bf16*>(ws + room.h);

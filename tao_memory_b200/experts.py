@@ -4,7 +4,6 @@ read the chosen experts.  Weights in bf16 or 4 bits (``Weight4`` stacks).
 """
 
 import ctypes
-import weakref
 
 import torch
 
@@ -14,6 +13,7 @@ from .norm import _rows
 
 _BF16 = torch.bfloat16
 _TOKENS = 64  # of one launch
+_HEADER = 256  # bytes of a workspace that have to be zero at first
 
 
 class ExpertWeights:
@@ -52,6 +52,7 @@ class ExpertWeights:
             router = router.contiguous()
         self._weights = router, gate, up, down
         self._four, self._layer_at = all(four), None
+        self._error = _error_word(self.device)
         lib = _lib.lib()
         self._workspace_bytes = lib.tao_expert_workspace_bytes(self.layer(), _TOKENS)
         if self._workspace_bytes == 0:
@@ -73,7 +74,7 @@ class ExpertWeights:
             strides = [0] * 6 if self._four else [s for w in weights for s in w.stride()[:2]]
             self._layer = _lib.TaoExperts(*at, *(None,) * (10 - len(at)), *strides, self.width, self.inner,
                                           self.experts, self.top_k, weights[0].group if self._four else 0,
-                                          int(self.renormalize))
+                                          int(self.renormalize), self._error.data_ptr())
             self._layer_at = at
         return ctypes.byref(self._layer)
 
@@ -90,18 +91,28 @@ def _aligned(t):
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+_ERRORS = {}
+
+
+def _error_word(device):
+    """The device's word of waits that ran out, which outlives workspaces and the graphs that hold one."""
+    if device not in _ERRORS:
+        _ERRORS[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return _ERRORS[device]
+
+
 class _Room:
     """Workspaces of the expert layer: zeroed once, one for a device and stream, so calls on
-    two streams do not meet in one; a captured call gets one of its own, zeroed by its graph."""
+    two streams do not meet in one; a captured call gets one of its own, whose header its graph
+    zeroes."""
 
     cache = {}
-    captured = {}
 
     @classmethod
     def get(cls, device, stream, nbytes):
         if torch.cuda.is_current_stream_capturing():
-            buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-            cls.captured.setdefault(device, weakref.WeakSet()).add(buf)
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            buf[:_HEADER].zero_()
             return buf
         buf = cls.cache.get((device, stream))
         if buf is None or buf.numel() < nbytes:
@@ -110,7 +121,7 @@ class _Room:
 
     @classmethod
     def on_device(cls, device):
-        return [b for (d, _), b in list(cls.cache.items()) if d == device] + list(cls.captured.get(device, ()))
+        return [b for (d, _), b in list(cls.cache.items()) if d == device]
 
 
 def expert_layer(x, weights, out=None, return_routing=False):
@@ -154,11 +165,20 @@ def expert_layer(x, weights, out=None, return_routing=False):
 
 
 def check_workspaces(device):
-    """Raise if an expert layer on ``device`` reported an error since the last check (part of
-    ``stream.check_device``; the device is synchronised)."""
+    """Raise if an expert layer on ``device``, in a graph or not, reported an error since the last check
+    (part of ``stream.check_device``; the device is synchronised)."""
     stream = torch.cuda.current_stream(device).cuda_stream
+    failed = False
     for ws in _Room.on_device(device):
-        _lib.check(_lib.lib().tao_expert_check(ws.data_ptr(), ws.numel(), None, stream))
+        rc = _lib.lib().tao_expert_check(ws.data_ptr(), ws.numel(), None, stream)
+        if rc != _lib.TAO_ERR_DEVICE:
+            _lib.check(rc)
+        failed |= rc != _lib.TAO_OK
+    if device in _ERRORS and int(_ERRORS[device]):
+        _ERRORS[device].zero_()
+        failed = True
+    if failed:  # said once, with every word cleared
+        raise _lib.TaoError("an expert layer's blocks did not meet in time")
 
 
 __all__ = ["ExpertWeights", "expert_layer"]
