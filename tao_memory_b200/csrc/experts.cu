@@ -739,8 +739,11 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaMemcpyAsync(&host, workspace, sizeof(int), cudaMemcpyDeviceToHost, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  // a wait that ran out leaves the barrier anywhere: all of it starts again
-  if (e == cudaSuccess && host) e = cudaMemsetAsync(workspace, 0, workspace_bytes, s);
+  // a wait that ran out leaves the barrier anywhere: all of it starts again, before a launch on any stream
+  if (e == cudaSuccess && host) {
+    e = cudaMemsetAsync(workspace, 0, workspace_bytes, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
   if (e != cudaSuccess) return efail(TAO_ERR_CUDA, cudaGetErrorString(e));
   if (flags) *flags = host;
   return host ? efail(TAO_ERR_DEVICE, "an expert layer's blocks did not meet in time") : TAO_OK;

@@ -82,3 +82,17 @@ def test_an_error_survives_its_workspace():
     with pytest.raises(_lib.TaoError, match="did not meet"):
         check_device()
     assert check_device() == 0
+
+
+def test_a_workspace_is_reset_when_its_check_returns():
+    """A launch on another stream may use it at once."""
+    from tao_memory_b200 import _lib
+    room = torch.full((1 << 30,), 7, device="cuda", dtype=torch.uint8)  # its reset takes 100 us and more
+    room[:4] = torch.tensor([1, 0, 0, 0], dtype=torch.uint8)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    flags = ctypes.c_int(0)
+    rc = _lib.lib().tao_expert_check(room.data_ptr(), room.numel(), ctypes.byref(flags), side.cuda_stream)
+    done = side.query()
+    assert rc == _lib.TAO_ERR_DEVICE and flags.value == 1 and done
+    assert not room.any()
