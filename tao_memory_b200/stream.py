@@ -830,7 +830,9 @@ class _BatchGraph:
 
 def check_device(device=None):
     """Raise if a kernel on ``device`` reported an error since the last check."""
-    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    dev = torch.device("cuda" if device is None else device)
+    if dev.index is None:  # the buffers are known by the index
+        dev = torch.device("cuda", torch.cuda.current_device())
     current = torch.cuda.current_stream(dev).cuda_stream
     flags = ctypes.c_int(0)
     total = 0

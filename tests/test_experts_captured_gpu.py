@@ -96,3 +96,15 @@ def test_a_workspace_is_reset_when_its_check_returns():
     done = side.query()
     assert rc == _lib.TAO_ERR_DEVICE and flags.value == 1 and done
     assert not room.any()
+
+
+@pytest.mark.parametrize("device", ["cuda", "cuda:0", 0, None])
+def test_a_device_without_its_index_is_the_current_one(device):
+    from tao_memory_b200 import _lib, experts
+    from tao_memory_b200.stream import check_device
+    _layer()
+    assert check_device(device) == 0
+    experts._error_word(torch.device("cuda", 0)).fill_(1)
+    with pytest.raises(_lib.TaoError, match="did not meet"):
+        check_device(device)
+    assert check_device(device) == 0
