@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .linear4 import Weight4
-from .norm import _rows
+from .norm import _rows, refuse_tangents
 
 _BF16 = torch.bfloat16
 _TOKENS = 64  # of one launch
@@ -62,6 +62,12 @@ class ExpertWeights:
     gate = property(lambda self: self._weights[1])
     up = property(lambda self: self._weights[2])
     down = property(lambda self: self._weights[3])
+
+    @property
+    def floats(self):
+        """The tensors that a derivative could be taken of."""
+        router, *weights = self._weights
+        return (router, *(w.scales if self._four else w for w in weights))
 
     def layer(self):
         """What tao_expert_layer takes of it, of the tensors as they are now."""
@@ -140,6 +146,7 @@ def expert_layer(x, weights, out=None, return_routing=False):
         raise ValueError(f"activations have {weights.width} channels, as the layer")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("expert_layer has no gradient: call it under torch.no_grad()")
+    refuse_tangents("expert_layer", x, *weights.floats)
     rows = _rows(x, weights.width)
     if rows.data_ptr() % 16 or rows.stride(0) % 8:
         rows = rows.clone(memory_format=torch.contiguous_format)

@@ -7,6 +7,7 @@ that adds the blocks' parts in a fixed order.
 """
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -20,6 +21,13 @@ def _rows(t, width):
     if t.dim() != 2:
         t = t.reshape(-1, width)
     return t if t.stride(1) == 1 or width == 1 else t.contiguous()
+
+
+def refuse_tangents(operator, *operands):
+    """Forward-mode derivatives would be dropped with the operands' addresses."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in operands):
+        raise ValueError(f"{operator} has no forward-mode derivative")
 
 
 def _check(x, weight, residual):
@@ -116,8 +124,9 @@ def add_rms_norm(x, weight=None, residual=None, eps=RMS_EPS):
     """(y, s): s = x + residual rounded to x's type (the stream the next block adds to; x
     itself without a residual) and y = s * rsqrt(mean(s^2) + eps) * weight over the last axis,
     in fp32, rounded once.  x, residual [..., width] bf16, fp16 or fp32; weight [width] of the
-    same type or None (ones).  Differentiable in x, residual and weight."""
+    same type or None (ones).  Differentiable (in reverse mode) in x, residual and weight."""
     _check(x, weight, residual)
+    refuse_tangents("add_rms_norm", x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         if residual is None:
@@ -131,6 +140,7 @@ def add_rms_norm_fp8(x, weight=None, residual=None, eps=RMS_EPS, group=None):
     (``group=None``: scale [..., 1], as ``linear4`` and row-scaled products take it) or one for
     128 channels (``group=128``: [..., ceil(width / 128)]).  Not differentiable."""
     _check(x, weight, residual)
+    refuse_tangents("add_rms_norm_fp8", x, weight, residual)
     if group not in (None, 128):
         raise ValueError("8-bit scales are by row (None) or by 128 channels")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
