@@ -9,7 +9,7 @@ the codes in the order in which the kernel's warps read them (laid out once, her
 import torch
 
 from . import _lib
-from .norm import TYPES, _rows, refuse_tangents
+from .norm import TYPES, _rows, refuse_tangents, wants_gradient
 
 GROUPS = (32, 64, 128)
 E4M3 = 3  # the library's code of the type, beside TYPES
@@ -156,8 +156,8 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
         code = E4M3
     elif x.dtype != dtype:
         raise ValueError("activations have the type of the weight's scales, or are e4m3")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("linear4 has no gradient: call it under torch.no_grad()")
+    if wants_gradient(x, x_scale, bias, weight.scales):
+        raise ValueError("linear4 has no gradient, for activations or weights: call it under torch.no_grad()")
     refuse_tangents("linear4", x, x_scale, bias, weight.scales)
     rows = _rows(x, k)
     count = rows.shape[0]

@@ -23,6 +23,14 @@ def _rows(t, width):
     return t if t.stride(1) == 1 or width == 1 else t.contiguous()
 
 
+def wants_gradient(*operands):
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def refuse_tangents(operator, *operands):
     """Forward-mode derivatives would be dropped with the operands' addresses."""
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
@@ -127,8 +135,7 @@ def add_rms_norm(x, weight=None, residual=None, eps=RMS_EPS):
     same type or None (ones).  Differentiable (in reverse mode) in x, residual and weight."""
     _check(x, weight, residual)
     refuse_tangents("add_rms_norm", x, weight, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if wants_gradient(x, weight, residual):
         if residual is None:
             return _AddNorm.apply(x, weight, None, eps), x
         return _AddNorm.apply(x, weight, residual, eps)
@@ -143,8 +150,7 @@ def add_rms_norm_fp8(x, weight=None, residual=None, eps=RMS_EPS, group=None):
     refuse_tangents("add_rms_norm_fp8", x, weight, residual)
     if group not in (None, 128):
         raise ValueError("8-bit scales are by row (None) or by 128 channels")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if wants_gradient(x, weight, residual):
         raise ValueError("the 8-bit norm has no gradient: call it under torch.no_grad()")
     width = x.shape[-1]
     rows = _rows(x, width)
