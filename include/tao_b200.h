@@ -493,7 +493,8 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
  * W[n][k] = (code - zero) * scale, one scale (and zero point) for `group` (32, 64 or 128)
  * consecutive k of a row, codes and zeros 0..15, zeros NULL: 8.  `type`: bf16 or fp16, the
  * type of scales, bias and y.  x_type: the same, or TAO_TYPE_E4M3 with x_scale [rows] fp32 (NULL: ones).
- * Products are summed in fp32 over a group, scaled, summed in fp32, rounded once.
+ * Products are summed in fp32 over a group, scaled, summed in fp32, rounded once; one or two rows of x are
+ * held as whole multiples of 2^-26 to 2^-27 of the largest magnitude of their 128 k, whose group sums are exact.
  * Layout (tiles = ceil(n / 16), blocks = ceil(k / 128), what lies beyond n or k has scale 0):
  *   codes  [tiles][blocks][2][32][16] bytes: byte 8i + 4f + e of lane 4g + t of half h holds the codes of
  *          k = 128 block + 64h + 32i + 8t + 4f + (0, 2, 1, 3)[e], of row 16 tile + g in its low nibble and

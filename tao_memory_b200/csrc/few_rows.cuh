@@ -10,10 +10,13 @@
 //
 // A few rows (product8): the codes 0..15 go as bytes into the integer mma.m16n8k32, three
 // instructions for eight of them.  The activations become sums of signed bytes under a power of
-// two s for each row and 128 k,  x = s (p0 + p1 / 2^7 + p2 / 2^14)  up to 2^-21 of the 128's largest
-// magnitude, a column of the mma for each piece (and an empty fourth).  Over a group
-//   sum of (q - zero) x = s 2^-7 (sum of q P - zero sum of P) + s 2^-14 (the same of p2),  P = 2^7 p0 + p1,
-// whole numbers below 2^31, so a group's product is exact; fp32 sums over the groups.
+// two s for each row and 128 k,  x = s (p0 + p1 / 2^7 + p2 / 2^14 + p3 / 2^21),  a column of the mma for
+// each piece.  The 128's largest magnitude is 32 s to 64 s, so x is held to 2^-27 of it, finer than the 2^-24 of
+// that magnitude to which fp32 sums of its products would go: no caller's channel is lost beside one 10^5 times larger.
+// Over a group
+//   sum of (q - zero) x = s 2^-7 (sum of q P - zero sum of P) + s 2^-21 (the same of Q),
+//   P = 2^7 p0 + p1,  Q = 2^7 p2 + p3,
+// whole numbers below 2^24, so a group's product is exact in fp32; fp32 sums over the groups.
 // More rows (product16): codes become 16-bit floats with their zero point subtracted, exactly, for
 // mma.m16n8k16: eleven instructions for eight, but one column a row.
 //
@@ -91,36 +94,32 @@ struct MmaF16 {
   }
 };
 
-// 2^14 / s and s / 2^7 of a 128's largest magnitude: x / s is below 64.  A magnitude that is no finite
+// 2^21 / s and s / 2^7 of a 128's largest magnitude: x / s is below 64.  A magnitude that is no finite
 // number makes both no numbers.
 TAO_DEVI void units_of(float most, float& up, float& unit) {
   const uint32_t e = __float_as_uint(most) >> 23;  // of a magnitude: no sign
-  const uint32_t f = e > 22 ? e - 5 : 17u;         // the exponent of s; 2^14 / s and s / 2^14 are normal numbers
-  up = __uint_as_float(e == 255 ? 0x7fc00000u : (254 + 14 - f) << 23);
+  const uint32_t f = e > 26 ? e - 5 : 21u;         // the exponent of s; 2^21 / s is a normal number
+  up = __uint_as_float(e == 255 ? 0x7fc00000u : (254 + 21 - f) << 23);
   unit = __uint_as_float(e == 255 ? 0x7fc00000u : (f - 7) << 23);
 }
 
-// Eight 2^14 x / s (below 2^20 in magnitude), rounded to whole numbers, as three pieces of 8 signed
-// bytes each in the order of the codes (digits of -64..63, the first up to 64), and the sums of P = 2^7 p0 + p1 and of p2.
-TAO_DEVI void split8(const float (&x)[8], uint2 (&p)[3], int& sum, int& sum2) {
-  uint32_t w[3][2] = {};
-  int all = 0;
-  sum2 = 0;
+// Eight 2^21 x / s (below 2^27 in magnitude), rounded to whole numbers, as four pieces of 8 signed
+// bytes each in the order of the codes (digits of -64..63, the first up to 64), and the sums of P and of Q.
+TAO_DEVI void split8(const float (&x)[8], uint2 (&p)[4], int& sum, int& sum2) {
+  uint32_t w[4][2] = {};
+  sum = sum2 = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // the addition rounds to a whole number and leaves it in the low bits (conversions are slow)
-    const int v = __float_as_int(x[i] + 12582912.f) - 0x4b400000;
-    const int v1 = (v + 64) >> 7, p2 = v - (v1 << 7);
-    const int v0 = (v1 + 64) >> 7, p1 = v1 - (v0 << 7);
-    const int q[3] = {v0, p1, p2};
+    const int v = __float2int_rn(x[i]);
+    const int v2 = (v + 64) >> 7, v1 = (v2 + 64) >> 7, v0 = (v1 + 64) >> 7;
+    const int q[4] = {v0, v1 - (v0 << 7), v2 - (v1 << 7), v - (v2 << 7)};
 #pragma unroll
-    for (int j = 0; j < 3; ++j) w[j][i / 4] |= (uint32_t)(q[j] & 0xff) << (8 * (i % 4 * 2 % 3 + i % 4 / 3 * 3));
-    all += v1;
-    sum2 += p2;
+    for (int j = 0; j < 4; ++j) w[j][i / 4] |= (uint32_t)(q[j] & 0xff) << (8 * (i % 4 * 2 % 3 + i % 4 / 3 * 3));
+    sum += v1;
+    sum2 += v - (v1 << 14);
   }
-  sum = all;
 #pragma unroll
-  for (int j = 0; j < 3; ++j) p[j] = make_uint2(w[j][0], w[j][1]);
+  for (int j = 0; j < 4; ++j) p[j] = make_uint2(w[j][0], w[j][1]);
 }
 
 // A 4-bit matrix laid out in blocks of 16 rows x 128 k, row tiles outermost.
@@ -182,11 +181,11 @@ struct Block4 {
   }
 
   // Adds to acc[n][0..1] rows g and g + 8 of the block's product with the row of x whose pieces 0 and 1
-  // (t even) or 2 (t odd) are columns 2t, 2t + 1 of column tile n; the row's whole product is the sum over
+  // (t even) or 2 and 3 (t odd) are columns 2t, 2t + 1 of column tile n; the row's whole product is the sum over
   // the two lanes.  `b(h, n)`: the lane's 16 bytes of half h; `xsum(j, n)`: the sum over group j of P (t odd:
-  // of p2); `unit(n)`: s / 2^7 (t odd: s / 2^14).
+  // of Q); `unit(n)`: s / 2^7 (t odd: s / 2^21).
   template <bool BF16_SCALES, int NT, class B, class X, class U>
-  TAO_DEVI void product8(float (&acc)[NT][2], bool odd, B b, X xsum, U unit) const {
+  TAO_DEVI void product8(float (&acc)[NT][2], B b, X xsum, U unit) const {
     constexpr uint32_t MASK = 0x0f0f0f0fu;
     uint32_t a[4][4];
 #pragma unroll
@@ -196,7 +195,6 @@ struct Block4 {
         a[u][2 * i] = word(u, i) & MASK;
         a[u][2 * i + 1] = word(u, i) >> 4 & MASK;
       }
-    const int m0 = odd ? 1 : 128, m1 = odd ? 0 : 1;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint4 x0 = b(0, n), x1 = b(1, n);
@@ -217,8 +215,8 @@ struct Block4 {
         const int z0 = zeros(j) & 0xff, z1 = zeros(j) >> 8 & 0xff;
         const int xs = xsum(j, n);
         const float2 sc = scales<BF16_SCALES>(j);
-        acc[n][0] += sc.x * un * (float)(d[0] * m0 + d[1] * m1 - z0 * xs);
-        acc[n][1] += sc.y * un * (float)(d[2] * m0 + d[3] * m1 - z1 * xs);
+        acc[n][0] += sc.x * un * (float)(d[0] * 128 + d[1] - z0 * xs);
+        acc[n][1] += sc.y * un * (float)(d[2] * 128 + d[3] - z1 * xs);
       }
     }
   }

@@ -36,15 +36,15 @@ constexpr int kMaxK = 65536;  // two rows' pieces of a cluster of 8's part fit b
 struct Bytes {};
 
 // COLS: columns of the mma for a row; WARPS: of a block; DEPTH: blocks of a warp's ring.  Shared memory of a
-// block's 128 k of x: bytes have a row's three pieces as [half][3 row + piece][t] 16 bytes, a lane's
-// operands in the order of the lanes, then [row] s / 2^7, then [group][row] the sums (P, p2); 16 bits have
+// block's 128 k of x: bytes have a row's four pieces as [half][4 row + piece][t] 16 bytes, a lane's
+// operands in the order of the lanes, then [row] s / 2^7, then [group][row] the sums (P, Q); 16 bits have
 // [32-k part][row][t] 16 bytes.
 template <class M, int GROUP, int NT>
 struct Form {
   static constexpr bool BYTES = std::is_same<M, Bytes>::value;
   static constexpr int COLS = BYTES ? 4 : 1, ROWS = 8 * NT / COLS, GROUPS = 128 / GROUP;
   static constexpr int WARPS = 16, DEPTH = 6;
-  static constexpr int UNITS = ROWS * 384, SUMS = UNITS + ROWS * 4 + ROWS * 4 % 8;
+  static constexpr int UNITS = ROWS * 512, SUMS = UNITS + ROWS * 4 + ROWS * 4 % 8;
   static constexpr int XBLOCK = BYTES ? (SUMS + GROUPS * ROWS * 8 + 15) / 16 * 16 : ROWS * 256;
 };
 
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_ker
         units_of(most, up, unit);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= up;
-        uint2 p[3];
+        uint2 p[4];
         int2 sum;
         split8(f, p, sum.x, sum.y);
 #pragma unroll
@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_ker
           if (l == 0) reinterpret_cast<float*>(to + F::UNITS)[m] = unit;
           if (l % (GROUP / 8) == 0) reinterpret_cast<int2*>(to + F::SUMS)[l / (GROUP / 8) * ROWS + m] = sum;
 #pragma unroll
-          for (int c = 0; c < 3; ++c)
-            *reinterpret_cast<uint2*>(to + ((l / 8 * ROWS * 3 + m * 3 + c) * 4 + l % 4) * 16 + l / 4 % 2 * 8) = p[c];
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint2*>(to + ((l / 8 * ROWS * 4 + m * 4 + c) * 4 + l % 4) * 16 + l / 4 % 2 * 8) = p[c];
         }
       } else if (in) {
         *reinterpret_cast<uint4*>(to + ((l / 4 * ROWS + m) * 4 + l % 4) * 16) = v;
@@ -155,15 +155,14 @@ __global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_ker
   }
   __syncthreads();
 
-  // What this lane reads of a block of x.  Columns without a row hold anything, a row's empty fourth
-  // reads another piece; nothing uses what they give.
+  // What this lane reads of a block of x.  Columns without a row hold anything; nothing uses what they give.
   constexpr int OUTS = BYTES ? 2 : 4;
-  constexpr int NEXT = BYTES ? 2 * 3 * 64 : 8 * 64;  // bytes to the next column tile
+  constexpr int NEXT = 8 * 64;  // bytes to the next column tile
   const uint8_t* const xfirst = smem + kw * F::XBLOCK;
   const uint8_t* xblock = xfirst;
-  const int xlane = ((BYTES ? g / 4 * 3 + min(g % 4, 2) : g) * 4 + t) * 16;
+  const int xlane = (g * 4 + t) * 16;
   const int ulane = F::UNITS + t / 2 * 4, slane = F::SUMS + t / 2 * 8 + (t & 1) * 4;
-  const float part = t & 1 ? 1.f / 128.f : 1.f;
+  const float part = t & 1 ? 1.f / 16384.f : 1.f;
   const int slot = rows * 16;  // floats of a warp's sums of a tile
   float* const sums = reinterpret_cast<float*>(smem + a.sums);  // [step][warp][row][16]
   float* to = sums + warp * slot;
@@ -172,8 +171,8 @@ __global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_ker
   auto product = [&](const B4& b) {
     if constexpr (BYTES) {
       b.template product8<BF16, NT>(
-          acc, t & 1,
-          [&](int h, int n) { return *reinterpret_cast<const uint4*>(xblock + xlane + n * NEXT + h * ROWS * 192); },
+          acc,
+          [&](int h, int n) { return *reinterpret_cast<const uint4*>(xblock + xlane + n * NEXT + h * ROWS * 256); },
           [&](int j, int n) { return *reinterpret_cast<const int*>(xblock + slane + (j * ROWS + n * 2) * 8); },
           [&](int n) { return *reinterpret_cast<const float*>(xblock + ulane + n * 8) * part; });
     } else {

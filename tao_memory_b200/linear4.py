@@ -141,8 +141,9 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
     (``x_scale`` [..., 1], as ``add_rms_norm_fp8`` gives them); returns [..., n] in the weight's type.
 
     Made for few rows (a decode step's): the weight is read once for up to 64 rows, and from L2
-    for each 64 more.  ``out`` must not overlap an operand.  One or two rows are taken as fixed-point numbers, to 2^-21 of the largest
-    magnitude of their 128 channels; more rows as they are.  No gradient."""
+    for each 64 more.  One or two rows are taken as fixed-point numbers, to 2^-27 of the largest
+    magnitude of their 128 channels; more rows as they are.  ``out`` must not overlap an operand.
+    No gradient."""
     if not isinstance(weight, Weight4) or len(weight.shape) != 2:
         raise ValueError("linear4 takes one Weight4 matrix")
     n, k = weight.shape
