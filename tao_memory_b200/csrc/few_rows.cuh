@@ -94,13 +94,14 @@ struct MmaF16 {
   }
 };
 
-// 2^21 / s and s / 2^7 of a 128's largest magnitude: x / s is below 64.  A magnitude that is no finite
-// number makes both no numbers.
+// 2^21 / s and s / 2^7 of a 128's largest magnitude: x / s is below 64.  What has no such form, a magnitude
+// that is no finite number or whose 2^21 / s would not be one, makes both no numbers, and with them the row's sums.
 TAO_DEVI void units_of(float most, float& up, float& unit) {
   const uint32_t e = __float_as_uint(most) >> 23;  // of a magnitude: no sign
   const uint32_t f = e > 26 ? e - 5 : 21u;         // the exponent of s; 2^21 / s is a normal number
-  up = __uint_as_float(e == 255 ? 0x7fc00000u : (254 + 21 - f) << 23);
-  unit = __uint_as_float(e == 255 ? 0x7fc00000u : (f - 7) << 23);
+  const bool none = e == 255 || (e < 27 && most > 0.f);
+  up = __uint_as_float(none ? 0x7fc00000u : (254 + 21 - f) << 23);
+  unit = __uint_as_float(none ? 0x7fc00000u : (f - 7) << 23);
 }
 
 // Eight 2^21 x / s (below 2^27 in magnitude), rounded to whole numbers, as four pieces of 8 signed

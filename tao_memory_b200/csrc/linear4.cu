@@ -48,6 +48,42 @@ struct Form {
   static constexpr int XBLOCK = BYTES ? (SUMS + GROUPS * ROWS * 8 + 15) / 16 * 16 : ROWS * 256;
 };
 
+// Outputs n..n + 3 (n a multiple of 4) of row m term by term, for rows of x that signed bytes cannot hold.  Rare
+// (an infinity, a NaN, 128 channels that are all below 2^-100 and not all zero) and slow: a row of k = n = 8192
+// takes 0.65 ms.
+template <bool BF16, int GROUP>
+TAO_DEVI float4 by_terms(const Linear4Args& a, long long m, int n) {
+  constexpr int GROUPS = 128 / GROUP;
+  float s[4] = {};
+#pragma unroll 1
+  for (int c = 0; c < a.kblocks * 16; ++c) {  // chunks of 8 k
+    const long long block = (long long)(n / 16) * a.kblocks + c / 16;
+    const int l = c % 16, group = l / (GROUP / 8);
+    uint4 v = chunk_of(a, m, c * 8);
+    if (a.x_type == TAO_TYPE_E4M3) v = widen_e4m3(v);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int g = n % 8 + e, high = n / 8 % 2;  // rows g and g + 8 of the tile share their bytes
+      const uint2 codes = __ldg(reinterpret_cast<const uint2*>(a.w.codes + block * 1024 + (l / 8) * 512 +
+                                                               (4 * g + l % 4) * 16 + l / 4 % 2 * 8));
+      const long long at = (block * 8 + g) * (GROUPS * 2) + group * 2 + high;
+      const uint16_t bits = __ldg(reinterpret_cast<const uint16_t*>(a.w.scales) + at);
+      const float scale = BF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+      const int zero = a.w.zeros ? __ldg(a.w.zeros + at) : 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 h = a.x_type == TAO_TYPE_BF16 ? make_float2(lo_f(w[i / 2]), hi_f(w[i / 2]))
+                                                   : __half22float2(*reinterpret_cast<const __half2*>(&w[i / 2]));
+        // byte b of word f is k 4f + (0, 2, 1, 3)[b]
+        const uint32_t byte = (i < 4 ? codes.x : codes.y) >> (8 * (i % 4 * 2 % 3 + i % 4 / 3 * 3));
+        s[e] += (float)((int)(byte >> (4 * high) & 15u) - zero) * scale * (i % 2 ? h.y : h.x);
+      }
+    }
+  }
+  return make_float4(s[0], s[1], s[2], s[3]);
+}
+
 // M: the form.  BF16: the type of scales, bias and y.  NT: column tiles of 8 columns of the mma.
 template <class M, bool BF16, int GROUP, int NT>
 __global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_kernel(const Linear4Args a) {
@@ -242,6 +278,16 @@ __global__ void __launch_bounds__(32 * Form<M, GROUP, NT>::WARPS, 1) linear4_ker
       for (int w = 0; w < 1 << (wks + a.shift); ++w) {
         const float4 v = ld_cluster(smem_u32(at + (w >> a.shift) * slot), w & ((1 << a.shift) - 1));
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+    }
+    if constexpr (BYTES) {
+      const bool x = s.x != s.x, y = s.y != s.y, z = s.z != s.z, w = s.w != s.w;
+      if (x || y || z || w) {
+        const float4 v = by_terms<BF16, GROUP>(a, m0 + m, n);
+        if (x) s.x = v.x;
+        if (y) s.y = v.y;
+        if (z) s.z = v.z;
+        if (w) s.w = v.w;
       }
     }
     const float xs = a.x_scale ? a.x_scale[m0 + m] : 1.f;

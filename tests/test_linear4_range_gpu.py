@@ -66,3 +66,48 @@ def test_a_row_alone_and_among_others(dtype):
         y = linear4(x[:count], w).double()
         off = _bound(xd[:count], wide, dtype, count, ref[:count]) + _bound(xd[:count], wide, dtype, 24, ref[:count])
         assert ((y - all_rows[:count]).abs() <= off).all()
+
+
+@pytest.mark.parametrize("size", [0.0, 1e-41, 1e-38, 2.0 ** -101, 2.0 ** -99, 1e-20, 1e20, 3e35])
+def test_one_row_of_any_magnitude(size):
+    """From subnormal rows to rows whose products are near the type's largest."""
+    from tao_memory_b200 import linear4
+    w, wide, _ = _case(1, 64, 512, 128, torch.bfloat16, 1.0, seed=2)
+    x = (torch.randn(2, 512, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).double() * size)
+    x = x.float().bfloat16()
+    x[1, 128:256] *= 2.0 ** -60  # of another size than its neighbours
+    xd = x.double()
+    ref = xd @ wide.T
+    y = linear4(x, w).double()
+    # y's own subnormals are 2^-133 apart
+    assert ((y - ref).abs() <= _bound(xd, wide, torch.bfloat16, 2, ref) + 2.0 ** -132).all()
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16, "fp8"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 9, 20])
+def test_infinities_and_nans_are_those_of_the_sum(rows, act, group):
+    """An infinity gives one of the weight's sign, none under a zero weight (infinity times zero is no
+    number), and two of unlike sign give no number: as in a sum term by term.  Other rows are untouched."""
+    from tao_memory_b200 import linear4
+    dtype = torch.bfloat16 if act == "fp8" else act
+    n, k, inf = 70, 1000, float("inf")
+    w, wide, clean = _case(rows, n, k, group, dtype, 1.0, seed=4)
+    for at, values in ((0, [(3, inf)]), (rows - 1, [(3, inf), (700, -inf)]), (0, [(5, -inf)]), (rows - 1, [(999, float("nan"))])):
+        x = clean.clone()
+        for c, v in values:
+            x[at, c] = v
+        scale = None
+        if act == "fp8":  # has no infinities: a NaN in their place
+            x = torch.where(x.isinf(), torch.full_like(x, float("nan")), x).to(torch.float8_e4m3fn)
+            scale = torch.rand(rows, 1, device="cuda") + 0.5
+        xd = x.to(torch.float32).double() * (1 if scale is None else scale.double())
+        terms = xd[at] * wide  # [n, k]
+        y = linear4(x, w, x_scale=scale)
+        bad = ~xd[at].isfinite()
+        want = terms[:, bad].sum(-1)  # decides over what is finite
+        assert torch.equal(y[at].isnan(), want.isnan())
+        assert torch.equal(y[at].isposinf(), want == inf) and torch.equal(y[at].isneginf(), want == -inf)
+        others = [i for i in range(rows) if i != at]
+        ref = xd[others] @ wide.T
+        assert ((y[others].double() - ref).abs() <= _bound(xd[others], wide, dtype, rows, ref)).all()
