@@ -126,9 +126,12 @@ def quantize4(weight, group=128, zeros=False):
     else:
         scales = torch.maximum(w.amax(-1) / 7, -w.amin(-1) / 8).to(dtype)
     step = scales.float()
+    # steps whose reciprocal would be infinite are taken 2^64 times as large, the weights with them
+    grow = torch.where(step < 2.0 ** -100, 2.0 ** 64, 1.0)
+    step, w = step * grow, w * grow.unsqueeze(-1)
     up = torch.where(step > 0, 1 / step, torch.zeros_like(step)).unsqueeze(-1)
     if zeros:
-        zero = (-low * up.squeeze(-1)).round().clamp(0, 15)
+        zero = (-low * grow * up.squeeze(-1)).round().clamp(0, 15)
         codes = ((w * up).round() + zero.unsqueeze(-1)).clamp(0, 15)
     else:
         zero, codes = None, ((w * up).round() + 8).clamp(0, 15)
