@@ -53,7 +53,7 @@ struct ExpertArgs {
   long long x_stride;
   Matrix16 router, gate16, up16, down16;
   Four gate4, up4, down4;
-  int tokens, width, inner, experts, top_k, group;
+  int tokens, width, inner, experts, top_k;
   bool renormalize;
   bf16* out;
   int* ids;          // [tokens][top_k] and their weights, or null
@@ -711,7 +711,6 @@ int tao_expert_layer(const TaoExperts* p, const void* x, long long x_stride, int
     a.inner = p->inner;
     a.experts = p->experts;
     a.top_k = p->top_k;
-    a.group = p->group;
     a.renormalize = p->renormalize != 0;
     a.out = static_cast<bf16*>(out) + (long long)at * p->width;
     a.ids = ids ? ids + (long long)at * p->top_k : nullptr;
