@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .linear4 import Weight4
-from .norm import _rows, refuse_tangents, wants_gradient
+from .norm import _rows, refuse_derivatives
 
 _BF16 = torch.bfloat16
 _TOKENS = 64  # of one launch
@@ -144,9 +144,7 @@ def expert_layer(x, weights, out=None, return_routing=False):
         raise ValueError("expert_layer takes bf16 CUDA activations on the weights' device (no CPU fallback)")
     if x.dim() == 0 or x.shape[-1] != weights.width:
         raise ValueError(f"activations have {weights.width} channels, as the layer")
-    if wants_gradient(x, *weights.floats):
-        raise ValueError("expert_layer has no gradient, for activations or weights: call it under torch.no_grad()")
-    refuse_tangents("expert_layer", x, *weights.floats)
+    refuse_derivatives("expert_layer", x, *weights.floats)
     rows = _rows(x, weights.width)
     if rows.data_ptr() % 16 or rows.stride(0) % 8:
         rows = rows.clone(memory_format=torch.contiguous_format)

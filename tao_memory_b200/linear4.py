@@ -9,7 +9,7 @@ the codes in the order in which the kernel's warps read them (laid out once, her
 import torch
 
 from . import _lib
-from .norm import TYPES, _rows, refuse_tangents, wants_gradient
+from .norm import TYPES, _rows, refuse_derivatives
 
 GROUPS = (32, 64, 128)
 E4M3 = 3  # the library's code of the type, beside TYPES
@@ -40,7 +40,7 @@ class Weight4:
 
     @property
     def args(self):
-        """What tao_linear4 takes of it: of the tensors as they are now, which a copy or a file keeps apart."""
+        """What tao_linear4 takes of it: of the tensors as they are now, not as they were before a copy or a file."""
         codes, scales, zeros = self._tensors
         return (codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), self.group,
                 TYPES[scales.dtype])
@@ -150,7 +150,8 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
     if not isinstance(weight, Weight4) or len(weight.shape) != 2:
         raise ValueError("linear4 takes one Weight4 matrix")
     n, k = weight.shape
-    device, dtype = weight.device, weight.dtype
+    scales = weight.scales
+    device, dtype = scales.device, scales.dtype
     if x.device != device or device.type != "cuda":
         raise ValueError("linear4 takes CUDA activations on the weight's device (no CPU fallback)")
     if x.dim() == 0 or x.shape[-1] != k:
@@ -160,9 +161,7 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
         code = E4M3
     elif x.dtype != dtype:
         raise ValueError("activations have the type of the weight's scales, or are e4m3")
-    if wants_gradient(x, x_scale, bias, weight.scales):
-        raise ValueError("linear4 has no gradient, for activations or weights: call it under torch.no_grad()")
-    refuse_tangents("linear4", x, x_scale, bias, weight.scales)
+    refuse_derivatives("linear4", x, x_scale, bias, scales)
     rows = _rows(x, k)
     count = rows.shape[0]
     scale_at = bias_at = None
@@ -176,9 +175,9 @@ def linear4(x, weight, bias=None, x_scale=None, out=None):
             raise ValueError("the bias is one value per output, of the weight's type and device")
         bias = bias.contiguous()
         bias_at = bias.data_ptr()
-    shape = (*x.shape[:-1], n)
+    shape = (count, n) if x.dim() == 2 else (*x.shape[:-1], n)
     if out is None:
-        out = x.new_empty(shape, dtype=dtype)
+        out = x.new_empty(shape, dtype=dtype) if code == E4M3 else x.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError("out is a contiguous tensor of the result's shape, type and device")
     _lib.on_device(device.index, _lib.lib().tao_linear4, rows.data_ptr(), rows.stride(0), code, scale_at,

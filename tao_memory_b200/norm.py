@@ -33,9 +33,20 @@ def wants_gradient(*operands):
 
 def refuse_tangents(operator, *operands):
     """Forward-mode derivatives would be dropped with the operands' addresses."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                              for t in operands):
+    if forward_ad._current_level < 0:  # none is being taken
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
         raise ValueError(f"{operator} has no forward-mode derivative")
+
+
+def refuse_derivatives(operator, *operands):
+    """For an operator without a gradient."""
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{operator} has no gradient, for activations or weights: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        refuse_tangents(operator, *operands)
 
 
 def _check(x, weight, residual):
@@ -51,6 +62,8 @@ def _check(x, weight, residual):
 
 
 def _new(x, dtype=None):
+    if dtype is None and x.is_contiguous():
+        return torch.empty_like(x)
     return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
 
 
@@ -147,11 +160,9 @@ def add_rms_norm_fp8(x, weight=None, residual=None, eps=RMS_EPS, group=None):
     (``group=None``: scale [..., 1], as ``linear4`` and row-scaled products take it) or one for
     128 channels (``group=128``: [..., ceil(width / 128)]).  Not differentiable."""
     _check(x, weight, residual)
-    refuse_tangents("add_rms_norm_fp8", x, weight, residual)
+    refuse_derivatives("add_rms_norm_fp8", x, weight, residual)
     if group not in (None, 128):
         raise ValueError("8-bit scales are by row (None) or by 128 channels")
-    if wants_gradient(x, weight, residual):
-        raise ValueError("the 8-bit norm has no gradient: call it under torch.no_grad()")
     width = x.shape[-1]
     rows = _rows(x, width)
     q = _new(x, torch.float8_e4m3fn)
