@@ -111,3 +111,57 @@ def test_experts_of_many_channels(tokens, width, inner, experts, top_k, four):
                                      + (slack[t] + d).unsqueeze(-1) * y.abs()))
     bad = (out.double() - ref).abs() > 2.0 ** -8 * ref.abs() + off + 1e-30
     assert not bad.any(), (int(bad.sum()), (out.double() - ref).abs().max().item())
+
+
+@pytest.mark.parametrize("group", [None, 128])
+@pytest.mark.parametrize("dtype,width", [(torch.bfloat16, 65536), (torch.float16, 65535), (torch.float32, 32768),
+                                         (torch.float32, 32767), (torch.bfloat16, 20001)])
+@pytest.mark.parametrize("rows", [1, 160])
+def test_e4m3_of_the_widest_rows(rows, width, dtype, group):
+    from tao_memory_b200 import add_rms_norm_fp8
+    g = torch.Generator(device="cuda").manual_seed(width + rows)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    x, res, w = n(rows, width).to(dtype), (3 * n(rows, width)).to(dtype), (1 + 0.3 * n(width)).to(dtype)
+    q, scale, s = add_rms_norm_fp8(x, w, res, eps=EPS, group=group)
+    want_s = (x.float() + res.float()).to(dtype)
+    assert torch.equal(s, want_s)
+    sd = want_s.double()
+    y = sd * (sd.square().mean(-1, keepdim=True) + EPS).rsqrt() * w.double()
+    lost = 128 * 2.0 ** -24
+    for i, c in enumerate(y.split(width if group is None else 128, -1)):
+        top = c.abs().amax(-1).clamp_min(1e-30)
+        assert ((scale[..., i].double() - top / 448).abs() <= lost * top / 448).all()
+        v = c * (448 / top).unsqueeze(-1)
+        at = i * (width if group is None else 128)
+        # e4m3: unit roundoff 2^-4 and half a subnormal step 2^-10
+        assert ((q[..., at:at + c.shape[-1]].double() - v).abs() <= (2.0 ** -4 + lost) * v.abs() + 2.0 ** -10).all()
+
+
+def test_operators_on_two_streams_at_once():
+    """Calls on two streams share no workspace: every result is that of the call alone."""
+    from tao_memory_b200 import ExpertWeights, add_rms_norm, expert_layer, linear4, quantize4
+    from tao_memory_b200.stream import check_device
+    g = torch.Generator(device="cuda").manual_seed(0)
+    n = lambda *s: (torch.randn(*s, device="cuda", generator=g) * s[-1] ** -0.5).bfloat16()
+    layer = ExpertWeights(n(16, 512), n(16, 256, 512), n(16, 256, 512), n(16, 512, 256), top_k=4)
+    w4 = quantize4(n(512, 512))
+    xs = [torch.randn(rows, 512, device="cuda", generator=g).bfloat16() for rows in (3, 40)]
+    weight = torch.ones(512, device="cuda", dtype=torch.bfloat16)
+
+    def block(x):
+        h, s = add_rms_norm(x, weight, x)
+        return expert_layer(linear4(h, w4), layer), s
+
+    want = [block(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(25):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(block(xs[i]))
+    torch.cuda.synchronize()
+    assert check_device() == 0
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
