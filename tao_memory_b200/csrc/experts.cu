@@ -18,8 +18,8 @@
 // unit to unit (part 3's starts before the barrier).
 // h is kept as the sum of two bf16 (16 mantissa bits), which are two columns of one mma: with bf16
 // alone its rounding would add as much to the error as the output's own.  Every sum's order is fixed.
-// Of 64 experts (2048, 1024) with 8 for a token: one token 32.5 us (3.1 TB/s), 8 tokens 103 us (5.1), in 4 bits 63.7
-// (2.1: the unpacking's instructions); 64 tokens of 128 experts (2048, 768) 230 us (5.2).
+// Of 64 experts (2048, 1024) with 8 for a token: one token 30.3 us (3.3 TB/s), 8 tokens 101 us (5.2), in 4 bits 63.1
+// (2.2: the unpacking's instructions); 64 tokens of 128 experts (2048, 768) 230 us (5.2).
 #include <cuda_runtime.h>
 
 #include <algorithm>

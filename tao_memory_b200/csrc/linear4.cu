@@ -12,7 +12,7 @@
 // (registers would do, but a warp's few scoreboards make a load wait for later ones).  A warp leaves its sums
 // of a tile in shared memory; these are added at the end, a cluster's blocks' through distributed shared
 // memory, in a fixed order.
-// With k = n = 8192 and groups of 128 one row takes 10.3 us (3.4 TB/s of its bytes), 8 rows 14.2, 16 rows 16.3: half of
+// With k = n = 8192 and groups of 128 one row takes 10.4 us (3.3 TB/s of its bytes), 8 rows 14.2, 16 rows 16.3: half of
 // the issue slots, the rest waits at the few meetings.  A single row of k = 2048, n = 6144 takes 4.4 us, of which
 // the bytes are 1: launch, x and the first weights follow one another.
 #include <cuda_runtime.h>
@@ -411,7 +411,7 @@ int launch_tc(Linear4Args a, cudaStream_t s) {
 }
 
 // The bytes' form costs four columns a row and little else, the 16-bit one eight more instructions for
-// eight weights: of k = n = 8192 one row takes 10.3 us (13.3 in 16 bits), two 11.3 (13.8), four 13.7 (14.2 as
+// eight weights: of k = n = 8192 one row takes 10.4 us (13.3 in 16 bits), two 11.2 (13.8), four 13.7 (14.2 as
 // bytes in two column tiles, a form that is not kept).  tcgen05 needs the weights in shared memory: 16 rows
 // 26.7 us (16.2 here), 17 26.9 (28.8), 64 29.5 (60.6); of k = 2048, n = 6144 17 rows 9.9 (8.7), 32 10.3 (10.7),
 // 64 11.1 (18.9).  A form whose x does not fit a cluster of 8 blocks'
