@@ -458,7 +458,7 @@ int tao_qkv_split_norm_backward(const void* raw_q, const void* raw_k, const void
                                 const void* dv, const void* d_raw_q, const void* d_raw_k, long long rows,
                                 int heads, int width, float eps, void* d_projected, void* stream);
 
-/* Element types of the block operators below. */
+/* Element types of the block operators below.  Their operands start on a whole element (TAO_ERR_ARG). */
 #define TAO_TYPE_BF16 0
 #define TAO_TYPE_FP16 1
 #define TAO_TYPE_FP32 2

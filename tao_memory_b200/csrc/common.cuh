@@ -6,7 +6,9 @@
 // FMA across the rounding point.
 #pragma once
 #include <cuda_bf16.h>
+#include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 #define TAO_DEVI __device__ __forceinline__
 
@@ -46,6 +48,17 @@ TAO_DEVI float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// Whether each operand's address is a multiple of its elements' size (an absent one's is).
+struct Operand {
+  const void* at;
+  size_t size;
+};
+inline bool on_elements(std::initializer_list<Operand> operands) {
+  for (const Operand& o : operands)
+    if (reinterpret_cast<uintptr_t>(o.at) % o.size) return false;
+  return true;
 }
 
 // Whether rows of `bytes` bytes, `stride` bytes apart from x on, share any with the `size` bytes from y on.

@@ -676,6 +676,8 @@ int tao_expert_layer(const TaoExperts* p, const void* x, long long x_stride, int
     if (reinterpret_cast<uintptr_t>(q) % 16) return efail(TAO_ERR_ARG, "the expert layer's operands start on 16 bytes");
   // (8 bytes are stored at a time; a row is whole 16 bytes)
   if (reinterpret_cast<uintptr_t>(out) % 8) return efail(TAO_ERR_ARG, "the expert layer's output starts on 8 bytes");
+  if (!on_elements({{ids, sizeof(int)}, {id_weights, sizeof(float)}, {p->error, sizeof(int)}}))
+    return efail(TAO_ERR_ARG, "operands start on a whole element");
   const long long strides[] = {x_stride, p->gate_expert, p->gate_row, p->up_expert, p->up_row, p->down_expert,
                                p->down_row};
   for (int i = 0; i < (p->group ? 1 : 7); ++i)

@@ -454,6 +454,8 @@ int tao_linear4(const void* x, long long x_stride, int x_type, const float* x_sc
   for (const void* p : {codes, scales, zeros})
     if (reinterpret_cast<uintptr_t>(p) % 16) return lfail(TAO_ERR_ARG, "a laid-out weight starts on 16 bytes");
   const int size = x_type == TAO_TYPE_E4M3 ? 1 : 2;
+  if (!on_elements({{x, (size_t)size}, {x_scale, sizeof(float)}, {bias, 2}, {y, 2}}))
+    return lfail(TAO_ERR_ARG, "operands start on a whole element");
   // a block writes its part of y while others still read theirs of x
   if (rows_overlap(x, rows, x_stride * size, (long long)k * size, y, rows * n * 2) ||
       (x_scale && rows_overlap(x_scale, 1, 0, rows * 4, y, rows * n * 2)) ||

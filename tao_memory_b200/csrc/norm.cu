@@ -523,6 +523,9 @@ int tao_add_rms_norm(const void* x, long long x_stride, const void* residual, lo
   if (int rc = check(rows, width, type)) return rc;
   if (rows == 0) return TAO_OK;
   if (!x || !y || (residual && !s)) return nfail(TAO_ERR_ARG, "null pointer");
+  const size_t size = size_of(type);
+  if (!on_elements({{x, size}, {residual, size}, {weight, size}, {s, size}, {y, size}}))
+    return nfail(TAO_ERR_ARG, "operands start on a whole element");
   return forward({x, residual, weight, x_stride, r_stride, rows, width, 0, eps, 1.f / width, s, y, nullptr}, type, false,
                  stream);
 }
@@ -535,6 +538,9 @@ int tao_add_rms_norm_fp8(const void* x, long long x_stride, const void* residual
   if (group != 0 && group != 128) return nfail(TAO_ERR_ARG, "8-bit scales are by row (0) or by 128 channels");
   if (rows == 0) return TAO_OK;
   if (!x || !q || !scale || (residual && !s)) return nfail(TAO_ERR_ARG, "null pointer");
+  const size_t size = size_of(type);
+  if (!on_elements({{x, size}, {residual, size}, {weight, size}, {s, size}, {scale, sizeof(float)}}))
+    return nfail(TAO_ERR_ARG, "operands start on a whole element");
   return forward({x, residual, weight, x_stride, r_stride, rows, width, group, eps, 1.f / width, s, q, scale}, type, true,
                  stream);
 }
@@ -560,6 +566,8 @@ int tao_add_rms_norm_backward(const void* dy, long long dy_stride, const void* d
     return TAO_OK;
   }
   if (!dy || !s || !dx) return nfail(TAO_ERR_ARG, "null pointer");
+  if (!on_elements({{dy, size}, {ds, size}, {s, size}, {weight, size}, {dx, size}, {dw, size}, {workspace, sizeof(float)}}))
+    return nfail(TAO_ERR_ARG, "operands start on a whole element");
   if (dw && (!workspace || workspace_bytes < tao_add_rms_norm_workspace_bytes(rows, width, type)))
     return nfail(TAO_ERR_ARG, "workspace too small for the norm's weight gradient");
   const NormGradArgs a = {dy,    ds,  s,  weight, dy_stride, ds_stride, s_stride, rows, width, eps, 1.f / width, dx,

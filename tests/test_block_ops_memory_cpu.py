@@ -58,3 +58,39 @@ def test_an_expert_layers_output_does_not_overlap_a_later_launchs_tokens():
     # a launch writes after its last read of x; the same rows; rows next to each other
     for out, tokens in ((x, 64), (x + row, 64), (x, 200), (x + 200 * row, 200), (x - 200 * row, 200)):
         assert not refused(out, tokens), (out - x, tokens)
+
+
+def test_operands_start_on_their_elements():
+    """A misaligned address would be a fault of the GPU; each is refused (only such calls are made here)."""
+    lib, arg, at = _lib.lib(), _lib.TAO_ERR_ARG, 1 << 20
+    names = lambda rc: rc == arg and b"element" in lib.tao_last_error()
+
+    def norm(type, fp8=False, **k):
+        a = {**dict(x=at, r=at, w=at, s=at, y=at, scale=at), **k}
+        head = (a["x"], 64, a["r"], 64, a["w"], 3, 64, type, 1e-6)
+        if fp8:
+            return lib.tao_add_rms_norm_fp8(*head, 0, a["s"], a["y"], a["scale"], None)
+        return lib.tao_add_rms_norm(*head, a["s"], a["y"], None)
+
+    for type, size in ((0, 2), (1, 2), (2, 4)):
+        for name in ("x", "r", "w", "s"):
+            assert names(norm(type, **{name: at + size // 2})) and names(norm(type, fp8=True, **{name: at + 1}))
+        assert names(norm(type, y=at + 1)) and names(norm(type, fp8=True, scale=at + 2))
+        room = 1 << 20
+        back = dict(dy=at, ds=at, s=at, w=at, dx=at, dw=at, ws=at)
+        for name in back:
+            b = {**back, name: at + (2 if name == "ws" else size // 2)}
+            assert names(lib.tao_add_rms_norm_backward(b["dy"], 64, b["ds"], 64, b["s"], 64, b["w"], 3, 64, type, 1e-6,
+                                                       b["dx"], b["dw"], b["ws"], room, None)), (type, name)
+
+    def product(x=at, x_type=0, x_scale=None, bias=None, y=1 << 22):
+        return lib.tao_linear4(x, 128, x_type, x_scale, at, at, None, 128, 0, bias, 1, 16, 128, y, None)
+
+    assert names(product(x=at + 1)) and names(product(y=at + 4097)) and names(product(bias=at + 9001))
+    assert names(product(x_type=3, x_scale=at + 9002))
+
+    def layer(ids=None, weights=None, error=None):
+        return lib.tao_expert_layer(ctypes.byref(_layer(error=error)), at, 8, 1, 1 << 22, ids, weights, 1 << 21, 1 << 20,
+                                    None)
+
+    assert names(layer(at + 2, at)) and names(layer(at, at + 1)) and names(layer(error=at + 2))
