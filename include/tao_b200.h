@@ -537,6 +537,78 @@ int tao_expert_layer(const TaoExperts* layer, const void* x, long long x_stride,
                      void* stream);
 int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* stream);
 
+/* Activations of the 16-bit products: gelu by the error function, gelu_tanh by its tanh form. */
+#define TAO_ACT_NONE 0
+#define TAO_ACT_RELU 1
+#define TAO_ACT_SILU 2
+#define TAO_ACT_GELU 3
+#define TAO_ACT_GELU_TANH 4
+
+/* Products of bf16 or fp16 matrices (`type`), fp32 sums, rounded once; strides in elements, last axes contiguous.
+ *   y [rows][n] = act(x [rows][k] W^T + bias) + residual            (W [n][k]; bias, residual may be NULL)
+ * or, with offsets [experts + 1] (int32, device memory), of the experts' weights W [experts][n][k] (matrices
+ * w_expert apart) for rows sorted by expert, offsets[e] .. offsets[e + 1] - 1 those of expert e:
+ *   y = act(x W_e^T), or with `up` the gated act(x W_e^T) * (x U_e^T).
+ * offsets[0] is taken as 0, values are held between the one before and `rows`, and rows from offsets[experts] on
+ * give zeros.  z, u [rows][z_stride]: what act and its factor are applied to, for the gradient, or NULL.
+ * x, W, up and their rows start on 16 bytes; y, z, u, bias and the residual on whole elements.  y may be the
+ * residual itself (r_stride n); it must not overlap another operand.  Up to 512 experts. */
+int tao_linear(const void* x, long long x_stride, const void* w, long long w_stride, long long w_expert, const void* up,
+               long long up_stride, long long up_expert, const void* bias, const void* residual, long long r_stride,
+               const int* offsets, int experts, long long rows, int n, int k, int type, int activation, void* y, void* z,
+               void* u, long long z_stride, void* stream);
+
+/* The gradient of tao_linear.  First dz = dy act'(z), or with u the gated dz = dy u act'(z), du = dy act(z)
+ * (rounded to the type, [rows][d_stride]; z NULL: dz is dy, written if dz is not NULL), and db [n] = the sum of
+ * dz over the rows, in a fixed order (NULL: not wanted; workspace: tao_linear_slope_workspace_bytes). */
+size_t tao_linear_slope_workspace_bytes(long long rows, int n);
+int tao_linear_slope(const void* dy, long long dy_stride, const void* z, const void* u, long long z_stride,
+                     long long rows, int n, int type, int activation, void* dz, void* du, long long d_stride, void* db,
+                     void* workspace, size_t workspace_bytes, void* stream);
+/* Then dx [rows][k] = dz W (+ du U), zeros for rows of no expert, ... */
+int tao_linear_input_gradient(const void* dz, const void* du, long long d_stride, const void* w, long long w_stride,
+                              long long w_expert, const void* up, long long up_stride, long long up_expert,
+                              const int* offsets, int experts, long long rows, int n, int k, int type, void* dx,
+                              void* stream);
+/* ... and dw [experts][n][k] = dz^T x (dup: du^T x) over each expert's rows, zeros for an expert without.  dz,
+ * du, x, W, up and their rows start on 16 bytes. */
+int tao_linear_weight_gradient(const void* dz, const void* du, long long d_stride, const void* x, long long x_stride,
+                               const int* offsets, int experts, long long rows, int n, int k, int type, void* dw,
+                               void* dup, void* stream);
+/* The current device's error word of the 16-bit products (a wait that ran out), read and cleared. */
+int tao_product_check(int* flags, void* stream);
+
+/* Tokens sorted by expert.  ids [pairs] (int32 or int64: id_bytes 4 or 8), pair t * top_k + j being token t's choice
+ * j; an id outside of 0 .. experts - 1 is no expert.  sorted [pairs]: the pairs by expert, stably, those of no
+ * expert last; places [pairs]: its inverse; offsets [experts + 1]: the first place of each expert and the number of
+ * pairs that have one.  Up to 512 experts and 2^30 pairs.  workspace: tao_sort_tokens_workspace_bytes. */
+size_t tao_sort_tokens_workspace_bytes(long long pairs, int experts);
+int tao_sort_tokens(const void* ids, int id_bytes, long long pairs, int experts, int* sorted, int* places, int* offsets,
+                    void* workspace, size_t workspace_bytes, void* stream);
+/* xs [tokens * top_k][width]: xs[places[t][j]] = x[t]; bf16, fp16 or fp32.  A place outside of the pairs is passed over. */
+int tao_gather_tokens(const void* x, long long x_stride, const int* places, long long tokens, int top_k, int width,
+                      int type, void* xs, void* stream);
+/* y [tokens][width] = sum over j of weights[t][j] ys[places[t][j]], in fp32 in j's order, rounded once.  weights: fp32 or
+ * `type` (weight_type), NULL: ones.  kept (device memory, NULL: all): pairs at places from *kept on do not count. */
+int tao_return_tokens(const void* ys, long long ys_stride, const int* places, const int* kept, const void* weights,
+                      int weight_type, long long tokens, int top_k, int width, int type, void* y, void* stream);
+/* Its gradient: dys[places[t][j]] = weights[t][j] dy[t], dw[t][j] = dy[t] . ys[places[t][j]] (either may be NULL; dw
+ * needs ys and weights), zeros for pairs that do not count. */
+int tao_return_tokens_gradient(const void* dy, long long dy_stride, const void* ys, long long ys_stride, const int* places,
+                               const int* kept, const void* weights, int weight_type, long long tokens, int top_k,
+                               int width, int type, void* dys, void* dw, void* stream);
+
+/* y [n][width] = scale * table[ids[i]] (table [vocab][width], rows `stride` apart; bf16, fp16 or fp32), zeros for an id
+ * outside of the table. */
+int tao_embed(const void* ids, int id_bytes, long long n, const void* table, long long stride, long long vocab, int width,
+              int type, float scale, void* y, void* stream);
+/* dtable [vocab][width] = scale * the sum of dy over the tokens of each id, in fp32 in a fixed order, rounded once.
+ * workspace: tao_embed_gradient_workspace_bytes, on 16 bytes.  Up to 2^26 rows. */
+size_t tao_embed_gradient_workspace_bytes(long long n, long long vocab, int width);
+int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* dy, long long dy_stride, long long vocab,
+                       int width, int type, float scale, void* dtable, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,22 @@ _SIGNATURES = {
     "tao_expert_workspace_bytes": (_SZ, [ctypes.POINTER(TaoExperts), _I]),
     "tao_expert_layer": (_I, [ctypes.POINTER(TaoExperts), _VP, _I64, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "tao_expert_check": (_I, [_VP, _SZ, ctypes.POINTER(_I), _VP]),
+    "tao_linear": (_I, [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I, _I64, _I, _I, _I, _I, _VP,
+                        _VP, _VP, _I64, _VP]),
+    "tao_linear_slope_workspace_bytes": (_SZ, [_I64, _I]),
+    "tao_linear_slope": (_I, [_VP, _I64, _VP, _VP, _I64, _I64, _I, _I, _I, _VP, _VP, _I64, _VP, _VP, _SZ, _VP]),
+    "tao_linear_input_gradient": (_I, [_VP, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I, _I64, _I, _I, _I, _VP,
+                                       _VP]),
+    "tao_linear_weight_gradient": (_I, [_VP, _VP, _I64, _VP, _I64, _VP, _I, _I64, _I, _I, _I, _VP, _VP, _VP]),
+    "tao_product_check": (_I, [ctypes.POINTER(_I), _VP]),
+    "tao_sort_tokens_workspace_bytes": (_SZ, [_I64, _I]),
+    "tao_sort_tokens": (_I, [_VP, _I, _I64, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "tao_gather_tokens": (_I, [_VP, _I64, _VP, _I64, _I, _I, _I, _VP, _VP]),
+    "tao_return_tokens": (_I, [_VP, _I64, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _VP, _VP]),
+    "tao_return_tokens_gradient": (_I, [_VP, _I64, _VP, _I64, _VP, _VP, _VP, _I, _I64, _I, _I, _I, _VP, _VP, _VP]),
+    "tao_embed": (_I, [_VP, _I, _I64, _VP, _I64, _I64, _I, _I, _F, _VP, _VP]),
+    "tao_embed_gradient_workspace_bytes": (_SZ, [_I64, _I64, _I]),
+    "tao_embed_gradient": (_I, [_VP, _I, _I64, _VP, _I64, _I64, _I, _I, _F, _VP, _VP, _SZ, _VP]),
     "tao_feature_read_forward": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP]),
     "tao_feature_read_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
     "tao_train_pairs": (_I, [_I]),

@@ -1,0 +1,252 @@
+// Rows of a table by tokens' ids, scaled, and the table's gradient.
+//
+// Forward: bound by its bytes (and for a few tokens by the launch); a thread has 16 bytes of a row.
+// Gradient: the tokens are sorted by id (sort.cuh, stably), and a block adds the rows of a run of kRun sorted
+// tokens, in fp32 and in their order, a sum for each id.  An id whose tokens lie within the run is written at
+// once; the sums of one that goes on in the next run are joined by a second kernel, in the runs' order, so a word
+// that comes 10000 times is added by 160 blocks and the result does not depend on when they ran.  Rows of no
+// token are zeros.
+#include <cuda_runtime.h>
+
+#include "rows.cuh"
+#include "sort.cuh"
+
+void tao_set_last_error(const char* msg);
+
+namespace tao {
+namespace {
+
+using namespace rows;
+
+constexpr int kRun = 64;
+
+int efail(int code, const char* msg) {
+  tao_set_last_error(msg);
+  return code;
+}
+int launched(cudaError_t e) { return e == cudaSuccess ? TAO_OK : efail(TAO_ERR_CUDA, cudaGetErrorString(e)); }
+
+struct EmbedArgs {
+  const void* ids;
+  long long n, vocab, stride;
+  int width;
+  bool wide_ids;
+  float scale;
+  const void* in;
+  void* out;
+};
+
+template <class T, int N>
+__global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
+  const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (t >= a.n || c >= a.width) return;
+  const long long id = a.wide_ids ? static_cast<const long long*>(a.ids)[t] : static_cast<const int*>(a.ids)[t];
+  float f[N] = {};
+  if (id >= 0 && id < a.vocab) {
+    reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + id * a.stride + c)->widen(f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] *= a.scale;
+  }
+  *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + t * a.width + c) = Vec<T, N>::of(f);
+}
+
+struct SumArgs {
+  const int *tokens, *ids;  // sorted by id
+  int n, vocab, width;
+  float scale;
+  const void* dy;
+  long long dy_stride;
+  void* out;
+  float* parts;  // [runs][2][width]: of an id that began before the run, and of one that goes on behind it
+};
+
+// Sums of run blockIdx.x, for the vector of columns that a thread has.
+template <class T, int N>
+__global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
+  __shared__ int ids[kRun + 2], tokens[kRun];  // ids[0] and ids[count + 1]: the neighbours'
+  const int begin = blockIdx.x * kRun, count = min(kRun, a.n - begin);
+  for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
+    const int at = begin + i - 1;
+    ids[i] = at >= 0 && at < a.n ? a.ids[at] : -1;
+    if (i < count) tokens[i] = a.tokens[begin + i];
+  }
+  __syncthreads();
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (c >= a.width) return;
+  float sum[N] = {};
+  constexpr int AHEAD = 8;
+  for (int i0 = 0; i0 < count; i0 += AHEAD) {
+    Vec<T, N> v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i0 + i < count)
+        v[i] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.dy) + tokens[i0 + i] * a.dy_stride + c);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (i0 + i >= count) break;
+      const int id = ids[i0 + i + 1], next = ids[i0 + i + 2];
+      float f[N];
+      v[i].widen(f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] += f[e];
+      const bool last = i0 + i == count - 1;
+      if (id == next && !last) continue;
+      if (id < a.vocab) {
+        const bool older = id == ids[0] && ids[1] == id;  // sorted: all from the run's first on
+        if (older || id == next) {
+          float* part = a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width + c;
+#pragma unroll
+          for (int e = 0; e < N; ++e) part[e] = sum[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e] *= a.scale;
+          *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)id * a.width + c) = Vec<T, N>::of(sum);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] = 0.f;
+    }
+  }
+}
+
+// The id that begins in run blockIdx.x and goes on behind it.
+template <class T, int N>
+__global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
+  const int begin = blockIdx.x * kRun, end = begin + kRun;
+  if (end >= a.n) return;
+  const int id = a.ids[end - 1];
+  if (a.ids[end] != id || id >= a.vocab || (begin > 0 && a.ids[begin] == id && a.ids[begin - 1] == id)) return;
+  int low = end, high = a.n;  // the first place behind the id's
+  while (low < high) {
+    const int mid = low + (high - low) / 2;
+    if (a.ids[mid] == id) low = mid + 1;
+    else high = mid;
+  }
+  const int last = (low - 1) / kRun;
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (c >= a.width) return;
+  float sum[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[e] = a.parts[((long long)blockIdx.x * 2 + 1) * a.width + c + e];
+#pragma unroll 8
+  for (int r = blockIdx.x + 1; r <= last; ++r)
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] += a.parts[(long long)r * 2 * a.width + c + e];
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[e] *= a.scale;
+  *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)id * a.width + c) = Vec<T, N>::of(sum);
+}
+
+// Passes of the sort and bits of each, for ids 0 .. vocab (vocab: none).
+int bits_of(long long vocab, int* passes) {
+  int bits = 1;
+  while (vocab >> bits) ++bits;
+  *passes = (bits + 8) / 9;
+  return (bits + *passes - 1) / *passes;
+}
+
+// Parts of the gradient's workspace.
+struct Room {
+  size_t values[2], ids, counts, parts, bytes;
+};
+Room room_of(long long n, long long vocab, int width) {
+  int passes;
+  const int bits = bits_of(vocab, &passes);
+  Room r;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  r.values[0] = take(n * 4);
+  r.values[1] = take(n * 4);
+  r.ids = take(n * 4);
+  r.counts = take(sorting::counts_bytes(n, 1 << bits));
+  r.parts = take((size_t)((n + kRun - 1) / kRun) * 2 * width * 4);
+  r.bytes = at;
+  return r;
+}
+
+int check(int id_bytes, long long n, long long vocab, int width, int type) {
+  if (id_bytes != 4 && id_bytes != 8) return efail(TAO_ERR_ARG, "ids have 32 or 64 bits");
+  if (!known(type)) return efail(TAO_ERR_ARG, "a table is bf16, fp16 or fp32");
+  if (n < 0 || n > (1ll << 30) || vocab < 1 || vocab > (1ll << 26) || width < 1 || width > (1 << 24))
+    return efail(TAO_ERR_ARG, "there are up to 2^30 ids and 1 to 2^26 rows of 1 to 2^24 channels");
+  return TAO_OK;
+}
+
+}  // namespace
+}  // namespace tao
+
+extern "C" {
+
+int tao_embed(const void* ids, int id_bytes, long long n, const void* table, long long stride, long long vocab, int width,
+              int type, float scale, void* y, void* stream) {
+  using namespace tao;
+  if (int rc = check(id_bytes, n, vocab, width, type)) return rc;
+  if (n == 0) return TAO_OK;
+  const size_t size = size_of(type);
+  if (!ids || !table || !y) return efail(TAO_ERR_ARG, "null pointer");
+  if (!on_elements({{ids, (size_t)id_bytes}, {table, size}, {y, size}}))
+    return efail(TAO_ERR_ARG, "operands start on a whole element");
+  const EmbedArgs a = {ids, n, vocab, stride, width, id_bytes == 8, scale, table, y};
+  const bool wide = width * size % 16 == 0 && on16(table, stride, size) && on16(y, 0, size);
+  return by_vector(type, wide, [&](auto t, auto v) {
+    const Mapping m = mapping(n, (width + decltype(v)::value - 1) / decltype(v)::value);
+    embed_kernel<decltype(t), decltype(v)::value><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    return launched(cudaGetLastError());
+  });
+}
+
+size_t tao_embed_gradient_workspace_bytes(long long n, long long vocab, int width) {
+  return n <= 0 || vocab < 1 || width < 1 ? 0 : tao::room_of(n, vocab, width).bytes;
+}
+
+int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* dy, long long dy_stride, long long vocab,
+                       int width, int type, float scale, void* dtable, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  using namespace tao;
+  if (int rc = check(id_bytes, n, vocab, width, type)) return rc;
+  const size_t size = size_of(type);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!dtable) return efail(TAO_ERR_ARG, "null pointer");
+  if (!on_elements({{ids, (size_t)id_bytes}, {dy, size}, {dtable, size}}))
+    return efail(TAO_ERR_ARG, "operands start on a whole element");
+  if (n > 0) {
+    if (!ids || !dy) return efail(TAO_ERR_ARG, "null pointer");
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+        workspace_bytes < tao_embed_gradient_workspace_bytes(n, vocab, width))
+      return efail(TAO_ERR_ARG, "workspace too small for the embedding's gradient, or off 16 bytes");
+  }
+  cudaError_t e = cudaMemsetAsync(dtable, 0, (size_t)vocab * width * size, s);
+  if (e != cudaSuccess || n == 0) return launched(e);
+  const Room r = room_of(n, vocab, width);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  int passes;
+  const int bits = bits_of(vocab, &passes);
+  sorting::Pass p = {};
+  p.ids = ids, p.limit = vocab, p.n = (int)n, p.bins = 1 << bits, p.wide = id_bytes == 8;
+  for (int i = 0; i < passes; ++i) {
+    p.shift = i * bits;
+    p.sorted = reinterpret_cast<int*>(ws + r.values[i & 1]);
+    p.keys = i + 1 == passes ? reinterpret_cast<int*>(ws + r.ids) : nullptr;
+    e = sorting::run(p, reinterpret_cast<int*>(ws + r.counts), s);
+    if (e != cudaSuccess) return launched(e);
+    p.values = p.sorted;
+  }
+  const SumArgs a = {p.values, reinterpret_cast<const int*>(ws + r.ids), (int)n, (int)vocab, width, scale, dy, dy_stride,
+                     dtable, reinterpret_cast<float*>(ws + r.parts)};
+  const bool wide = width * size % 16 == 0 && on16(dy, dy_stride, size) && on16(dtable, 0, size);
+  return by_vector(type, wide, [&](auto t, auto v) {
+    constexpr int N = decltype(v)::value;
+    const int vectors = (width + N - 1) / N, threads = std::min(256, (vectors + 31) / 32 * 32);
+    const dim3 grid((unsigned)((n + kRun - 1) / kRun), (vectors + threads - 1) / threads);
+    run_kernel<decltype(t), N><<<grid, threads, 0, s>>>(a);
+    if (grid.x > 1) join_kernel<decltype(t), N><<<grid, threads, 0, s>>>(a);
+    return launched(cudaGetLastError());
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,699 @@
+// Products of 16-bit matrices on tcgen05 with everything around them in one kernel: the forward product
+// with bias, activation, gate and residual, the two products of its gradient, and each of them for the rows
+// of many experts at once.  fp32 accumulators in TMEM, one rounding when a value is stored.
+//
+//   FORWARD  y[t][c] = act(sum_k x[t][k] W[c][k] + bias[c]) + residual[t][c], or act(x W^T) * (x U^T)
+//   FEW      the same for few rows: W is the operand of 128 rows, x the one of 16 to 64 columns, so that
+//            a tile does not multiply rows that are not there
+//   INPUT    dx[t][k] = sum_c dz[t][c] W[c][k] (+ du U)
+//   WEIGHT   dW[c][k] = sum_t dz[t][c] x[t][k]
+//
+// Operands arrive as they lie in memory: one whose terms are next to each other (K-major) and one whose
+// rows are (MN-major) differ in the box that TMA fetches and in the descriptor only, so nothing is transposed.
+// A block keeps one CTA an SM busy over many tiles: a warp fetches 64 terms at a time into a ring, a
+// warp issues the products into one of two accumulators, and eight warps turn the other one into outputs.
+// Tiles go in bands of 16 row tiles, so that the blocks at work share operands in L2.
+//
+// SPLIT: a product with fewer tiles than SMs deals the terms of a tile to the blocks of a cluster, which add
+// their parts through each other's shared memory in the order of their ranks.
+//
+// Experts: rows of x are sorted by expert, offsets[e] .. offsets[e + 1] are those of expert e.  Every block
+// makes the list of tiles itself from the offsets, so the host never reads them.  A row tile never spans
+// two experts; rows of a tile behind its expert's last are computed and not stored, and as terms of WEIGHT
+// they are set to zero in shared memory in both operands (another expert's may be infinite).
+#pragma once
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include "../../include/tao_b200.h"
+#include "common.cuh"
+#include "linear4.cuh"
+#include "tcgen05.cuh"
+
+namespace tao {
+namespace product {
+
+static __device__ int g_error;  // an expired wait, until tao_product_check
+
+enum Form { FORWARD, FEW, INPUT, WEIGHT };
+
+constexpr int kTerms = 64;         // of a step of the ring: 128 bytes, the swizzle's width
+constexpr int kMostGroups = 512;   // experts
+constexpr int kWorkers = 8;        // warps that read accumulators
+constexpr int kThreads = 32 * (kWorkers + 2);
+constexpr int kBand = 16;          // row tiles of a band
+
+struct Args {
+  const int* offsets;  // of the experts, or null: one group of all rows
+  int groups, rows;
+  int cols;            // of an output row
+  int depth;           // terms of a sum (FORWARD, FEW: k, INPUT: n); WEIGHT: rows of an output matrix
+  int pairs;           // INPUT: pairs of operands whose products are added; WEIGHT: matrices of an expert
+  int type, act;
+  const void *bias, *residual;
+  long long r_stride;
+  void *y, *z, *u;     // z, u: act's argument and the gate's factor (FORWARD, FEW); u: the second matrix (WEIGHT)
+  long long z_stride;
+  bool wide;           // rows of y, z, u and the residual start on 16 bytes, and cols is a multiple of 8
+  int split;           // blocks of a cluster
+};
+
+template <int FORM, int BN, bool GATED, bool SPLIT>
+struct Cfg {
+  static constexpr bool A_MN = FORM == WEIGHT, B_MN = FORM == INPUT || FORM == WEIGHT;
+  static constexpr int TT = FORM == FEW ? BN : 128;                              // token rows of a tile
+  static constexpr int CT = FORM == FEW ? 128 : GATED ? BN / 2 : BN;             // output columns of a tile
+  static constexpr int A = (FORM == FEW && GATED ? 2 : 1) * 128 * 128, B = BN * 128, STAGE = A + B;
+  static constexpr int STAGING = FORM == FEW || SPLIT ? 0 : kWorkers * 2048;
+  static constexpr int LISTS = SPLIT ? 0 : (2 * kMostGroups + 4) * 4;
+  static constexpr int REST = STAGING + LISTS + 512;
+  static constexpr int FIT = (227 * 1024 - REST) / STAGE, STAGES = FIT < 12 ? FIT : 12;
+  static constexpr int SUMS = SPLIT ? (FORM == FEW ? BN * 132 : 128 * (BN + 4)) * 4 : 0;
+  static constexpr int SMEM = STAGES * STAGE + REST;
+  static constexpr int ACC = FORM == FEW && GATED ? 2 * BN : BN;
+  static constexpr int SETS = SPLIT ? 1 : 2, USED = SETS * ACC;
+  static constexpr int TMEM = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+  static_assert(USED <= 512 && STAGES >= 3 && SUMS <= STAGES * STAGE && SMEM <= 227 * 1024, "");
+};
+
+// Waits at most about four seconds; a wait that runs out, or another's of this block, ends all of them.
+TAO_DEVI bool wait_for(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  unsigned long long began = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if (i & 63u) continue;
+    if (*abort) return false;
+    unsigned long long now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (!began) began = now;
+    if (now - began > 4000000000ull) break;
+  }
+  *abort = 1;
+  atomicOr(&g_error, kErrWaitTimeout);
+  return false;
+}
+TAO_DEVI bool warp_wait_for(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  return __all_sync(0xffffffffu, wait_for(bar, phase, abort));
+}
+
+TAO_DEVI void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// N consecutive fp32 columns of this thread's TMEM lane.
+template <int N>
+TAO_DEVI void load_columns(uint32_t at, float (&v)[N]) {
+  static_assert(N == 8 || N == 16 || N == 32, "");
+  if constexpr (N == 32) {
+    tc::tmem_ld32(at, v);
+  } else {
+    uint32_t r[N];
+    if constexpr (N == 16)
+      asm volatile(
+          "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+            "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          : "r"(at));
+    else
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                   : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+
+// -- 16-bit values of either type -----------------------------------------
+TAO_DEVI uint32_t pack(float lo, float hi, bool is_bf16) {
+  if (is_bf16) return bf16x2(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+TAO_DEVI uint16_t pack1(float v, bool is_bf16) { return (uint16_t)pack(v, 0.f, is_bf16); }
+TAO_DEVI float2 unpack(uint32_t w, bool is_bf16) {
+  if (is_bf16) return make_float2(lo_f(w), hi_f(w));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+TAO_DEVI float unpack1(uint16_t w, bool is_bf16) { return unpack(w, is_bf16).x; }
+TAO_DEVI float load1(const void* p, long long i, bool is_bf16) {
+  return unpack1(static_cast<const uint16_t*>(p)[i], is_bf16);
+}
+
+// -- activations ------------------------------------------------------------
+// 1 / (1 + e^-q), by the fast exponential and reciprocal: to some 2^-21 of it, far below a 16-bit step.
+TAO_DEVI float sigmoid(float q) { return __fdividef(1.f, 1.f + __expf(-q)); }
+constexpr float kGeluRoot = 0.7978845608028654f, kGeluCube = 0.044715f;  // sqrt(2 / pi)
+
+// gelu by the error function of the other side, whose small values keep their relative precision.
+TAO_DEVI float activate(float z, int act) {
+  switch (act) {
+    case TAO_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
+    case TAO_ACT_SILU: return z * sigmoid(z);
+    case TAO_ACT_GELU: return 0.5f * z * erfcf(-0.7071067811865476f * z);
+    case TAO_ACT_GELU_TANH: return z * sigmoid(2.f * kGeluRoot * (z + kGeluCube * z * z * z));
+  }
+  return z;
+}
+// act(z) and act'(z).
+TAO_DEVI float2 activate_slope(float z, int act) {
+  switch (act) {
+    case TAO_ACT_RELU: return make_float2(z > 0.f || z != z ? z : 0.f, z > 0.f ? 1.f : 0.f);
+    case TAO_ACT_SILU: {
+      const float s = sigmoid(z);
+      return make_float2(z * s, s * (1.f + z * (1.f - s)));
+    }
+    case TAO_ACT_GELU: {
+      const float p = 0.5f * erfcf(-0.7071067811865476f * z);
+      return make_float2(z * p, p + z * 0.3989422804014327f * __expf(-0.5f * z * z));
+    }
+    case TAO_ACT_GELU_TANH: {
+      const float s = sigmoid(2.f * kGeluRoot * (z + kGeluCube * z * z * z));
+      const float near = fminf(fmaxf(z, -32.f), 32.f);  // where s (1 - s) is 0 the square would be infinite
+      return make_float2(z * s, s + near * s * (1.f - s) * 2.f * kGeluRoot * (1.f + 3.f * kGeluCube * near * near));
+    }
+  }
+  return make_float2(z, 1.f);
+}
+template <int N>
+TAO_DEVI void activate_all(float (&v)[N], int act) {
+#define TAO_EACH(code)                                        \
+  case code:                                                  \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = activate(v[i], code); \
+    break;
+  switch (act) {  // the choice outside of the loop
+    TAO_EACH(TAO_ACT_RELU)
+    TAO_EACH(TAO_ACT_SILU)
+    TAO_EACH(TAO_ACT_GELU)
+    TAO_EACH(TAO_ACT_GELU_TANH)
+  }
+#undef TAO_EACH
+}
+
+// -- tiles ----------------------------------------------------------------------
+struct Tile {
+  int row0, rows;  // token rows: the first, and how many of the tile's there are; WEIGHT: rows of the matrix
+  int col0;
+  int group, second;  // expert; WEIGHT: which of its matrices
+  int from, upto;     // WEIGHT: its token rows
+  int blocks;         // steps of the ring; 0: zeros
+};
+
+// The experts' last rows (not before the one before, not behind the last row) and the tiles before each;
+// rows of no expert are one more group.  By one warp.
+template <class C>
+TAO_DEVI void make_lists(const Args& a, int* first, int* ends, int lane) {
+  const int col_tiles = (a.cols + C::CT - 1) / C::CT;
+  int end = 0, tiles = 0;
+  for (int base = 0; base <= a.groups; base += 32) {
+    const int e = base + lane;
+    int v = e < a.groups ? min(max(a.offsets[e + 1], 0), a.rows) : a.rows;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int w = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = max(v, w);
+    }
+    v = max(v, end);
+    int before = __shfl_up_sync(0xffffffffu, v, 1);
+    if (lane == 0) before = end;
+    int n = e <= a.groups ? (v - before + C::TT - 1) / C::TT * col_tiles : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int w = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += w;
+    }
+    if (e <= a.groups) {
+      ends[e] = v;
+      first[e + 1] = tiles + n;
+    }
+    end = __shfl_sync(0xffffffffu, v, 31);
+    tiles += __shfl_sync(0xffffffffu, n, 31);
+  }
+  if (lane == 0) first[0] = 0;
+}
+
+// Tile t of all; `group` is the one of the caller's tile before (0 at first).
+template <int FORM, class C>
+TAO_DEVI Tile tile_of(const Args& a, const int* first, const int* ends, int t, int& group) {
+  Tile tile;
+  const int col_tiles = (a.cols + C::CT - 1) / C::CT;
+  tile.second = tile.from = tile.upto = 0;
+  if constexpr (FORM == WEIGHT) {
+    const int row_tiles = (a.depth + 127) / 128, per = row_tiles * col_tiles;
+    const int matrix = t / per, at = t - matrix * per;
+    group = matrix / a.pairs;
+    tile.second = matrix - group * a.pairs;
+    tile.row0 = at % row_tiles * 128;
+    tile.col0 = at / row_tiles * C::CT;
+    tile.rows = min(128, a.depth - tile.row0);
+    if (a.offsets) {
+      tile.from = group ? ends[group - 1] : 0;
+      tile.upto = ends[group];
+    } else {
+      tile.upto = a.rows;
+    }
+    tile.blocks = (tile.upto - tile.from + kTerms - 1) / kTerms;
+  } else {
+    int begin = 0, end = a.rows;
+    if (a.offsets) {
+      while (t >= first[group + 1]) ++group;
+      t -= first[group];
+      begin = group ? ends[group - 1] : 0;
+      end = ends[group];
+    }
+    const int row_tiles = (end - begin + C::TT - 1) / C::TT;
+    const int band = t / (kBand * col_tiles), in = t - band * (kBand * col_tiles);
+    const int high = min(kBand, row_tiles - band * kBand), column = in / high;
+    tile.row0 = begin + (band * kBand + in - column * high) * C::TT;
+    tile.col0 = column * C::CT;
+    tile.rows = min(C::TT, end - tile.row0);
+    tile.blocks = a.offsets && group == a.groups ? 0 : (a.depth + kTerms - 1) / kTerms * (FORM == INPUT ? a.pairs : 1);
+  }
+  tile.group = group;
+  return tile;
+}
+
+// -- 32 x 32 values between a warp's threads, a row each, and memory ----------------
+// Through 2 KB of shared memory, 16-byte chunks of a row turned so that eight rows' meet all banks.
+TAO_DEVI int staged(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1 & 3)) << 4); }
+
+TAO_DEVI void store_rows(uint8_t* staging, void* to, long long stride, int rows, int cols, bool wide, int lane) {
+  uint16_t* const out = static_cast<uint16_t*>(to);
+  if (wide) {
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      if (r < rows && c * 8 < cols)
+        *reinterpret_cast<uint4*>(out + r * stride + c * 8) = *reinterpret_cast<const uint4*>(staging + staged(r, c));
+    }
+  } else {
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && lane < cols)
+        out[r * stride + lane] = *reinterpret_cast<const uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2);
+  }
+}
+TAO_DEVI void fetch_rows(uint8_t* staging, const void* from, long long stride, int rows, int cols, bool wide, int lane) {
+  const uint16_t* const in = static_cast<const uint16_t*>(from);
+  if (wide) {
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      if (r < rows && c * 8 < cols)
+        *reinterpret_cast<uint4*>(staging + staged(r, c)) = *reinterpret_cast<const uint4*>(in + r * stride + c * 8);
+    }
+  } else {
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && lane < cols)
+        *reinterpret_cast<uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2) = in[r * stride + lane];
+  }
+}
+// This thread's row of v, rounded, to memory.  All lanes of the warp.
+TAO_DEVI void put_rows(uint8_t* staging, const float (&v)[32], bool is_bf16, void* to, long long stride, int rows,
+                       int cols, bool wide, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(staging + staged(lane, c)) =
+        make_uint4(pack(v[c * 8], v[c * 8 + 1], is_bf16), pack(v[c * 8 + 2], v[c * 8 + 3], is_bf16),
+                   pack(v[c * 8 + 4], v[c * 8 + 5], is_bf16), pack(v[c * 8 + 6], v[c * 8 + 7], is_bf16));
+  __syncwarp();
+  store_rows(staging, to, stride, rows, cols, wide, lane);
+  __syncwarp();
+}
+
+// One output of a FORWARD, FEW or WEIGHT product that was split, from its whole sum.
+template <int FORM>
+TAO_DEVI float finish(const Args& a, float v, long long row, int col, bool is_bf16) {
+  if constexpr (FORM == FORWARD || FORM == FEW) {
+    if (a.bias) v += load1(a.bias, col, is_bf16);
+    if (a.z) static_cast<uint16_t*>(a.z)[row * a.z_stride + col] = pack1(v, is_bf16);
+    v = activate(v, a.act);
+    if (a.residual) v += load1(a.residual, row * a.r_stride + col, is_bf16);
+  }
+  return v;
+}
+
+// Maps: FORWARD: x, W, -, U.  FEW: W, x, U, -.  INPUT: dz, W, du, U.  WEIGHT: dz, x, du, -.
+template <int FORM, int BN, bool GATED, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_a2, const __grid_constant__ CUtensorMap map_b2,
+                   const Args a) {
+  using namespace tc;
+  using C = Cfg<FORM, BN, GATED, SPLIT>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint8_t* const staging_all = sm + C::STAGES * C::STAGE;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(staging_all + C::STAGING);
+  uint64_t* const empty = full + C::STAGES;
+  uint64_t* const acc_full = empty + C::STAGES;  // [2]
+  uint64_t* const acc_empty = acc_full + 2;      // [2]
+  uint64_t* const over = acc_empty + 2;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(over + 1);
+  volatile int* const abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* const first = reinterpret_cast<int*>(staging_all + C::STAGING + 512);  // [groups + 2]
+  int* const ends = first + kMostGroups + 2;                                  // [groups + 1]
+
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  if (smem_u32(sm) & 1023u) {  // 128-byte swizzled tiles start on 1024 bytes
+    if (tid == 0) atomicOr(&g_error, kErrState);
+    return;
+  }
+  const bool is_bf16 = a.type == TAO_TYPE_BF16;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 32) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], kWorkers);
+    }
+    mbar_init(over, 1);
+    *abort = 0;
+    fence_mbar_init();
+  }
+  if constexpr (!SPLIT)
+    if (warp == 2 && a.offsets) make_lists<C>(a, first, ends, lane);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tbase = *tmem_slot;
+
+  const int rank = SPLIT ? (int)cluster_rank() : 0;
+  const int start = SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
+  int total;
+  if (FORM == WEIGHT)
+    total = (a.depth + 127) / 128 * ((a.cols + C::CT - 1) / C::CT) * a.groups * a.pairs;
+  else
+    total = a.offsets ? first[a.groups + 1] : (a.rows + C::TT - 1) / C::TT * ((a.cols + C::CT - 1) / C::CT);
+  // this block's part of a tile's steps
+  auto part = [&](const Tile& t, int& k0) {
+    if constexpr (!SPLIT) return k0 = 0, t.blocks;
+    k0 = (int)((long long)t.blocks * rank / a.split);
+    return (int)((long long)t.blocks * (rank + 1) / a.split) - k0;
+  };
+
+  int group = 0;
+  if (warp == kWorkers) {
+    // ---- fetches operands
+    uint32_t fetched = 0;
+    int s = 0, phase = 0;
+    bool ok = true;
+    for (int t = start; ok && t < total; t += step) {
+      const Tile tile = tile_of<FORM, C>(a, first, ends, t, group);
+      int k0;
+      const int blocks = part(tile, k0);
+      for (int kb = k0; kb < k0 + blocks; ++kb) {
+        if (!(ok = warp_wait_for(&empty[s], phase ^ 1, abort))) break;
+        if (lane == 0) {
+          uint8_t* const sa = sm + s * C::STAGE;
+          uint8_t* const sb = sa + C::A;
+          mbar_expect_tx(&full[s], C::STAGE);
+          if constexpr (FORM == FORWARD) {
+            const int k = kb * kTerms;
+            tma_3d(sa, &map_a, k, tile.row0, 0, &full[s]);
+            tma_3d(sb, &map_b, k, tile.col0, tile.group, &full[s]);
+            if constexpr (GATED) tma_3d(sb + C::B / 2, &map_b2, k, tile.col0, tile.group, &full[s]);
+          } else if constexpr (FORM == FEW) {
+            const int k = kb * kTerms;
+            tma_3d(sa, &map_a, k, tile.col0, tile.group, &full[s]);
+            if constexpr (GATED) tma_3d(sa + C::A / 2, &map_a2, k, tile.col0, tile.group, &full[s]);
+            tma_3d(sb, &map_b, k, tile.row0, 0, &full[s]);
+          } else if constexpr (FORM == INPUT) {
+            const int each = tile.blocks / a.pairs;
+            const bool other = kb >= each;
+            const int k = (kb - (other ? each : 0)) * kTerms;
+            tma_3d(sa, other ? &map_a2 : &map_a, k, tile.row0, 0, &full[s]);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j)
+              tma_3d(sb + j * 8192, other ? &map_b2 : &map_b, tile.col0 + j * 64, k, tile.group, &full[s]);
+          } else {
+            const int k = tile.from + kb * kTerms;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              tma_3d(sa + j * 8192, tile.second ? &map_a2 : &map_a, tile.row0 + j * 64, k, 0, &full[s]);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_3d(sb + j * 8192, &map_b, tile.col0 + j * 64, k, 0, &full[s]);
+          }
+        }
+        __syncwarp();
+        ++fetched;
+        if (++s == C::STAGES) s = 0, phase ^= 1;
+      }
+    }
+    if (!ok) {  // copies in flight have their time before the block ends
+      const uint32_t last = fetched < C::STAGES ? 0 : fetched - C::STAGES;
+      for (uint32_t i = last; i < fetched; ++i) mbar_wait(&full[i % C::STAGES], i / C::STAGES & 1, nullptr);
+    }
+  } else if (warp == kWorkers + 1) {
+    // ---- issues the products
+    const uint32_t type_bits = is_bf16 ? 1u << 7 | 1u << 10 : 0u;
+    const uint32_t idesc = (idesc_bf16(128, BN, C::A_MN, C::B_MN) & ~(1u << 7 | 1u << 10)) | type_bits;
+    int s = 0, phase = 0, set = 0, set_phase = 0;
+    bool ok = true;
+    for (int t = start; ok && t < total; t += step) {
+      const Tile tile = tile_of<FORM, C>(a, first, ends, t, group);
+      int k0;
+      const int blocks = part(tile, k0);
+      if (blocks == 0) continue;
+      if (!(ok = warp_wait_for(&acc_empty[set], set_phase ^ 1, abort))) break;
+      fence_after();
+      const uint32_t acc = tbase + set * C::ACC;
+      for (int kb = 0; kb < blocks; ++kb) {
+        if (!(ok = warp_wait_for(&full[s], phase, abort))) break;
+        fence_after();
+        const uint32_t sa = smem_u32(sm + s * C::STAGE), sb = sa + C::A;
+        int steps = kTerms / 16;
+        if constexpr (FORM == WEIGHT) {
+          const int left = tile.upto - tile.from - (k0 + kb) * kTerms;
+          if (left < kTerms) {
+            steps = (left + 15) / 16;
+            const int rows = steps * 16 - left;  // terms of the last product that are other rows'
+            if (a.offsets && rows > 0) {
+              for (int i = lane; i < rows * 8 * (2 + BN / 64); i += 32)
+                *reinterpret_cast<uint4*>(sm + s * C::STAGE + (i / (rows * 8)) * 8192 + (left + i / 8 % rows) * 128 +
+                                          (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async();
+              __syncwarp();
+            }
+          }
+        }
+        if (lane == 0) {
+          for (int k = 0; k < steps; ++k) {
+            const uint64_t db = C::B_MN ? sdesc(sb + k * 2048, 8192, 1024) : sdesc(sb + k * 32, 16, 1024);
+            const uint64_t da = C::A_MN ? sdesc(sa + k * 2048, 8192, 1024) : sdesc(sa + k * 32, 16, 1024);
+            mma(acc, da, db, idesc, kb > 0 || k > 0);
+            if constexpr (FORM == FEW && GATED)
+              mma(acc + BN, sdesc(sa + C::A / 2 + k * 32, 16, 1024), db, idesc, kb > 0 || k > 0);
+          }
+          commit(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == C::STAGES) s = 0, phase ^= 1;
+      }
+      if (!ok) break;
+      if (lane == 0) commit(&acc_full[set]);
+      __syncwarp();
+      if (++set == C::SETS) set = 0, set_phase ^= 1;
+    }
+    if (lane == 0) {  // nothing is in flight when the block ends
+      commit(over);
+      mbar_wait(over, 0, nullptr);
+    }
+    __syncwarp();
+  } else {
+    // ---- turns sums into outputs: a warp has the rows of its quarter of TMEM, and half of the columns
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    uint8_t* const staging = staging_all + warp * 2048;
+    int set = 0, set_phase = 0;
+    bool ok = true;
+    for (int t = start; ok && t < total; t += step) {
+      const Tile tile = tile_of<FORM, C>(a, first, ends, t, group);
+      int k0;
+      const int blocks = part(tile, k0);
+      const uint32_t acc = tbase + set * C::ACC + lanes;
+      if (blocks) {
+        if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort))) break;
+        fence_after();
+      }
+      if constexpr (SPLIT) {
+        constexpr int W = BN / 2 < 32 ? BN / 2 : 32;
+        float* const sums = reinterpret_cast<float*>(sm);
+        const int r = quarter * 32 + lane;
+#pragma unroll 1
+        for (int c0 = half * (BN / 2); c0 < (half + 1) * (BN / 2); c0 += W) {
+          float v[W];
+          if (blocks) {
+            load_columns(acc + c0, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = 0.f;
+          }
+          if constexpr (FORM == FEW) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) sums[(c0 + i) * 132 + r] = v[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; i += 4)
+              *reinterpret_cast<float4*>(sums + r * (BN + 4) + c0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        }
+      } else if constexpr (FORM == FEW) {
+        constexpr int W = BN / 2;
+        const int col = tile.col0 + quarter * 32 + lane, rows = tile.rows - half * W;
+        if (rows > 0) {  // the same for the warp
+          float v[W], u[GATED ? W : 1];
+          if (blocks) {
+            load_columns(acc + half * W, v);
+            if constexpr (GATED) load_columns(acc + BN + half * W, u);
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = 0.f, u[GATED ? i : 0] = 0.f;
+          }
+          if (col < a.cols) {
+            const long long row0 = tile.row0 + half * W;
+            const float bias = a.bias ? load1(a.bias, col, is_bf16) : 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              v[i] += bias;
+              if (a.z && i < rows) {
+                static_cast<uint16_t*>(a.z)[(row0 + i) * a.z_stride + col] = pack1(v[i], is_bf16);
+                if constexpr (GATED) static_cast<uint16_t*>(a.u)[(row0 + i) * a.z_stride + col] = pack1(u[i], is_bf16);
+              }
+            }
+            activate_all(v, a.act);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              if constexpr (GATED) v[i] *= u[i];
+              if (i < rows) {
+                if (a.residual) v[i] += load1(a.residual, (row0 + i) * a.r_stride + col, is_bf16);
+                static_cast<uint16_t*>(a.y)[(row0 + i) * a.cols + col] = pack1(v[i], is_bf16);
+              }
+            }
+          }
+        }
+        if (blocks) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[set]);
+        }
+      } else {
+        constexpr int HALF = C::CT / 2;
+        const long long row0 = tile.row0 + quarter * 32;
+        const int rows = tile.rows - quarter * 32;
+        uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
+        if constexpr (FORM == WEIGHT) y += (long long)tile.group * a.depth * a.cols;
+#pragma unroll 1
+        for (int c0 = half * HALF; c0 < (half + 1) * HALF; c0 += 32) {
+          const int col = tile.col0 + c0, cols = a.cols - col;
+          float v[32], u[GATED ? 32 : 1];
+          if (blocks) {
+            load_columns(acc + c0, v);
+            if constexpr (GATED) load_columns(acc + BN / 2 + c0, u);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f, u[GATED ? i : 0] = 0.f;
+          }
+          if (rows <= 0 || cols <= 0) continue;  // the same for the warp
+          if constexpr (FORM == FORWARD) {
+            if (a.bias) {
+              const float bias = lane < cols ? load1(a.bias, col + lane, is_bf16) : 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bias, i);
+            }
+            if (a.z) {
+              put_rows(staging, v, is_bf16, static_cast<uint16_t*>(a.z) + row0 * a.z_stride + col, a.z_stride, rows,
+                       cols, a.wide, lane);
+              if constexpr (GATED)
+                put_rows(staging, u, is_bf16, static_cast<uint16_t*>(a.u) + row0 * a.z_stride + col, a.z_stride, rows,
+                         cols, a.wide, lane);
+            }
+            activate_all(v, a.act);
+            if constexpr (GATED) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] *= u[i];
+            }
+            if (a.residual) {
+              fetch_rows(staging, static_cast<const uint16_t*>(a.residual) + row0 * a.r_stride + col, a.r_stride, rows,
+                         cols, a.wide, lane);
+              __syncwarp();
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const uint4 w = *reinterpret_cast<const uint4*>(staging + staged(lane, c));
+                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = unpack(words[i], is_bf16);
+                  v[c * 8 + i * 2] += f.x;
+                  v[c * 8 + i * 2 + 1] += f.y;
+                }
+              }
+              __syncwarp();
+            }
+          }
+          put_rows(staging, v, is_bf16, y + row0 * a.cols + col, a.cols, rows, cols, a.wide, lane);
+        }
+        if (blocks) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[set]);
+        }
+      }
+      if (blocks && ++set == C::SETS) set = 0, set_phase ^= 1;
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
+
+  if constexpr (SPLIT) {
+    // every block has its part in shared memory; each adds a share of the tile's outputs
+    cluster_sync();
+    const Tile tile = tile_of<FORM, C>(a, first, ends, start, group);
+    constexpr int ACROSS = FORM == FEW ? 32 : BN / 4, DOWN = FORM == FEW ? BN : 128, ROW = FORM == FEW ? 132 : BN + 4;
+    uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
+    for (int i = rank * kThreads + tid; i < ACROSS * DOWN; i += kThreads * a.split) {
+      const int r = i / ACROSS, c = i % ACROSS * 4;
+      if (r >= tile.rows || tile.col0 + c >= a.cols) continue;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t at = smem_u32(reinterpret_cast<const float*>(sm) + r * ROW + c);
+#pragma unroll 4
+      for (int q = 0; q < a.split; ++q) {
+        const float4 w = ld_cluster(at, q);
+        v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+      }
+      const long long row = tile.row0 + r;
+      const int col = tile.col0 + c;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < a.cols) v[j] = finish<FORM>(a, v[j], row, col + j, is_bf16);
+      uint16_t* const out = y + row * a.cols + col;
+      if (a.wide) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack(v[0], v[1], is_bf16), pack(v[2], v[3], is_bf16));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < a.cols) out[j] = pack1(v[j], is_bf16);
+      }
+    }
+    cluster_sync();  // the others' reads of this block's part are over
+  }
+}
+
+}  // namespace product
+}  // namespace tao

@@ -1,0 +1,166 @@
+// A stable sort of a few thousand to some millions of small whole numbers by counting: tokens by expert in one
+// pass, tokens by word in two or three passes of up to nine bits.
+//
+// A pass counts, for each block's run of elements, how many fall into each bin (count_kernel), and then places
+// each element (place_kernel): a bin begins behind all smaller bins, a block's elements behind those of the
+// blocks before, a warp's behind those of the warps before, and of 32 elements at a time each finds those before
+// it in its bin by a match across the warp.  No atomics: the order, and all that is summed by it, is fixed.
+// Up to kSmallSort elements one block does it in one launch.  What bounds it is latency: launches, and each
+// warp's chain of some rounds of 32 (its elements are read as they are needed, 262144 are 64 blocks' work).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace tao {
+namespace sorting {
+
+constexpr int kMostBins = 513;  // 512 and one for what belongs to none
+constexpr int kSmallSort = 8192;
+constexpr int kMostBlocks = 128;
+
+// A pass over n elements.  The key of element i is ids[value], value = values[i] or (values null) i: the whole id
+// for `shift` < 0, else `bits` bits of it from `shift` on.  Ids outside of 0 .. limit - 1 count as `limit`.
+struct Pass {
+  const void* ids;
+  const int* values;
+  long long limit;
+  int n, shift, bins, per;  // per: elements of a warp
+  bool wide;                // ids have 64 bits
+  const int* counts;        // [blocks][bins], of all blocks; null: this block is the only one
+  int blocks;
+  int* sorted;              // values in order
+  int* places;              // where element i went, or null
+  int* keys;                // whole ids in order, or null
+  int* offsets;             // the first place of each bin, or null
+};
+
+TAO_DEVI int id_of(const Pass& p, int value) {
+  const long long id = p.wide ? static_cast<const long long*>(p.ids)[value] : static_cast<const int*>(p.ids)[value];
+  return (int)(id < 0 || id >= p.limit ? p.limit : id);
+}
+TAO_DEVI int bin_of(const Pass& p, int id) { return p.shift < 0 ? id : id >> p.shift & (p.bins - 1); }
+
+// counts[warp][bin] of this block's warps, in shared memory.
+TAO_DEVI void count_warps(const Pass& p, int* counts, int warps) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < warps * p.bins; i += blockDim.x) counts[i] = 0;
+  __syncthreads();
+  const long long begin = ((long long)blockIdx.x * warps + warp) * p.per;
+  const int end = (int)min(begin + p.per, (long long)p.n);
+  int* const mine = counts + warp * p.bins;
+  for (long long i = begin + lane; i < end; i += 32) atomicAdd(mine + bin_of(p, id_of(p, p.values ? p.values[i] : (int)i)), 1);
+  __syncthreads();
+}
+
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) count_kernel(const Pass p, int* out) {
+  extern __shared__ int counts[];
+  count_warps(p, counts, WARPS);
+  for (int b = threadIdx.x; b < p.bins; b += 32 * WARPS) {
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += counts[w * p.bins + b];
+    out[(long long)blockIdx.x * p.bins + b] = s;
+  }
+}
+
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) place_kernel(const Pass p) {
+  extern __shared__ int counts[];
+  __shared__ int first[kMostBins], before[kMostBins];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  count_warps(p, counts, WARPS);
+  for (int b = threadIdx.x; b < p.bins; b += 32 * WARPS) {
+    int all = 0, earlier = 0;
+    if (p.counts) {
+#pragma unroll 8
+      for (int k = 0; k < p.blocks; ++k) {
+        const int c = p.counts[(long long)k * p.bins + b];
+        all += c;
+        if (k < (int)blockIdx.x) earlier += c;
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) all += counts[w * p.bins + b];
+    }
+    first[b] = all;
+    before[b] = earlier;
+  }
+  __syncthreads();
+  if (warp == 0) {  // the bins' sizes to their first places
+    int sum = 0;
+    for (int base = 0; base < p.bins; base += 32) {
+      const int b = base + lane, mine = b < p.bins ? first[b] : 0;
+      int s = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+      }
+      if (b < p.bins) first[b] = sum + s - mine;
+      sum += __shfl_sync(0xffffffffu, s, 31);
+    }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.bins; b += 32 * WARPS) {
+    if (p.offsets && blockIdx.x == 0) p.offsets[b] = first[b];
+    int at = first[b] + before[b];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const int c = counts[w * p.bins + b];
+      counts[w * p.bins + b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  const long long begin = ((long long)blockIdx.x * WARPS + warp) * p.per;
+  const int end = (int)min(begin + p.per, (long long)p.n);
+  int* const mine = counts + warp * p.bins;
+  for (long long base = begin; base < end; base += 32) {
+    const long long i = base + lane;
+    const bool in = i < end;
+    const int value = in ? (p.values ? p.values[i] : (int)i) : 0;
+    const int id = in ? id_of(p, value) : 0, bin = in ? bin_of(p, id) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, bin);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    const int at = in ? mine[bin] + rank : 0;
+    __syncwarp();
+    if (in && rank == 0) mine[bin] += __popc(same);
+    __syncwarp();
+    if (in) {
+      p.sorted[at] = value;
+      if (p.places) p.places[i] = at;
+      if (p.keys) p.keys[at] = id;
+    }
+  }
+}
+
+inline int blocks_of(long long n) { return n <= kSmallSort ? 1 : (int)std::min<long long>((n + 4095) / 4096, kMostBlocks); }
+inline size_t counts_bytes(long long n, int bins) { return n <= kSmallSort ? 0 : (size_t)blocks_of(n) * bins * sizeof(int); }
+
+// `counts`: counts_bytes of scratch.
+inline cudaError_t run(Pass p, int* counts, cudaStream_t s) {
+  p.blocks = blocks_of(p.n);
+  if (p.blocks == 1) {
+    p.counts = nullptr;
+    p.per = (p.n + 1023) / 1024 * 32;
+    static_assert(32 * kMostBins * sizeof(int) <= 96 * 1024, "");
+    const cudaError_t e = cudaFuncSetAttribute(place_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               32 * kMostBins * (int)sizeof(int));
+    if (e != cudaSuccess) return e;
+    place_kernel<32><<<1, 1024, 32 * p.bins * sizeof(int), s>>>(p);
+    return cudaGetLastError();
+  }
+  const int warps = p.blocks * 8;
+  p.per = (int)(((long long)p.n + warps - 1) / warps + 31) / 32 * 32;
+  p.counts = counts;
+  count_kernel<8><<<p.blocks, 256, 8 * p.bins * sizeof(int), s>>>(p, counts);
+  place_kernel<8><<<p.blocks, 256, 8 * p.bins * sizeof(int), s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace sorting
+}  // namespace tao

@@ -1,0 +1,232 @@
+// Tokens sorted by expert and back: the order (sort.cuh), rows copied to their pairs' places, and the experts'
+// rows added into their tokens by weight, with the gradients.  All bound by their bytes: a thread has 16 bytes of
+// a token's row and goes over the token's pairs, so that x is read and y written once; a token's pairs are added
+// in the order of its choices.
+#include <cuda_runtime.h>
+
+#include "rows.cuh"
+#include "sort.cuh"
+
+void tao_set_last_error(const char* msg);
+
+namespace tao {
+namespace {
+
+using namespace rows;
+
+int tfail(int code, const char* msg) {
+  tao_set_last_error(msg);
+  return code;
+}
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TAO_OK : tfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
+struct TokenArgs {
+  const int* places;  // [tokens][k]
+  const int* kept;    // pairs that have an expert (their places come first), or null: all
+  long long tokens, pairs;
+  int k, width;
+  const void *in, *other, *weights;  // rows; weights null: ones
+  long long in_stride, other_stride;
+  int weight_type;
+  void *out, *dw;
+};
+
+TAO_DEVI int kept_of(const TokenArgs& a) { return a.kept ? (int)min((long long)*a.kept, a.pairs) : (int)a.pairs; }
+
+template <class T, int N>
+__global__ void __launch_bounds__(256) gather_kernel(const TokenArgs a) {
+  const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (t >= a.tokens || c >= a.width) return;
+  const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + t * a.in_stride + c);
+#pragma unroll 4
+  for (int j = 0; j < a.k; ++j) {
+    const int place = a.places[t * a.k + j];
+    if ((unsigned)place < (unsigned)a.pairs)
+      *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)place * a.width + c) = v;
+  }
+}
+
+// out[t] = sum over j of weights[t][j] in[places[t][j]]
+template <class T, int N>
+__global__ void __launch_bounds__(256) return_kernel(const TokenArgs a) {
+  const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (t >= a.tokens || c >= a.width) return;
+  const int kept = kept_of(a);
+  float sum[N] = {};
+  constexpr int AT_ONCE = 4;  // rows on their way
+  for (int j0 = 0; j0 < a.k; j0 += AT_ONCE) {
+    Vec<T, N> v[AT_ONCE];
+    float w[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int place = j0 + j < a.k ? a.places[t * a.k + j0 + j] : -1;
+      const bool in = (unsigned)place < (unsigned)kept;
+      w[j] = in ? 1.f : 0.f;
+      if (in) {
+        v[j] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + place * a.in_stride + c);
+        if (a.weights) w[j] = value_of(a.weights, t * a.k + j0 + j, a.weight_type);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[j].v[i] = rounded<T>(0.f);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      float f[N];
+      v[j].widen(f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] += w[j] * f[i];
+    }
+  }
+  *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + t * a.width + c) = Vec<T, N>::of(sum);
+}
+
+// A warp a pair: out[place] = weight in[t], dw = in[t] . other[place]; zeros for a pair of no expert.
+template <class T, int N>
+__global__ void __launch_bounds__(256) return_gradient_kernel(const TokenArgs a) {
+  const long long pair = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (pair >= a.pairs) return;
+  const int place = a.places[pair];
+  if ((unsigned)place >= (unsigned)a.pairs) return;
+  const bool in = place < kept_of(a);
+  const float w = !in ? 0.f : a.weights ? value_of(a.weights, pair, a.weight_type) : 1.f;
+  const T* const dy = static_cast<const T*>(a.in) + pair / a.k * a.in_stride;
+  const T* const y = static_cast<const T*>(a.other) + place * a.other_stride;
+  T* const out = static_cast<T*>(a.out) + (long long)place * a.width;
+  float dot = 0.f;
+#pragma unroll 4
+  for (int c = lane * N; c < a.width; c += 32 * N) {
+    float d[N] = {};
+    if (in) {
+      reinterpret_cast<const Vec<T, N>*>(dy + c)->widen(d);
+      if (a.dw) {
+        float f[N];
+        reinterpret_cast<const Vec<T, N>*>(y + c)->widen(f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) dot += d[i] * f[i];
+      }
+    }
+    if (a.out) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = in ? d[i] * w : 0.f;
+      *reinterpret_cast<Vec<T, N>*>(out + c) = Vec<T, N>::of(d);
+    }
+  }
+  if (a.dw) {
+    dot = warp_sum(dot);
+    if (lane == 0) set_value(a.dw, pair, dot, a.weight_type);
+  }
+}
+
+int check(const TokenArgs& a, int type) {
+  if (!known(type)) return tfail(TAO_ERR_ARG, "tokens are bf16, fp16 or fp32");
+  if (a.weights && a.weight_type != TAO_TYPE_FP32 && a.weight_type != type)
+    return tfail(TAO_ERR_ARG, "weights are fp32 or of the rows' type");
+  if (a.tokens < 0 || a.k < 1 || a.width < 1 || a.k > (1 << 20) || a.width > (1 << 24) || a.tokens > (1ll << 30) / a.k)
+    return tfail(TAO_ERR_ARG, "a token has at least one choice and one channel, and there are up to 2^30 pairs");
+  return TAO_OK;
+}
+
+}  // namespace
+}  // namespace tao
+
+extern "C" {
+
+size_t tao_sort_tokens_workspace_bytes(long long pairs, int experts) {
+  return pairs <= 0 || experts < 1 ? 0 : tao::sorting::counts_bytes(pairs, experts + 1);
+}
+
+int tao_sort_tokens(const void* ids, int id_bytes, long long pairs, int experts, int* sorted, int* places, int* offsets,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace tao;
+  if (id_bytes != 4 && id_bytes != 8) return tfail(TAO_ERR_ARG, "ids have 32 or 64 bits");
+  if (experts < 1 || experts >= sorting::kMostBins) return tfail(TAO_ERR_ARG, "there are 1 to 512 experts");
+  if (pairs < 0 || pairs > (1ll << 30)) return tfail(TAO_ERR_ARG, "there are up to 2^30 pairs");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!offsets) return tfail(TAO_ERR_ARG, "null pointer");
+  if (!on_elements({{ids, (size_t)id_bytes}, {sorted, 4}, {places, 4}, {offsets, 4}, {workspace, 4}}))
+    return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  if (pairs == 0) {
+    const cudaError_t e = cudaMemsetAsync(offsets, 0, (experts + 1) * sizeof(int), s);
+    return e == cudaSuccess ? TAO_OK : tfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+  }
+  if (!ids || !sorted || !places) return tfail(TAO_ERR_ARG, "null pointer");
+  const size_t need = tao_sort_tokens_workspace_bytes(pairs, experts);
+  if (need && (!workspace || workspace_bytes < need)) return tfail(TAO_ERR_ARG, "workspace too small for the sort");
+  sorting::Pass p = {};
+  p.ids = ids, p.limit = experts, p.n = (int)pairs, p.shift = -1, p.bins = experts + 1, p.wide = id_bytes == 8;
+  p.sorted = sorted, p.places = places, p.offsets = offsets;
+  const cudaError_t e = sorting::run(p, static_cast<int*>(workspace), s);
+  return e == cudaSuccess ? TAO_OK : tfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int tao_gather_tokens(const void* x, long long x_stride, const int* places, long long tokens, int top_k, int width,
+                      int type, void* xs, void* stream) {
+  using namespace tao;
+  TokenArgs a = {};
+  a.places = places, a.tokens = tokens, a.k = top_k, a.width = width, a.in = x, a.in_stride = x_stride, a.out = xs;
+  if (int rc = check(a, type)) return rc;
+  if (tokens == 0) return TAO_OK;
+  a.pairs = tokens * top_k;
+  const size_t size = size_of(type);
+  if (!x || !places || !xs) return tfail(TAO_ERR_ARG, "null pointer");
+  if (!on_elements({{x, size}, {xs, size}, {places, 4}})) return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  const bool wide = width * size % 16 == 0 && on16(x, x_stride, size) && on16(xs, 0, size);
+  return by_vector(type, wide, [&](auto t, auto n) {
+    const Mapping m = mapping(tokens, (width + decltype(n)::value - 1) / decltype(n)::value);
+    gather_kernel<decltype(t), decltype(n)::value><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    return launched();
+  });
+}
+
+int tao_return_tokens(const void* ys, long long ys_stride, const int* places, const int* kept, const void* weights,
+                      int weight_type, long long tokens, int top_k, int width, int type, void* y, void* stream) {
+  using namespace tao;
+  TokenArgs a = {};
+  a.places = places, a.kept = kept, a.tokens = tokens, a.k = top_k, a.width = width, a.in = ys, a.in_stride = ys_stride;
+  a.weights = weights, a.weight_type = weight_type, a.out = y;
+  if (int rc = check(a, type)) return rc;
+  if (tokens == 0) return TAO_OK;
+  a.pairs = tokens * top_k;
+  const size_t size = size_of(type);
+  if (!ys || !places || !y) return tfail(TAO_ERR_ARG, "null pointer");
+  if (!on_elements({{ys, size}, {y, size}, {places, 4}, {kept, 4}, {weights, weights ? size_of(weight_type) : 1}}))
+    return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  const bool wide = width * size % 16 == 0 && on16(ys, ys_stride, size) && on16(y, 0, size);
+  return by_vector(type, wide, [&](auto t, auto n) {
+    const Mapping m = mapping(tokens, (width + decltype(n)::value - 1) / decltype(n)::value);
+    return_kernel<decltype(t), decltype(n)::value><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    return launched();
+  });
+}
+
+int tao_return_tokens_gradient(const void* dy, long long dy_stride, const void* ys, long long ys_stride, const int* places,
+                               const int* kept, const void* weights, int weight_type, long long tokens, int top_k,
+                               int width, int type, void* dys, void* dw, void* stream) {
+  using namespace tao;
+  TokenArgs a = {};
+  a.places = places, a.kept = kept, a.tokens = tokens, a.k = top_k, a.width = width, a.in = dy, a.in_stride = dy_stride;
+  a.other = ys, a.other_stride = ys_stride, a.weights = weights, a.weight_type = weight_type, a.out = dys, a.dw = dw;
+  if (int rc = check(a, type)) return rc;
+  if (tokens == 0) return TAO_OK;
+  a.pairs = tokens * top_k;
+  const size_t size = size_of(type);
+  if (!dy || !places || (!dys && !dw) || (dw && (!ys || !weights))) return tfail(TAO_ERR_ARG, "null pointer");
+  const size_t weight_size = weights ? size_of(weight_type) : 1;
+  if (!on_elements({{dy, size}, {ys, size}, {dys, size}, {places, 4}, {kept, 4}, {weights, weight_size}, {dw, weight_size}}))
+    return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  const bool wide = width * size % 16 == 0 && on16(dy, dy_stride, size) && on16(ys, ys_stride, size) && on16(dys, 0, size);
+  return by_vector(type, wide, [&](auto t, auto n) {
+    const unsigned grid = (unsigned)((a.pairs + 7) / 8);
+    return_gradient_kernel<decltype(t), decltype(n)::value><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    return launched();
+  });
+}
+
+}  // extern "C"

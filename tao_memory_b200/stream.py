@@ -846,6 +846,7 @@ def check_device(device=None):
     check_workspaces(dev)
     with torch.cuda.device(dev):
         _lib.check(_lib.lib().tao_linear4_check(None, current))
+        _lib.check(_lib.lib().tao_product_check(None, current))
     return total
 
 
