@@ -544,37 +544,40 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
 #define TAO_ACT_GELU 3
 #define TAO_ACT_GELU_TANH 4
 
-/* Products of bf16 or fp16 matrices (`type`), fp32 sums, rounded once; strides in elements, last axes contiguous.
- *   y [rows][n] = act(x [rows][k] W^T + bias) + residual            (W [n][k]; bias, residual may be NULL)
- * or, with offsets [experts + 1] (int32, device memory), of the experts' weights W [experts][n][k] (matrices
- * w_expert apart) for rows sorted by expert, offsets[e] .. offsets[e + 1] - 1 those of expert e:
- *   y = act(x W_e^T), or with `up` the gated act(x W_e^T) * (x U_e^T).
+/* Products of bf16 or fp16 matrices (`type`), fp32 sums, rounded once; strides in elements.
+ *   y [rows][n] = act(x [rows][k] W^T + bias) + residual            (W [n][k]; bias, residual may be NULL; experts 1)
+ * or, with offsets [experts + 1] (int32, device memory), of the experts' weights W [experts][n][k] for rows sorted
+ * by expert, offsets[e] .. offsets[e + 1] - 1 those of expert e:
+ *   y = act(x W_e^T), or with `up` (like W) the gated act(x W_e^T) * (x U_e^T).
  * offsets[0] is taken as 0, values are held between the one before and `rows`, and rows from offsets[experts] on
- * give zeros.  z, u [rows][z_stride]: what act and its factor are applied to, for the gradient, or NULL.
- * x, W, up and their rows start on 16 bytes; y, z, u, bias and the residual on whole elements.  y may be the
- * residual itself (r_stride n); it must not overlap another operand.  Up to 512 experts. */
-int tao_linear(const void* x, long long x_stride, const void* w, long long w_stride, long long w_expert, const void* up,
-               long long up_stride, long long up_expert, const void* bias, const void* residual, long long r_stride,
-               const int* offsets, int experts, long long rows, int n, int k, int type, int activation, void* y, void* z,
-               void* u, long long z_stride, void* stream);
-
-/* The gradient of tao_linear.  First dz = dy act'(z), or with u the gated dz = dy u act'(z), du = dy act(z)
- * (rounded to the type, [rows][d_stride]; z NULL: dz is dy, written if dz is not NULL), and db [n] = the sum of
- * dz over the rows, in a fixed order (NULL: not wanted; workspace: tao_linear_slope_workspace_bytes). */
-size_t tao_linear_slope_workspace_bytes(long long rows, int n);
-int tao_linear_slope(const void* dy, long long dy_stride, const void* z, const void* u, long long z_stride,
-                     long long rows, int n, int type, int activation, void* dz, void* du, long long d_stride, void* db,
-                     void* workspace, size_t workspace_bytes, void* stream);
-/* Then dx [rows][k] = dz W (+ du U), zeros for rows of no expert, ... */
-int tao_linear_input_gradient(const void* dz, const void* du, long long d_stride, const void* w, long long w_stride,
-                              long long w_expert, const void* up, long long up_stride, long long up_expert,
-                              const int* offsets, int experts, long long rows, int n, int k, int type, void* dx,
-                              void* stream);
-/* ... and dw [experts][n][k] = dz^T x (dup: du^T x) over each expert's rows, zeros for an expert without.  dz,
- * du, x, W, up and their rows start on 16 bytes. */
-int tao_linear_weight_gradient(const void* dz, const void* du, long long d_stride, const void* x, long long x_stride,
-                               const int* offsets, int experts, long long rows, int n, int k, int type, void* dw,
-                               void* dup, void* stream);
+ * give zeros.  z, u [rows][z_row]: what act and its factor are applied to, for the gradient, or NULL.
+ *
+ * The gradient (tao_linear_gradient) of dy [rows][n] (neighbours next to each other), with dz = dy act'(z), or gated
+ * dz = dy u act'(z) and du = dy act(z), rounded to the type for the products: dx [rows][k] = dz W (+ du U), zeros for
+ * rows of no expert; dw [experts][n][k] = dz^T x, dup = du^T x over each expert's rows, zeros for an expert
+ * without; db [n] = the sum of dz over the rows, in a fixed order.  Each may be NULL (dw and dup together); z (and u)
+ * are needed where there is an activation or a gate, x for dw, W and U for dx.
+ *
+ * x, W and U of any strides: what does not lie with neighbours next to each other and everything else on 16 bytes
+ * is copied into the workspace first (tao_linear_workspace_bytes of the same structure, on 256 bytes; each
+ * call's own until it is over).  y, dx, dw, dup are contiguous; y may be the residual (r_row n), outputs must not
+ * overlap operands otherwise.  Up to 512 experts, 2^30 rows, n and k 2^24. */
+typedef struct TaoLinear {
+  const void *x, *w, *up, *bias, *residual;
+  const int* offsets;
+  long long x_row, x_col, w_expert, w_row, w_col, up_expert, up_row, up_col, r_row, z_row, rows;
+  int n, k, experts, type, activation;
+  void *y, *z, *u;
+  const void* dy;
+  long long dy_row;
+  void *dx, *dw, *dup, *db;
+  void* workspace;
+  size_t workspace_bytes;
+} TaoLinear;
+size_t tao_linear_sizeof(void);
+size_t tao_linear_workspace_bytes(const TaoLinear* p, int gradient);
+int tao_linear(const TaoLinear* p, void* stream);
+int tao_linear_gradient(const TaoLinear* p, void* stream);
 /* The current device's error word of the 16-bit products (a wait that ran out), read and cleared. */
 int tao_product_check(int* flags, void* stream);
 

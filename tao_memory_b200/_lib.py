@@ -48,6 +48,16 @@ class TaoExperts(ctypes.Structure):
                 + [("error", ctypes.c_void_p)])
 
 
+class TaoLinear(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "up", "bias", "residual", "offsets")]
+                + [(n, ctypes.c_longlong) for n in ("x_row", "x_col", "w_expert", "w_row", "w_col", "up_expert", "up_row",
+                                                    "up_col", "r_row", "z_row", "rows")]
+                + [(n, ctypes.c_int) for n in ("n", "k", "experts", "type", "activation")]
+                + [(n, ctypes.c_void_p) for n in ("y", "z", "u", "dy")] + [("dy_row", ctypes.c_longlong)]
+                + [(n, ctypes.c_void_p) for n in ("dx", "dw", "dup", "db", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)])
+
+
 class TaoError(RuntimeError):
     """A CUDA or device-side failure reported by the library."""
 
@@ -104,13 +114,10 @@ _SIGNATURES = {
     "tao_expert_workspace_bytes": (_SZ, [ctypes.POINTER(TaoExperts), _I]),
     "tao_expert_layer": (_I, [ctypes.POINTER(TaoExperts), _VP, _I64, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "tao_expert_check": (_I, [_VP, _SZ, ctypes.POINTER(_I), _VP]),
-    "tao_linear": (_I, [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I, _I64, _I, _I, _I, _I, _VP,
-                        _VP, _VP, _I64, _VP]),
-    "tao_linear_slope_workspace_bytes": (_SZ, [_I64, _I]),
-    "tao_linear_slope": (_I, [_VP, _I64, _VP, _VP, _I64, _I64, _I, _I, _I, _VP, _VP, _I64, _VP, _VP, _SZ, _VP]),
-    "tao_linear_input_gradient": (_I, [_VP, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I, _I64, _I, _I, _I, _VP,
-                                       _VP]),
-    "tao_linear_weight_gradient": (_I, [_VP, _VP, _I64, _VP, _I64, _VP, _I, _I64, _I, _I, _I, _VP, _VP, _VP]),
+    "tao_linear_sizeof": (_SZ, []),
+    "tao_linear_workspace_bytes": (_SZ, [ctypes.POINTER(TaoLinear), _I]),
+    "tao_linear": (_I, [ctypes.POINTER(TaoLinear), _VP]),
+    "tao_linear_gradient": (_I, [ctypes.POINTER(TaoLinear), _VP]),
     "tao_product_check": (_I, [ctypes.POINTER(_I), _VP]),
     "tao_sort_tokens_workspace_bytes": (_SZ, [_I64, _I]),
     "tao_sort_tokens": (_I, [_VP, _I, _I64, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
@@ -147,6 +154,8 @@ def lib():
             fn.argtypes = args
         if handle.tao_state_sizeof() != ctypes.sizeof(TaoState):
             raise RuntimeError("TaoState layout mismatch between Python and libtao_b200.so")
+        if handle.tao_linear_sizeof() != ctypes.sizeof(TaoLinear):
+            raise RuntimeError("TaoLinear layout mismatch between Python and libtao_b200.so")
         _lib = handle
     return _lib
 

@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "product.cuh"
+#include "product_few.cuh"
 
 void tao_set_last_error(const char* msg);
 
@@ -73,10 +74,40 @@ struct Operands {
   Operand2 a, b, a2, b2;
 };
 
-template <int FORM, int BN, bool GATED, bool SPLIT>
-int start(const Operands& o, Args a, int split, cudaStream_t stream) {
+// Clusters of `split` blocks that the device runs at once (how many blocks of a cluster find room in one GPC).
+template <int FORM, int BN>
+int clusters_of(int split) {
+  static std::atomic<int> known[16][9];  // of the first 16 devices
+  int device = 0;
+  if (split == 1 || cudaGetDevice(&device) != cudaSuccess) return sms();
+  if (device < 16)
+    if (const int n = known[device][split].load(std::memory_order_relaxed)) return n;
+  using C = Cfg<FORM, BN, false, true>;
+  auto kernel = product_kernel<FORM, BN, false, true, true>;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(split);
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = C::SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  c.attrs = attr;
+  c.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &c) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 1;
+  }
+  if (device < 16) known[device][split].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <int FORM, int BN, bool GATED, bool SPLIT, bool BF16>
+int start_typed(const Operands& o, Args a, int split, cudaStream_t stream) {
   using C = Cfg<FORM, BN, GATED, SPLIT>;
-  auto kernel = product_kernel<FORM, BN, GATED, SPLIT>;
+  auto kernel = product_kernel<FORM, BN, GATED, SPLIT, BF16>;
   CUtensorMap maps[4];
   constexpr int A_BOX = C::A_MN ? kTerms : 128, B_BOX = C::B_MN ? kTerms : FORM == FORWARD ? C::CT : BN;
   const Operand2* ops[4] = {&o.a, &o.b, &o.a2, &o.b2};
@@ -116,31 +147,75 @@ int start(const Operands& o, Args a, int split, cudaStream_t stream) {
   return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
 }
 
-// Blocks that share a tile's terms: as many as the SMs hold beside the other tiles', of four steps each at least.
-int split_of(long long tiles, int blocks) {
-  const long long fit = tiles > 0 ? sms() / tiles : 1;
-  return (int)std::max<long long>(1, std::min<long long>({fit, 8, blocks / 4}));
+template <int FORM, int BN, bool GATED, bool SPLIT>
+int start(const Operands& o, const Args& a, int split, cudaStream_t stream) {
+  return a.type == TAO_TYPE_BF16 ? start_typed<FORM, BN, GATED, SPLIT, true>(o, a, split, stream)
+                                 : start_typed<FORM, BN, GATED, SPLIT, false>(o, a, split, stream);
+}
+
+// Blocks that share a tile's terms, and what it takes in steps of the ring: rounds of all clusters, each of its
+// steps and of `join` more for what the blocks give each other (none: of a few for the first and last tile).
+struct Split {
+  int blocks;
+  double cost;
+};
+template <int FORM, int BN>
+Split split_of(long long tiles, int steps, double join) {
+  Split best = {1, (double)((tiles + sms() - 1) / sms()) * (steps + 6)};
+  for (int s = 2; s <= 8 && s <= steps; ++s) {
+    const int fit = clusters_of<FORM, BN>(s);
+    const double cost = (double)((tiles + fit - 1) / fit) * ((steps + s - 1) / s + join);
+    if (cost < best.cost) best = {s, cost};
+  }
+  return best;
+}
+
+// FORWARD and INPUT of many rows, by what a tile of 256, 128 or 64 columns costs in steps of a 128 tile (about 0.2 us):
+// 1.6 of them a step for 256 columns, and for a split some 32 more.  Measured (us), 256 columns / 128 / 64 and split:
+// 2048x768x2304 9.2 / 9.9 / 46; 512x2048x2048 14.4 / 10.1 / 17.3; 128x8192x2048 48.5 / 29.6 / 16.7.
+template <int FORM>
+int start_rows(const Operands& o, const Args& a, long long row_tiles, int steps, cudaStream_t s) {
+  const int n = sms();
+  const auto rounds = [&](int width) { return (row_tiles * ((a.cols + width - 1) / width) + n - 1) / n; };
+  const double wide = rounds(256) * (1.6 * steps), narrow = (double)rounds(128) * steps;
+  if (!a.offsets) {
+    const Split split = split_of<FORM, 64>(row_tiles * ((a.cols + 63) / 64), steps, 32);
+    if (split.blocks > 1 && split.cost < std::min(wide, narrow)) return start<FORM, 64, false, true>(o, a, split.blocks, s);
+  }
+  if (narrow < wide || a.cols <= 128) return start<FORM, 128, false, false>(o, a, 1, s);
+  return start<FORM, 256, false, false>(o, a, 1, s);
+}
+
+template <int EIGHTS, int WARPS, int AHEAD>
+int start_few(const FewArgs& a, int type, cudaStream_t s) {
+  const unsigned grid = (a.n + 15) / 16;
+  if (type == TAO_TYPE_BF16)
+    few_kernel<EIGHTS, WARPS, AHEAD, true><<<grid, 32 * WARPS, 0, s>>>(a);
+  else
+    few_kernel<EIGHTS, WARPS, AHEAD, false><<<grid, 32 * WARPS, 0, s>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
+// Up to 32 rows; `false`: the tcgen05 form is the faster one.
+bool few_rows(const FewArgs& a, int type, cudaStream_t s, int* rc) {
+  const int outputs = (a.n + 15) / 16, rounds = (a.k + 31) / 32;
+  const bool narrow = outputs <= 148 && rounds >= 48;
+  if (a.rows <= 8)
+    *rc = rounds <= 16 ? start_few<1, 4, 4>(a, type, s)
+          : narrow || (rounds > 64 && outputs <= 296) ? start_few<1, 16, 4>(a, type, s)
+          : rounds <= 64 ? start_few<1, 8, 4>(a, type, s)
+                         : start_few<1, 8, 8>(a, type, s);
+  else if (a.rows <= 16)
+    *rc = narrow ? start_few<2, 16, 4>(a, type, s) : start_few<2, 8, 2>(a, type, s);
+  else if (outputs > 512)
+    return false;
+  else
+    *rc = outputs <= 148 ? start_few<4, 16, 2>(a, type, s) : start_few<4, 8, 1>(a, type, s);
+  return true;
 }
 
 bool on16(const void* p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
-
-int check_sizes(long long rows, int n, int k, int type, int act, const int* offsets, int experts) {
-  if (type != TAO_TYPE_BF16 && type != TAO_TYPE_FP16) return pfail(TAO_ERR_ARG, "16-bit products take bf16 or fp16");
-  if (act < TAO_ACT_NONE || act > TAO_ACT_GELU_TANH) return pfail(TAO_ERR_ARG, "unknown activation");
-  if (rows < 0 || n <= 0 || k <= 0) return pfail(TAO_ERR_ARG, "rows must not be negative, n and k must be positive");
-  if (rows > (1ll << 30) || n > (1 << 24) || k > (1 << 24))
-    return pfail(TAO_ERR_ARG, "rows are limited to 2^30, n and k to 2^24");
-  if (offsets ? experts < 1 || experts > kMostGroups : experts != 1)
-    return pfail(TAO_ERR_ARG, "offsets are those of 1 to 512 experts; without them there is one matrix");
-  if (reinterpret_cast<uintptr_t>(offsets) % 4) return pfail(TAO_ERR_ARG, "operands start on a whole element");
-  return TAO_OK;
-}
-
-// Operands of the tensor maps: on 16 bytes, rows (and matrices) too, and rows that do not overlap.
-bool laid(const Operand2& o) {
-  return !o.at || (on16(o.at, 0) && (o.rows <= 1 || (o.stride % 8 == 0 && o.stride >= o.inner && o.stride < (1ll << 38))) &&
-                   (o.count <= 1 || (o.matrix % 8 == 0 && o.matrix > 0 && o.matrix < (1ll << 38))));
-}
 
 // -- the gradient's elementwise part ------------------------------------------
 struct SlopeArgs {
@@ -153,58 +228,75 @@ struct SlopeArgs {
 };
 
 // dz = dy act'(z), or dy u act'(z) and du = dy act(z); sums over a block's rows of dz as it is before rounding.
-// A thread has VEC columns of a slab of 32 VEC and every eighth row.
-template <int VEC>
+// A thread has VEC columns of a slab of 32 VEC and every eighth row, some rows' loads on their way at once: it is
+// bound by its bytes.
+template <int VEC, int ACT, bool SLOPED, bool GATED, bool BF16>
 __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool is_bf16 = a.type == TAO_TYPE_BF16;
   const int col = (blockIdx.x * 32 + lane) * VEC;
   const long long begin = (long long)blockIdx.y * a.per, end = min(begin + a.per, a.rows);
-  float sum[VEC] = {};
-  if (col < a.n) {
-#pragma unroll 2
-    for (long long r = begin + warp; r < end; r += 8) {
-      float dy[VEC], z[VEC], u[VEC];
-      auto load = [&](const void* p, long long stride, float (&v)[VEC]) {
-        const uint16_t* at = static_cast<const uint16_t*>(p) + r * stride + col;
-        if constexpr (VEC == 8) {
-          const uint4 w = *reinterpret_cast<const uint4*>(at);
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+  using Word = std::conditional_t<VEC == 8, uint4, uint16_t>;
+  auto widen = [](const Word& w, float (&v)[VEC]) {
+    if constexpr (VEC == 8) {
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack(words[i], is_bf16);
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-          }
-        } else {
-          v[0] = unpack1(*at, is_bf16);
-        }
-      };
-      auto store = [&](void* p, const float (&v)[VEC]) {
-        uint16_t* at = static_cast<uint16_t*>(p) + r * a.d_stride + col;
-        if constexpr (VEC == 8)
-          *reinterpret_cast<uint4*>(at) = make_uint4(pack(v[0], v[1], is_bf16), pack(v[2], v[3], is_bf16),
-                                                     pack(v[4], v[5], is_bf16), pack(v[6], v[7], is_bf16));
-        else
-          *at = pack1(v[0], is_bf16);
-      };
-      load(a.dy, a.dy_stride, dy);
-      if (a.z) load(a.z, a.z_stride, z);
-      if (a.u) load(a.u, a.z_stride, u);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (a.z) {
-          const float2 f = activate_slope(z[i], a.act);
-          if (a.u) {
-            z[i] = dy[i] * f.x;  // du
-            dy[i] *= u[i] * f.y;
-          } else {
-            dy[i] *= f.y;
-          }
-        }
-        sum[i] += dy[i];
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack(words[i], BF16);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
       }
-      if (a.dz) store(a.dz, dy);
-      if (a.u) store(a.du, z);
+    } else {
+      v[0] = unpack1(w, BF16);
+    }
+  };
+  auto store = [&](void* p, long long r, const float (&v)[VEC]) {
+    uint16_t* at = static_cast<uint16_t*>(p) + r * a.d_stride + col;
+    if constexpr (VEC == 8)
+      *reinterpret_cast<uint4*>(at) =
+          make_uint4(pack(v[0], v[1], BF16), pack(v[2], v[3], BF16), pack(v[4], v[5], BF16), pack(v[6], v[7], BF16));
+    else
+      *at = pack1(v[0], BF16);
+  };
+  auto load = [&](const void* p, long long r, long long stride) {
+    return *reinterpret_cast<const Word*>(static_cast<const uint16_t*>(p) + r * stride + col);
+  };
+  float sum[VEC] = {};
+  constexpr int AHEAD = GATED ? 2 : 4;
+  if (col < a.n) {
+    for (long long r0 = begin + warp; r0 < end; r0 += 8 * AHEAD) {
+      Word wy[AHEAD], wz[AHEAD], wu[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const long long r = r0 + 8 * j;
+        if (r >= end) break;
+        wy[j] = load(a.dy, r, a.dy_stride);
+        if constexpr (SLOPED) wz[j] = load(a.z, r, a.z_stride);
+        if constexpr (GATED) wu[j] = load(a.u, r, a.z_stride);
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const long long r = r0 + 8 * j;
+        if (r >= end) break;
+        float dy[VEC], z[VEC], u[VEC];
+        widen(wy[j], dy);
+        if constexpr (SLOPED) {
+          widen(wz[j], z);
+          if constexpr (GATED) widen(wu[j], u);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float2 f = activate_slope(z[i], ACT);
+            if constexpr (GATED) {
+              z[i] = dy[i] * f.x;  // du
+              dy[i] *= u[i] * f.y;
+            } else {
+              dy[i] *= f.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] += dy[i];
+        if (a.dz) store(a.dz, r, dy);
+        if constexpr (GATED) store(a.du, r, z);
+      }
     }
   }
   if (!a.sums) return;
@@ -219,6 +311,33 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
     const int c = (blockIdx.x * 32 + (i & 31)) * VEC + i / 32;
     if (c < a.n) a.sums[(long long)blockIdx.y * a.n + c] = s;
   }
+}
+
+template <int VEC, int ACT, bool SLOPED, bool GATED>
+void start_slope(const SlopeArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.type == TAO_TYPE_BF16)
+    slope_kernel<VEC, ACT, SLOPED, GATED, true><<<grid, 256, 0, s>>>(a);
+  else
+    slope_kernel<VEC, ACT, SLOPED, GATED, false><<<grid, 256, 0, s>>>(a);
+}
+template <int VEC, int ACT>
+void start_slope(const SlopeArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.u)
+    start_slope<VEC, ACT, true, true>(a, grid, s);
+  else if (ACT != TAO_ACT_NONE)  // without one dz is dy
+    start_slope<VEC, ACT, true, false>(a, grid, s);
+  else
+    start_slope<VEC, ACT, false, false>(a, grid, s);
+}
+template <int VEC>
+void start_slope(const SlopeArgs& a, dim3 grid, cudaStream_t s) {
+  switch (a.act) {
+    case TAO_ACT_RELU: return start_slope<VEC, TAO_ACT_RELU>(a, grid, s);
+    case TAO_ACT_SILU: return start_slope<VEC, TAO_ACT_SILU>(a, grid, s);
+    case TAO_ACT_GELU: return start_slope<VEC, TAO_ACT_GELU>(a, grid, s);
+    case TAO_ACT_GELU_TANH: return start_slope<VEC, TAO_ACT_GELU_TANH>(a, grid, s);
+  }
+  start_slope<VEC, TAO_ACT_NONE>(a, grid, s);
 }
 
 // Adds the blocks' sums in their order: eight runs of them side by side, then those.
@@ -253,151 +372,261 @@ int slope_blocks(long long rows, int n) {
 }  // namespace product
 }  // namespace tao
 
-extern "C" {
+namespace tao {
+namespace product {
+namespace {
 
-int tao_linear(const void* x, long long x_stride, const void* w, long long w_stride, long long w_expert, const void* up,
-               long long up_stride, long long up_expert, const void* bias, const void* residual, long long r_stride,
-               const int* offsets, int experts, long long rows, int n, int k, int type, int activation, void* y, void* z,
-               void* u, long long z_stride, void* stream) {
-  using namespace tao;
-  using namespace tao::product;
-  if (int rc = check_sizes(rows, n, k, type, activation, offsets, experts)) return rc;
-  if (rows == 0) return TAO_OK;
-  if (!x || !w || !y || (up && z && !u)) return pfail(TAO_ERR_ARG, "null pointer");
-  if (offsets ? bias || residual : up != nullptr)
+// A matrix or matrices as a caller has them.
+struct Given {
+  const void* at;
+  long long rows, cols, count, row, col, matrix;  // strides in elements
+};
+
+// Whether TMA can fetch it as it lies: neighbours next to each other, everything else on 16 bytes, no overlaps.
+bool fetchable(const Given& g) {
+  return reinterpret_cast<uintptr_t>(g.at) % 16 == 0 && (g.cols == 1 || g.col == 1) &&
+         (g.rows == 1 || (g.row % 8 == 0 && g.row >= g.cols && g.row < (1ll << 38))) &&
+         (g.count == 1 || (g.matrix % 8 == 0 && g.matrix >= (g.rows - 1) * g.row + g.cols && g.matrix < (1ll << 38)));
+}
+
+// 16-bit values to rows of `stride` from whatever strides they have.
+__global__ void __launch_bounds__(256) lay_kernel(const Given g, uint16_t* out, long long stride) {
+  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= g.rows * g.count) return;
+  const long long matrix = row / g.rows;
+  const uint16_t* in = static_cast<const uint16_t*>(g.at) + matrix * g.matrix + (row - matrix * g.rows) * g.row;
+  for (long long c = threadIdx.x; c < g.cols; c += blockDim.x) out[row * stride + c] = in[c * g.col];
+}
+
+// Rooms of a workspace, one behind the other; without a base only their size is counted.
+struct Rooms {
+  uint8_t* base;
+  size_t used;
+  void* take(size_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+long long padded(long long cols) { return (cols + 7) / 8 * 8; }
+
+// An operand that TMA can fetch: as given, or laid in the workspace (of a Rooms without a base nothing is launched).
+Operand2 operand(const Given& g, Rooms& rooms, cudaStream_t s) {
+  if (!g.at) return {};
+  if (fetchable(g)) return {g.at, g.cols, g.rows, g.row, g.count, g.matrix};
+  const long long stride = padded(g.cols);
+  void* to = rooms.take((size_t)(g.rows * g.count * stride * 2));
+  if (rooms.base) {
+    const dim3 block(g.cols <= 64 ? 32 : 256, g.cols <= 64 ? 8 : 1);
+    lay_kernel<<<(unsigned)((g.rows * g.count + block.y - 1) / block.y), block, 0, s>>>(g, static_cast<uint16_t*>(to), stride);
+  }
+  return {to, g.cols, g.rows, stride, g.count, g.rows * stride};
+}
+
+Given given_x(const TaoLinear& p) { return {p.x, p.rows, p.k, 1, p.x_row, p.x_col, 0}; }
+Given given_w(const TaoLinear& p) { return {p.w, p.n, p.k, p.experts, p.w_row, p.w_col, p.w_expert}; }
+Given given_up(const TaoLinear& p) { return {p.up, p.n, p.k, p.experts, p.up_row, p.up_col, p.up_expert}; }
+
+int check(const TaoLinear* p) {
+  if (!p) return pfail(TAO_ERR_ARG, "null pointer");
+  if (p->type != TAO_TYPE_BF16 && p->type != TAO_TYPE_FP16) return pfail(TAO_ERR_ARG, "16-bit products take bf16 or fp16");
+  if (p->activation < TAO_ACT_NONE || p->activation > TAO_ACT_GELU_TANH) return pfail(TAO_ERR_ARG, "unknown activation");
+  if (p->rows < 0 || p->n <= 0 || p->k <= 0)
+    return pfail(TAO_ERR_ARG, "rows must not be negative, n and k must be positive");
+  if (p->rows > (1ll << 30) || p->n > (1 << 24) || p->k > (1 << 24))
+    return pfail(TAO_ERR_ARG, "rows are limited to 2^30, n and k to 2^24");
+  if (p->offsets ? p->experts < 1 || p->experts > kMostGroups : p->experts != 1)
+    return pfail(TAO_ERR_ARG, "offsets are those of 1 to 512 experts; without them there is one matrix");
+  if (p->offsets ? p->bias || p->residual : p->up != nullptr)
     return pfail(TAO_ERR_ARG, "experts have no bias or residual, and a gate needs experts");
-  if (!on_elements({{bias, 2}, {residual, 2}, {y, 2}, {z, 2}, {u, 2}}))
+  if (!on_elements({{p->x, 2}, {p->w, 2}, {p->up, 2}, {p->bias, 2}, {p->residual, 2}, {p->y, 2}, {p->z, 2}, {p->u, 2},
+                    {p->offsets, 4}, {p->dy, 2}, {p->dx, 2}, {p->dw, 2}, {p->dup, 2}, {p->db, 2}}))
     return pfail(TAO_ERR_ARG, "operands start on a whole element");
-  const Operand2 ox = {x, k, rows, x_stride, 1, 0}, ow = {w, k, n, w_stride, experts, w_expert},
-                 ou = {up, k, n, up_stride, experts, up_expert}, none = {};
-  if (!laid(ox) || !laid(ow) || !laid(ou))
-    return pfail(TAO_ERR_ARG, "operands of a 16-bit product and their rows start on 16 bytes");
+  return TAO_OK;
+}
+
+int check_room(const TaoLinear& p, size_t need) {
+  if (need && (!p.workspace || reinterpret_cast<uintptr_t>(p.workspace) % 256 || p.workspace_bytes < need))
+    return pfail(TAO_ERR_ARG, "the products' workspace is too small, or off 256 bytes");
+  return TAO_OK;
+}
+
+int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
+  const Operand2 ox = operand(given_x(p), rooms, s), ow = operand(given_w(p), rooms, s), ou = operand(given_up(p), rooms, s),
+                 none = {};
+  if (!rooms.base) return TAO_OK;
+  const int n = p.n, k = p.k;
+  const long long rows = p.rows;
   Args a = {};
-  a.offsets = offsets, a.groups = experts, a.rows = (int)rows, a.cols = n, a.depth = k, a.pairs = 1;
-  a.type = type, a.act = activation, a.bias = bias, a.residual = residual, a.r_stride = r_stride;
-  a.y = y, a.z = z, a.u = z ? u : nullptr, a.z_stride = z_stride;
-  a.wide = n % 8 == 0 && on16(y, 0) && on16(z, z_stride) && on16(u, 0) && on16(residual, r_stride);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int blocks = (k + kTerms - 1) / kTerms;
-  if (offsets) {
-    const long long mean = rows / experts;
+  a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)rows, a.cols = n, a.depth = k, a.pairs = 1;
+  a.type = p.type, a.act = p.activation, a.bias = p.bias, a.residual = p.residual, a.r_stride = p.r_row;
+  a.y = p.y, a.z = p.z, a.u = p.z ? p.u : nullptr, a.z_stride = p.z_row;
+  a.wide = n % 8 == 0 && on16(p.y, 0) && on16(p.z, p.z_row) && on16(p.u, 0) && on16(p.residual, p.r_row);
+  const int steps = (k + kTerms - 1) / kTerms;
+  if (p.offsets) {
+    const long long mean = rows / p.experts;
     const Operands few = {ow, ox, ou, none}, many = {ox, ow, none, ou};
-    if (up) {
+    if (p.up) {
       if (mean <= 32) return start<FEW, 32, true, false>(few, a, 1, s);
       return start<FORWARD, 256, true, false>(many, a, 1, s);
     }
     if (mean <= 32) return start<FEW, 32, false, false>(few, a, 1, s);
-    return start<FORWARD, 256, false, false>(many, a, 1, s);
+    return start_rows<FORWARD>(many, a, (rows + 127) / 128 + p.experts / 2, steps, s);
+  }
+  if (rows <= 32) {
+    const FewArgs f = {ox.at, ow.at, p.bias, p.residual, rows > 1 ? ox.stride : 0, n > 1 ? ow.stride : 0, p.r_row,
+                       (int)rows, n, k, p.activation, p.y, p.z, p.z_row};
+    int rc;
+    if (few_rows(f, p.type, s, &rc)) return rc;
   }
   if (rows <= 64) {
     const Operands o = {ow, ox, none, none};
-    const int split = split_of((n + 127) / 128, blocks);
-    if (rows <= 16) return start<FEW, 16, false, true>(o, a, split, s);
-    if (rows <= 32) return start<FEW, 32, false, true>(o, a, split, s);
-    return start<FEW, 64, false, true>(o, a, split, s);
+    const int split = split_of<FEW, 64>((n + 127) / 128, steps, 9).blocks;
+    if (split == 1)
+      return rows <= 32 ? start<FEW, 32, false, false>(o, a, 1, s) : start<FEW, 64, false, false>(o, a, 1, s);
+    return rows <= 32 ? start<FEW, 32, false, true>(o, a, split, s) : start<FEW, 64, false, true>(o, a, split, s);
   }
   const Operands o = {ox, ow, none, none};
   const long long row_tiles = (rows + 127) / 128;
-  if (row_tiles * ((n + 255) / 256) >= 120) return start<FORWARD, 256, false, false>(o, a, 1, s);
-  if (row_tiles * ((n + 127) / 128) >= 100) return start<FORWARD, 128, false, false>(o, a, 1, s);
-  return start<FORWARD, 64, false, true>(o, a, split_of(row_tiles * ((n + 63) / 64), blocks), s);
+  return start_rows<FORWARD>(o, a, row_tiles, steps, s);
 }
 
-int tao_linear_input_gradient(const void* dz, const void* du, long long d_stride, const void* w, long long w_stride,
-                              long long w_expert, const void* up, long long up_stride, long long up_expert,
-                              const int* offsets, int experts, long long rows, int n, int k, int type, void* dx,
-                              void* stream) {
-  using namespace tao;
-  using namespace tao::product;
-  if (int rc = check_sizes(rows, n, k, type, TAO_ACT_NONE, offsets, experts)) return rc;
-  if (rows == 0) return TAO_OK;
-  if (!dz || !w || !dx || !du != !up) return pfail(TAO_ERR_ARG, "null pointer");
-  if (!on_elements({{dx, 2}})) return pfail(TAO_ERR_ARG, "operands start on a whole element");
-  const Operand2 oz = {dz, n, rows, d_stride, 1, 0}, od = {du, n, rows, d_stride, 1, 0},
-                 ow = {w, k, n, w_stride, experts, w_expert}, ou = {up, k, n, up_stride, experts, up_expert};
-  if (!laid(oz) || !laid(od) || !laid(ow) || !laid(ou))
-    return pfail(TAO_ERR_ARG, "operands of a 16-bit product and their rows start on 16 bytes");
+int input_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_t s) {
+  const int n = p.n, k = p.k;
   Args a = {};
-  a.offsets = offsets, a.groups = experts, a.rows = (int)rows, a.cols = k, a.depth = n, a.pairs = du ? 2 : 1;
-  a.type = type, a.y = dx;
-  a.wide = k % 8 == 0 && on16(dx, 0);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Operands o = {oz, ow, od, ou};
-  const int blocks = (n + kTerms - 1) / kTerms * a.pairs;
-  const long long row_tiles = (rows + 127) / 128 + (offsets ? experts / 2 : 0);
-  if (row_tiles * ((k + 255) / 256) >= 120) return start<INPUT, 256, false, false>(o, a, 1, s);
-  if (offsets || row_tiles * ((k + 127) / 128) >= 100) return start<INPUT, 128, false, false>(o, a, 1, s);
-  return start<INPUT, 64, false, true>(o, a, split_of(row_tiles * ((k + 63) / 64), blocks), s);
+  a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)p.rows, a.cols = k, a.depth = n, a.pairs = pairs;
+  a.type = p.type, a.y = p.dx;
+  a.wide = k % 8 == 0 && on16(p.dx, 0);
+  const int steps = (n + kTerms - 1) / kTerms * pairs;
+  const long long row_tiles = (p.rows + 127) / 128 + (p.offsets ? p.experts / 2 : 0);
+  return start_rows<INPUT>({o.a, o.b, o.a2, o.b2}, a, row_tiles, steps, s);
 }
 
-int tao_linear_weight_gradient(const void* dz, const void* du, long long d_stride, const void* x, long long x_stride,
-                               const int* offsets, int experts, long long rows, int n, int k, int type, void* dw,
-                               void* dup, void* stream) {
-  using namespace tao;
-  using namespace tao::product;
-  if (int rc = check_sizes(rows, n, k, type, TAO_ACT_NONE, offsets, experts)) return rc;
-  if (!dw || !du != !dup) return pfail(TAO_ERR_ARG, "null pointer");
-  if (!on_elements({{dw, 2}, {dup, 2}})) return pfail(TAO_ERR_ARG, "operands start on a whole element");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (rows == 0) {
-    const size_t size = (size_t)experts * n * k * 2;
-    cudaError_t e = cudaMemsetAsync(dw, 0, size, s);
-    if (e == cudaSuccess && dup) e = cudaMemsetAsync(dup, 0, size, s);
-    return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
-  }
-  if (!dz || !x) return pfail(TAO_ERR_ARG, "null pointer");
-  const Operand2 oz = {dz, n, rows, d_stride, 1, 0}, od = {du, n, rows, d_stride, 1, 0},
-                 ox = {x, k, rows, x_stride, 1, 0}, none = {};
-  if (!laid(oz) || !laid(od) || !laid(ox))
-    return pfail(TAO_ERR_ARG, "operands of a 16-bit product and their rows start on 16 bytes");
+int weight_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_t s) {
+  const int n = p.n, k = p.k;
   Args a = {};
-  a.offsets = offsets, a.groups = experts, a.rows = (int)rows, a.cols = k, a.depth = n, a.pairs = du ? 2 : 1;
-  a.type = type, a.y = dw, a.u = dup;
-  a.wide = k % 8 == 0 && on16(dw, 0) && on16(dup, 0);
-  const Operands o = {oz, ox, od, none};
-  const long long down = (long long)(n + 127) / 128 * experts * a.pairs;
-  if (down * ((k + 255) / 256) >= 120) return start<WEIGHT, 256, false, false>(o, a, 1, s);
-  const int blocks = (int)std::min<long long>((rows + kTerms - 1) / kTerms, 1 << 20);
-  if (offsets) return start<WEIGHT, 128, false, false>(o, a, 1, s);
-  const long long tiles = down * ((k + 127) / 128);
-  if (tiles >= 100) return start<WEIGHT, 128, false, false>(o, a, 1, s);
-  return start<WEIGHT, 128, false, true>(o, a, split_of(tiles, blocks), s);
-}
-
-size_t tao_linear_slope_workspace_bytes(long long rows, int n) {
-  if (rows <= 0 || n <= 0) return 0;
-  return (size_t)tao::product::slope_blocks(rows, n) * n * sizeof(float);
-}
-
-int tao_linear_slope(const void* dy, long long dy_stride, const void* z, const void* u, long long z_stride,
-                     long long rows, int n, int type, int activation, void* dz, void* du, long long d_stride, void* db,
-                     void* workspace, size_t workspace_bytes, void* stream) {
-  using namespace tao;
-  using namespace tao::product;
-  if (int rc = check_sizes(rows, n, 1, type, activation, nullptr, 1)) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (rows == 0) {
-    if (db && cudaMemsetAsync(db, 0, (size_t)n * 2, s) != cudaSuccess)
-      return pfail(TAO_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
-    return TAO_OK;
+  a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)p.rows, a.cols = k, a.depth = n, a.pairs = pairs;
+  a.type = p.type, a.y = p.dw, a.u = p.dup;
+  a.wide = k % 8 == 0 && on16(p.dw, 0) && on16(p.dup, 0);
+  if (p.offsets) {
+    if (k > 128) return start<WEIGHT, 256, false, false>(o, a, 1, s);
+    return start<WEIGHT, 128, false, false>(o, a, 1, s);
   }
-  if (!dy || (u && (!z || !du)) || (z && !dz) || (!dz && !db)) return pfail(TAO_ERR_ARG, "null pointer");
-  if (!on_elements({{dy, 2}, {z, 2}, {u, 2}, {dz, 2}, {du, 2}, {db, 2}, {workspace, 4}}))
-    return pfail(TAO_ERR_ARG, "operands start on a whole element");
-  if (db && (!workspace || workspace_bytes < tao_linear_slope_workspace_bytes(rows, n)))
-    return pfail(TAO_ERR_ARG, "workspace too small for the bias's gradient");
-  SlopeArgs a = {dy, z, u, dy_stride, z_stride, d_stride, dz, du, db ? static_cast<float*>(workspace) : nullptr,
-                 rows, n, type, activation, slope_rows(rows, n)};
-  const bool wide = n % 8 == 0 && on16(dy, dy_stride) && on16(z, z_stride) && on16(u, 0) && on16(dz, d_stride) && on16(du, 0);
-  const int blocks = slope_blocks(rows, n), slab = wide ? 256 : 32;
-  const dim3 grid((n + slab - 1) / slab, blocks);
-  if (wide)
-    slope_kernel<8><<<grid, 256, 0, s>>>(a);
-  else
-    slope_kernel<1><<<grid, 256, 0, s>>>(a);
-  if (db) column_sum_kernel<<<(n + 31) / 32, 256, 0, s>>>(a.sums, blocks, n, type, db);
+  const long long down = (n + 127) / 128;
+  const int steps = (int)((p.rows + kTerms - 1) / kTerms);
+  if (k > 128) {
+    const int split = split_of<WEIGHT, 256>(down * ((k + 255) / 256), steps, 26).blocks;
+    if (split > 1) return start<WEIGHT, 256, false, true>(o, a, split, s);
+    return start<WEIGHT, 256, false, false>(o, a, 1, s);
+  }
+  const int split = split_of<WEIGHT, 128>(down, steps, 20).blocks;
+  if (split > 1) return start<WEIGHT, 128, false, true>(o, a, split, s);
+  return start<WEIGHT, 128, false, false>(o, a, 1, s);
+}
+
+int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
+  const bool sloped = p.activation != TAO_ACT_NONE || p.up, products = p.dx || p.dw;
+  const int pairs = p.up ? 2 : 1;
+  // dz and du, or dy itself
+  Given gz = {p.dy, p.rows, p.n, 1, p.dy_row, 1, 0}, gd = {};
+  if (sloped || p.db) {
+    SlopeArgs a = {p.dy, sloped ? p.z : nullptr, p.up ? p.u : nullptr, p.dy_row, p.z_row, padded(p.n), nullptr, nullptr,
+                   nullptr, p.rows, p.n, p.type, p.activation, slope_rows(p.rows, p.n)};
+    if (sloped && products) {
+      const size_t size = (size_t)(p.rows * a.d_stride * 2);
+      a.dz = rooms.take(size);
+      gz = {a.dz, p.rows, p.n, 1, a.d_stride, 1, 0};
+      if (p.up) {
+        a.du = rooms.take(size);
+        gd = {a.du, p.rows, p.n, 1, a.d_stride, 1, 0};
+      }
+    }
+    const int blocks = slope_blocks(p.rows, p.n);
+    if (p.db) a.sums = static_cast<float*>(rooms.take((size_t)blocks * p.n * sizeof(float)));
+    if (rooms.base) {
+      const bool wide = p.n % 8 == 0 && on16(p.dy, p.dy_row) && (!sloped || (on16(p.z, p.z_row) && on16(p.u, 0)));
+      const dim3 grid((p.n + (wide ? 255 : 31)) / (wide ? 256 : 32), blocks);
+      if (wide)
+        start_slope<8>(a, grid, s);
+      else
+        start_slope<1>(a, grid, s);
+      if (p.db) column_sum_kernel<<<(p.n + 31) / 32, 256, 0, s>>>(a.sums, blocks, p.n, p.type, p.db);
+    }
+  }
+  if (products) {
+    if (sloped && !rooms.base) gz.at = gd.at = nullptr;  // their rooms are counted, and they are laid as they are made
+    const Operand2 oz = sloped ? Operand2{gz.at, gz.cols, gz.rows, gz.row, 1, 0} : operand(gz, rooms, s),
+                   od = p.up ? Operand2{gd.at, gd.cols, gd.rows, gd.row, 1, 0} : Operand2{};
+    if (p.dx) {
+      const Operand2 ow = operand(given_w(p), rooms, s), ou = operand(given_up(p), rooms, s);
+      if (rooms.base)
+        if (int rc = input_gradient(p, {oz, ow, od, ou}, pairs, s)) return rc;
+    }
+    if (p.dw) {
+      const Operand2 ox = operand(given_x(p), rooms, s);
+      if (rooms.base)
+        if (int rc = weight_gradient(p, {oz, ox, od, {}}, pairs, s)) return rc;
+    }
+  }
+  if (!rooms.base) return TAO_OK;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int missing(const TaoLinear& p, bool gradient) {
+  if (!gradient) return !p.x || !p.w || !p.y || (p.up && p.z && !p.u);
+  const bool sloped = p.activation != TAO_ACT_NONE || p.up;
+  return !p.dy || (p.up ? !p.dw != !p.dup : p.dup != nullptr) || (p.dx && (!p.w)) || (p.dw && !p.x) ||
+         (sloped && (!p.z || (p.up && !p.u)));
+}
+
+}  // namespace
+}  // namespace product
+}  // namespace tao
+
+extern "C" {
+
+size_t tao_linear_sizeof(void) { return sizeof(TaoLinear); }
+
+size_t tao_linear_workspace_bytes(const TaoLinear* p, int gradient) {
+  using namespace tao::product;
+  if (check(p) || p->rows == 0) return 0;
+  Rooms rooms = {nullptr, 0};
+  if (gradient)
+    backward(*p, rooms, nullptr);
+  else
+    forward(*p, rooms, nullptr);
+  return rooms.used;
+}
+
+int tao_linear(const TaoLinear* p, void* stream) {
+  using namespace tao::product;
+  if (int rc = check(p)) return rc;
+  if (p->rows == 0) return TAO_OK;
+  if (missing(*p, false)) return pfail(TAO_ERR_ARG, "null pointer");
+  if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 0))) return rc;
+  static uint8_t none[1];  // where no room is needed
+  Rooms rooms = {p->workspace ? static_cast<uint8_t*>(p->workspace) : none, 0};
+  return forward(*p, rooms, static_cast<cudaStream_t>(stream));
+}
+
+int tao_linear_gradient(const TaoLinear* p, void* stream) {
+  using namespace tao::product;
+  if (int rc = check(p)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->rows == 0) {
+    const size_t size = (size_t)p->experts * p->n * p->k * 2;
+    cudaError_t e = cudaSuccess;
+    if (p->dw) e = cudaMemsetAsync(p->dw, 0, size, s);
+    if (e == cudaSuccess && p->dup) e = cudaMemsetAsync(p->dup, 0, size, s);
+    if (e == cudaSuccess && p->db) e = cudaMemsetAsync(p->db, 0, (size_t)p->n * 2, s);
+    return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
+  }
+  if (missing(*p, true)) return pfail(TAO_ERR_ARG, "null pointer");
+  if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 1))) return rc;
+  static uint8_t none[1];
+  Rooms rooms = {p->workspace ? static_cast<uint8_t*>(p->workspace) : none, 0};
+  return backward(*p, rooms, s);
 }
 
 int tao_product_check(int* flags, void* stream) {

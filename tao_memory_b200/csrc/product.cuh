@@ -66,15 +66,26 @@ struct Cfg {
   static constexpr int A = (FORM == FEW && GATED ? 2 : 1) * 128 * 128, B = BN * 128, STAGE = A + B;
   static constexpr int STAGING = FORM == FEW || SPLIT ? 0 : kWorkers * 2048;
   static constexpr int LISTS = SPLIT ? 0 : (2 * kMostGroups + 4) * 4;
-  static constexpr int REST = STAGING + LISTS + 512;
+  // parts of a split tile: of few rows in a place of their own, else over the ring
+  static constexpr int PARTS = !SPLIT ? 0 : FORM == FEW ? (BN + 7) * 128 * 4 : 128 * (BN + 4) * 4;
+  static constexpr int REST = STAGING + LISTS + 512 + (FORM == FEW ? PARTS : 0);
   static constexpr int FIT = (227 * 1024 - REST) / STAGE, STAGES = FIT < 12 ? FIT : 12;
-  static constexpr int SUMS = SPLIT ? (FORM == FEW ? BN * 132 : 128 * (BN + 4)) * 4 : 0;
   static constexpr int SMEM = STAGES * STAGE + REST;
   static constexpr int ACC = FORM == FEW && GATED ? 2 * BN : BN;
   static constexpr int SETS = SPLIT ? 1 : 2, USED = SETS * ACC;
   static constexpr int TMEM = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
-  static_assert(USED <= 512 && STAGES >= 3 && SUMS <= STAGES * STAGE && SMEM <= 227 * 1024, "");
+  static_assert(USED <= 512 && STAGES >= 3 && (FORM == FEW || PARTS <= STAGES * STAGE) && SMEM <= 227 * 1024, "");
 };
+
+// Whether a phase is over, without waiting (try_wait may suspend the thread for a while).
+TAO_DEVI bool arrived(uint64_t* bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(phase)
+               : "memory");
+  return ok != 0;
+}
 
 // Waits at most about four seconds; a wait that runs out, or another's of this block, ends all of them.
 TAO_DEVI bool wait_for(uint64_t* bar, uint32_t phase, volatile int* abort) {
@@ -102,6 +113,36 @@ TAO_DEVI void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uin
           smem_u32(dst)),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+
+// The cluster's barrier in two steps, by whole warps.
+TAO_DEVI void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+TAO_DEVI void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Where a block of the cluster has what is at `at` in this one.
+TAO_DEVI uint32_t peer(uint32_t at, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+TAO_DEVI void put_peer(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// One lane of a warp that has met, the same for all that ask.
+TAO_DEVI bool elected() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+// 128 rows of A times B^T, 16 terms, onto (or, more = 0, into) the accumulator.
+TAO_DEVI void multiply(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(acc),
+      "l"(a), "l"(b), "r"(idesc), "r"(more));
 }
 
 // N consecutive fp32 columns of this thread's TMEM lane.
@@ -149,12 +190,31 @@ TAO_DEVI float load1(const void* p, long long i, bool is_bf16) {
 TAO_DEVI float sigmoid(float q) { return __fdividef(1.f, 1.f + __expf(-q)); }
 constexpr float kGeluRoot = 0.7978845608028654f, kGeluCube = 0.044715f;  // sqrt(2 / pi)
 
-// gelu by the error function of the other side, whose small values keep their relative precision.
+// The normal distribution's integral from the tail of z's side: with t = 1 / (1 + 0.35 x), x = |z| / sqrt(2),
+// erfc(x) e^(x^2) / t is smooth on (0, 1], and half of it a polynomial in t (fitted here at Chebyshev nodes to 2^-20).
+// So small values keep their relative precision, at two special-function instructions.  `density` is e^(-z^2 / 2).
+TAO_DEVI float normal_integral(float z, float& density) {
+  const float t = __fdividef(1.f, 1.f + 0.35f * 0.7071067811865476f * fabsf(z));
+  density = __expf(-0.5f * z * z);
+  float q = fmaf(-0.042552598f, t, 0.100604653f);
+  q = fmaf(q, t, -0.0072748783f);
+  q = fmaf(q, t, 0.0814718946f);
+  q = fmaf(q, t, 0.0773361512f);
+  q = fmaf(q, t, 0.0929546698f);
+  q = fmaf(q, t, 0.098726552f);
+  q = fmaf(q, t, 0.0987331438f);
+  const float tail = density * t * q;
+  return z < 0.f ? tail : 1.f - tail;
+}
+
 TAO_DEVI float activate(float z, int act) {
   switch (act) {
     case TAO_ACT_RELU: return z > 0.f || z != z ? z : 0.f;
     case TAO_ACT_SILU: return z * sigmoid(z);
-    case TAO_ACT_GELU: return 0.5f * z * erfcf(-0.7071067811865476f * z);
+    case TAO_ACT_GELU: {
+      float density;
+      return z * normal_integral(z, density);
+    }
     case TAO_ACT_GELU_TANH: return z * sigmoid(2.f * kGeluRoot * (z + kGeluCube * z * z * z));
   }
   return z;
@@ -168,8 +228,9 @@ TAO_DEVI float2 activate_slope(float z, int act) {
       return make_float2(z * s, s * (1.f + z * (1.f - s)));
     }
     case TAO_ACT_GELU: {
-      const float p = 0.5f * erfcf(-0.7071067811865476f * z);
-      return make_float2(z * p, p + z * 0.3989422804014327f * __expf(-0.5f * z * z));
+      float density;
+      const float p = normal_integral(z, density);
+      return make_float2(z * p, p + z * 0.3989422804014327f * density);
     }
     case TAO_ACT_GELU_TANH: {
       const float s = sigmoid(2.f * kGeluRoot * (z + kGeluCube * z * z * z));
@@ -341,7 +402,7 @@ TAO_DEVI float finish(const Args& a, float v, long long row, int col, bool is_bf
 }
 
 // Maps: FORWARD: x, W, -, U.  FEW: W, x, U, -.  INPUT: dz, W, du, U.  WEIGHT: dz, x, du, -.
-template <int FORM, int BN, bool GATED, bool SPLIT>
+template <int FORM, int BN, bool GATED, bool SPLIT, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_a2, const __grid_constant__ CUtensorMap map_b2,
@@ -365,24 +426,75 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) atomicOr(&g_error, kErrState);
     return;
   }
-  const bool is_bf16 = a.type == TAO_TYPE_BF16;
+  constexpr bool is_bf16 = BF16;
+  const int rank = SPLIT ? (int)cluster_rank() : 0;
+  const int start = SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
+  // this block's part of a tile's steps
+  auto part = [&](const Tile& t, int& k0) {
+    if constexpr (!SPLIT) return k0 = 0, t.blocks;
+    k0 = (int)((long long)t.blocks * rank / a.split);
+    return (int)((long long)t.blocks * (rank + 1) / a.split) - k0;
+  };
+  // 64 terms of a tile into slot s, by one thread
+  auto fetch = [&](const Tile& tile, int kb, int s) {
+    uint8_t* const sa = sm + s * C::STAGE;
+    uint8_t* const sb = sa + C::A;
+    mbar_expect_tx(&full[s], C::STAGE);
+    if constexpr (FORM == FORWARD) {
+      const int k = kb * kTerms;
+      tma_3d(sa, &map_a, k, tile.row0, 0, &full[s]);
+      tma_3d(sb, &map_b, k, tile.col0, tile.group, &full[s]);
+      if constexpr (GATED) tma_3d(sb + C::B / 2, &map_b2, k, tile.col0, tile.group, &full[s]);
+    } else if constexpr (FORM == FEW) {
+      const int k = kb * kTerms;
+      tma_3d(sa, &map_a, k, tile.col0, tile.group, &full[s]);
+      if constexpr (GATED) tma_3d(sa + C::A / 2, &map_a2, k, tile.col0, tile.group, &full[s]);
+      tma_3d(sb, &map_b, k, tile.row0, 0, &full[s]);
+    } else if constexpr (FORM == INPUT) {
+      const int each = tile.blocks / a.pairs;
+      const bool other = kb >= each;
+      const int k = (kb - (other ? each : 0)) * kTerms;
+      tma_3d(sa, other ? &map_a2 : &map_a, k, tile.row0, 0, &full[s]);
+#pragma unroll
+      for (int j = 0; j < BN / 64; ++j)
+        tma_3d(sb + j * 8192, other ? &map_b2 : &map_b, tile.col0 + j * 64, k, tile.group, &full[s]);
+    } else {
+      const int k = tile.from + kb * kTerms;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        tma_3d(sa + j * 8192, tile.second ? &map_a2 : &map_a, tile.row0 + j * 64, k, 0, &full[s]);
+#pragma unroll
+      for (int j = 0; j < BN / 64; ++j) tma_3d(sb + j * 8192, &map_b, tile.col0 + j * 64, k, 0, &full[s]);
+    }
+  };
+  int early = 0, group = 0;  // steps of the first tile that are fetched while the rest of the block sets itself up
+  if (warp == kWorkers) {
+    if (lane == 0) {
+      for (int i = 0; i < C::STAGES; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&acc_full[i], 1);
+        mbar_init(&acc_empty[i], kWorkers);
+      }
+      mbar_init(over, 1);
+      *abort = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    if (!a.offsets) {
+      const Tile tile = tile_of<FORM, C>(a, first, ends, start, group);  // there is one: no block is launched without
+      int k0;
+      early = min(part(tile, k0), C::STAGES);
+      if (lane == 0)
+        for (int i = 0; i < early; ++i) fetch(tile, k0 + i, i);
+    }
+  }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(C::TMEM));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  if (tid == 32) {
-    for (int i = 0; i < C::STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kWorkers);
-    }
-    mbar_init(over, 1);
-    *abort = 0;
-    fence_mbar_init();
   }
   if constexpr (!SPLIT)
     if (warp == 2 && a.offsets) make_lists<C>(a, first, ends, lane);
@@ -390,77 +502,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tbase = *tmem_slot;
+  if constexpr (SPLIT) cluster_arrive();  // this block has begun: its shared memory can be written to
 
-  const int rank = SPLIT ? (int)cluster_rank() : 0;
-  const int start = SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
   int total;
   if (FORM == WEIGHT)
     total = (a.depth + 127) / 128 * ((a.cols + C::CT - 1) / C::CT) * a.groups * a.pairs;
   else
     total = a.offsets ? first[a.groups + 1] : (a.rows + C::TT - 1) / C::TT * ((a.cols + C::CT - 1) / C::CT);
-  // this block's part of a tile's steps
-  auto part = [&](const Tile& t, int& k0) {
-    if constexpr (!SPLIT) return k0 = 0, t.blocks;
-    k0 = (int)((long long)t.blocks * rank / a.split);
-    return (int)((long long)t.blocks * (rank + 1) / a.split) - k0;
-  };
 
-  int group = 0;
   if (warp == kWorkers) {
     // ---- fetches operands
-    uint32_t fetched = 0;
-    int s = 0, phase = 0;
+    int fetched = 0, s = 0, phase = 0;
     bool ok = true;
     for (int t = start; ok && t < total; t += step) {
       const Tile tile = tile_of<FORM, C>(a, first, ends, t, group);
       int k0;
       const int blocks = part(tile, k0);
       for (int kb = k0; kb < k0 + blocks; ++kb) {
-        if (!(ok = warp_wait_for(&empty[s], phase ^ 1, abort))) break;
-        if (lane == 0) {
-          uint8_t* const sa = sm + s * C::STAGE;
-          uint8_t* const sb = sa + C::A;
-          mbar_expect_tx(&full[s], C::STAGE);
-          if constexpr (FORM == FORWARD) {
-            const int k = kb * kTerms;
-            tma_3d(sa, &map_a, k, tile.row0, 0, &full[s]);
-            tma_3d(sb, &map_b, k, tile.col0, tile.group, &full[s]);
-            if constexpr (GATED) tma_3d(sb + C::B / 2, &map_b2, k, tile.col0, tile.group, &full[s]);
-          } else if constexpr (FORM == FEW) {
-            const int k = kb * kTerms;
-            tma_3d(sa, &map_a, k, tile.col0, tile.group, &full[s]);
-            if constexpr (GATED) tma_3d(sa + C::A / 2, &map_a2, k, tile.col0, tile.group, &full[s]);
-            tma_3d(sb, &map_b, k, tile.row0, 0, &full[s]);
-          } else if constexpr (FORM == INPUT) {
-            const int each = tile.blocks / a.pairs;
-            const bool other = kb >= each;
-            const int k = (kb - (other ? each : 0)) * kTerms;
-            tma_3d(sa, other ? &map_a2 : &map_a, k, tile.row0, 0, &full[s]);
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j)
-              tma_3d(sb + j * 8192, other ? &map_b2 : &map_b, tile.col0 + j * 64, k, tile.group, &full[s]);
-          } else {
-            const int k = tile.from + kb * kTerms;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              tma_3d(sa + j * 8192, tile.second ? &map_a2 : &map_a, tile.row0 + j * 64, k, 0, &full[s]);
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_3d(sb + j * 8192, &map_b, tile.col0 + j * 64, k, 0, &full[s]);
-          }
+        if (fetched >= early) {
+          if (!(ok = warp_wait_for(&empty[s], phase ^ 1, abort))) break;
+          if (lane == 0) fetch(tile, kb, s);
+          __syncwarp();
         }
-        __syncwarp();
         ++fetched;
         if (++s == C::STAGES) s = 0, phase ^= 1;
       }
     }
     if (!ok) {  // copies in flight have their time before the block ends
-      const uint32_t last = fetched < C::STAGES ? 0 : fetched - C::STAGES;
-      for (uint32_t i = last; i < fetched; ++i) mbar_wait(&full[i % C::STAGES], i / C::STAGES & 1, nullptr);
+      fetched = max(fetched, early);
+      for (int i = max(fetched - C::STAGES, 0); i < fetched; ++i) mbar_wait(&full[i % C::STAGES], i / C::STAGES & 1, nullptr);
     }
   } else if (warp == kWorkers + 1) {
     // ---- issues the products
     const uint32_t type_bits = is_bf16 ? 1u << 7 | 1u << 10 : 0u;
     const uint32_t idesc = (idesc_bf16(128, BN, C::A_MN, C::B_MN) & ~(1u << 7 | 1u << 10)) | type_bits;
+    constexpr int STEP_A = (C::A_MN ? 2048 : 32) >> 4, STEP_B = (C::B_MN ? 2048 : 32) >> 4;  // 16 terms on
+    const uint64_t desc_a = sdesc(smem_u32(sm), C::A_MN ? 8192 : 16, 1024);
+    const uint64_t desc_b = sdesc(smem_u32(sm) + C::A, C::B_MN ? 8192 : 16, 1024);
     int s = 0, phase = 0, set = 0, set_phase = 0;
     bool ok = true;
     for (int t = start; ok && t < total; t += step) {
@@ -471,12 +549,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(ok = warp_wait_for(&acc_empty[set], set_phase ^ 1, abort))) break;
       fence_after();
       const uint32_t acc = tbase + set * C::ACC;
+      bool ready = arrived(&full[s], phase);
+#pragma unroll 1
       for (int kb = 0; kb < blocks; ++kb) {
-        if (!(ok = warp_wait_for(&full[s], phase, abort))) break;
+        if (!__all_sync(0xffffffffu, ready) && !(ok = warp_wait_for(&full[s], phase, abort))) break;
         fence_after();
-        const uint32_t sa = smem_u32(sm + s * C::STAGE), sb = sa + C::A;
+        const int next = s + 1 == C::STAGES ? 0 : s + 1, next_phase = s + 1 == C::STAGES ? phase ^ 1 : phase;
+        ready = arrived(&full[next], next_phase);  // its answer is on its way while these products are issued
         int steps = kTerms / 16;
-        if constexpr (FORM == WEIGHT) {
+        if constexpr (FORM == WEIGHT) {  // the last rows may be fewer than 64
           const int left = tile.upto - tile.from - (k0 + kb) * kTerms;
           if (left < kTerms) {
             steps = (left + 15) / 16;
@@ -490,25 +571,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (lane == 0) {
-          for (int k = 0; k < steps; ++k) {
-            const uint64_t db = C::B_MN ? sdesc(sb + k * 2048, 8192, 1024) : sdesc(sb + k * 32, 16, 1024);
-            const uint64_t da = C::A_MN ? sdesc(sa + k * 2048, 8192, 1024) : sdesc(sa + k * 32, 16, 1024);
-            mma(acc, da, db, idesc, kb > 0 || k > 0);
+        // descriptors count 16 bytes and are added up
+        const uint64_t da = desc_a + s * (C::STAGE >> 4), db = desc_b + s * (C::STAGE >> 4);
+        if (elected()) {
+#pragma unroll
+          for (int k = 0; k < kTerms / 16; ++k) {
+            if (FORM == WEIGHT && k >= steps) break;
+            multiply(acc, da + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
             if constexpr (FORM == FEW && GATED)
-              mma(acc + BN, sdesc(sa + C::A / 2 + k * 32, 16, 1024), db, idesc, kb > 0 || k > 0);
+              multiply(acc + BN, da + (C::A / 2 >> 4) + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
           }
           commit(&empty[s]);
         }
         __syncwarp();
-        if (++s == C::STAGES) s = 0, phase ^= 1;
+        s = next, phase = next_phase;
       }
       if (!ok) break;
-      if (lane == 0) commit(&acc_full[set]);
+      if (elected()) commit(&acc_full[set]);
       __syncwarp();
       if (++set == C::SETS) set = 0, set_phase ^= 1;
     }
-    if (lane == 0) {  // nothing is in flight when the block ends
+    if (elected()) {  // nothing is in flight when the block ends
       commit(over);
       mbar_wait(over, 0, nullptr);
     }
@@ -530,59 +613,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after();
       }
       if constexpr (SPLIT) {
-        constexpr int W = BN / 2 < 32 ? BN / 2 : 32;
-        float* const sums = reinterpret_cast<float*>(sm);
-        const int r = quarter * 32 + lane;
-#pragma unroll 1
-        for (int c0 = half * (BN / 2); c0 < (half + 1) * (BN / 2); c0 += W) {
-          float v[W];
-          if (blocks) {
-            load_columns(acc + c0, v);
-          } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = 0.f;
-          }
-          if constexpr (FORM == FEW) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) sums[(c0 + i) * 132 + r] = v[i];
-          } else {
-#pragma unroll
-            for (int i = 0; i < W; i += 4)
-              *reinterpret_cast<float4*>(sums + r * (BN + 4) + c0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          }
-        }
+        break;  // the block's one tile: below
       } else if constexpr (FORM == FEW) {
         constexpr int W = BN / 2;
         const int col = tile.col0 + quarter * 32 + lane, rows = tile.rows - half * W;
         if (rows > 0) {  // the same for the warp
-          float v[W], u[GATED ? W : 1];
+          float v[W], u[W];
           if (blocks) {
             load_columns(acc + half * W, v);
             if constexpr (GATED) load_columns(acc + BN + half * W, u);
           } else {
 #pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = 0.f, u[GATED ? i : 0] = 0.f;
+            for (int i = 0; i < W; ++i) v[i] = 0.f, u[i] = 0.f;
           }
           if (col < a.cols) {
             const long long row0 = tile.row0 + half * W;
-            const float bias = a.bias ? load1(a.bias, col, is_bf16) : 0.f;
+            if (a.bias) {
+              const float bias = load1(a.bias, col, is_bf16);
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-              v[i] += bias;
-              if (a.z && i < rows) {
-                static_cast<uint16_t*>(a.z)[(row0 + i) * a.z_stride + col] = pack1(v[i], is_bf16);
-                if constexpr (GATED) static_cast<uint16_t*>(a.u)[(row0 + i) * a.z_stride + col] = pack1(u[i], is_bf16);
-              }
+              for (int i = 0; i < W; ++i) v[i] += bias;
+            }
+            // a column of W values, a row apart
+            auto put = [&](void* to, long long stride, const float (&w)[W]) {
+              uint16_t* out = static_cast<uint16_t*>(to) + row0 * stride + col;
+#pragma unroll
+              for (int i = 0; i < W; ++i, out += stride)
+                if (i < rows) *out = pack1(w[i], is_bf16);
+            };
+            if (a.z) {
+              put(a.z, a.z_stride, v);
+              if constexpr (GATED) put(a.u, a.z_stride, u);
             }
             activate_all(v, a.act);
+            if constexpr (GATED) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-              if constexpr (GATED) v[i] *= u[i];
-              if (i < rows) {
-                if (a.residual) v[i] += load1(a.residual, (row0 + i) * a.r_stride + col, is_bf16);
-                static_cast<uint16_t*>(a.y)[(row0 + i) * a.cols + col] = pack1(v[i], is_bf16);
-              }
+              for (int i = 0; i < W; ++i) v[i] *= u[i];
             }
+            if (a.residual) {
+              const uint16_t* in = static_cast<const uint16_t*>(a.residual) + row0 * a.r_stride + col;
+#pragma unroll
+              for (int i = 0; i < W; ++i, in += a.r_stride)
+                if (i < rows) v[i] += unpack1(*in, is_bf16);
+            }
+            put(a.y, a.cols, v);
           }
         }
         if (blocks) {
@@ -658,41 +731,94 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp == 0)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
 
   if constexpr (SPLIT) {
-    // every block has its part in shared memory; each adds a share of the tile's outputs
-    cluster_sync();
+    // Every block adds a share of the tile's outputs, the blocks' parts in order of their ranks.  FEW: the parts of a
+    // row of x (128 outputs, neighbours in a warp) are written to the block that adds them, one barrier.  Else a
+    // thread has a row of the tile, whose remote writes would not meet: each block keeps its part, the others read it.
+    fence_after();
     const Tile tile = tile_of<FORM, C>(a, first, ends, start, group);
-    constexpr int ACROSS = FORM == FEW ? 32 : BN / 4, DOWN = FORM == FEW ? BN : 128, ROW = FORM == FEW ? 132 : BN + 4;
-    uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
-    for (int i = rank * kThreads + tid; i < ACROSS * DOWN; i += kThreads * a.split) {
-      const int r = i / ACROSS, c = i % ACROSS * 4;
-      if (r >= tile.rows || tile.col0 + c >= a.cols) continue;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      const uint32_t at = smem_u32(reinterpret_cast<const float*>(sm) + r * ROW + c);
-#pragma unroll 4
-      for (int q = 0; q < a.split; ++q) {
-        const float4 w = ld_cluster(at, q);
-        v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
-      }
-      const long long row = tile.row0 + r;
-      const int col = tile.col0 + c;
+    int k0;
+    const int blocks = part(tile, k0);
+    const int share = FORM == FEW ? (min(BN, tile.rows) + a.split - 1) / a.split : 0;  // rows of x of a block
+    constexpr int ROW = FORM == FEW ? 128 : BN + 4;                                   // floats of a row of a part
+    float* const sums = reinterpret_cast<float*>(FORM == FEW ? staging_all + 512 : sm);
+    cluster_wait();
+    if (warp < kWorkers) {
+      constexpr int W = BN / 2 < 32 ? BN / 2 : 32;
+      const int r = (warp & 3) * 32 + lane, begin = (warp >> 2) * (BN / 2);
+      const uint32_t acc = tbase + ((uint32_t)((warp & 3) * 32) << 16);
+      int to = FORM == FEW ? begin / share : 0, in = begin - to * share;
+#pragma unroll 1
+      for (int c0 = begin; c0 < begin + BN / 2; c0 += W) {
+        if (FORM == FEW && c0 >= tile.rows) break;
+        float v[W];
+        if (blocks) {
+          load_columns(acc + c0, v);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < a.cols) v[j] = finish<FORM>(a, v[j], row, col + j, is_bf16);
-      uint16_t* const out = y + row * a.cols + col;
-      if (a.wide) {
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack(v[0], v[1], is_bf16), pack(v[2], v[3], is_bf16));
-      } else {
+          for (int i = 0; i < W; ++i) v[i] = 0.f;
+        }
+        if constexpr (FORM == FEW) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < a.cols) out[j] = pack1(v[j], is_bf16);
+          for (int i = 0; i < W; ++i) {
+            if (c0 + i < tile.rows) put_peer(peer(smem_u32(sums + (rank * share + in) * ROW + r), to), v[i]);
+            if (++in == share) in = 0, ++to;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < W; i += 4)
+            *reinterpret_cast<float4*>(sums + r * ROW + c0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
       }
     }
-    cluster_sync();  // the others' reads of this block's part are over
+    cluster_sync();
+    uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
+    constexpr int ACROSS = FORM == FEW ? 32 : BN / 4;
+    const int first_row = FORM == FEW ? rank * share : 0, rows = FORM == FEW ? min(share, tile.rows - first_row) : tile.rows;
+    const int begin = FORM == FEW ? tid : rank * kThreads + tid, stride = FORM == FEW ? kThreads : kThreads * a.split;
+    constexpr int AT_ONCE = 4;  // sums whose parts are on their way
+    for (int i0 = begin; i0 < ACROSS * rows; i0 += stride * AT_ONCE) {
+      float4 v[AT_ONCE];
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < a.split; ++q) {
+        float4 w[AT_ONCE];
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) {
+          const int i = min(i0 + e * stride, ACROSS * rows - 1), r = i / ACROSS, c = i % ACROSS * 4;
+          w[e] = FORM == FEW ? *reinterpret_cast<const float4*>(sums + (q * share + r) * ROW + c)
+                             : ld_cluster(smem_u32(sums + r * ROW + c), q);
+        }
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) v[e].x += w[e].x, v[e].y += w[e].y, v[e].z += w[e].z, v[e].w += w[e].w;
+      }
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int i = i0 + e * stride, r = i / ACROSS, col = tile.col0 + i % ACROSS * 4;
+        if (i >= ACROSS * rows || col >= a.cols) continue;
+        const long long row = tile.row0 + first_row + r;
+        float o[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+        if (FORM == FORWARD || FORM == FEW) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col + j < a.cols) o[j] = finish<FORM>(a, o[j], row, col + j, is_bf16);
+        }
+        uint16_t* const out = y + row * a.cols + col;
+        if (a.wide) {
+          *reinterpret_cast<uint2*>(out) = make_uint2(pack(o[0], o[1], is_bf16), pack(o[2], o[3], is_bf16));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col + j < a.cols) out[j] = pack1(o[j], is_bf16);
+        }
+      }
+    }
+    __syncwarp();
+    if constexpr (FORM != FEW) cluster_sync();  // the others' reads of this block's part are over
   }
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
 }
 
 }  // namespace product

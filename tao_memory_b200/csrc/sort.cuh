@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -148,8 +149,15 @@ inline cudaError_t run(Pass p, int* counts, cudaStream_t s) {
     p.counts = nullptr;
     p.per = (p.n + 1023) / 1024 * 32;
     static_assert(32 * kMostBins * sizeof(int) <= 96 * 1024, "");
-    const cudaError_t e = cudaFuncSetAttribute(place_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               32 * kMostBins * (int)sizeof(int));
+    static std::atomic<uint64_t> ready{0};  // of the first 64 devices
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t mark = device < 64 ? 1ull << device : 0;
+    if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & mark)) {
+      e = cudaFuncSetAttribute(place_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               32 * kMostBins * (int)sizeof(int));
+      if (e == cudaSuccess) ready |= mark;
+    }
     if (e != cudaSuccess) return e;
     place_kernel<32><<<1, 1024, 32 * p.bins * sizeof(int), s>>>(p);
     return cudaGetLastError();

@@ -3,8 +3,10 @@ residual) and ``expert_linear`` (rows sorted by expert, each through its expert'
 
 Forward one library kernel; the gradient is one for the activation's slope (where there is an activation or a
 bias), one for the input and one for the weights.  Operands whose rows do not start on 16 bytes are copied to
-rows that do first.
+rows that do first, by the library.
 """
+
+from ctypes import byref
 
 import torch
 
@@ -13,26 +15,6 @@ from .norm import TYPES, _rows, refuse_tangents, wants_gradient
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 MOST_EXPERTS = 512
-
-
-def _room(like, *shape):
-    """An uninitialised [..., width] whose rows start on 16 bytes."""
-    width = shape[-1]
-    return like.new_empty((*shape[:-1], -(-width // 8) * 8))[..., :width]
-
-
-def _laid(t):
-    """``t`` [..., rows, width] as the products fetch it: neighbours next to each other, everything else on 16 bytes."""
-    width = t.shape[-1]
-    if (t.stride(-1) == 1 or width == 1) and t.data_ptr() % 16 == 0:
-        least = width  # rows do not overlap, nor do matrices
-        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-            if size > 1 and (stride % 8 or stride < least):
-                break
-            least = max(least, stride * size)
-        else:
-            return t
-    return _room(t, *t.shape).copy_(t)
 
 
 def _check(name, x, weight, activation):
@@ -48,41 +30,51 @@ def _check(name, x, weight, activation):
         raise ValueError(f"activation is one of {tuple(ACTIVATIONS)}")
 
 
-def _forward(rows, weight, up, bias, residual, offsets, act, keep):
-    """(y, z, u) of laid-out operands: z, u are None unless ``keep``."""
-    count, n, k = rows.shape[0], weight.shape[-2], weight.shape[-1]
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _describe(rows, weight, up, bias, residual, offsets, act):
+    """The library's description of a product, without its outputs."""
+    n, k = weight.shape[-2:]
+    grouped = offsets is not None
+    w = weight.stride() if grouped else (0, *weight.stride())
+    u = (0, 0, 0) if up is None else up.stride()
+    x = rows.stride()
+    return _lib.TaoLinear(
+        rows.data_ptr(), weight.data_ptr(), _address(up), _address(bias), _address(residual), _address(offsets), x[0], x[1],
+        w[0], w[1], w[2], u[0], u[1], u[2], 0 if residual is None else residual.stride(0), 0, rows.shape[0], n, k,
+        weight.shape[0] if grouped else 1, TYPES[rows.dtype], act)
+
+
+def _room(p, rows, gradient):
+    """The workspace that ``p`` needs, held by the caller until the launch; the allocator orders its next use."""
+    size = _lib.lib().tao_linear_workspace_bytes(byref(p), gradient)
+    if size == 0:
+        return None
+    room = torch.empty(size + 256, dtype=torch.uint8, device=rows.device)
+    at = room.data_ptr()
+    p.workspace, p.workspace_bytes = at + -at % 256, size
+    return room
+
+
+def _forward(p, rows, up, keep):
+    """(y, z, u) of a described product: z, u are None unless ``keep``."""
+    count, n = rows.shape[0], p.n
     y = rows.new_empty((count, n))
+    p.y = y.data_ptr()
     z = u = None
     if keep:
-        z = _room(rows, count, n)
-        u = None if up is None else _room(rows, count, n)
-    grouped = offsets is not None
-    _lib.on_device(
-        rows.device.index, _lib.lib().tao_linear, rows.data_ptr(), rows.stride(0), weight.data_ptr(), weight.stride(-2),
-        weight.stride(0) if grouped else 0, None if up is None else up.data_ptr(), 0 if up is None else up.stride(-2),
-        0 if up is None else up.stride(0), None if bias is None else bias.data_ptr(),
-        None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-        offsets.data_ptr() if grouped else None, weight.shape[0] if grouped else 1, count, n, k, TYPES[rows.dtype], act,
-        y.data_ptr(), None if z is None else z.data_ptr(), None if u is None else u.data_ptr(),
-        0 if z is None else z.stride(0))
+        p.z_row = -(-n // 8) * 8
+        z = rows.new_empty((count, p.z_row))
+        p.z = z.data_ptr()
+        if up is not None:
+            u = rows.new_empty((count, p.z_row))
+            p.u = u.data_ptr()
+    room = _room(p, rows, 0)
+    _lib.on_device(rows.device.index, _lib.lib().tao_linear, byref(p))
+    del room
     return y, z, u
-
-
-def _slope(dy, z, u, act, db):
-    """(dz, du) of dy [rows, n], and the rows' sum into ``db``."""
-    count, n = dy.shape
-    lib = _lib.lib()
-    dz = None if z is None else _room(dy, count, n)
-    du = None if u is None else _room(dy, count, n)
-    room = None
-    if db is not None:
-        room = dy.new_empty(lib.tao_linear_slope_workspace_bytes(count, n), dtype=torch.uint8)
-    _lib.on_device(
-        dy.device.index, lib.tao_linear_slope, dy.data_ptr(), dy.stride(0), None if z is None else z.data_ptr(),
-        None if u is None else u.data_ptr(), 0 if z is None else z.stride(0), count, n, TYPES[dy.dtype], act,
-        None if dz is None else dz.data_ptr(), None if du is None else du.data_ptr(), 0 if dz is None else dz.stride(0),
-        None if db is None else db.data_ptr(), None if room is None else room.data_ptr(), 0 if room is None else room.numel())
-    return dy if dz is None else dz, du
 
 
 class _Product(torch.autograd.Function):
@@ -90,13 +82,11 @@ class _Product(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, up, bias, residual, offsets, act):
-        rows, w = _laid(x), _laid(weight)
-        u_w = None if up is None else _laid(up)
+        p = _describe(x, weight, up, bias, residual, offsets, act)
         sloped = any(ctx.needs_input_grad[:4]) and (act != 0 or up is not None)
-        y, z, u = _forward(rows, w, u_w, bias, residual, offsets, act, sloped)
-        ctx.save_for_backward(rows, w, u_w, z, u, offsets)
+        y, z, u = _forward(p, x, up, sloped)
+        ctx.save_for_backward(x, weight, up, z, u, offsets)
         ctx.act = act
-        ctx.has_bias = bias is not None
         ctx.set_materialize_grads(False)
         return y
 
@@ -106,38 +96,32 @@ class _Product(torch.autograd.Function):
             raise RuntimeError("linear and expert_linear are differentiable once (their gradients have none)")
         if dy is None:
             return (None,) * 7
-        rows, weight, up, z, u, offsets = ctx.saved_tensors
         want_x, want_w, want_up, want_b, want_res = ctx.needs_input_grad[:5]
         dx = dw = dup = db = None
         if want_x or want_w or want_up or want_b:
-            (count, k), n = rows.shape, weight.shape[-2]
-            lib, device, code = _lib.lib(), rows.device.index, TYPES[rows.dtype]
-            grad = _rows(dy, n)
-            du = None
-            if want_b:
-                db = dy.new_empty(n)
-            if z is not None or want_b:
-                dz, du = _slope(grad, z, u, ctx.act, db)
-            else:
-                dz = grad
-            grouped = offsets is not None
-            at, experts = (offsets.data_ptr(), weight.shape[0]) if grouped else (None, 1)
-            if want_x or want_w or want_up:
-                dz = _laid(dz)
-                du_at = None if du is None else du.data_ptr()
+            x, weight, up, z, u, offsets = ctx.saved_tensors
+            p = _describe(x, weight, up, None, None, offsets, ctx.act)
+            grad = _rows(dy, p.n)
+            p.dy, p.dy_row = grad.data_ptr(), grad.stride(0)
+            if z is not None:
+                p.z, p.z_row = z.data_ptr(), z.stride(0)
+                if u is not None:
+                    p.u = u.data_ptr()
             if want_x:
-                dx = rows.new_empty((count, k))
-                _lib.on_device(
-                    device, lib.tao_linear_input_gradient, dz.data_ptr(), du_at, dz.stride(0), weight.data_ptr(),
-                    weight.stride(-2), weight.stride(0) if grouped else 0, None if up is None else up.data_ptr(),
-                    0 if up is None else up.stride(-2), 0 if up is None else up.stride(0), at, experts, count, n, k, code,
-                    dx.data_ptr())
+                dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                p.dx = dx.data_ptr()
             if want_w or want_up:
-                dw = weight.new_empty(weight.shape)
-                dup = None if up is None else weight.new_empty(weight.shape)
-                _lib.on_device(
-                    device, lib.tao_linear_weight_gradient, dz.data_ptr(), du_at, dz.stride(0), rows.data_ptr(),
-                    rows.stride(0), at, experts, count, n, k, code, dw.data_ptr(), None if dup is None else dup.data_ptr())
+                dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
+                p.dw = dw.data_ptr()
+                if up is not None:
+                    dup = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
+                    p.dup = dup.data_ptr()
+            if want_b:
+                db = torch.empty(p.n, dtype=x.dtype, device=x.device)
+                p.db = db.data_ptr()
+            room = _room(p, x, 1)
+            _lib.on_device(x.device.index, _lib.lib().tao_linear_gradient, byref(p))
+            del room
         return (dx, dw if want_w else None, dup if want_up else None, db, dy if want_res else None, None, None)
 
 
@@ -159,7 +143,7 @@ def linear(x, weight, bias=None, residual=None, activation=None):
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("the residual has the output's shape and the activations' type and device")
     refuse_tangents("linear", x, weight, bias, residual)
-    rows = _rows(x, k)
+    rows = x if x.dim() == 2 else x.reshape(-1, k)
     if bias is not None:
         bias = bias.contiguous()
     if residual is not None:
@@ -168,7 +152,7 @@ def linear(x, weight, bias=None, residual=None, activation=None):
     if wants_gradient(x, weight, bias, residual):
         y = _Product.apply(rows, weight, None, bias, residual, None, act)
     else:
-        y, _, _ = _forward(_laid(rows), _laid(weight), None, bias, residual, None, act, False)
+        y, _, _ = _forward(_describe(rows, weight, None, bias, residual, None, act), rows, None, False)
     return y if x.dim() == 2 else y.view(shape)
 
 
@@ -195,10 +179,9 @@ def expert_linear(x, weight, offsets, up=None, activation=None):
     refuse_tangents("expert_linear", x, weight, up)
     offsets = offsets.contiguous()
     act = ACTIVATIONS[activation]
-    rows = _rows(x, x.shape[1])
     if wants_gradient(x, weight, up):
-        return _Product.apply(rows, weight, up, None, None, offsets, act)
-    return _forward(_laid(rows), _laid(weight), None if up is None else _laid(up), None, None, offsets, act, False)[0]
+        return _Product.apply(x, weight, up, None, None, offsets, act)
+    return _forward(_describe(x, weight, up, None, None, offsets, act), x, up, False)[0]
 
 
 __all__ = ["linear", "expert_linear", "ACTIVATIONS"]

@@ -150,8 +150,9 @@ def test_residual_in_place_of_the_output():
     from tao_memory_b200 import _lib
     x, w, _, res, _ = _inputs(300, 128, 96, torch.bfloat16, residual=True)
     want = Product(x, w, torch.bfloat16, residual=res)
-    _lib.on_device(0, _lib.lib().tao_linear, x.data_ptr(), 128, w.data_ptr(), 128, 0, None, 0, 0, None, res.data_ptr(), 96,
-                   None, 1, 300, 96, 128, 0, 0, res.data_ptr(), None, None, 0)
+    p = _lib.TaoLinear(x=x.data_ptr(), x_row=128, x_col=1, w=w.data_ptr(), w_row=128, w_col=1, residual=res.data_ptr(), r_row=96,
+                       rows=300, n=96, k=128, experts=1, y=res.data_ptr())
+    _lib.on_device(0, _lib.lib().tao_linear, p)
     close(res, want.y, want.y_off)
 
 

@@ -1,7 +1,5 @@
 """What the trained block's operators refuse, checked before any launch (no GPU needed)."""
 
-import ctypes
-
 import pytest
 import torch
 
@@ -20,54 +18,54 @@ def test_no_cpu_fallback():
             bad()
 
 
-def _linear(**kw):
-    a = dict(x=16, xs=64, w=16, ws=64, we=0, up=None, us=0, ue=0, bias=None, res=None, rs=0, off=None, e=1, rows=4, n=32,
-             k=64, type=0, act=0, y=16, z=None, u=None, zs=0)
+def _described(**kw):
+    a = dict(x=256, w=256, x_row=64, x_col=1, w_row=64, w_col=1, rows=4, n=32, k=64, experts=1, y=256)
     a.update(kw)
-    return _lib.lib().tao_linear(*a.values(), None)
+    return _lib.TaoLinear(**a)
+
+
+EXPERTS = dict(offsets=16, experts=2, w_expert=2048)
 
 
 def test_linear_refusals():
-    for bad in (dict(type=2), dict(act=5), dict(act=-1), dict(rows=-1), dict(n=0), dict(k=0), dict(x=None), dict(w=None),
-                dict(y=None), dict(x=18), dict(w=24), dict(xs=63), dict(xs=56), dict(ws=60), dict(y=17), dict(bias=17),
-                dict(res=17, rs=32), dict(e=2), dict(e=0), dict(off=16, e=513), dict(off=18, e=2, we=2048),
-                dict(off=16, e=2, we=2047), dict(off=16, e=2, we=0), dict(up=16, us=64),
-                dict(off=16, e=2, we=2048, bias=16), dict(off=16, e=2, we=2048, up=16, us=64, ue=2048, z=16, zs=32),
-                dict(rows=(1 << 30) + 1), dict(n=(1 << 24) + 1)):
-        assert _linear(**bad) == ARG, bad
-    assert _linear(rows=0) == _lib.TAO_OK
+    lib = _lib.lib()
+    for bad in (dict(type=2), dict(activation=5), dict(activation=-1), dict(rows=-1), dict(n=0), dict(k=0), dict(x=None),
+                dict(w=None), dict(y=None), dict(x=17), dict(w=19), dict(y=17), dict(bias=17), dict(residual=17, r_row=32),
+                dict(experts=2), dict(experts=0), dict(offsets=16, experts=513), dict(EXPERTS, offsets=18),
+                dict(up=256, up_row=64, up_col=1), dict(EXPERTS, bias=16), dict(EXPERTS, residual=16, r_row=32),
+                dict(EXPERTS, up=256, up_row=64, up_col=1, up_expert=2048, z=16, z_row=32), dict(rows=(1 << 30) + 1),
+                dict(n=(1 << 24) + 1), dict(k=(1 << 24) + 1),
+                # what has to be copied first has no room, too little, or one off its alignment
+                dict(x_row=63), dict(x_col=2), dict(w=24), dict(x_row=0), dict(x_row=63, workspace=256, workspace_bytes=256),
+                dict(x_row=63, workspace=128, workspace_bytes=1 << 20), dict(EXPERTS, w_expert=2047),
+                dict(EXPERTS, w_expert=0)):
+        assert lib.tao_linear(_described(**bad), None) == ARG, bad
+    assert lib.tao_linear(_described(rows=0), None) == _lib.TAO_OK
+    assert lib.tao_linear(None, None) == ARG
+
+
+def test_linear_workspace():
+    size = lambda gradient, **kw: _lib.lib().tao_linear_workspace_bytes(_described(**kw), gradient)
+    assert size(0) == 0 and size(0, rows=0, x_row=63) == 0 and size(0, type=7) == 0
+    assert size(0, x_row=63) == 512 and size(0, x=258, rows=1) == 256 and size(0, rows=1, x_row=63) == 0
+    assert size(0, w_row=1, w_col=64) == 4096 and size(0, **dict(EXPERTS, w_expert=0)) == 8192
+    grad = dict(dy=256, dy_row=32, dx=256, dw=256)
+    assert size(1, **grad) == 0 and size(1, **dict(grad, dy_row=33)) == 256
+    assert size(1, activation=2, z=256, z_row=32, **grad) == 256 and size(1, db=256, **grad) == 256
+    assert size(1, db=256, activation=2, z=256, z_row=32, **dict(grad, dx=None, dw=None)) == 256
+    gated = dict(EXPERTS, up=256, up_row=64, up_col=1, up_expert=2048, u=256, z=256, z_row=32, dup=256)
+    assert size(1, **grad, **gated) == 512
 
 
 def test_gradient_refusals():
     lib = _lib.lib()
-
-    def dinput(**kw):
-        a = dict(dz=16, du=None, ds=32, w=16, ws=64, we=0, up=None, us=0, ue=0, off=None, e=1, rows=4, n=32, k=64, type=0,
-                 dx=16)
-        a.update(kw)
-        return lib.tao_linear_input_gradient(*a.values(), None)
-
-    def dweight(**kw):
-        a = dict(dz=16, du=None, ds=32, x=16, xs=64, off=None, e=1, rows=4, n=32, k=64, type=0, dw=16, dup=None)
-        a.update(kw)
-        return lib.tao_linear_weight_gradient(*a.values(), None)
-
-    def slope(**kw):
-        a = dict(dy=16, dys=32, z=16, u=None, zs=32, rows=4, n=32, type=0, act=2, dz=16, du=None, ds=32, db=None, ws=None,
-                 size=0)
-        a.update(kw)
-        return lib.tao_linear_slope(*a.values(), None)
-
-    for bad in (dict(dz=None), dict(dx=None), dict(du=16), dict(up=16), dict(ds=30), dict(dz=20), dict(w=20), dict(type=3),
-                dict(dx=17)):
-        assert dinput(**bad) == ARG, bad
-    for bad in (dict(dz=None), dict(dw=None), dict(du=16), dict(dup=16), dict(xs=62), dict(x=24), dict(dw=17), dict(e=0)):
-        assert dweight(**bad) == ARG, bad
-    for bad in (dict(dy=None), dict(dz=None), dict(u=16), dict(dy=17), dict(db=16), dict(db=16, ws=16, size=64),
-                dict(act=9), dict(z=None, dz=None)):
-        assert slope(**bad) == ARG, bad
-    assert dinput(rows=0) == _lib.TAO_OK and slope(rows=0) == _lib.TAO_OK
-    assert lib.tao_linear_slope_workspace_bytes(0, 8) == 0 and lib.tao_linear_slope_workspace_bytes(1, 8) == 32
+    grad = dict(dy=256, dy_row=32, dx=256, dw=256)
+    for bad in (dict(dy=None), dict(dy=17), dict(dx=17), dict(dw=17), dict(db=17), dict(x=None), dict(w=None), dict(dup=256),
+                dict(activation=2), dict(activation=2, z=256, z_row=32), dict(db=256), dict(dy_row=33),
+                dict(EXPERTS, up=256, up_row=64, up_col=1, up_expert=2048, z=256, u=256, z_row=32),
+                dict(EXPERTS, up=256, up_row=64, up_col=1, up_expert=2048, z=256, z_row=32, dup=256)):
+        assert lib.tao_linear_gradient(_described(**dict(grad, **bad)), None) == ARG, bad
+    assert lib.tao_linear_gradient(_described(rows=0), None) == _lib.TAO_OK
 
 
 def test_token_refusals():
