@@ -4,7 +4,7 @@
 // Gradient: the tokens are sorted by id (sort.cuh, stably), and a block adds the rows of a run of kRun sorted
 // tokens, in fp32 and in their order, a sum for each id.  An id whose tokens lie within the run is written at
 // once; the sums of one that goes on in the next run are joined by a second kernel, in the runs' order, so a word
-// that comes 10000 times is added by 160 blocks and the result does not depend on when they ran.  Rows of no
+// that comes 10000 times is added by 313 blocks and the result does not depend on when they ran.  Rows of no
 // token are zeros.
 #include <cuda_runtime.h>
 
@@ -18,7 +18,7 @@ namespace {
 
 using namespace rows;
 
-constexpr int kRun = 64;
+constexpr int kRun = 32;
 
 int efail(int code, const char* msg) {
   tao_set_last_error(msg);
@@ -36,19 +36,33 @@ struct EmbedArgs {
   void* out;
 };
 
-template <class T, int N>
+// EACH: tokens of a thread, whose rows are on their way at once.
+template <class T, int N, int EACH>
 __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
-  const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
-  if (t >= a.n || c >= a.width) return;
-  const long long id = a.wide_ids ? static_cast<const long long*>(a.ids)[t] : static_cast<const int*>(a.ids)[t];
-  float f[N] = {};
-  if (id >= 0 && id < a.vocab) {
-    reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + id * a.stride + c)->widen(f);
+  if (c >= a.width) return;
+  const long long t0 = (long long)blockIdx.x * (blockDim.y * EACH) + threadIdx.y;
+  long long id[EACH];
+  Vec<T, N> v[EACH];
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] *= a.scale;
+  for (int j = 0; j < EACH; ++j) {
+    const long long t = min(t0 + j * (int)blockDim.y, a.n - 1);
+    id[j] = a.wide_ids ? static_cast<const long long*>(a.ids)[t] : static_cast<const int*>(a.ids)[t];
   }
-  *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + t * a.width + c) = Vec<T, N>::of(f);
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    if (id[j] < 0 || id[j] >= a.vocab) id[j] = -1;
+    v[j] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + max(id[j], 0ll) * a.stride + c);
+  }
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const long long t = t0 + j * (int)blockDim.y;
+    float f[N];
+    v[j].widen(f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = id[j] < 0 ? 0.f : f[i] * a.scale;
+    if (t < a.n) *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + t * a.width + c) = Vec<T, N>::of(f);
+  }
 }
 
 struct SumArgs {
@@ -60,6 +74,28 @@ struct SumArgs {
   void* out;
   float* parts;  // [runs][2][width]: of an id that began before the run, and of one that goes on behind it
 };
+
+template <int N>
+TAO_DEVI void put_part(float* to, const float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  } else {
+    *to = v[0];
+  }
+}
+template <int N>
+TAO_DEVI void add_part(const float* from, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float4 w = *reinterpret_cast<const float4*>(from + e);
+      v[e] += w.x, v[e + 1] += w.y, v[e + 2] += w.z, v[e + 3] += w.w;
+    }
+  } else {
+    v[0] += *from;
+  }
+}
 
 // Sums of run blockIdx.x, for the vector of columns that a thread has.
 template <class T, int N>
@@ -75,29 +111,29 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
   if (c >= a.width) return;
   float sum[N] = {};
-  constexpr int AHEAD = 8;
-  for (int i0 = 0; i0 < count; i0 += AHEAD) {
-    Vec<T, N> v[AHEAD];
+  constexpr int AHEAD = 8;  // rows on their way
+  Vec<T, N> v[AHEAD];
+  auto fetch = [&](int i) {
+    return *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.dy) + tokens[min(i, count - 1)] * a.dy_stride + c);
+  };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (i0 + i < count)
-        v[i] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.dy) + tokens[i0 + i] * a.dy_stride + c);
+  for (int i = 0; i < AHEAD; ++i) v[i] = fetch(i);
+  for (int i0 = 0; i0 < count; i0 += AHEAD) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (i0 + i >= count) break;
       const int id = ids[i0 + i + 1], next = ids[i0 + i + 2];
       float f[N];
       v[i].widen(f);
+      v[i] = fetch(i0 + i + AHEAD);
 #pragma unroll
       for (int e = 0; e < N; ++e) sum[e] += f[e];
       const bool last = i0 + i == count - 1;
       if (id == next && !last) continue;
       if (id < a.vocab) {
-        const bool older = id == ids[0] && ids[1] == id;  // sorted: all from the run's first on
+        const bool older = id == ids[0];  // sorted: all from the run's first on
         if (older || id == next) {
-          float* part = a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width + c;
-#pragma unroll
-          for (int e = 0; e < N; ++e) part[e] = sum[e];
+          put_part<N>(a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width + c, sum);
         } else {
 #pragma unroll
           for (int e = 0; e < N; ++e) sum[e] *= a.scale;
@@ -110,31 +146,39 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
   }
 }
 
-// The id that begins in run blockIdx.x and goes on behind it.
+// The id that begins in run blockIdx.x and goes on behind it.  A warp has 32 vectors of columns; the warps share out
+// the runs, and their sums are added in their order.
 template <class T, int N>
 __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
+  __shared__ float sums[8][N][33];
   const int begin = blockIdx.x * kRun, end = begin + kRun;
-  if (end >= a.n) return;
-  const int id = a.ids[end - 1];
-  if (a.ids[end] != id || id >= a.vocab || (begin > 0 && a.ids[begin] == id && a.ids[begin - 1] == id)) return;
-  int low = end, high = a.n;  // the first place behind the id's
-  while (low < high) {
-    const int mid = low + (high - low) / 2;
-    if (a.ids[mid] == id) low = mid + 1;
-    else high = mid;
+  const int id = a.ids[end - 1], before = a.ids[max(begin - 1, 0)], first = a.ids[begin], next = a.ids[end];
+  if (next != id || id >= a.vocab || (begin > 0 && first == id && before == id)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = (a.n + kRun - 1) / kRun;
+  int last = blockIdx.x + 1;  // the last run that begins with the id, 32 more looked at at once
+  for (bool more = true; more;) {
+    const int run = last + 1 + lane;
+    const uint32_t same = __ballot_sync(0xffffffffu, run < runs && a.ids[min(run, runs - 1) * kRun] == id);
+    last += ~same ? __ffs(~same) - 1 : 32;
+    more = same == 0xffffffffu;
   }
-  const int last = (low - 1) / kRun;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
-  if (c >= a.width) return;
-  float sum[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) sum[e] = a.parts[((long long)blockIdx.x * 2 + 1) * a.width + c + e];
+  const int c = (blockIdx.y * 32 + lane) * N, count = last - blockIdx.x;
+  float sum[N] = {};
+  if (c < a.width) {
+    if (warp == 0) add_part<N>(a.parts + ((long long)blockIdx.x * 2 + 1) * a.width + c, sum);
 #pragma unroll 8
-  for (int r = blockIdx.x + 1; r <= last; ++r)
+    for (int r = count * warp / 8; r < count * (warp + 1) / 8; ++r)
+      add_part<N>(a.parts + ((long long)blockIdx.x + 1 + r) * 2 * a.width + c, sum);
+  }
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[e] += a.parts[(long long)r * 2 * a.width + c + e];
+  for (int e = 0; e < N; ++e) sums[warp][e][lane] = sum[e];
+  __syncthreads();
+  if (warp || c >= a.width) return;
 #pragma unroll
-  for (int e = 0; e < N; ++e) sum[e] *= a.scale;
+  for (int e = 0; e < N; ++e) {
+    for (int w = 1; w < 8; ++w) sum[e] += sums[w][e][lane];
+    sum[e] *= a.scale;
+  }
   *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)id * a.width + c) = Vec<T, N>::of(sum);
 }
 
@@ -195,7 +239,13 @@ int tao_embed(const void* ids, int id_bytes, long long n, const void* table, lon
   const bool wide = width * size % 16 == 0 && on16(table, stride, size) && on16(y, 0, size);
   return by_vector(type, wide, [&](auto t, auto v) {
     const Mapping m = mapping(n, (width + decltype(v)::value - 1) / decltype(v)::value);
-    embed_kernel<decltype(t), decltype(v)::value><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if ((long long)m.grid.x * m.grid.y < 148 * 8) {  // all at once, a token a thread
+      embed_kernel<decltype(t), decltype(v)::value, 1><<<m.grid, m.block, 0, s>>>(a);
+    } else {
+      const dim3 grid((m.grid.x + 3) / 4, m.grid.y);
+      embed_kernel<decltype(t), decltype(v)::value, 4><<<grid, m.block, 0, s>>>(a);
+    }
     return launched(cudaGetLastError());
   });
 }
@@ -244,7 +294,8 @@ int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* d
     const int vectors = (width + N - 1) / N, threads = std::min(256, (vectors + 31) / 32 * 32);
     const dim3 grid((unsigned)((n + kRun - 1) / kRun), (vectors + threads - 1) / threads);
     run_kernel<decltype(t), N><<<grid, threads, 0, s>>>(a);
-    if (grid.x > 1) join_kernel<decltype(t), N><<<grid, threads, 0, s>>>(a);
+    if (grid.x > 1)  // the last run goes on nowhere
+      join_kernel<decltype(t), N><<<dim3(grid.x - 1, (vectors + 31) / 32), 256, 0, s>>>(a);
     return launched(cudaGetLastError());
   });
 }

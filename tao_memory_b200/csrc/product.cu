@@ -112,8 +112,10 @@ int start_typed(const Operands& o, Args a, int split, cudaStream_t stream) {
   constexpr int A_BOX = C::A_MN ? kTerms : 128, B_BOX = C::B_MN ? kTerms : FORM == FORWARD ? C::CT : BN;
   const Operand2* ops[4] = {&o.a, &o.b, &o.a2, &o.b2};
   for (int i = 0; i < 4; ++i) {
-    const Operand2& x = ops[i]->at ? *ops[i] : *ops[i & 1];
-    if (!make_map(&maps[i], x, a.type, i & 1 ? B_BOX : A_BOX)) return pfail(TAO_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    if (!ops[i]->at)
+      maps[i] = maps[i & 1];
+    else if (!make_map(&maps[i], *ops[i], a.type, i & 1 ? B_BOX : A_BOX))
+      return pfail(TAO_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   }
   static std::atomic<uint64_t> ready{0};  // of the first 64 devices
   int device = 0;
@@ -389,13 +391,23 @@ bool fetchable(const Given& g) {
          (g.count == 1 || (g.matrix % 8 == 0 && g.matrix >= (g.rows - 1) * g.row + g.cols && g.matrix < (1ll << 38)));
 }
 
-// 16-bit values to rows of `stride` from whatever strides they have.
-__global__ void __launch_bounds__(256) lay_kernel(const Given g, uint16_t* out, long long stride) {
-  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= g.rows * g.count) return;
-  const long long matrix = row / g.rows;
-  const uint16_t* in = static_cast<const uint16_t*>(g.at) + matrix * g.matrix + (row - matrix * g.rows) * g.row;
-  for (long long c = threadIdx.x; c < g.cols; c += blockDim.x) out[row * stride + c] = in[c * g.col];
+// Up to three of them to rows of whole 16 bytes, from whatever strides they have.
+struct Laying {
+  Given from[3];
+  uint16_t* to[3];
+  long long stride[3];
+  int count;
+};
+__global__ void __launch_bounds__(256) lay_kernel(const Laying l) {
+  const Given& g = l.from[blockIdx.y];
+  const long long rows = g.rows * g.count;
+  for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.x * 8) {
+    const long long matrix = row / g.rows;
+    const uint16_t* in = static_cast<const uint16_t*>(g.at) + matrix * g.matrix + (row - matrix * g.rows) * g.row;
+    uint16_t* const out = l.to[blockIdx.y] + row * l.stride[blockIdx.y];
+#pragma unroll 8
+    for (int c = threadIdx.x & 31; c < (int)g.cols; c += 32) out[c] = in[c * g.col];
+  }
 }
 
 // Rooms of a workspace, one behind the other; without a base only their size is counted.
@@ -410,17 +422,19 @@ struct Rooms {
 };
 long long padded(long long cols) { return (cols + 7) / 8 * 8; }
 
-// An operand that TMA can fetch: as given, or laid in the workspace (of a Rooms without a base nothing is launched).
-Operand2 operand(const Given& g, Rooms& rooms, cudaStream_t s) {
+// An operand that TMA can fetch: as given, or in the workspace, to be laid there.
+Operand2 operand(const Given& g, Rooms& rooms, Laying& l) {
   if (!g.at) return {};
   if (fetchable(g)) return {g.at, g.cols, g.rows, g.row, g.count, g.matrix};
   const long long stride = padded(g.cols);
   void* to = rooms.take((size_t)(g.rows * g.count * stride * 2));
-  if (rooms.base) {
-    const dim3 block(g.cols <= 64 ? 32 : 256, g.cols <= 64 ? 8 : 1);
-    lay_kernel<<<(unsigned)((g.rows * g.count + block.y - 1) / block.y), block, 0, s>>>(g, static_cast<uint16_t*>(to), stride);
-  }
+  l.from[l.count] = g, l.to[l.count] = static_cast<uint16_t*>(to), l.stride[l.count++] = stride;
   return {to, g.cols, g.rows, stride, g.count, g.rows * stride};
+}
+void lay(const Laying& l, cudaStream_t s) {
+  long long rows = 0;
+  for (int i = 0; i < l.count; ++i) rows = std::max(rows, l.from[i].rows * l.from[i].count);
+  if (l.count) lay_kernel<<<dim3((unsigned)std::min<long long>((rows + 7) / 8, 148 * 8), l.count), 256, 0, s>>>(l);
 }
 
 Given given_x(const TaoLinear& p) { return {p.x, p.rows, p.k, 1, p.x_row, p.x_col, 0}; }
@@ -452,9 +466,11 @@ int check_room(const TaoLinear& p, size_t need) {
 }
 
 int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
-  const Operand2 ox = operand(given_x(p), rooms, s), ow = operand(given_w(p), rooms, s), ou = operand(given_up(p), rooms, s),
-                 none = {};
+  Laying laying = {};
+  const Operand2 ox = operand(given_x(p), rooms, laying), ow = operand(given_w(p), rooms, laying),
+                 ou = operand(given_up(p), rooms, laying), none = {};
   if (!rooms.base) return TAO_OK;
+  lay(laying, s);
   const int n = p.n, k = p.k;
   const long long rows = p.rows;
   Args a = {};
@@ -512,16 +528,18 @@ int weight_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream
     if (k > 128) return start<WEIGHT, 256, false, false>(o, a, 1, s);
     return start<WEIGHT, 128, false, false>(o, a, 1, s);
   }
+  // in steps of a 128 tile, as start_rows; a split of 256 columns takes 26 steps of its own more
   const long long down = (n + 127) / 128;
-  const int steps = (int)((p.rows + kTerms - 1) / kTerms);
-  if (k > 128) {
-    const int split = split_of<WEIGHT, 256>(down * ((k + 255) / 256), steps, 26).blocks;
-    if (split > 1) return start<WEIGHT, 256, false, true>(o, a, split, s);
-    return start<WEIGHT, 256, false, false>(o, a, 1, s);
+  const int steps = (int)((p.rows + kTerms - 1) / kTerms), all = sms();
+  const long long narrow = (down * ((k + 127) / 128) + all - 1) / all * steps;
+  const Split split = split_of<WEIGHT, 256>(down * ((k + 255) / 256), steps, 26);
+  if (k <= 128 || narrow < 1.6 * split.cost) {
+    const Split half = split_of<WEIGHT, 128>(down * ((k + 127) / 128), steps, 32);
+    if (half.blocks > 1 && half.cost < narrow) return start<WEIGHT, 128, false, true>(o, a, half.blocks, s);
+    return start<WEIGHT, 128, false, false>(o, a, 1, s);
   }
-  const int split = split_of<WEIGHT, 128>(down, steps, 20).blocks;
-  if (split > 1) return start<WEIGHT, 128, false, true>(o, a, split, s);
-  return start<WEIGHT, 128, false, false>(o, a, 1, s);
+  if (split.blocks > 1) return start<WEIGHT, 256, false, true>(o, a, split.blocks, s);
+  return start<WEIGHT, 256, false, false>(o, a, 1, s);
 }
 
 int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
@@ -555,16 +573,17 @@ int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
   }
   if (products) {
     if (sloped && !rooms.base) gz.at = gd.at = nullptr;  // their rooms are counted, and they are laid as they are made
-    const Operand2 oz = sloped ? Operand2{gz.at, gz.cols, gz.rows, gz.row, 1, 0} : operand(gz, rooms, s),
+    Laying laying = {};
+    const Operand2 oz = sloped ? Operand2{gz.at, gz.cols, gz.rows, gz.row, 1, 0} : operand(gz, rooms, laying),
                    od = p.up ? Operand2{gd.at, gd.cols, gd.rows, gd.row, 1, 0} : Operand2{};
-    if (p.dx) {
-      const Operand2 ow = operand(given_w(p), rooms, s), ou = operand(given_up(p), rooms, s);
-      if (rooms.base)
+    Operand2 ow = {}, ou = {}, ox = {};
+    if (p.dx) ow = operand(given_w(p), rooms, laying), ou = operand(given_up(p), rooms, laying);
+    if (p.dw) ox = operand(given_x(p), rooms, laying);  // with dy, W and U three at most: dz is made where there is U
+    if (rooms.base) {
+      lay(laying, s);
+      if (p.dx)
         if (int rc = input_gradient(p, {oz, ow, od, ou}, pairs, s)) return rc;
-    }
-    if (p.dw) {
-      const Operand2 ox = operand(given_x(p), rooms, s);
-      if (rooms.base)
+      if (p.dw)
         if (int rc = weight_gradient(p, {oz, ox, od, {}}, pairs, s)) return rc;
     }
   }

@@ -353,7 +353,7 @@ TAO_DEVI void store_rows(uint8_t* staging, void* to, long long stride, int rows,
         *reinterpret_cast<uint4*>(out + r * stride + c * 8) = *reinterpret_cast<const uint4*>(staging + staged(r, c));
     }
   } else {
-#pragma unroll 4
+#pragma unroll 8
     for (int r = 0; r < 32; ++r)
       if (r < rows && lane < cols)
         out[r * stride + lane] = *reinterpret_cast<const uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2);
@@ -370,10 +370,11 @@ TAO_DEVI void fetch_rows(uint8_t* staging, const void* from, long long stride, i
         *reinterpret_cast<uint4*>(staging + staged(r, c)) = *reinterpret_cast<const uint4*>(in + r * stride + c * 8);
     }
   } else {
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r)
-      if (r < rows && lane < cols)
-        *reinterpret_cast<uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2) = in[r * stride + lane];
+    uint16_t v[32];  // all on their way
+#pragma unroll
+    for (int r = 0; r < 32; ++r) v[r] = r < rows && lane < cols ? in[r * stride + lane] : (uint16_t)0;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) *reinterpret_cast<uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2) = v[r];
   }
 }
 // This thread's row of v, rounded, to memory.  All lanes of the warp.

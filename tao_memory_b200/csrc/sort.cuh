@@ -4,7 +4,7 @@
 // A pass counts, for each block's run of elements, how many fall into each bin (count_kernel), and then places
 // each element (place_kernel): a bin begins behind all smaller bins, a block's elements behind those of the
 // blocks before, a warp's behind those of the warps before, and of 32 elements at a time each finds those before
-// it in its bin by a match across the warp.  No atomics: the order, and all that is summed by it, is fixed.
+// it in its bin by a match across the warp.  Only whole numbers are added atomically: the order is fixed.
 // Up to kSmallSort elements one block does it in one launch.  What bounds it is latency: launches, and each
 // warp's chain of some rounds of 32 (its elements are read as they are needed, 262144 are 64 blocks' work).
 #pragma once
@@ -44,6 +44,10 @@ TAO_DEVI int id_of(const Pass& p, int value) {
 }
 TAO_DEVI int bin_of(const Pass& p, int id) { return p.shift < 0 ? id : id >> p.shift & (p.bins - 1); }
 
+constexpr int kAhead = 4;  // rounds whose ids are on their way
+// The value of element i, -1 behind the last.
+TAO_DEVI int value_at(const Pass& p, long long i, int end) { return i >= end ? -1 : p.values ? p.values[i] : (int)i; }
+
 // counts[warp][bin] of this block's warps, in shared memory.
 TAO_DEVI void count_warps(const Pass& p, int* counts, int warps) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -52,7 +56,16 @@ TAO_DEVI void count_warps(const Pass& p, int* counts, int warps) {
   const long long begin = ((long long)blockIdx.x * warps + warp) * p.per;
   const int end = (int)min(begin + p.per, (long long)p.n);
   int* const mine = counts + warp * p.bins;
-  for (long long i = begin + lane; i < end; i += 32) atomicAdd(mine + bin_of(p, id_of(p, p.values ? p.values[i] : (int)i)), 1);
+  for (long long i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
+    int value[kAhead], id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) value[j] = value_at(p, i0 + 32 * j, end);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) id[j] = value[j] < 0 ? 0 : id_of(p, value[j]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (value[j] >= 0) atomicAdd(mine + bin_of(p, id[j]), 1);
+  }
   __syncthreads();
 }
 
@@ -75,20 +88,30 @@ __global__ void __launch_bounds__(32 * WARPS) place_kernel(const Pass p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   count_warps(p, counts, WARPS);
   for (int b = threadIdx.x; b < p.bins; b += 32 * WARPS) {
-    int all = 0, earlier = 0;
-    if (p.counts) {
-#pragma unroll 8
-      for (int k = 0; k < p.blocks; ++k) {
-        const int c = p.counts[(long long)k * p.bins + b];
-        all += c;
-        if (k < (int)blockIdx.x) earlier += c;
-      }
-    } else {
+    int all = 0;
+    if (!p.counts) {
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) all += counts[w * p.bins + b];
     }
     first[b] = all;
-    before[b] = earlier;
+    before[b] = 0;
+  }
+  __syncthreads();
+  if (p.counts) {  // threads that are not needed for the bins share out the blocks
+    const int across = min((p.bins + 31) / 32 * 32, 32 * WARPS), parts = 32 * WARPS / across, part = threadIdx.x / across;
+    if (part < parts) {
+      for (int b = threadIdx.x - part * across; b < p.bins; b += across) {
+        int all = 0, earlier = 0;
+#pragma unroll 8
+        for (int k = part; k < p.blocks; k += parts) {
+          const int c = p.counts[(long long)k * p.bins + b];
+          all += c;
+          earlier += k < (int)blockIdx.x ? c : 0;
+        }
+        atomicAdd(first + b, all);
+        atomicAdd(before + b, earlier);
+      }
+    }
   }
   __syncthreads();
   if (warp == 0) {  // the bins' sizes to their first places
@@ -120,26 +143,32 @@ __global__ void __launch_bounds__(32 * WARPS) place_kernel(const Pass p) {
   const long long begin = ((long long)blockIdx.x * WARPS + warp) * p.per;
   const int end = (int)min(begin + p.per, (long long)p.n);
   int* const mine = counts + warp * p.bins;
-  for (long long base = begin; base < end; base += 32) {
-    const long long i = base + lane;
-    const bool in = i < end;
-    const int value = in ? (p.values ? p.values[i] : (int)i) : 0;
-    const int id = in ? id_of(p, value) : 0, bin = in ? bin_of(p, id) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, bin);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    const int at = in ? mine[bin] + rank : 0;
-    __syncwarp();
-    if (in && rank == 0) mine[bin] += __popc(same);
-    __syncwarp();
-    if (in) {
-      p.sorted[at] = value;
-      if (p.places) p.places[i] = at;
-      if (p.keys) p.keys[at] = id;
+  for (long long base = begin; base < end; base += 32 * kAhead) {
+    int value[kAhead], id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) value[j] = value_at(p, base + 32 * j + lane, end);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) id[j] = value[j] < 0 ? 0 : id_of(p, value[j]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const bool in = value[j] >= 0;
+      const int bin = in ? bin_of(p, id[j]) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, bin);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      const int at = in ? mine[bin] + rank : 0;
+      __syncwarp();
+      if (in && rank == 0) mine[bin] += __popc(same);
+      __syncwarp();
+      if (in) {
+        p.sorted[at] = value[j];
+        if (p.places) p.places[base + 32 * j + lane] = at;
+        if (p.keys) p.keys[at] = id[j];
+      }
     }
   }
 }
 
-inline int blocks_of(long long n) { return n <= kSmallSort ? 1 : (int)std::min<long long>((n + 4095) / 4096, kMostBlocks); }
+inline int blocks_of(long long n) { return n <= kSmallSort ? 1 : (int)std::min<long long>((n + 1023) / 1024, kMostBlocks); }
 inline size_t counts_bytes(long long n, int bins) { return n <= kSmallSort ? 0 : (size_t)blocks_of(n) * bins * sizeof(int); }
 
 // `counts`: counts_bytes of scratch.
