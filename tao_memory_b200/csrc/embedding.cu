@@ -37,13 +37,13 @@ struct EmbedArgs {
 };
 
 // EACH: tokens of a thread, whose rows are on their way at once.
-template <class T, int N, int EACH>
+template <class T, int N, bool WIDE, int EACH>
 __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  const int c = first_of<N, WIDE>(blockIdx.y, blockDim.x, threadIdx.x), step = blockDim.x;
   if (c >= a.width) return;
   const long long t0 = (long long)blockIdx.x * (blockDim.y * EACH) + threadIdx.y;
   long long id[EACH];
-  Vec<T, N> v[EACH];
+  Part<T, N, WIDE> v[EACH];
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
     const long long t = min(t0 + j * (int)blockDim.y, a.n - 1);
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
     if (id[j] < 0 || id[j] >= a.vocab) id[j] = -1;
-    v[j] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + max(id[j], 0ll) * a.stride + c);
+    v[j].load(static_cast<const T*>(a.in) + max(id[j], 0ll) * a.stride, c, step, a.width);
   }
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) embed_kernel(const EmbedArgs a) {
     v[j].widen(f);
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = id[j] < 0 ? 0.f : f[i] * a.scale;
-    if (t < a.n) *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + t * a.width + c) = Vec<T, N>::of(f);
+    if (t < a.n) Part<T, N, WIDE>::of(f).store(static_cast<T*>(a.out) + t * a.width, c, step, a.width);
   }
 }
 
@@ -75,30 +75,37 @@ struct SumArgs {
   float* parts;  // [runs][2][width]: of an id that began before the run, and of one that goes on behind it
 };
 
-template <int N>
-TAO_DEVI void put_part(float* to, const float (&v)[N]) {
-  if constexpr (N % 4 == 0) {
+// A thread's sums in fp32, in the workspace.
+template <int N, bool WIDE>
+TAO_DEVI void put_sums(float* row, int first, int step, int width, const float (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-  } else {
-    *to = v[0];
+  for (int e = 0; e < N; e += 4) {
+    if constexpr (WIDE) {
+      *reinterpret_cast<float4*>(row + first + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else {
+#pragma unroll
+      for (int i = e; i < e + 4; ++i)
+        if (first + i * step < width) row[first + i * step] = v[i];
+    }
   }
 }
-template <int N>
-TAO_DEVI void add_part(const float* from, float (&v)[N]) {
-  if constexpr (N % 4 == 0) {
+template <int N, bool WIDE>
+TAO_DEVI void add_sums(const float* row, int first, int step, int width, float (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < N; e += 4) {
-      const float4 w = *reinterpret_cast<const float4*>(from + e);
+  for (int e = 0; e < N; e += 4) {
+    if constexpr (WIDE) {
+      const float4 w = *reinterpret_cast<const float4*>(row + first + e);
       v[e] += w.x, v[e + 1] += w.y, v[e + 2] += w.z, v[e + 3] += w.w;
+    } else {
+#pragma unroll
+      for (int i = e; i < e + 4; ++i)
+        if (first + i * step < width) v[i] += row[first + i * step];
     }
-  } else {
-    v[0] += *from;
   }
 }
 
-// Sums of run blockIdx.x, for the vector of columns that a thread has.
-template <class T, int N>
+// Sums of run blockIdx.x, for the columns that a thread has.
+template <class T, int N, bool WIDE>
 __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
   __shared__ int ids[kRun + 2], tokens[kRun];  // ids[0] and ids[count + 1]: the neighbours'
   const int begin = blockIdx.x * kRun, count = min(kRun, a.n - begin);
@@ -108,16 +115,16 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
     if (i < count) tokens[i] = a.tokens[begin + i];
   }
   __syncthreads();
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  const int c = first_of<N, WIDE>(blockIdx.y, blockDim.x, threadIdx.x), step = blockDim.x;
   if (c >= a.width) return;
   float sum[N] = {};
   constexpr int AHEAD = 8;  // rows on their way
-  Vec<T, N> v[AHEAD];
-  auto fetch = [&](int i) {
-    return *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.dy) + tokens[min(i, count - 1)] * a.dy_stride + c);
+  Part<T, N, WIDE> v[AHEAD];
+  auto fetch = [&](Part<T, N, WIDE>& to, int i) {
+    to.load(static_cast<const T*>(a.dy) + tokens[min(i, count - 1)] * a.dy_stride, c, step, a.width);
   };
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) v[i] = fetch(i);
+  for (int i = 0; i < AHEAD; ++i) fetch(v[i], i);
   for (int i0 = 0; i0 < count; i0 += AHEAD) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
@@ -125,7 +132,7 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
       const int id = ids[i0 + i + 1], next = ids[i0 + i + 2];
       float f[N];
       v[i].widen(f);
-      v[i] = fetch(i0 + i + AHEAD);
+      fetch(v[i], i0 + i + AHEAD);
 #pragma unroll
       for (int e = 0; e < N; ++e) sum[e] += f[e];
       const bool last = i0 + i == count - 1;
@@ -133,11 +140,11 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
       if (id < a.vocab) {
         const bool older = id == ids[0];  // sorted: all from the run's first on
         if (older || id == next) {
-          put_part<N>(a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width + c, sum);
+          put_sums<N, WIDE>(a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width, c, step, a.width, sum);
         } else {
 #pragma unroll
           for (int e = 0; e < N; ++e) sum[e] *= a.scale;
-          *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)id * a.width + c) = Vec<T, N>::of(sum);
+          Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, step, a.width);
         }
       }
 #pragma unroll
@@ -148,7 +155,7 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
 
 // The id that begins in run blockIdx.x and goes on behind it.  A warp has 32 vectors of columns; the warps share out
 // the runs, and their sums are added in their order.
-template <class T, int N>
+template <class T, int N, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
   __shared__ float sums[8][N][33];
   const int begin = blockIdx.x * kRun, end = begin + kRun;
@@ -162,13 +169,13 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
     last += ~same ? __ffs(~same) - 1 : 32;
     more = same == 0xffffffffu;
   }
-  const int c = (blockIdx.y * 32 + lane) * N, count = last - blockIdx.x;
+  const int c = first_of<N, WIDE>(blockIdx.y, 32, lane), count = last - blockIdx.x;
   float sum[N] = {};
   if (c < a.width) {
-    if (warp == 0) add_part<N>(a.parts + ((long long)blockIdx.x * 2 + 1) * a.width + c, sum);
+    if (warp == 0) add_sums<N, WIDE>(a.parts + ((long long)blockIdx.x * 2 + 1) * a.width, c, 32, a.width, sum);
 #pragma unroll 8
     for (int r = count * warp / 8; r < count * (warp + 1) / 8; ++r)
-      add_part<N>(a.parts + ((long long)blockIdx.x + 1 + r) * 2 * a.width + c, sum);
+      add_sums<N, WIDE>(a.parts + ((long long)blockIdx.x + 1 + r) * 2 * a.width, c, 32, a.width, sum);
   }
 #pragma unroll
   for (int e = 0; e < N; ++e) sums[warp][e][lane] = sum[e];
@@ -179,7 +186,7 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
     for (int w = 1; w < 8; ++w) sum[e] += sums[w][e][lane];
     sum[e] *= a.scale;
   }
-  *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)id * a.width + c) = Vec<T, N>::of(sum);
+  Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, 32, a.width);
 }
 
 // Passes of the sort and bits of each, for ids 0 .. vocab (vocab: none).
@@ -237,14 +244,14 @@ int tao_embed(const void* ids, int id_bytes, long long n, const void* table, lon
     return efail(TAO_ERR_ARG, "operands start on a whole element");
   const EmbedArgs a = {ids, n, vocab, stride, width, id_bytes == 8, scale, table, y};
   const bool wide = width * size % 16 == 0 && on16(table, stride, size) && on16(y, 0, size);
-  return by_vector(type, wide, [&](auto t, auto v) {
+  return by_part(type, wide, [&](auto t, auto v, auto w) {
     const Mapping m = mapping(n, (width + decltype(v)::value - 1) / decltype(v)::value);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if ((long long)m.grid.x * m.grid.y < 148 * 8) {  // all at once, a token a thread
-      embed_kernel<decltype(t), decltype(v)::value, 1><<<m.grid, m.block, 0, s>>>(a);
+      embed_kernel<decltype(t), decltype(v)::value, decltype(w)::value, 1><<<m.grid, m.block, 0, s>>>(a);
     } else {
       const dim3 grid((m.grid.x + 3) / 4, m.grid.y);
-      embed_kernel<decltype(t), decltype(v)::value, 4><<<grid, m.block, 0, s>>>(a);
+      embed_kernel<decltype(t), decltype(v)::value, decltype(w)::value, 4><<<grid, m.block, 0, s>>>(a);
     }
     return launched(cudaGetLastError());
   });
@@ -289,13 +296,13 @@ int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* d
   const SumArgs a = {p.values, reinterpret_cast<const int*>(ws + r.ids), (int)n, (int)vocab, width, scale, dy, dy_stride,
                      dtable, reinterpret_cast<float*>(ws + r.parts)};
   const bool wide = width * size % 16 == 0 && on16(dy, dy_stride, size) && on16(dtable, 0, size);
-  return by_vector(type, wide, [&](auto t, auto v) {
+  return by_part(type, wide, [&](auto t, auto v, auto w) {
     constexpr int N = decltype(v)::value;
     const int vectors = (width + N - 1) / N, threads = std::min(256, (vectors + 31) / 32 * 32);
     const dim3 grid((unsigned)((n + kRun - 1) / kRun), (vectors + threads - 1) / threads);
-    run_kernel<decltype(t), N><<<grid, threads, 0, s>>>(a);
+    run_kernel<decltype(t), N, decltype(w)::value><<<grid, threads, 0, s>>>(a);
     if (grid.x > 1)  // the last run goes on nowhere
-      join_kernel<decltype(t), N><<<dim3(grid.x - 1, (vectors + 31) / 32), 256, 0, s>>>(a);
+      join_kernel<decltype(t), N, decltype(w)::value><<<dim3(grid.x - 1, (vectors + 31) / 32), 256, 0, s>>>(a);
     return launched(cudaGetLastError());
   });
 }

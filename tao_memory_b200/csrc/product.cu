@@ -217,7 +217,17 @@ bool few_rows(const FewArgs& a, int type, cudaStream_t s, int* rc) {
   return true;
 }
 
-bool on16(const void* p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
+// Neighbours that can move at once in rows of `cols` whose addresses and strides (in bytes) have these bits.
+int unit_of(int cols, unsigned long long bits) {
+  for (int u = 8; u > 1; u /= 2)
+    if (cols % u == 0 && bits % (2 * u) == 0) return u;
+  return 1;
+}
+unsigned long long bits_of(const void* p, long long stride) {
+  return reinterpret_cast<uintptr_t>(p) | (unsigned long long)stride * 2;
+}
+
+
 
 // -- the gradient's elementwise part ------------------------------------------
 struct SlopeArgs {
@@ -237,7 +247,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (blockIdx.x * 32 + lane) * VEC;
   const long long begin = (long long)blockIdx.y * a.per, end = min(begin + a.per, a.rows);
-  using Word = std::conditional_t<VEC == 8, uint4, uint16_t>;
+  using Word = typename Unit<VEC>::Type;
   auto widen = [](const Word& w, float (&v)[VEC]) {
     if constexpr (VEC == 8) {
       const uint32_t words[4] = {w.x, w.y, w.z, w.w};
@@ -246,6 +256,9 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
         const float2 f = unpack(words[i], BF16);
         v[2 * i] = f.x, v[2 * i + 1] = f.y;
       }
+    } else if constexpr (VEC == 2) {
+      const float2 f = unpack(w, BF16);
+      v[0] = f.x, v[1] = f.y;
     } else {
       v[0] = unpack1(w, BF16);
     }
@@ -255,6 +268,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
     if constexpr (VEC == 8)
       *reinterpret_cast<uint4*>(at) =
           make_uint4(pack(v[0], v[1], BF16), pack(v[2], v[3], BF16), pack(v[4], v[5], BF16), pack(v[6], v[7], BF16));
+    else if constexpr (VEC == 2)
+      *reinterpret_cast<uint32_t*>(at) = pack(v[0], v[1], BF16);
     else
       *at = pack1(v[0], BF16);
   };
@@ -398,15 +413,51 @@ struct Laying {
   long long stride[3];
   int count;
 };
+// A warp a row.  Neighbours go two at a time: words of the row as they lie, and, where it starts between two words, each
+// made of two.
 __global__ void __launch_bounds__(256) lay_kernel(const Laying l) {
   const Given& g = l.from[blockIdx.y];
   const long long rows = g.rows * g.count;
+  const int lane = threadIdx.x & 31, cols = (int)g.cols;
+  constexpr int AHEAD = 8;
   for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (long long)gridDim.x * 8) {
     const long long matrix = row / g.rows;
-    const uint16_t* in = static_cast<const uint16_t*>(g.at) + matrix * g.matrix + (row - matrix * g.rows) * g.row;
+    const uint16_t* const in = static_cast<const uint16_t*>(g.at) + matrix * g.matrix + (row - matrix * g.rows) * g.row;
     uint16_t* const out = l.to[blockIdx.y] + row * l.stride[blockIdx.y];
+    if (g.col != 1) {
 #pragma unroll 8
-    for (int c = threadIdx.x & 31; c < (int)g.cols; c += 32) out[c] = in[c * g.col];
+      for (int c = lane; c < cols; c += 32) out[c] = in[c * g.col];
+      continue;
+    }
+    const int odd = reinterpret_cast<uintptr_t>(in) >> 1 & 1;  // elements before the first whole word
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(in + odd);
+    const int whole = (cols - odd) / 2;  // words of the row
+    uint32_t* const to = reinterpret_cast<uint32_t*>(out);
+    if (!odd) {
+#pragma unroll 8
+      for (int c = lane; c < whole; c += 32) to[c] = words[c];
+      if (lane == 0 && cols & 1) out[cols - 1] = in[cols - 1];
+      continue;
+    }
+    // word c of the output: the upper half of word c - 1 and the lower one of word c
+    for (int c0 = 0; c0 <= whole; c0 += 32 * AHEAD) {
+      uint32_t before[AHEAD], v[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int c = c0 + j * 32 + lane;
+        v[j] = c < whole ? words[c] : c == whole && 2 * c < cols - 1 ? (uint32_t)in[2 * c + 1] : 0u;
+        before[j] = c > whole ? 0u : c == 0 ? (uint32_t)in[0] << 16 : words[c - 1];
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int c = c0 + j * 32 + lane;
+        const uint32_t w = before[j] >> 16 | v[j] << 16;
+        if (2 * c + 1 < cols)
+          to[c] = w;
+        else if (2 * c < cols)
+          out[2 * c] = (uint16_t)w;
+      }
+    }
   }
 }
 
@@ -477,7 +528,8 @@ int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)rows, a.cols = n, a.depth = k, a.pairs = 1;
   a.type = p.type, a.act = p.activation, a.bias = p.bias, a.residual = p.residual, a.r_stride = p.r_row;
   a.y = p.y, a.z = p.z, a.u = p.z ? p.u : nullptr, a.z_stride = p.z_row;
-  a.wide = n % 8 == 0 && on16(p.y, 0) && on16(p.z, p.z_row) && on16(p.u, 0) && on16(p.residual, p.r_row);
+  a.unit = unit_of(n, bits_of(p.y, n) | (p.z ? bits_of(p.z, p.z_row) : 0) | bits_of(a.u, 0) |
+                          (p.residual ? bits_of(p.residual, p.r_row) : 0));
   const int steps = (k + kTerms - 1) / kTerms;
   if (p.offsets) {
     const long long mean = rows / p.experts;
@@ -512,7 +564,7 @@ int input_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_
   Args a = {};
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)p.rows, a.cols = k, a.depth = n, a.pairs = pairs;
   a.type = p.type, a.y = p.dx;
-  a.wide = k % 8 == 0 && on16(p.dx, 0);
+  a.unit = unit_of(k, bits_of(p.dx, k));
   const int steps = (n + kTerms - 1) / kTerms * pairs;
   const long long row_tiles = (p.rows + 127) / 128 + (p.offsets ? p.experts / 2 : 0);
   return start_rows<INPUT>({o.a, o.b, o.a2, o.b2}, a, row_tiles, steps, s);
@@ -523,7 +575,7 @@ int weight_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream
   Args a = {};
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)p.rows, a.cols = k, a.depth = n, a.pairs = pairs;
   a.type = p.type, a.y = p.dw, a.u = p.dup;
-  a.wide = k % 8 == 0 && on16(p.dw, 0) && on16(p.dup, 0);
+  a.unit = unit_of(k, bits_of(p.dw, k) | bits_of(p.dup, 0));
   if (p.offsets) {
     if (k > 128) return start<WEIGHT, 256, false, false>(o, a, 1, s);
     return start<WEIGHT, 128, false, false>(o, a, 1, s);
@@ -562,10 +614,13 @@ int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
     const int blocks = slope_blocks(p.rows, p.n);
     if (p.db) a.sums = static_cast<float*>(rooms.take((size_t)blocks * p.n * sizeof(float)));
     if (rooms.base) {
-      const bool wide = p.n % 8 == 0 && on16(p.dy, p.dy_row) && (!sloped || (on16(p.z, p.z_row) && on16(p.u, 0)));
-      const dim3 grid((p.n + (wide ? 255 : 31)) / (wide ? 256 : 32), blocks);
-      if (wide)
+      const int unit = unit_of(p.n, bits_of(p.dy, p.dy_row) | (sloped ? bits_of(p.z, p.z_row) | bits_of(p.u, 0) : 0));
+      const int across = unit == 8 ? 256 : unit > 1 ? 64 : 32;
+      const dim3 grid((p.n + across - 1) / across, blocks);
+      if (unit == 8)
         start_slope<8>(a, grid, s);
+      else if (unit > 1)
+        start_slope<2>(a, grid, s);
       else
         start_slope<1>(a, grid, s);
       if (p.db) column_sum_kernel<<<(p.n + 31) / 32, 256, 0, s>>>(a.sums, blocks, p.n, p.type, p.db);

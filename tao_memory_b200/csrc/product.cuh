@@ -54,7 +54,7 @@ struct Args {
   long long r_stride;
   void *y, *z, *u;     // z, u: act's argument and the gate's factor (FORWARD, FEW); u: the second matrix (WEIGHT)
   long long z_stride;
-  bool wide;           // rows of y, z, u and the residual start on 16 bytes, and cols is a multiple of 8
+  int unit;            // neighbours of y, z, u and the residual that move at once: 8, 4, 2 or 1
   int split;           // blocks of a cluster
 };
 
@@ -186,16 +186,22 @@ TAO_DEVI float load1(const void* p, long long i, bool is_bf16) {
 }
 
 // -- activations ------------------------------------------------------------
-// 1 / (1 + e^-q), by the fast exponential and reciprocal: to some 2^-21 of it, far below a 16-bit step.
-TAO_DEVI float sigmoid(float q) { return __fdividef(1.f, 1.f + __expf(-q)); }
+// By the special-function unit's 2^x and reciprocal (subnormal numbers are zero): to some 2^-21, far below a 16-bit step.
+TAO_DEVI float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+TAO_DEVI float sigmoid(float q) { return reciprocal(1.f + tc::ex2(-kLog2E * q)); }
 constexpr float kGeluRoot = 0.7978845608028654f, kGeluCube = 0.044715f;  // sqrt(2 / pi)
 
 // The normal distribution's integral from the tail of z's side: with t = 1 / (1 + 0.35 x), x = |z| / sqrt(2),
 // erfc(x) e^(x^2) / t is smooth on (0, 1], and half of it a polynomial in t (fitted here at Chebyshev nodes to 2^-20).
 // So small values keep their relative precision, at two special-function instructions.  `density` is e^(-z^2 / 2).
 TAO_DEVI float normal_integral(float z, float& density) {
-  const float t = __fdividef(1.f, 1.f + 0.35f * 0.7071067811865476f * fabsf(z));
-  density = __expf(-0.5f * z * z);
+  const float t = reciprocal(fmaf(0.35f * 0.7071067811865476f, fabsf(z), 1.f));
+  density = tc::ex2(-0.5f * kLog2E * z * z);
   float q = fmaf(-0.042552598f, t, 0.100604653f);
   q = fmaf(q, t, -0.0072748783f);
   q = fmaf(q, t, 0.0814718946f);
@@ -342,51 +348,58 @@ TAO_DEVI Tile tile_of(const Args& a, const int* first, const int* ends, int t, i
 // Through 2 KB of shared memory, 16-byte chunks of a row turned so that eight rows' meet all banks.
 TAO_DEVI int staged(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1 & 3)) << 4); }
 
-TAO_DEVI void store_rows(uint8_t* staging, void* to, long long stride, int rows, int cols, bool wide, int lane) {
-  uint16_t* const out = static_cast<uint16_t*>(to);
-  if (wide) {
-    const int c = lane & 3;
+// `unit` neighbours at a time (8, 4, 2 or 1: what the rows' addresses allow), all rows on their way.
+template <int U>
+struct Unit;
+template <>
+struct Unit<8> { using Type = uint4; };
+template <>
+struct Unit<4> { using Type = uint2; };
+template <>
+struct Unit<2> { using Type = uint32_t; };
+template <>
+struct Unit<1> { using Type = uint16_t; };
+
+template <int U>
+TAO_DEVI void move_rows(uint8_t* staging, uint16_t* memory, long long stride, int rows, int cols, bool in, int lane) {
+  using W = typename Unit<U>::Type;
+  constexpr int ACROSS = 32 / U;
+  const int c = lane % ACROSS * U, first = lane / ACROSS;
+  memory += first * stride + c;
+  auto at = [&](int r) { return reinterpret_cast<W*>(staging + staged(r, c >> 3) + (c & 7) * 2); };
+  if (in) {
+    W v[ACROSS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      if (r < rows && c * 8 < cols)
-        *reinterpret_cast<uint4*>(out + r * stride + c * 8) = *reinterpret_cast<const uint4*>(staging + staged(r, c));
-    }
+    for (int i = 0; i < ACROSS; ++i)
+      if (i * U + first < rows && c < cols) v[i] = *reinterpret_cast<const W*>(memory + i * U * stride);
+#pragma unroll
+    for (int i = 0; i < ACROSS; ++i)
+      if (i * U + first < rows && c < cols) *at(i * U + first) = v[i];
   } else {
 #pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      if (r < rows && lane < cols)
-        out[r * stride + lane] = *reinterpret_cast<const uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2);
+    for (int i = 0; i < ACROSS; ++i)
+      if (i * U + first < rows && c < cols) *reinterpret_cast<W*>(memory + i * U * stride) = *at(i * U + first);
   }
 }
-TAO_DEVI void fetch_rows(uint8_t* staging, const void* from, long long stride, int rows, int cols, bool wide, int lane) {
-  const uint16_t* const in = static_cast<const uint16_t*>(from);
-  if (wide) {
-    const int c = lane & 3;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      if (r < rows && c * 8 < cols)
-        *reinterpret_cast<uint4*>(staging + staged(r, c)) = *reinterpret_cast<const uint4*>(in + r * stride + c * 8);
-    }
-  } else {
-    uint16_t v[32];  // all on their way
-#pragma unroll
-    for (int r = 0; r < 32; ++r) v[r] = r < rows && lane < cols ? in[r * stride + lane] : (uint16_t)0;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) *reinterpret_cast<uint16_t*>(staging + staged(r, lane >> 3) + (lane & 7) * 2) = v[r];
+TAO_DEVI void move_rows(uint8_t* staging, void* memory, long long stride, int rows, int cols, int unit, bool in, int lane) {
+  uint16_t* const m = static_cast<uint16_t*>(memory);
+  switch (unit) {
+    case 8: return move_rows<8>(staging, m, stride, rows, cols, in, lane);
+    case 4: return move_rows<4>(staging, m, stride, rows, cols, in, lane);
+    case 2: return move_rows<2>(staging, m, stride, rows, cols, in, lane);
   }
+  move_rows<1>(staging, m, stride, rows, cols, in, lane);
 }
 // This thread's row of v, rounded, to memory.  All lanes of the warp.
 TAO_DEVI void put_rows(uint8_t* staging, const float (&v)[32], bool is_bf16, void* to, long long stride, int rows,
-                       int cols, bool wide, int lane) {
+                       int cols, int unit, int lane) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     *reinterpret_cast<uint4*>(staging + staged(lane, c)) =
         make_uint4(pack(v[c * 8], v[c * 8 + 1], is_bf16), pack(v[c * 8 + 2], v[c * 8 + 3], is_bf16),
                    pack(v[c * 8 + 4], v[c * 8 + 5], is_bf16), pack(v[c * 8 + 6], v[c * 8 + 7], is_bf16));
   __syncwarp();
-  store_rows(staging, to, stride, rows, cols, wide, lane);
+  move_rows(staging, to, stride, rows, cols, unit, false, lane);
   __syncwarp();
 }
 
@@ -609,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int k0;
       const int blocks = part(tile, k0);
       const uint32_t acc = tbase + set * C::ACC + lanes;
-      if (blocks) {
+      if (blocks && (SPLIT || FORM == FEW)) {
         if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort))) break;
         fence_after();
       }
@@ -670,6 +683,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rows = tile.rows - quarter * 32;
         uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
         if constexpr (FORM == WEIGHT) y += (long long)tile.group * a.depth * a.cols;
+        const auto bias_of = [&](int c0) {  // of column `lane` of a chunk
+          const int col = tile.col0 + c0 + lane;
+          return FORM == FORWARD && a.bias && c0 < (half + 1) * HALF && col < a.cols ? load1(a.bias, col, is_bf16) : 0.f;
+        };
+        float bias = bias_of(half * HALF);
+        if (blocks) {  // all that is not the sums is on its way before them
+          if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort))) break;
+          fence_after();
+        }
 #pragma unroll 1
         for (int c0 = half * HALF; c0 < (half + 1) * HALF; c0 += 32) {
           const int col = tile.col0 + c0, cols = a.cols - col;
@@ -684,16 +706,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rows <= 0 || cols <= 0) continue;  // the same for the warp
           if constexpr (FORM == FORWARD) {
             if (a.bias) {
-              const float bias = lane < cols ? load1(a.bias, col + lane, is_bf16) : 0.f;
+              const float next = bias_of(c0 + 32);
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bias, i);
+              bias = next;
             }
             if (a.z) {
               put_rows(staging, v, is_bf16, static_cast<uint16_t*>(a.z) + row0 * a.z_stride + col, a.z_stride, rows,
-                       cols, a.wide, lane);
+                       cols, a.unit, lane);
               if constexpr (GATED)
                 put_rows(staging, u, is_bf16, static_cast<uint16_t*>(a.u) + row0 * a.z_stride + col, a.z_stride, rows,
-                         cols, a.wide, lane);
+                         cols, a.unit, lane);
             }
             activate_all(v, a.act);
             if constexpr (GATED) {
@@ -701,8 +724,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 32; ++i) v[i] *= u[i];
             }
             if (a.residual) {
-              fetch_rows(staging, static_cast<const uint16_t*>(a.residual) + row0 * a.r_stride + col, a.r_stride, rows,
-                         cols, a.wide, lane);
+              move_rows(staging, const_cast<uint16_t*>(static_cast<const uint16_t*>(a.residual)) + row0 * a.r_stride + col,
+                        a.r_stride, rows, cols, a.unit, true, lane);
               __syncwarp();
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
@@ -718,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
             }
           }
-          put_rows(staging, v, is_bf16, y + row0 * a.cols + col, a.cols, rows, cols, a.wide, lane);
+          put_rows(staging, v, is_bf16, y + row0 * a.cols + col, a.cols, rows, cols, a.unit, lane);
         }
         if (blocks) {
           fence_before();
@@ -806,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (col + j < a.cols) o[j] = finish<FORM>(a, o[j], row, col + j, is_bf16);
         }
         uint16_t* const out = y + row * a.cols + col;
-        if (a.wide) {
+        if (a.unit >= 4) {
           *reinterpret_cast<uint2*>(out) = make_uint2(pack(o[0], o[1], is_bf16), pack(o[2], o[3], is_bf16));
         } else {
 #pragma unroll

@@ -25,20 +25,44 @@ TAO_DEVI T rounded(float v) {
   else return v;
 }
 
-template <class T, int N>
-struct alignas(sizeof(T) * N) Vec {
+// N values of a row that a thread has: neighbours, read and written at once (WIDE), or `step` apart, one by one, so
+// that a warp's are neighbours.  What lies beyond the width reads as zeros and is not written.
+template <class T, int N, bool WIDE>
+struct alignas(sizeof(T) * N) Part {
   T v[N];
+  TAO_DEVI void load(const T* row, int first, int step, int width) {
+    if constexpr (WIDE) {
+      *this = *reinterpret_cast<const Part*>(row + first);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = first + i * step < width ? row[first + i * step] : rounded<T>(0.f);
+    }
+  }
+  TAO_DEVI void store(T* row, int first, int step, int width) const {
+    if constexpr (WIDE) {
+      *reinterpret_cast<Part*>(row + first) = *this;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (first + i * step < width) row[first + i * step] = v[i];
+    }
+  }
   TAO_DEVI void widen(float (&f)[N]) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = wide_of(v[i]);
   }
-  static TAO_DEVI Vec of(const float (&f)[N]) {
-    Vec r;
+  static TAO_DEVI Part of(const float (&f)[N]) {
+    Part r;
 #pragma unroll
     for (int i = 0; i < N; ++i) r.v[i] = rounded<T>(f[i]);
     return r;
   }
 };
+// The first of thread `x` of `across` in slab `slab` of N x across values.
+template <int N, bool WIDE>
+TAO_DEVI int first_of(int slab, int across, int x) {
+  return WIDE ? (slab * across + x) * N : slab * across * N + x;
+}
 
 // A value of a type known at run time.
 TAO_DEVI float value_of(const void* p, long long i, int type) {
@@ -62,15 +86,17 @@ inline bool on16(const void* p, long long stride, size_t size) {
   return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (long long)size % 16 == 0);
 }
 
-// f(element type, elements of a vector) as compile-time constants.
+// f(element type, values of a thread, whether they are neighbours) as compile-time constants.
 template <class F>
-int by_vector(int type, bool wide, F f) {
-  if (type == TAO_TYPE_FP32) return wide ? f(float(), Int<4>()) : f(float(), Int<1>());
-  if (type == TAO_TYPE_FP16) return wide ? f(__half(), Int<8>()) : f(__half(), Int<1>());
-  return wide ? f(bf16(), Int<8>()) : f(bf16(), Int<1>());
+int by_part(int type, bool wide, F f) {
+  using True = std::true_type;
+  using False = std::false_type;
+  if (type == TAO_TYPE_FP32) return wide ? f(float(), Int<4>(), True()) : f(float(), Int<4>(), False());
+  if (type == TAO_TYPE_FP16) return wide ? f(__half(), Int<8>(), True()) : f(__half(), Int<8>(), False());
+  return wide ? f(bf16(), Int<8>(), True()) : f(bf16(), Int<8>(), False());
 }
 
-// A vector of a row a thread: blocks of `across` x 256 / across threads, and their grid over rows and slabs.
+// A part of a row a thread: blocks of `across` x 256 / across threads, and their grid over rows and slabs.
 struct Mapping {
   dim3 grid, block;
 };

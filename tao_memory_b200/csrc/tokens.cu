@@ -37,40 +37,41 @@ struct TokenArgs {
 TAO_DEVI int kept_of(const TokenArgs& a) { return a.kept ? (int)min((long long)*a.kept, a.pairs) : (int)a.pairs; }
 
 // out[places[t][j]] = in[t], or, WEIGHTED, weights[t][j] in[t] (zeros for a pair that is not kept).
-template <class T, int N, bool WEIGHTED>
+template <class T, int N, bool WIDE, bool WEIGHTED>
 __global__ void __launch_bounds__(256) gather_kernel(const TokenArgs a) {
   const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  const int c = first_of<N, WIDE>(blockIdx.y, blockDim.x, threadIdx.x), step = blockDim.x;
   if (t >= a.tokens || c >= a.width) return;
   const int kept = WEIGHTED ? kept_of(a) : 0;
-  const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + t * a.in_stride + c);
+  Part<T, N, WIDE> v;
+  v.load(static_cast<const T*>(a.in) + t * a.in_stride, c, step, a.width);
 #pragma unroll 4
   for (int j = 0; j < a.k; ++j) {
     const int place = a.places[t * a.k + j];
     if ((unsigned)place >= (unsigned)a.pairs) continue;
-    Vec<T, N>* const to = reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + (long long)place * a.width + c);
+    T* const to = static_cast<T*>(a.out) + (long long)place * a.width;
     if constexpr (WEIGHTED) {
       const float w = a.weights ? value_of(a.weights, t * a.k + j, a.weight_type) : 1.f;
       float f[N];
       v.widen(f);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = place < kept ? f[i] * w : 0.f;
-      *to = Vec<T, N>::of(f);
+      Part<T, N, WIDE>::of(f).store(to, c, step, a.width);
     } else {
-      *to = v;
+      v.store(to, c, step, a.width);
     }
   }
 }
 
 // out[t] = sum over j of weights[t][j] in[places[t][j]]
-template <class T, int N>
+// AT_ONCE: rows on their way; no branch stands between their places and their loads.
+template <class T, int N, bool WIDE, int AT_ONCE>
 __global__ void __launch_bounds__(256) return_kernel(const TokenArgs a) {
   const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  const int c = first_of<N, WIDE>(blockIdx.y, blockDim.x, threadIdx.x), step = blockDim.x;
   if (t >= a.tokens || c >= a.width) return;
   const int kept = kept_of(a);
   float sum[N] = {};
-  constexpr int AT_ONCE = 4;  // rows on their way: no branch stands between their places and their loads
   for (int j0 = 0; j0 < a.k; j0 += AT_ONCE) {
     int place[AT_ONCE];
     float w[AT_ONCE];
@@ -78,11 +79,11 @@ __global__ void __launch_bounds__(256) return_kernel(const TokenArgs a) {
     for (int j = 0; j < AT_ONCE; ++j) place[j] = a.places[t * a.k + min(j0 + j, a.k - 1)];
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) w[j] = a.weights ? value_of(a.weights, t * a.k + min(j0 + j, a.k - 1), a.weight_type) : 1.f;
-    Vec<T, N> v[AT_ONCE];
+    Part<T, N, WIDE> v[AT_ONCE];
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
       const bool in = j0 + j < a.k && (unsigned)place[j] < (unsigned)kept;
-      v[j] = *reinterpret_cast<const Vec<T, N>*>(static_cast<const T*>(a.in) + (in ? place[j] : 0) * a.in_stride + c);
+      v[j].load(static_cast<const T*>(a.in) + (in ? place[j] : 0) * a.in_stride, c, step, a.width);
       place[j] = in;
     }
 #pragma unroll
@@ -93,17 +94,18 @@ __global__ void __launch_bounds__(256) return_kernel(const TokenArgs a) {
       for (int i = 0; i < N; ++i) sum[i] = place[j] ? sum[i] + w[j] * f[i] : sum[i];
     }
   }
-  *reinterpret_cast<Vec<T, N>*>(static_cast<T*>(a.out) + t * a.width + c) = Vec<T, N>::of(sum);
+  Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + t * a.width, c, step, a.width);
 }
 
-// dw[t][j] = in[t] . other[places[t][j]], zero for a pair that is not kept.  A warp a token, four experts' rows on
-// their way at once.  (In one kernel with the rows' gradient, which writes as much as this reads, the two took 115 to
-// 156 us for 32768 tokens of 768 channels and 4 experts.)
-template <class T, int N>
+// dw[t][j] = in[t] . other[places[t][j]], zero for a pair that is not kept.  WARPS a token (one, or where that leaves the
+// device empty eight, whose sums are added in their order), AT_ONCE experts' rows on their way at once.  (In one
+// kernel with the rows' gradient, which writes as much as this reads, the two took 115 to 156 us for 32768 tokens of 768
+// channels and 4 experts.)
+template <class T, int N, bool WIDE, int AT_ONCE, int WARPS>
 __global__ void __launch_bounds__(256) weight_gradient_kernel(const TokenArgs a) {
-  constexpr int AT_ONCE = 4;
-  const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  __shared__ float parts[AT_ONCE][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = WARPS == 1 ? (long long)blockIdx.x * 8 + warp : (long long)blockIdx.x;
   if (t >= a.tokens) return;
   const int kept = kept_of(a);
   const T* const dy = static_cast<const T*>(a.in) + t * a.in_stride;
@@ -118,12 +120,13 @@ __global__ void __launch_bounds__(256) weight_gradient_kernel(const TokenArgs a)
       rows[j] = static_cast<const T*>(a.other) + (in[j] ? place : 0) * a.other_stride;
     }
 #pragma unroll 2
-    for (int c = lane * N; c < a.width; c += 32 * N) {
-      Vec<T, N> v[AT_ONCE];
+    for (int c = first_of<N, WIDE>(WARPS == 1 ? 0 : warp, 32, lane); c < a.width; c += WARPS * 32 * N) {
+      Part<T, N, WIDE> v[AT_ONCE], y;
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) v[j] = *reinterpret_cast<const Vec<T, N>*>(rows[j] + c);
+      for (int j = 0; j < AT_ONCE; ++j) v[j].load(rows[j], c, 32, a.width);
       float d[N], f[N];
-      reinterpret_cast<const Vec<T, N>*>(dy + c)->widen(d);
+      y.load(dy, c, 32, a.width);
+      y.widen(d);
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
         v[j].widen(f);
@@ -133,10 +136,26 @@ __global__ void __launch_bounds__(256) weight_gradient_kernel(const TokenArgs a)
     }
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
-      const float s = warp_sum(dot[j]);
-      if (lane == 0 && j0 + j < a.k) set_value(a.dw, t * a.k + j0 + j, in[j] ? s : 0.f, a.weight_type);
+      float s = warp_sum(dot[j]);
+      if constexpr (WARPS > 1) {
+        if (lane == 0) parts[j][warp] = s;
+        __syncthreads();
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) s += parts[j][w];
+      }
+      if (lane == 0 && (WARPS == 1 || warp == 0) && j0 + j < a.k)
+        set_value(a.dw, t * a.k + j0 + j, in[j] ? s : 0.f, a.weight_type);
     }
+    if constexpr (WARPS > 1) __syncthreads();
   }
+}
+template <class T, int N, bool WIDE, int AT_ONCE>
+void start_weight_gradient(const TokenArgs& a, cudaStream_t s) {
+  if (a.tokens <= 148 * 8)
+    weight_gradient_kernel<T, N, WIDE, AT_ONCE, 8><<<(unsigned)a.tokens, 256, 0, s>>>(a);
+  else
+    weight_gradient_kernel<T, N, WIDE, AT_ONCE, 1><<<(unsigned)((a.tokens + 7) / 8), 256, 0, s>>>(a);
 }
 
 int check(const TokenArgs& a, int type) {
@@ -193,9 +212,9 @@ int tao_gather_tokens(const void* x, long long x_stride, const int* places, long
   if (!x || !places || !xs) return tfail(TAO_ERR_ARG, "null pointer");
   if (!on_elements({{x, size}, {xs, size}, {places, 4}})) return tfail(TAO_ERR_ARG, "operands start on a whole element");
   const bool wide = width * size % 16 == 0 && on16(x, x_stride, size) && on16(xs, 0, size);
-  return by_vector(type, wide, [&](auto t, auto n) {
+  return by_part(type, wide, [&](auto t, auto n, auto w) {
     const Mapping m = mapping(tokens, (width + decltype(n)::value - 1) / decltype(n)::value);
-    gather_kernel<decltype(t), decltype(n)::value, false><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    gather_kernel<decltype(t), decltype(n)::value, decltype(w)::value, false><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
     return launched();
   });
 }
@@ -214,9 +233,18 @@ int tao_return_tokens(const void* ys, long long ys_stride, const int* places, co
   if (!on_elements({{ys, size}, {y, size}, {places, 4}, {kept, 4}, {weights, weights ? size_of(weight_type) : 1}}))
     return tfail(TAO_ERR_ARG, "operands start on a whole element");
   const bool wide = width * size % 16 == 0 && on16(ys, ys_stride, size) && on16(y, 0, size);
-  return by_vector(type, wide, [&](auto t, auto n) {
+  return by_part(type, wide, [&](auto t, auto n, auto w) {
     const Mapping m = mapping(tokens, (width + decltype(n)::value - 1) / decltype(n)::value);
-    return_kernel<decltype(t), decltype(n)::value><<<m.grid, m.block, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    using T = decltype(t);
+    constexpr int N = decltype(n)::value;
+    constexpr bool WIDE = decltype(w)::value;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (top_k == 1)
+      return_kernel<T, N, WIDE, 1><<<m.grid, m.block, 0, s>>>(a);
+    else if (top_k == 2)
+      return_kernel<T, N, WIDE, 2><<<m.grid, m.block, 0, s>>>(a);
+    else
+      return_kernel<T, N, WIDE, 4><<<m.grid, m.block, 0, s>>>(a);
     return launched();
   });
 }
@@ -237,13 +265,19 @@ int tao_return_tokens_gradient(const void* dy, long long dy_stride, const void* 
   if (!on_elements({{dy, size}, {ys, size}, {dys, size}, {places, 4}, {kept, 4}, {weights, weight_size}, {dw, weight_size}}))
     return tfail(TAO_ERR_ARG, "operands start on a whole element");
   const bool wide = width * size % 16 == 0 && on16(dy, dy_stride, size) && on16(ys, ys_stride, size) && on16(dys, 0, size);
-  return by_vector(type, wide, [&](auto t, auto n) {
+  return by_part(type, wide, [&](auto t, auto n, auto w) {
     using T = decltype(t);
     constexpr int N = decltype(n)::value;
+    constexpr bool WIDE = decltype(w)::value;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const Mapping m = mapping(tokens, (width + N - 1) / N);
-    if (dys) gather_kernel<T, N, true><<<m.grid, m.block, 0, s>>>(a);
-    if (dw) weight_gradient_kernel<T, N><<<(unsigned)((tokens + 7) / 8), 256, 0, s>>>(a);
+    if (dys) gather_kernel<T, N, WIDE, true><<<m.grid, m.block, 0, s>>>(a);
+    if (dw && top_k == 1)
+      start_weight_gradient<T, N, WIDE, 1>(a, s);
+    else if (dw && top_k == 2)
+      start_weight_gradient<T, N, WIDE, 2>(a, s);
+    else if (dw)
+      start_weight_gradient<T, N, WIDE, 4>(a, s);
     return launched();
   });
 }
