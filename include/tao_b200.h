@@ -561,7 +561,7 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
  * x, W and U of any strides: what does not lie with neighbours next to each other and everything else on 16 bytes
  * is copied into the workspace first (tao_linear_workspace_bytes of the same structure, on 256 bytes; each
  * call's own until it is over).  y, dx, dw, dup are contiguous; y may be the residual (r_row n), outputs must not
- * overlap operands otherwise.  Up to 512 experts, 2^30 rows, n and k 2^24. */
+ * overlap operands, or one another, otherwise (TAO_ERR_ARG; by all that an operand's strides reach over).  Up to 512 experts, 2^30 rows, n and k 2^24. */
 typedef struct TaoLinear {
   const void *x, *w, *up, *bias, *residual;
   const int* offsets;
@@ -596,7 +596,8 @@ int tao_gather_tokens(const void* x, long long x_stride, const int* places, long
 int tao_return_tokens(const void* ys, long long ys_stride, const int* places, const int* kept, const void* weights,
                       int weight_type, long long tokens, int top_k, int width, int type, void* y, void* stream);
 /* Its gradient: dys[places[t][j]] = weights[t][j] dy[t], dw[t][j] = dy[t] . ys[places[t][j]] (either may be NULL; dw
- * needs ys and weights), zeros for pairs that do not count. */
+ * needs ys and weights), zeros for pairs that do not count.  Outputs of these four must not overlap their operands
+ * (TAO_ERR_ARG); rows have up to 2^20 channels. */
 int tao_return_tokens_gradient(const void* dy, long long dy_stride, const void* ys, long long ys_stride, const int* places,
                                const int* kept, const void* weights, int weight_type, long long tokens, int top_k,
                                int width, int type, void* dys, void* dw, void* stream);
@@ -606,7 +607,8 @@ int tao_return_tokens_gradient(const void* dy, long long dy_stride, const void* 
 int tao_embed(const void* ids, int id_bytes, long long n, const void* table, long long stride, long long vocab, int width,
               int type, float scale, void* y, void* stream);
 /* dtable [vocab][width] = scale * the sum of dy over the tokens of each id, in fp32 in a fixed order, rounded once.
- * workspace: tao_embed_gradient_workspace_bytes, on 16 bytes.  Up to 2^26 rows. */
+ * workspace: tao_embed_gradient_workspace_bytes, on 16 bytes.  Up to 2^26 rows of up to 2^20 channels.  Outputs must
+ * not overlap operands (TAO_ERR_ARG). */
 size_t tao_embed_gradient_workspace_bytes(long long n, long long vocab, int width);
 int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* dy, long long dy_stride, long long vocab,
                        int width, int type, float scale, void* dtable, void* workspace, size_t workspace_bytes,

@@ -74,6 +74,26 @@ inline bool rows_overlap(const void* x, long long rows, long long stride, long l
   return first < rows && first * stride < at + size;
 }
 
+// What an operand reaches over in memory: `rows` of `bytes` bytes, `stride` bytes apart (and `count` such matrices,
+// `matrix` bytes apart).
+struct Extent {
+  uintptr_t begin, end;
+};
+inline Extent extent(const void* p, long long rows, long long stride, long long bytes, long long count = 1,
+                     long long matrix = 0) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  if (!p || rows < 1 || count < 1) return {0, 0};
+  const long long down = (rows - 1) * stride, on = (count - 1) * matrix;
+  return {at + (down < 0 ? down : 0) + (on < 0 ? on : 0), at + (down > 0 ? down : 0) + (on > 0 ? on : 0) + bytes};
+}
+// Whether an output (contiguous, `bytes` from `out` on) shares memory with what any operand reaches over.
+inline bool overlaps(const void* out, long long bytes, std::initializer_list<Extent> operands) {
+  const Extent o = extent(out, 1, 0, bytes);
+  for (const Extent& e : operands)
+    if (out && e.begin < o.end && o.begin < e.end) return true;
+  return false;
+}
+
 // Products of two bf16 pairs rounded to bf16, lane by lane.  The product of two
 // bf16 values is exact in fp32, so this equals rb(a * b) for each lane.
 TAO_DEVI uint32_t hmul2u(uint32_t a, uint32_t b) {

@@ -223,8 +223,8 @@ Room room_of(long long n, long long vocab, int width) {
 int check(int id_bytes, long long n, long long vocab, int width, int type) {
   if (id_bytes != 4 && id_bytes != 8) return efail(TAO_ERR_ARG, "ids have 32 or 64 bits");
   if (!known(type)) return efail(TAO_ERR_ARG, "a table is bf16, fp16 or fp32");
-  if (n < 0 || n > (1ll << 30) || vocab < 1 || vocab > (1ll << 26) || width < 1 || width > (1 << 24))
-    return efail(TAO_ERR_ARG, "there are up to 2^30 ids and 1 to 2^26 rows of 1 to 2^24 channels");
+  if (n < 0 || n > (1ll << 30) || vocab < 1 || vocab > (1ll << 26) || width < 1 || width > (1 << 20))
+    return efail(TAO_ERR_ARG, "there are up to 2^30 ids and 1 to 2^26 rows of 1 to 2^20 channels");
   return TAO_OK;
 }
 
@@ -242,6 +242,8 @@ int tao_embed(const void* ids, int id_bytes, long long n, const void* table, lon
   if (!ids || !table || !y) return efail(TAO_ERR_ARG, "null pointer");
   if (!on_elements({{ids, (size_t)id_bytes}, {table, size}, {y, size}}))
     return efail(TAO_ERR_ARG, "operands start on a whole element");
+  if (overlaps(y, n * width * size, {extent(table, vocab, stride * size, width * size), extent(ids, 1, 0, n * id_bytes)}))
+    return efail(TAO_ERR_ARG, "embedded rows must not overlap the table or the ids");
   const EmbedArgs a = {ids, n, vocab, stride, width, id_bytes == 8, scale, table, y};
   const bool wide = width * size % 16 == 0 && on16(table, stride, size) && on16(y, 0, size);
   return by_part(type, wide, [&](auto t, auto v, auto w) {
@@ -277,6 +279,8 @@ int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* d
         workspace_bytes < tao_embed_gradient_workspace_bytes(n, vocab, width))
       return efail(TAO_ERR_ARG, "workspace too small for the embedding's gradient, or off 16 bytes");
   }
+  if (overlaps(dtable, vocab * width * size, {extent(dy, n, dy_stride * size, width * size), extent(ids, 1, 0, n * id_bytes)}))
+    return efail(TAO_ERR_ARG, "the table's gradient must not overlap the rows' or the ids");
   cudaError_t e = cudaMemsetAsync(dtable, 0, (size_t)vocab * width * size, s);
   if (e != cudaSuccess || n == 0) return launched(e);
   const Room r = room_of(n, vocab, width);

@@ -210,7 +210,7 @@ bool few_rows(const FewArgs& a, int type, cudaStream_t s, int* rc) {
                          : start_few<1, 8, 8>(a, type, s);
   else if (a.rows <= 16)
     *rc = narrow ? start_few<2, 16, 4>(a, type, s) : start_few<2, 8, 2>(a, type, s);
-  else if (outputs > 512)
+  else if (outputs >= 448)
     return false;
   else
     *rc = outputs <= 148 ? start_few<4, 16, 2>(a, type, s) : start_few<4, 8, 1>(a, type, s);
@@ -510,6 +510,31 @@ int check(const TaoLinear* p) {
   return TAO_OK;
 }
 
+Extent reach(const Given& g) {
+  if (!g.at) return {0, 0};
+  const long long across = (g.cols - 1) * g.col * 2;  // strides are not negative where they come from tensors
+  return extent(g.at, g.rows, g.row * 2, across + 2, g.count, g.matrix * 2);
+}
+bool any_overlap(const TaoLinear& p, bool gradient) {
+  const long long rows = p.rows, n = p.n, k = p.k, y = rows * n * 2, w = (long long)p.experts * n * k * 2;
+  const long long kept = ((rows - 1) * p.z_row + n) * 2;
+  const Extent x = reach(given_x(p)), weight = reach(given_w(p)), up = reach(given_up(p)), z = extent(p.z, 1, 0, kept),
+               u = extent(p.u, 1, 0, kept), offsets = extent(p.offsets, 1, 0, (p.experts + 1) * 4ll);
+  if (!gradient) {
+    const Extent bias = extent(p.bias, 1, 0, n * 2), residual = extent(p.residual, rows, p.r_row * 2, n * 2);
+    const bool in_place = p.residual == p.y && (p.r_row == n || rows == 1);
+    return overlaps(p.y, y, {x, weight, up, bias, in_place ? Extent{0, 0} : residual, z, p.z ? u : Extent{0, 0}, offsets}) ||
+           overlaps(p.z, kept, {x, weight, up, bias, residual, u, offsets}) ||
+           (p.z && overlaps(p.u, kept, {x, weight, up, offsets}));
+  }
+  const Extent dy = extent(p.dy, rows, p.dy_row * 2, n * 2), dx = extent(p.dx, 1, 0, rows * k * 2), dw = extent(p.dw, 1, 0, w),
+               dup = extent(p.dup, 1, 0, w);
+  return overlaps(p.dx, rows * k * 2, {x, weight, up, z, u, offsets, dy, dw, dup}) ||
+         overlaps(p.dw, w, {x, weight, up, z, u, offsets, dy, dup}) ||
+         overlaps(p.dup, w, {x, weight, up, z, u, offsets, dy}) ||
+         overlaps(p.db, n * 2, {x, weight, up, z, u, offsets, dy, dx, dw, dup});
+}
+
 int check_room(const TaoLinear& p, size_t need) {
   if (need && (!p.workspace || reinterpret_cast<uintptr_t>(p.workspace) % 256 || p.workspace_bytes < need))
     return pfail(TAO_ERR_ARG, "the products' workspace is too small, or off 256 bytes");
@@ -678,6 +703,7 @@ int tao_linear(const TaoLinear* p, void* stream) {
   if (int rc = check(p)) return rc;
   if (p->rows == 0) return TAO_OK;
   if (missing(*p, false)) return pfail(TAO_ERR_ARG, "null pointer");
+  if (any_overlap(*p, false)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 0))) return rc;
   static uint8_t none[1];  // where no room is needed
   Rooms rooms = {p->workspace ? static_cast<uint8_t*>(p->workspace) : none, 0};
@@ -697,6 +723,7 @@ int tao_linear_gradient(const TaoLinear* p, void* stream) {
     return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
   }
   if (missing(*p, true)) return pfail(TAO_ERR_ARG, "null pointer");
+  if (any_overlap(*p, true)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 1))) return rc;
   static uint8_t none[1];
   Rooms rooms = {p->workspace ? static_cast<uint8_t*>(p->workspace) : none, 0};

@@ -28,9 +28,10 @@ TAO_DEVI uint4 terms(const uint16_t* row, int k, int depth) {
     asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + k));
     return v;
   }
+  if (k >= depth) return make_uint4(0, 0, 0, 0);
   uint32_t w[4] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 7; ++i)
     if (k + i < depth) w[i / 2] |= (uint32_t)row[k + i] << (16 * (i & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }

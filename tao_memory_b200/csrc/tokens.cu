@@ -162,8 +162,8 @@ int check(const TokenArgs& a, int type) {
   if (!known(type)) return tfail(TAO_ERR_ARG, "tokens are bf16, fp16 or fp32");
   if (a.weights && a.weight_type != TAO_TYPE_FP32 && a.weight_type != type)
     return tfail(TAO_ERR_ARG, "weights are fp32 or of the rows' type");
-  if (a.tokens < 0 || a.k < 1 || a.width < 1 || a.k > (1 << 20) || a.width > (1 << 24) || a.tokens > (1ll << 30) / a.k)
-    return tfail(TAO_ERR_ARG, "a token has at least one choice and one channel, and there are up to 2^30 pairs");
+  if (a.tokens < 0 || a.k < 1 || a.width < 1 || a.k > (1 << 20) || a.width > (1 << 20) || a.tokens > (1ll << 30) / a.k)
+    return tfail(TAO_ERR_ARG, "a token has at least one choice and 1 to 2^20 channels, and there are up to 2^30 pairs");
   return TAO_OK;
 }
 
@@ -191,6 +191,10 @@ int tao_sort_tokens(const void* ids, int id_bytes, long long pairs, int experts,
     return e == cudaSuccess ? TAO_OK : tfail(TAO_ERR_CUDA, cudaGetErrorString(e));
   }
   if (!ids || !sorted || !places) return tfail(TAO_ERR_ARG, "null pointer");
+  const Extent id = extent(ids, 1, 0, pairs * id_bytes), by = extent(sorted, 1, 0, pairs * 4), at = extent(places, 1, 0, pairs * 4);
+  if (overlaps(sorted, pairs * 4, {id, at}) || overlaps(places, pairs * 4, {id}) ||
+      overlaps(offsets, (experts + 1) * 4ll, {id, by, at}))
+    return tfail(TAO_ERR_ARG, "an order's parts must not overlap each other or the ids");
   const size_t need = tao_sort_tokens_workspace_bytes(pairs, experts);
   if (need && (!workspace || workspace_bytes < need)) return tfail(TAO_ERR_ARG, "workspace too small for the sort");
   sorting::Pass p = {};
@@ -211,6 +215,8 @@ int tao_gather_tokens(const void* x, long long x_stride, const int* places, long
   const size_t size = size_of(type);
   if (!x || !places || !xs) return tfail(TAO_ERR_ARG, "null pointer");
   if (!on_elements({{x, size}, {xs, size}, {places, 4}})) return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  if (overlaps(xs, a.pairs * width * size, {extent(x, tokens, x_stride * size, width * size), extent(places, 1, 0, a.pairs * 4)}))
+    return tfail(TAO_ERR_ARG, "gathered rows must not overlap what they are gathered from");
   const bool wide = width * size % 16 == 0 && on16(x, x_stride, size) && on16(xs, 0, size);
   return by_part(type, wide, [&](auto t, auto n, auto w) {
     const Mapping m = mapping(tokens, (width + decltype(n)::value - 1) / decltype(n)::value);
@@ -232,6 +238,9 @@ int tao_return_tokens(const void* ys, long long ys_stride, const int* places, co
   if (!ys || !places || !y) return tfail(TAO_ERR_ARG, "null pointer");
   if (!on_elements({{ys, size}, {y, size}, {places, 4}, {kept, 4}, {weights, weights ? size_of(weight_type) : 1}}))
     return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  if (overlaps(y, tokens * width * size, {extent(ys, a.pairs, ys_stride * size, width * size), extent(places, 1, 0, a.pairs * 4),
+                                          extent(kept, 1, 0, 4), extent(weights, 1, 0, a.pairs * size_of(weight_type))}))
+    return tfail(TAO_ERR_ARG, "returned rows must not overlap what they are made of");
   const bool wide = width * size % 16 == 0 && on16(ys, ys_stride, size) && on16(y, 0, size);
   return by_part(type, wide, [&](auto t, auto n, auto w) {
     const Mapping m = mapping(tokens, (width + decltype(n)::value - 1) / decltype(n)::value);
@@ -264,6 +273,13 @@ int tao_return_tokens_gradient(const void* dy, long long dy_stride, const void* 
   const size_t weight_size = weights ? size_of(weight_type) : 1;
   if (!on_elements({{dy, size}, {ys, size}, {dys, size}, {places, 4}, {kept, 4}, {weights, weight_size}, {dw, weight_size}}))
     return tfail(TAO_ERR_ARG, "operands start on a whole element");
+  const long long out = a.pairs * width * size;
+  const Extent from = extent(dy, tokens, dy_stride * size, width * size), rows_of = extent(ys, a.pairs, ys_stride * size, width * size),
+               at = extent(places, 1, 0, a.pairs * 4), number = extent(kept, 1, 0, 4),
+               by = extent(weights, 1, 0, a.pairs * (long long)weight_size);
+  if (overlaps(dys, out, {from, rows_of, at, number, by}) ||
+      overlaps(dw, a.pairs * (long long)weight_size, {from, rows_of, at, number, by, extent(dys, 1, 0, out)}))
+    return tfail(TAO_ERR_ARG, "gradients must not overlap what they are made of");
   const bool wide = width * size % 16 == 0 && on16(dy, dy_stride, size) && on16(ys, ys_stride, size) && on16(dys, 0, size);
   return by_part(type, wide, [&](auto t, auto n, auto w) {
     using T = decltype(t);

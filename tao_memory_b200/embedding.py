@@ -5,7 +5,7 @@ import torch
 from . import _lib
 from .norm import TYPES, _rows, refuse_tangents, wants_gradient
 
-MOST_ROWS = 1 << 26
+MOST_ROWS, MOST_CHANNELS = 1 << 26, 1 << 20
 
 
 def _forward(ids, table, scale):
@@ -48,8 +48,8 @@ def embed(ids, table, scale=1.0):
     row's sum in fp32 in the order of the tokens, in runs of 32 of the sorted tokens, rounded once."""
     if table.dtype not in TYPES or not table.is_cuda or table.dim() != 2 or 0 in table.shape:
         raise ValueError("embed takes a bf16, fp16 or fp32 CUDA table [vocab, width] (no CPU fallback)")
-    if table.shape[0] > MOST_ROWS:
-        raise ValueError("a table has up to 2^26 rows")
+    if table.shape[0] > MOST_ROWS or table.shape[1] > MOST_CHANNELS:
+        raise ValueError("a table has up to 2^26 rows of up to 2^20 channels")
     if ids.dtype not in (torch.int32, torch.int64) or ids.device != table.device:
         raise ValueError("ids are an int32 or int64 tensor on the table's device")
     scale = float(scale)

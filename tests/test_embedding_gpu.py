@@ -86,6 +86,18 @@ def test_ids_that_are_none():
     assert (y[[0, 1, 2, 3, 5]] == 0).all() and torch.equal(y[4], table[9])
 
 
+def test_refusals():
+    from tao_memory_b200 import embed
+    table, ids = torch.randn(10, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    for bad in (lambda: embed(ids.float(), table), lambda: embed(ids.cpu(), table), lambda: embed(ids, table.double()),
+                lambda: embed(ids, table[0]), lambda: embed(ids, table[:0]), lambda: embed(ids.to(torch.int16), table)):
+        with pytest.raises(ValueError):
+            bad()
+    y = embed(ids, table.requires_grad_(True))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), table, create_graph=True)
+
+
 def test_same_result_again_captured_and_on_other_streams():
     from tao_memory_b200 import embed
     g = torch.Generator(device="cuda").manual_seed(4)

@@ -204,6 +204,21 @@ def test_gradient_has_no_gradient():
         torch.autograd.grad(y.sum(), x, create_graph=True)
 
 
+def test_refusals():
+    from tao_memory_b200 import linear
+    x, w, b, res, _ = _inputs(6, 64, 32, torch.bfloat16, True, True)
+    for bad in (lambda: linear(x.float(), w.float()), lambda: linear(x, w.half()), lambda: linear(x[:, :60], w),
+                lambda: linear(x, w[None]), lambda: linear(x, w, bias=b[:31]), lambda: linear(x, w, bias=b.float()),
+                lambda: linear(x, w, residual=res[:5]), lambda: linear(x, w, residual=res.half()),
+                lambda: linear(x, w, activation="tanh"), lambda: linear(x, w.cpu()), lambda: linear(x[:, :0], w[:, :0])):
+        with pytest.raises(ValueError):
+            bad()
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        with pytest.raises(ValueError):
+            linear(fwd.make_dual(x, x), w)
+
+
 def test_no_wait_ran_out():
     from tao_memory_b200.stream import check_device
     assert check_device() == 0

@@ -125,6 +125,52 @@ def test_pairs_of_no_expert_do_not_count():
     assert (dys[int(order.offsets[-1]):] == 0).all()
 
 
+def test_orders_made_elsewhere_and_what_is_refused():
+    """An order of a caller's own (places outside of the pairs are passed over), and the Python calls' refusals."""
+    from tao_memory_b200 import TokenOrder, expert_linear, gather_tokens, return_tokens, sort_tokens
+    ids = _ids(50, 3, 7)
+    made = sort_tokens(ids, 7)
+    order = TokenOrder(made.pairs, made.places.clone(), made.offsets)
+    order.places[3, 1], order.places[4, 0] = -5, 2 ** 31 - 1
+    ys = torch.randn(150, 40, device="cuda")
+    full, part = return_tokens(ys, made), return_tokens(ys, order)
+    keep = torch.ones(50, dtype=torch.bool, device="cuda")
+    keep[3] = keep[4] = False
+    assert torch.equal(full[keep], part[keep]) and not torch.equal(full[3], part[3])
+    x = torch.randn(50, 40, device="cuda")
+    same = gather_tokens(x, order) == gather_tokens(x, made)
+    missed = made.places[[3, 4], [1, 0]].long()
+    same[missed] = True
+    assert same.all()
+    w, offsets = torch.randn(7, 8, 40, device="cuda").bfloat16(), made.offsets
+    rows = ys.bfloat16()
+    for bad in (lambda: sort_tokens(ids.float(), 7), lambda: sort_tokens(ids[0], 7), lambda: sort_tokens(ids, 0),
+                lambda: sort_tokens(ids, 513), lambda: sort_tokens(ids[:, :0], 7), lambda: gather_tokens(x[:49], made),
+                lambda: gather_tokens(x.double(), made), lambda: gather_tokens(x, made.places), lambda: return_tokens(x, made),
+                lambda: return_tokens(ys, made, torch.ones(50, 2, device="cuda")),
+                lambda: return_tokens(ys, made, torch.ones(50, 3, device="cuda").half()),
+                lambda: return_tokens(ys, made, torch.ones(50, 3)), lambda: return_tokens(ys[:, :0], made),
+                lambda: TokenOrder(made.pairs, made.places.long(), offsets), lambda: TokenOrder(made.pairs, made.places.T, offsets),
+                lambda: TokenOrder(made.pairs[:9], made.places, offsets),
+                lambda: expert_linear(rows, w, offsets.long()), lambda: expert_linear(rows, w, offsets[1:]),
+                lambda: expert_linear(rows, w[0], offsets), lambda: expert_linear(rows, w.half(), offsets),
+                lambda: expert_linear(rows[:, 1:], w, offsets), lambda: expert_linear(rows, w, offsets, up=w[:, 1:]),
+                lambda: expert_linear(rows, w, offsets, activation="tanh"), lambda: expert_linear(ys, w.float(), offsets),
+                lambda: expert_linear(rows[None], w, offsets)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_what_was_saved_is_not_changed_in_between():
+    from tao_memory_b200 import return_tokens, sort_tokens
+    order = sort_tokens(_ids(20, 2, 4), 4)
+    ys = torch.randn(40, 8, device="cuda", requires_grad=True)
+    y = return_tokens(ys, order, torch.ones(20, 2, device="cuda"))
+    order.places.add_(0)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
 # -- the experts' products ----------------------------------------------------
 def _check_experts(x, w, up, offsets, name, dy, grad=True):
     from tao_memory_b200 import expert_linear
