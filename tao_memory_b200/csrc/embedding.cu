@@ -4,7 +4,7 @@
 // Gradient: the tokens are sorted by id (sort.cuh, stably), and a block adds the rows of a run of kRun sorted
 // tokens, in fp32 and in their order, a sum for each id.  An id whose tokens lie within the run is written at
 // once; the sums of one that goes on in the next run are joined by a second kernel, in the runs' order, so a word
-// that comes 10000 times is added by 313 blocks and the result does not depend on when they ran.  Rows of no
+// that comes 10000 times is added by 625 blocks and the result does not depend on when they ran.  Rows of no
 // token are zeros.
 #include <cuda_runtime.h>
 
@@ -18,7 +18,7 @@ namespace {
 
 using namespace rows;
 
-constexpr int kRun = 32;
+constexpr int kRun = 16;
 
 int efail(int code, const char* msg) {
   tao_set_last_error(msg);
@@ -118,38 +118,31 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
   const int c = first_of<N, WIDE>(blockIdx.y, blockDim.x, threadIdx.x), step = blockDim.x;
   if (c >= a.width) return;
   float sum[N] = {};
-  constexpr int AHEAD = 8;  // rows on their way
-  Part<T, N, WIDE> v[AHEAD];
-  auto fetch = [&](Part<T, N, WIDE>& to, int i) {
-    to.load(static_cast<const T*>(a.dy) + tokens[min(i, count - 1)] * a.dy_stride, c, step, a.width);
-  };
+  Part<T, N, WIDE> v[kRun];  // all rows on their way
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) fetch(v[i], i);
-  for (int i0 = 0; i0 < count; i0 += AHEAD) {
+  for (int i = 0; i < kRun; ++i)
+    v[i].load(static_cast<const T*>(a.dy) + tokens[min(i, count - 1)] * a.dy_stride, c, step, a.width);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      if (i0 + i >= count) break;
-      const int id = ids[i0 + i + 1], next = ids[i0 + i + 2];
-      float f[N];
-      v[i].widen(f);
-      fetch(v[i], i0 + i + AHEAD);
+  for (int i = 0; i < kRun; ++i) {
+    if (i >= count) break;
+    const int id = ids[i + 1], next = ids[i + 2];
+    float f[N];
+    v[i].widen(f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] += f[e];
-      const bool last = i0 + i == count - 1;
-      if (id == next && !last) continue;
-      if (id < a.vocab) {
-        const bool older = id == ids[0];  // sorted: all from the run's first on
-        if (older || id == next) {
-          put_sums<N, WIDE>(a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width, c, step, a.width, sum);
-        } else {
+    for (int e = 0; e < N; ++e) sum[e] += f[e];
+    if (id == next && i < count - 1) continue;
+    if (id < a.vocab) {
+      const bool older = id == ids[0];  // sorted: all from the run's first on
+      if (older || id == next) {
+        put_sums<N, WIDE>(a.parts + ((long long)blockIdx.x * 2 + (older ? 0 : 1)) * a.width, c, step, a.width, sum);
+      } else {
 #pragma unroll
-          for (int e = 0; e < N; ++e) sum[e] *= a.scale;
-          Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, step, a.width);
-        }
+        for (int e = 0; e < N; ++e) sum[e] *= a.scale;
+        Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, step, a.width);
       }
-#pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] = 0.f;
     }
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = 0.f;
   }
 }
 

@@ -83,7 +83,7 @@ int clusters_of(int split) {
   if (device < 16)
     if (const int n = known[device][split].load(std::memory_order_relaxed)) return n;
   using C = Cfg<FORM, BN, false, true>;
-  auto kernel = product_kernel<FORM, BN, false, true, true>;
+  auto kernel = product_kernel<FORM, BN, false, true, false, true>;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(split);
   c.blockDim = dim3(kThreads);
@@ -104,12 +104,12 @@ int clusters_of(int split) {
   return n;
 }
 
-template <int FORM, int BN, bool GATED, bool SPLIT, bool BF16>
+template <int FORM, int BN, bool GATED, bool SPLIT, bool PAIR, bool BF16>
 int start_typed(const Operands& o, Args a, int split, cudaStream_t stream) {
-  using C = Cfg<FORM, BN, GATED, SPLIT>;
-  auto kernel = product_kernel<FORM, BN, GATED, SPLIT, BF16>;
+  using C = Cfg<FORM, BN, GATED, SPLIT, PAIR>;
+  auto kernel = product_kernel<FORM, BN, GATED, SPLIT, PAIR, BF16>;
   CUtensorMap maps[4];
-  constexpr int A_BOX = C::A_MN ? kTerms : 128, B_BOX = C::B_MN ? kTerms : FORM == FORWARD ? C::CT : BN;
+  constexpr int A_BOX = C::A_MN ? kTerms : 128, B_BOX = C::B_MN ? kTerms : PAIR ? 128 : FORM == FORWARD ? C::CT : BN;
   const Operand2* ops[4] = {&o.a, &o.b, &o.a2, &o.b2};
   for (int i = 0; i < 4; ++i) {
     if (!ops[i]->at)
@@ -135,24 +135,25 @@ int start_typed(const Operands& o, Args a, int split, cudaStream_t stream) {
   if (tiles > (1 << 29)) return pfail(TAO_ERR_CAPACITY, "the product has too many tiles");
   a.split = split;
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3((unsigned)(SPLIT ? tiles * split : std::min<long long>(tiles, sms())));
+  const int together = SPLIT ? split : PAIR ? 2 : 1;  // blocks of a cluster
+  c.gridDim = dim3((unsigned)(together * (SPLIT ? tiles : std::min<long long>(tiles, sms() / together))));
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = C::SMEM;
   c.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.x = together;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   c.attrs = attr;
-  c.numAttrs = SPLIT ? 1 : 0;
+  c.numAttrs = SPLIT || PAIR ? 1 : 0;
   e = cudaLaunchKernelEx(&c, kernel, maps[0], maps[1], maps[2], maps[3], a);
   return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
 }
 
-template <int FORM, int BN, bool GATED, bool SPLIT>
+template <int FORM, int BN, bool GATED, bool SPLIT, bool PAIR = false>
 int start(const Operands& o, const Args& a, int split, cudaStream_t stream) {
-  return a.type == TAO_TYPE_BF16 ? start_typed<FORM, BN, GATED, SPLIT, true>(o, a, split, stream)
-                                 : start_typed<FORM, BN, GATED, SPLIT, false>(o, a, split, stream);
+  return a.type == TAO_TYPE_BF16 ? start_typed<FORM, BN, GATED, SPLIT, PAIR, true>(o, a, split, stream)
+                                 : start_typed<FORM, BN, GATED, SPLIT, PAIR, false>(o, a, split, stream);
 }
 
 // Blocks that share a tile's terms, and what it takes in steps of the ring: rounds of all clusters, each of its
@@ -172,20 +173,36 @@ Split split_of(long long tiles, int steps, double join) {
   return best;
 }
 
-// FORWARD and INPUT of many rows, by what a tile of 256, 128 or 64 columns costs in steps of a 128 tile (about 0.2 us):
-// 1.6 of them a step for 256 columns, and for a split some 32 more.  Measured (us), 256 columns / 128 / 64 and split:
-// 2048x768x2304 9.2 / 9.9 / 46; 512x2048x2048 14.4 / 10.1 / 17.3; 128x8192x2048 48.5 / 29.6 / 16.7.
-template <int FORM>
-int start_rows(const Operands& o, const Args& a, long long row_tiles, int steps, cudaStream_t s) {
-  const int n = sms();
-  const auto rounds = [&](int width) { return (row_tiles * ((a.cols + width - 1) / width) + n - 1) / n; };
-  const double wide = rounds(256) * (1.6 * steps), narrow = (double)rounds(128) * steps;
-  if (!a.offsets) {
-    const Split split = split_of<FORM, 64>(row_tiles * ((a.cols + 63) / 64), steps, 32);
-    if (split.blocks > 1 && split.cost < std::min(wide, narrow)) return start<FORM, 64, false, true>(o, a, split.blocks, s);
+// FORWARD and INPUT of many rows, by what the rounds of all SMs cost in steps of a 128 tile (about 0.2 us): a step of a
+// tile of 256 columns 1.6 of them, of a pair's 256 x 256 1.48 (INPUT: 1.4) and 6 for its start, and for a split of 64
+// columns some 32.  Half of an expert's last tile is taken as empty.  A pair's two blocks share one round of outputs,
+// so with short sums and an activation to compute it loses (32768x768x2304 with gelu 162.5 us, alone 154.0).
+// Measured (us), 256 columns / 128 / 64 and split: 2048x768x2304 9.2 / 9.9 / 46; 512x2048x2048 14.4 / 10.1 / 17.3;
+// 128x8192x2048 48.5 / 29.6 / 16.7.  256 columns / pair: 16384x2048x8192 379.8 / 353.3; 2048x2048x2048 22.0 / 23.3;
+// INPUT of 16384x8192x2048 523.6 / 364.0; gated 4096 tokens by 8 of 64 experts 240.5 / 249.2, 16384 by 2 of 16 208.6 / 195.2.
+template <int FORM, bool GATED = false>
+int start_rows(const Operands& o, const Args& a, int steps, cudaStream_t s) {
+  const int n = sms(), columns = GATED ? 128 : 256;
+  const auto rounds = [&](int down, int across, int at_once) {
+    const long long tiles = ((a.rows + down - 1) / down + (a.offsets ? a.groups / 2 : 0)) *
+                            (long long)((a.cols + across - 1) / across);
+    return (tiles + at_once - 1) / at_once;
+  };
+  const double wide = rounds(128, columns, n) * (1.6 * steps);
+  const double pair = a.act != TAO_ACT_NONE && steps < 16
+                          ? 2 * wide
+                          : rounds(256, columns, n / 2) * ((FORM == INPUT ? 1.4 : 1.48) * steps) + 6;
+  if constexpr (!GATED) {
+    const double narrow = (double)rounds(128, 128, n) * steps;
+    if (!a.offsets) {
+      const Split split = split_of<FORM, 64>(((a.rows + 127) / 128) * (long long)((a.cols + 63) / 64), steps, 32);
+      if (split.blocks > 1 && split.cost < std::min({wide, narrow, pair}))
+        return start<FORM, 64, false, true>(o, a, split.blocks, s);
+    }
+    if (narrow < std::min(wide, pair) || a.cols <= 128) return start<FORM, 128, false, false>(o, a, 1, s);
   }
-  if (narrow < wide || a.cols <= 128) return start<FORM, 128, false, false>(o, a, 1, s);
-  return start<FORM, 256, false, false>(o, a, 1, s);
+  if (pair < wide) return start<FORM, 256, GATED, false, true>(o, a, 1, s);
+  return start<FORM, 256, GATED, false>(o, a, 1, s);
 }
 
 template <int EIGHTS, int WARPS, int AHEAD>
@@ -561,10 +578,10 @@ int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
     const Operands few = {ow, ox, ou, none}, many = {ox, ow, none, ou};
     if (p.up) {
       if (mean <= 32) return start<FEW, 32, true, false>(few, a, 1, s);
-      return start<FORWARD, 256, true, false>(many, a, 1, s);
+      return start_rows<FORWARD, true>(many, a, steps, s);
     }
     if (mean <= 32) return start<FEW, 32, false, false>(few, a, 1, s);
-    return start_rows<FORWARD>(many, a, (rows + 127) / 128 + p.experts / 2, steps, s);
+    return start_rows<FORWARD>(many, a, steps, s);
   }
   if (rows <= 32) {
     const FewArgs f = {ox.at, ow.at, p.bias, p.residual, rows > 1 ? ox.stride : 0, n > 1 ? ow.stride : 0, p.r_row,
@@ -580,8 +597,7 @@ int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
     return rows <= 32 ? start<FEW, 32, false, true>(o, a, split, s) : start<FEW, 64, false, true>(o, a, split, s);
   }
   const Operands o = {ox, ow, none, none};
-  const long long row_tiles = (rows + 127) / 128;
-  return start_rows<FORWARD>(o, a, row_tiles, steps, s);
+  return start_rows<FORWARD>(o, a, steps, s);
 }
 
 int input_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_t s) {
@@ -591,8 +607,7 @@ int input_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_
   a.type = p.type, a.y = p.dx;
   a.unit = unit_of(k, bits_of(p.dx, k));
   const int steps = (n + kTerms - 1) / kTerms * pairs;
-  const long long row_tiles = (p.rows + 127) / 128 + (p.offsets ? p.experts / 2 : 0);
-  return start_rows<INPUT>({o.a, o.b, o.a2, o.b2}, a, row_tiles, steps, s);
+  return start_rows<INPUT>(o, a, steps, s);
 }
 
 int weight_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_t s) {

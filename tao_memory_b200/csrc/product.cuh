@@ -58,12 +58,12 @@ struct Args {
   int split;           // blocks of a cluster
 };
 
-template <int FORM, int BN, bool GATED, bool SPLIT>
+template <int FORM, int BN, bool GATED, bool SPLIT, bool PAIR = false>
 struct Cfg {
   static constexpr bool A_MN = FORM == WEIGHT, B_MN = FORM == INPUT || FORM == WEIGHT;
-  static constexpr int TT = FORM == FEW ? BN : 128;                              // token rows of a tile
+  static constexpr int TT = FORM == FEW ? BN : PAIR ? 256 : 128;                 // token rows of a tile
   static constexpr int CT = FORM == FEW ? 128 : GATED ? BN / 2 : BN;             // output columns of a tile
-  static constexpr int A = (FORM == FEW && GATED ? 2 : 1) * 128 * 128, B = BN * 128, STAGE = A + B;
+  static constexpr int A = (FORM == FEW && GATED ? 2 : 1) * 128 * 128, B = (PAIR ? BN / 2 : BN) * 128, STAGE = A + B;
   static constexpr int STAGING = FORM == FEW || SPLIT ? 0 : kWorkers * 2048;
   static constexpr int LISTS = SPLIT ? 0 : (2 * kMostGroups + 4) * 4;
   // parts of a split tile: of few rows in a place of their own, else over the ring
@@ -131,6 +131,31 @@ TAO_DEVI void put_peer(uint32_t at, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
 
+// PAIR: the same by the two blocks of a pair: the copy arrives at a barrier of either, the product takes 128 rows of A
+// and half of B's from each one's shared memory, and the end of products arrives at the same barrier of both.
+TAO_DEVI void tma_3d_pair(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+TAO_DEVI void multiply_pair(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(acc),
+      "l"(a), "l"(b), "r"(idesc), "r"(more));
+}
+TAO_DEVI void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+TAO_DEVI void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // One lane of a warp that has met, the same for all that ask.
 TAO_DEVI bool elected() {
   uint32_t p;
@@ -196,21 +221,56 @@ constexpr float kLog2E = 1.4426950408889634f;
 TAO_DEVI float sigmoid(float q) { return reciprocal(1.f + tc::ex2(-kLog2E * q)); }
 constexpr float kGeluRoot = 0.7978845608028654f, kGeluCube = 0.044715f;  // sqrt(2 / pi)
 
+// Two fp32 values at an instruction.
+struct Two {
+  uint64_t v;
+};
+TAO_DEVI Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+TAO_DEVI Two two(float a) { return two(a, a); }
+TAO_DEVI float2 apart(Two x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+  return r;
+}
+TAO_DEVI Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+TAO_DEVI Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 // The normal distribution's integral from the tail of z's side: with t = 1 / (1 + 0.35 x), x = |z| / sqrt(2),
 // erfc(x) e^(x^2) / t is smooth on (0, 1], and half of it a polynomial in t (fitted here at Chebyshev nodes to 2^-20).
 // So small values keep their relative precision, at two special-function instructions.  `density` is e^(-z^2 / 2).
+TAO_DEVI float2 normal_integral(float2 z, float2& density) {
+  const float slope = 0.35f * 0.7071067811865476f;
+  const Two t = two(reciprocal(fmaf(slope, fabsf(z.x), 1.f)), reciprocal(fmaf(slope, fabsf(z.y), 1.f)));
+  const Two both = two(z.x, z.y);
+  const float2 e = apart(mul2(mul2(both, both), two(-0.5f * kLog2E)));
+  density = make_float2(tc::ex2(e.x), tc::ex2(e.y));
+  Two q = fma2(two(-0.042552598f), t, two(0.100604653f));
+  q = fma2(q, t, two(-0.0072748783f));
+  q = fma2(q, t, two(0.0814718946f));
+  q = fma2(q, t, two(0.0773361512f));
+  q = fma2(q, t, two(0.0929546698f));
+  q = fma2(q, t, two(0.098726552f));
+  q = fma2(q, t, two(0.0987331438f));
+  const float2 tail = apart(mul2(mul2(two(density.x, density.y), t), q));
+  return make_float2(z.x < 0.f ? tail.x : 1.f - tail.x, z.y < 0.f ? tail.y : 1.f - tail.y);
+}
 TAO_DEVI float normal_integral(float z, float& density) {
-  const float t = reciprocal(fmaf(0.35f * 0.7071067811865476f, fabsf(z), 1.f));
-  density = tc::ex2(-0.5f * kLog2E * z * z);
-  float q = fmaf(-0.042552598f, t, 0.100604653f);
-  q = fmaf(q, t, -0.0072748783f);
-  q = fmaf(q, t, 0.0814718946f);
-  q = fmaf(q, t, 0.0773361512f);
-  q = fmaf(q, t, 0.0929546698f);
-  q = fmaf(q, t, 0.098726552f);
-  q = fmaf(q, t, 0.0987331438f);
-  const float tail = density * t * q;
-  return z < 0.f ? tail : 1.f - tail;
+  float2 d;
+  const float2 p = normal_integral(make_float2(z, z), d);
+  density = d.x;
+  return p.x;
 }
 
 TAO_DEVI float activate(float z, int act) {
@@ -248,17 +308,29 @@ TAO_DEVI float2 activate_slope(float z, int act) {
 }
 template <int N>
 TAO_DEVI void activate_all(float (&v)[N], int act) {
-#define TAO_EACH(code)                                        \
-  case code:                                                  \
-    _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = activate(v[i], code); \
-    break;
   switch (act) {  // the choice outside of the loop
-    TAO_EACH(TAO_ACT_RELU)
-    TAO_EACH(TAO_ACT_SILU)
-    TAO_EACH(TAO_ACT_GELU)
-    TAO_EACH(TAO_ACT_GELU_TANH)
+    case TAO_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], TAO_ACT_RELU);
+      break;
+    case TAO_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], TAO_ACT_SILU);
+      break;
+    case TAO_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        float2 density;
+        const float2 p = normal_integral(make_float2(v[i], v[i + 1]), density);
+        v[i] *= p.x;
+        v[i + 1] *= p.y;
+      }
+      break;
+    case TAO_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], TAO_ACT_GELU_TANH);
+      break;
   }
-#undef TAO_EACH
 }
 
 // -- tiles ----------------------------------------------------------------------
@@ -416,13 +488,14 @@ TAO_DEVI float finish(const Args& a, float v, long long row, int col, bool is_bf
 }
 
 // Maps: FORWARD: x, W, -, U.  FEW: W, x, U, -.  INPUT: dz, W, du, U.  WEIGHT: dz, x, du, -.
-template <int FORM, int BN, bool GATED, bool SPLIT, bool BF16>
+template <int FORM, int BN, bool GATED, bool SPLIT, bool PAIR, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_a2, const __grid_constant__ CUtensorMap map_b2,
                    const Args a) {
   using namespace tc;
-  using C = Cfg<FORM, BN, GATED, SPLIT>;
+  using C = Cfg<FORM, BN, GATED, SPLIT, PAIR>;
+  static_assert(!PAIR || ((FORM == FORWARD || FORM == INPUT) && BN == 256 && !SPLIT), "");
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* const staging_all = sm + C::STAGES * C::STAGE;
   uint64_t* const full = reinterpret_cast<uint64_t*>(staging_all + C::STAGING);
@@ -441,8 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   constexpr bool is_bf16 = BF16;
-  const int rank = SPLIT ? (int)cluster_rank() : 0;
-  const int start = SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x, step = SPLIT ? 1 << 30 : (int)gridDim.x;
+  const int rank = SPLIT || PAIR ? (int)cluster_rank() : 0;
+  const int start = SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x / (PAIR ? 2 : 1);
+  const int step = SPLIT ? 1 << 30 : (int)gridDim.x / (PAIR ? 2 : 1);
   // this block's part of a tile's steps
   auto part = [&](const Tile& t, int& k0) {
     if constexpr (!SPLIT) return k0 = 0, t.blocks;
@@ -453,6 +527,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto fetch = [&](const Tile& tile, int kb, int s) {
     uint8_t* const sa = sm + s * C::STAGE;
     uint8_t* const sb = sa + C::A;
+    if constexpr (PAIR) {  // this block's 128 rows of A and its half of B; both blocks' copies arrive at the first one's
+      if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+      const uint32_t bar = peer(smem_u32(&full[s]), 0);
+      const int each = tile.blocks / a.pairs;
+      const bool other = kb >= each;
+      const int k = (kb - (other ? each : 0)) * kTerms;
+      tma_3d_pair(sa, other ? &map_a2 : &map_a, k, tile.row0 + rank * 128, 0, bar);
+      if constexpr (FORM == FORWARD) {
+        if constexpr (GATED)
+          tma_3d_pair(sb, rank ? &map_b2 : &map_b, k, tile.col0, tile.group, bar);
+        else
+          tma_3d_pair(sb, &map_b, k, tile.col0 + rank * 128, tile.group, bar);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          tma_3d_pair(sb + j * 8192, other ? &map_b2 : &map_b, tile.col0 + rank * 128 + j * 64, k, tile.group, bar);
+      }
+      return;
+    }
     mbar_expect_tx(&full[s], C::STAGE);
     if constexpr (FORM == FORWARD) {
       const int k = kb * kTerms;
@@ -490,14 +583,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&acc_full[i], 1);
-        mbar_init(&acc_empty[i], kWorkers);
+        mbar_init(&acc_empty[i], PAIR ? 2 * kWorkers : kWorkers);
       }
       mbar_init(over, 1);
       *abort = 0;
       fence_mbar_init();
     }
     __syncwarp();
-    if (!a.offsets) {
+    if (!a.offsets && !PAIR) {
       const Tile tile = tile_of<FORM, C>(a, first, ends, start, group);  // there is one: no block is launched without
       int k0;
       early = min(part(tile, k0), C::STAGES);
@@ -506,14 +599,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(C::TMEM));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(C::TMEM));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(C::TMEM));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   if constexpr (!SPLIT)
     if (warp == 2 && a.offsets) make_lists<C>(a, first, ends, lane);
   fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // both blocks' barriers and accumulators are there
   fence_after();
   const uint32_t tbase = *tmem_slot;
   if constexpr (SPLIT) cluster_arrive();  // this block has begun: its shared memory can be written to
@@ -542,20 +642,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++s == C::STAGES) s = 0, phase ^= 1;
       }
     }
-    if (!ok) {  // copies in flight have their time before the block ends
+    if (!ok && !(PAIR && rank)) {  // copies in flight (PAIR: both blocks') have their time before the block ends
       fetched = max(fetched, early);
       for (int i = max(fetched - C::STAGES, 0); i < fetched; ++i) mbar_wait(&full[i % C::STAGES], i / C::STAGES & 1, nullptr);
     }
   } else if (warp == kWorkers + 1) {
     // ---- issues the products
     const uint32_t type_bits = is_bf16 ? 1u << 7 | 1u << 10 : 0u;
-    const uint32_t idesc = (idesc_bf16(128, BN, C::A_MN, C::B_MN) & ~(1u << 7 | 1u << 10)) | type_bits;
+    const uint32_t idesc = (idesc_bf16(PAIR ? 256 : 128, BN, C::A_MN, C::B_MN) & ~(1u << 7 | 1u << 10)) | type_bits;
     constexpr int STEP_A = (C::A_MN ? 2048 : 32) >> 4, STEP_B = (C::B_MN ? 2048 : 32) >> 4;  // 16 terms on
     const uint64_t desc_a = sdesc(smem_u32(sm), C::A_MN ? 8192 : 16, 1024);
     const uint64_t desc_b = sdesc(smem_u32(sm) + C::A, C::B_MN ? 8192 : 16, 1024);
     int s = 0, phase = 0, set = 0, set_phase = 0;
     bool ok = true;
-    for (int t = start; ok && t < total; t += step) {
+    for (int t = PAIR && rank ? total : start; ok && t < total; t += step) {  // PAIR: the first block's for both
       const Tile tile = tile_of<FORM, C>(a, first, ends, t, group);
       int k0;
       const int blocks = part(tile, k0);
@@ -591,23 +691,37 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < kTerms / 16; ++k) {
             if (FORM == WEIGHT && k >= steps) break;
-            multiply(acc, da + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
+            if constexpr (PAIR)
+              multiply_pair(acc, da + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
+            else
+              multiply(acc, da + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
             if constexpr (FORM == FEW && GATED)
               multiply(acc + BN, da + (C::A / 2 >> 4) + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
           }
-          commit(&empty[s]);
+          if constexpr (PAIR)
+            commit_pair(&empty[s]);
+          else
+            commit(&empty[s]);
         }
         __syncwarp();
         s = next, phase = next_phase;
       }
       if (!ok) break;
-      if (elected()) commit(&acc_full[set]);
+      if (elected()) {
+        if constexpr (PAIR)
+          commit_pair(&acc_full[set]);
+        else
+          commit(&acc_full[set]);
+      }
       __syncwarp();
       if (++set == C::SETS) set = 0, set_phase ^= 1;
     }
     if (elected()) {  // nothing is in flight when the block ends
-      commit(over);
-      mbar_wait(over, 0, nullptr);
+      if constexpr (!PAIR)
+        commit(over);
+      else if (rank == 0)
+        commit_pair(over);
+      if (!PAIR || rank == 0) mbar_wait(over, 0, nullptr);
     }
     __syncwarp();
   } else {
@@ -679,8 +793,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         constexpr int HALF = C::CT / 2;
-        const long long row0 = tile.row0 + quarter * 32;
-        const int rows = tile.rows - quarter * 32;
+        const int down = PAIR ? rank * 128 + quarter * 32 : quarter * 32;
+        const long long row0 = tile.row0 + down;
+        const int rows = tile.rows - down;
         uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
         if constexpr (FORM == WEIGHT) y += (long long)tile.group * a.depth * a.cols;
         const auto bias_of = [&](int c0) {  // of column `lane` of a chunk
@@ -706,10 +821,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rows <= 0 || cols <= 0) continue;  // the same for the warp
           if constexpr (FORM == FORWARD) {
             if (a.bias) {
-              const float next = bias_of(c0 + 32);
+              reinterpret_cast<float*>(staging)[lane] = bias;
+              __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bias, i);
-              bias = next;
+              for (int i = 0; i < 32; i += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(staging + i * 4);
+                v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
+              }
+              __syncwarp();
+              bias = bias_of(c0 + 32);
             }
             if (a.z) {
               put_rows(staging, v, is_bf16, static_cast<uint16_t*>(a.z) + row0 * a.z_stride + col, a.z_stride, rows,
@@ -746,7 +866,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (blocks) {
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[set]);
+          if (lane == 0) {
+            if constexpr (PAIR)
+              arrive_at(peer(smem_u32(&acc_empty[set]), 0));
+            else
+              mbar_arrive(&acc_empty[set]);
+          }
         }
       }
       if (blocks && ++set == C::SETS) set = 0, set_phase ^= 1;
@@ -841,8 +966,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if constexpr (FORM != FEW) cluster_sync();  // the others' reads of this block's part are over
   }
-  if (warp == 0)
+  if constexpr (PAIR) {
+    cluster_sync();  // neither's products, copies or arrivals need the other any more
+    if (warp == 0)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
+  } else if (warp == 0) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
+  }
 }
 
 }  // namespace product

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(32 * WARPS) place_kernel(const Pass p) {
   }
 }
 
-inline int blocks_of(long long n) { return n <= kSmallSort ? 1 : (int)std::min<long long>((n + 1023) / 1024, kMostBlocks); }
+inline int blocks_of(long long n) { return n <= kSmallSort ? 1 : (int)std::min<long long>((n + 511) / 512, kMostBlocks); }
 inline size_t counts_bytes(long long n, int bins) { return n <= kSmallSort ? 0 : (size_t)blocks_of(n) * bins * sizeof(int); }
 
 // `counts`: counts_bytes of scratch.

@@ -45,7 +45,7 @@ def embed(ids, table, scale=1.0):
     """scale * table[ids]: table [vocab, width] bf16, fp16 or fp32, ids int32 or int64 of any shape on its device;
     returns [*ids.shape, width], scaled in fp32 and rounded once.  An id outside of the table (padding) gives
     zeros and adds to no gradient.  Differentiable (in reverse mode, once) in the table: a dense gradient, each
-    row's sum in fp32 in the order of the tokens, in runs of 32 of the sorted tokens, rounded once."""
+    row's sum in fp32 in the order of the tokens, in runs of 16 of the sorted tokens, rounded once."""
     if table.dtype not in TYPES or not table.is_cuda or table.dim() != 2 or 0 in table.shape:
         raise ValueError("embed takes a bf16, fp16 or fp32 CUDA table [vocab, width] (no CPU fallback)")
     if table.shape[0] > MOST_ROWS or table.shape[1] > MOST_CHANNELS:
