@@ -53,7 +53,7 @@ class TaoLinear(ctypes.Structure):
                 + [(n, ctypes.c_longlong) for n in ("x_row", "x_col", "w_expert", "w_row", "w_col", "up_expert", "up_row",
                                                     "up_col", "r_row", "z_row", "rows")]
                 + [(n, ctypes.c_int) for n in ("n", "k", "experts", "type", "activation")]
-                + [(n, ctypes.c_void_p) for n in ("y", "z", "u", "dy")] + [("dy_row", ctypes.c_longlong)]
+                + [(n, ctypes.c_void_p) for n in ("y", "z", "u", "low", "dy")] + [("dy_row", ctypes.c_longlong)]
                 + [(n, ctypes.c_void_p) for n in ("dx", "dw", "dup", "db", "workspace")]
                 + [("workspace_bytes", ctypes.c_size_t)])
 

@@ -249,6 +249,7 @@ unsigned long long bits_of(const void* p, long long stride) {
 // -- the gradient's elementwise part ------------------------------------------
 struct SlopeArgs {
   const void *dy, *z, *u;
+  const uint8_t* low;  // gated: the lower bits of z and, rows * z_stride on, of u
   long long dy_stride, z_stride, d_stride;
   void *dz, *du;
   float* sums;  // [blocks][n] of dz, or null
@@ -265,6 +266,17 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
   const int col = (blockIdx.x * 32 + lane) * VEC;
   const long long begin = (long long)blockIdx.y * a.per, end = min(begin + a.per, a.rows);
   using Word = typename Unit<VEC>::Type;
+  using Low = std::conditional_t<VEC == 8, uint2, std::conditional_t<VEC == 2, uint16_t, uint8_t>>;
+  const auto widen24 = [](const Word& upper, const Low& lower, float (&v)[VEC]) {
+    uint32_t up[VEC / 2 + 1], low[2] = {};
+    if constexpr (VEC == 8) {
+      up[0] = upper.x, up[1] = upper.y, up[2] = upper.z, up[3] = upper.w, low[0] = lower.x, low[1] = lower.y;
+    } else {
+      up[0] = upper, low[0] = lower;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = of24(up[i / 2] >> (16 * (i & 1)) & 0xffffu, low[i / 4] >> (8 * (i & 3)) & 0xffu);
+  };
   auto widen = [](const Word& w, float (&v)[VEC]) {
     if constexpr (VEC == 8) {
       const uint32_t words[4] = {w.x, w.y, w.z, w.w};
@@ -298,13 +310,18 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
   if (col < a.n) {
     for (long long r0 = begin + warp; r0 < end; r0 += 8 * AHEAD) {
       Word wy[AHEAD], wz[AHEAD], wu[AHEAD];
+      Low lz[AHEAD], lu[AHEAD];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const long long r = r0 + 8 * j;
         if (r >= end) break;
         wy[j] = load(a.dy, r, a.dy_stride);
         if constexpr (SLOPED) wz[j] = load(a.z, r, a.z_stride);
-        if constexpr (GATED) wu[j] = load(a.u, r, a.z_stride);
+        if constexpr (GATED) {
+          wu[j] = load(a.u, r, a.z_stride);
+          lz[j] = *reinterpret_cast<const Low*>(a.low + r * a.z_stride + col);
+          lu[j] = *reinterpret_cast<const Low*>(a.low + (a.rows + r) * a.z_stride + col);
+        }
       }
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
@@ -313,8 +330,12 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
         float dy[VEC], z[VEC], u[VEC];
         widen(wy[j], dy);
         if constexpr (SLOPED) {
-          widen(wz[j], z);
-          if constexpr (GATED) widen(wu[j], u);
+          if constexpr (GATED) {
+            widen24(wz[j], lz[j], z);
+            widen24(wu[j], lu[j], u);
+          } else {
+            widen(wz[j], z);
+          }
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             const float2 f = activate_slope(z[i], ACT);
@@ -534,22 +555,30 @@ Extent reach(const Given& g) {
 }
 bool any_overlap(const TaoLinear& p, bool gradient) {
   const long long rows = p.rows, n = p.n, k = p.k, y = rows * n * 2, w = (long long)p.experts * n * k * 2;
-  const long long kept = ((rows - 1) * p.z_row + n) * 2;
+  const long long kept = p.up ? rows * p.z_row * 2 : ((rows - 1) * p.z_row + n) * 2;  // gated: whole rows
   const Extent x = reach(given_x(p)), weight = reach(given_w(p)), up = reach(given_up(p)), z = extent(p.z, 1, 0, kept),
-               u = extent(p.u, 1, 0, kept), offsets = extent(p.offsets, 1, 0, (p.experts + 1) * 4ll);
+               u = extent(p.u, 1, 0, kept), low = extent(p.up ? p.low : nullptr, 1, 0, kept), offsets = extent(p.offsets, 1, 0, (p.experts + 1) * 4ll);
   if (!gradient) {
     const Extent bias = extent(p.bias, 1, 0, n * 2), residual = extent(p.residual, rows, p.r_row * 2, n * 2);
     const bool in_place = p.residual == p.y && (p.r_row == n || rows == 1);
-    return overlaps(p.y, y, {x, weight, up, bias, in_place ? Extent{0, 0} : residual, z, p.z ? u : Extent{0, 0}, offsets}) ||
-           overlaps(p.z, kept, {x, weight, up, bias, residual, u, offsets}) ||
-           (p.z && overlaps(p.u, kept, {x, weight, up, offsets}));
+    return overlaps(p.y, y, {x, weight, up, bias, in_place ? Extent{0, 0} : residual, z, p.z ? u : Extent{0, 0}, p.z ? low : Extent{0, 0}, offsets}) ||
+           overlaps(p.z, kept, {x, weight, up, bias, residual, u, low, offsets}) ||
+           (p.z && overlaps(p.u, kept, {x, weight, up, low, offsets})) ||
+           (p.z && p.up && overlaps(p.low, kept, {x, weight, up, offsets}));
   }
   const Extent dy = extent(p.dy, rows, p.dy_row * 2, n * 2), dx = extent(p.dx, 1, 0, rows * k * 2), dw = extent(p.dw, 1, 0, w),
                dup = extent(p.dup, 1, 0, w);
-  return overlaps(p.dx, rows * k * 2, {x, weight, up, z, u, offsets, dy, dw, dup}) ||
-         overlaps(p.dw, w, {x, weight, up, z, u, offsets, dy, dup}) ||
-         overlaps(p.dup, w, {x, weight, up, z, u, offsets, dy}) ||
-         overlaps(p.db, n * 2, {x, weight, up, z, u, offsets, dy, dx, dw, dup});
+  return overlaps(p.dx, rows * k * 2, {x, weight, up, z, u, low, offsets, dy, dw, dup}) ||
+         overlaps(p.dw, w, {x, weight, up, z, u, low, offsets, dy, dup}) ||
+         overlaps(p.dup, w, {x, weight, up, z, u, low, offsets, dy}) ||
+         overlaps(p.db, n * 2, {x, weight, up, z, u, low, offsets, dy, dx, dw, dup});
+}
+
+// Gated: what is kept for the gradient goes by 16 bytes.
+bool kept_ok(const TaoLinear& p) {
+  return !p.up || !p.z || (p.z_row % 16 == 0 && p.z_row >= p.n &&
+                           (reinterpret_cast<uintptr_t>(p.z) | reinterpret_cast<uintptr_t>(p.u) |
+                            reinterpret_cast<uintptr_t>(p.low)) % 16 == 0);
 }
 
 int check_room(const TaoLinear& p, size_t need) {
@@ -569,8 +598,8 @@ int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
   Args a = {};
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)rows, a.cols = n, a.depth = k, a.pairs = 1;
   a.type = p.type, a.act = p.activation, a.bias = p.bias, a.residual = p.residual, a.r_stride = p.r_row;
-  a.y = p.y, a.z = p.z, a.u = p.z ? p.u : nullptr, a.z_stride = p.z_row;
-  a.unit = unit_of(n, bits_of(p.y, n) | (p.z ? bits_of(p.z, p.z_row) : 0) | bits_of(a.u, 0) |
+  a.y = p.y, a.z = p.z, a.u = p.z ? p.u : nullptr, a.low = static_cast<uint8_t*>(p.low), a.z_stride = p.z_row;
+  a.unit = unit_of(n, bits_of(p.y, n) | (p.z && !p.up ? bits_of(p.z, p.z_row) : 0) |
                           (p.residual ? bits_of(p.residual, p.r_row) : 0));
   const int steps = (k + kTerms - 1) / kTerms;
   if (p.offsets) {
@@ -640,7 +669,7 @@ int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
   // dz and du, or dy itself
   Given gz = {p.dy, p.rows, p.n, 1, p.dy_row, 1, 0}, gd = {};
   if (sloped || p.db) {
-    SlopeArgs a = {p.dy, sloped ? p.z : nullptr, p.up ? p.u : nullptr, p.dy_row, p.z_row, padded(p.n), nullptr, nullptr,
+    SlopeArgs a = {p.dy, sloped ? p.z : nullptr, p.up ? p.u : nullptr, static_cast<const uint8_t*>(p.low), p.dy_row, p.z_row, padded(p.n), nullptr, nullptr,
                    nullptr, p.rows, p.n, p.type, p.activation, slope_rows(p.rows, p.n)};
     if (sloped && products) {
       const size_t size = (size_t)(p.rows * a.d_stride * 2);
@@ -688,10 +717,10 @@ int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
 }
 
 int missing(const TaoLinear& p, bool gradient) {
-  if (!gradient) return !p.x || !p.w || !p.y || (p.up && p.z && !p.u);
+  if (!gradient) return !p.x || !p.w || !p.y || (p.up && p.z && (!p.u || !p.low));
   const bool sloped = p.activation != TAO_ACT_NONE || p.up;
   return !p.dy || (p.up ? !p.dw != !p.dup : p.dup != nullptr) || (p.dx && (!p.w)) || (p.dw && !p.x) ||
-         (sloped && (!p.z || (p.up && !p.u)));
+         (sloped && (!p.z || (p.up && (!p.u || !p.low))));
 }
 
 }  // namespace
@@ -718,6 +747,7 @@ int tao_linear(const TaoLinear* p, void* stream) {
   if (int rc = check(p)) return rc;
   if (p->rows == 0) return TAO_OK;
   if (missing(*p, false)) return pfail(TAO_ERR_ARG, "null pointer");
+  if (!kept_ok(*p)) return pfail(TAO_ERR_ARG, "a gate's kept factors start on 16 bytes, in rows of a multiple of 16");
   if (any_overlap(*p, false)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 0))) return rc;
   static uint8_t none[1];  // where no room is needed
@@ -738,6 +768,7 @@ int tao_linear_gradient(const TaoLinear* p, void* stream) {
     return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
   }
   if (missing(*p, true)) return pfail(TAO_ERR_ARG, "null pointer");
+  if (!kept_ok(*p)) return pfail(TAO_ERR_ARG, "a gate's kept factors start on 16 bytes, in rows of a multiple of 16");
   if (any_overlap(*p, true)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 1))) return rc;
   static uint8_t none[1];

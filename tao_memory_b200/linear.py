@@ -58,23 +58,28 @@ def _room(p, rows, gradient):
     return room
 
 
+def _point(p, kept, up):
+    p.z, p.z_row = kept.data_ptr(), kept.shape[-1]
+    if up is not None:
+        plane = 2 * kept.shape[1] * kept.shape[2]
+        p.u, p.low = p.z + plane, p.z + 2 * plane
+
+
 def _forward(p, rows, up, keep):
-    """(y, z, u) of a described product: z, u are None unless ``keep``."""
+    """(y, kept) of a described product: kept is None unless ``keep``."""
     count, n = rows.shape[0], p.n
     y = rows.new_empty((count, n))
     p.y = y.data_ptr()
-    z = u = None
+    kept = None
     if keep:
-        p.z_row = -(-n // 8) * 8
-        z = rows.new_empty((count, p.z_row))
-        p.z = z.data_ptr()
-        if up is not None:
-            u = rows.new_empty((count, p.z_row))
-            p.u = u.data_ptr()
+        row = -(-n // 16) * 16
+        # act's argument, or 24 bits each of a gate's two factors: their upper 16 and behind them their lower 8
+        kept = rows.new_empty((count, row) if up is None else (3, count, row))
+        _point(p, kept, up)
     room = _room(p, rows, 0)
     _lib.on_device(rows.device.index, _lib.lib().tao_linear, byref(p))
     del room
-    return y, z, u
+    return y, kept
 
 
 class _Product(torch.autograd.Function):
@@ -84,8 +89,8 @@ class _Product(torch.autograd.Function):
     def forward(ctx, x, weight, up, bias, residual, offsets, act):
         p = _describe(x, weight, up, bias, residual, offsets, act)
         sloped = any(ctx.needs_input_grad[:4]) and (act != 0 or up is not None)
-        y, z, u = _forward(p, x, up, sloped)
-        ctx.save_for_backward(x, weight, up, z, u, offsets)
+        y, kept = _forward(p, x, up, sloped)
+        ctx.save_for_backward(x, weight, up, kept, offsets)
         ctx.act = act
         ctx.set_materialize_grads(False)
         return y
@@ -99,14 +104,12 @@ class _Product(torch.autograd.Function):
         want_x, want_w, want_up, want_b, want_res = ctx.needs_input_grad[:5]
         dx = dw = dup = db = None
         if want_x or want_w or want_up or want_b:
-            x, weight, up, z, u, offsets = ctx.saved_tensors
+            x, weight, up, kept, offsets = ctx.saved_tensors
             p = _describe(x, weight, up, None, None, offsets, ctx.act)
             grad = _rows(dy, p.n)
             p.dy, p.dy_row = grad.data_ptr(), grad.stride(0)
-            if z is not None:
-                p.z, p.z_row = z.data_ptr(), z.stride(0)
-                if u is not None:
-                    p.u = u.data_ptr()
+            if kept is not None:
+                _point(p, kept, up)
             if want_x:
                 dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
                 p.dx = dx.data_ptr()
@@ -152,7 +155,7 @@ def linear(x, weight, bias=None, residual=None, activation=None):
     if wants_gradient(x, weight, bias, residual):
         y = _Product.apply(rows, weight, None, bias, residual, None, act)
     else:
-        y, _, _ = _forward(_describe(rows, weight, None, bias, residual, None, act), rows, None, False)
+        y, _ = _forward(_describe(rows, weight, None, bias, residual, None, act), rows, None, False)
     return y if x.dim() == 2 else y.view(shape)
 
 
@@ -163,7 +166,8 @@ def expert_linear(x, weight, offsets, up=None, activation=None):
     Rows behind the last expert's give zeros.  bf16 or fp16, sums and activation in fp32, rounded once.
 
     The offsets are read on the device only.  Differentiable (in reverse mode, once) in x, weight and up, as
-    ``linear`` is; an expert without rows has a gradient of zeros, rows of no expert too."""
+    ``linear`` is, but that a gate's two factors are kept in 24 bits; an expert without rows has a gradient of zeros,
+    rows of no expert too."""
     if weight.dim() != 3:
         raise ValueError("expert_linear takes weights [experts, n, k]")
     _check("expert_linear", x, weight, activation)

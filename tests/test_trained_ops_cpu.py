@@ -19,7 +19,7 @@ def test_no_cpu_fallback():
 
 
 # addresses a megabyte apart, none of which is read before a refusal
-X, W, UP, Y, Z, U, DY, DX, DW, DUP, DB, ROOM = (i << 20 for i in range(1, 13))
+X, W, UP, Y, Z, U, LOW, DY, DX, DW, DUP, DB, ROOM = (i << 20 for i in range(1, 14))
 
 
 def _described(**kw):
@@ -38,7 +38,10 @@ def test_linear_refusals():
                 dict(w=None), dict(y=None), dict(x=X + 1), dict(w=W + 3), dict(y=Y + 1), dict(bias=17),
                 dict(residual=17, r_row=32), dict(experts=2), dict(experts=0), dict(offsets=16, experts=513),
                 dict(EXPERTS, offsets=18), dict(up=UP, up_row=64, up_col=1), dict(EXPERTS, bias=16),
-                dict(EXPERTS, residual=16, r_row=32), dict(GATED, z=Z, z_row=32), dict(rows=(1 << 30) + 1),
+                dict(EXPERTS, residual=16, r_row=32), dict(GATED, z=Z, z_row=32), dict(GATED, z=Z, u=U, z_row=32),
+                dict(GATED, z=Z, u=U, low=LOW, z_row=40), dict(GATED, z=Z + 8, u=U, low=LOW, z_row=32),
+                dict(GATED, z=Z, u=U, low=LOW + 8, z_row=32), dict(GATED, z=Z, u=U, low=U + 128, z_row=32),
+                dict(rows=(1 << 30) + 1),
                 dict(n=(1 << 24) + 1), dict(k=(1 << 24) + 1),
                 # what has to be copied first has no room, too little, or one off its alignment
                 dict(x_row=63), dict(x_col=2), dict(w=W + 8), dict(x_row=0), dict(x_row=63, workspace=ROOM, workspace_bytes=256),
@@ -46,7 +49,7 @@ def test_linear_refusals():
                 dict(EXPERTS, w_expert=0),
                 # outputs over operands: the last row of x, the bias, a residual one row on, z over y
                 dict(y=X + 3 * 128), dict(y=W - 2), dict(bias=Y + 4), dict(residual=Y + 64, r_row=32),
-                dict(residual=Y, r_row=40), dict(z=Y, z_row=32), dict(z=X, z_row=32), dict(GATED, z=Z, u=Z, z_row=32),
+                dict(residual=Y, r_row=40), dict(z=Y, z_row=32), dict(z=X, z_row=32), dict(GATED, z=Z, u=Z, low=LOW, z_row=32),
                 dict(GATED, y=UP + 8000)):
         assert lib.tao_linear(_described(**bad), None) == ARG, bad
     assert lib.tao_linear(_described(rows=0), None) == _lib.TAO_OK
@@ -62,7 +65,7 @@ def test_linear_workspace():
     assert size(1, **grad) == 0 and size(1, **dict(grad, dy_row=33)) == 256
     assert size(1, activation=2, z=Z, z_row=32, **grad) == 256 and size(1, db=DB, **grad) == 256
     assert size(1, db=DB, activation=2, z=Z, z_row=32, **dict(grad, dx=None, dw=None)) == 256
-    assert size(1, **grad, **GATED, u=U, z=Z, z_row=32, dup=DUP) == 512
+    assert size(1, **grad, **GATED, u=U, z=Z, low=LOW, z_row=32, dup=DUP) == 512
 
 
 def test_gradient_refusals():
@@ -70,9 +73,10 @@ def test_gradient_refusals():
     grad = dict(dy=DY, dy_row=32, dx=DX, dw=DW)
     for bad in (dict(dy=None), dict(dy=DY + 1), dict(dx=DX + 1), dict(dw=DW + 1), dict(db=DB + 1), dict(x=None), dict(w=None),
                 dict(dup=DUP), dict(activation=2), dict(activation=2, z=Z, z_row=32), dict(db=DB), dict(dy_row=33),
-                dict(GATED, z=Z, u=U, z_row=32), dict(GATED, z=Z, z_row=32, dup=DUP), dict(dx=X), dict(dx=DY), dict(dw=W + 64),
+                dict(GATED, z=Z, u=U, low=LOW, z_row=32), dict(GATED, z=Z, z_row=32, dup=DUP),
+                dict(GATED, z=Z, u=U, z_row=32, dup=DUP, workspace=ROOM, workspace_bytes=1 << 20), dict(dx=X), dict(dx=DY), dict(dw=W + 64),
                 dict(dw=DX), dict(db=DY, workspace=ROOM, workspace_bytes=1 << 20),
-                dict(GATED, z=Z, u=U, z_row=32, dup=DW, workspace=ROOM, workspace_bytes=1 << 20)):
+                dict(GATED, z=Z, u=U, low=LOW, z_row=32, dup=DW, workspace=ROOM, workspace_bytes=1 << 20)):
         assert lib.tao_linear_gradient(_described(**dict(grad, **bad)), None) == ARG, bad
     assert lib.tao_linear_gradient(_described(rows=0), None) == _lib.TAO_OK
 
