@@ -40,14 +40,13 @@ def sort_tokens(ids, experts):
         raise ValueError(f"there are 1 to {MOST_EXPERTS} experts")
     ids = ids.contiguous()
     count, lib = ids.numel(), _lib.lib()
-    out = ids.new_empty(2 * count + experts + 1, dtype=torch.int32)
-    pairs, places, offsets = out[:count], out[count:2 * count], out[2 * count:]
+    pairs, places, offsets = (ids.new_empty(shape, dtype=torch.int32) for shape in (count, ids.shape, experts + 1))
     size = lib.tao_sort_tokens_workspace_bytes(count, experts)
     room = ids.new_empty(size, dtype=torch.uint8) if size else None
     _lib.on_device(ids.device.index, lib.tao_sort_tokens, ids.data_ptr(), ids.element_size(), count, experts,
                    pairs.data_ptr(), places.data_ptr(), offsets.data_ptr(), None if room is None else room.data_ptr(), size)
     order = TokenOrder.__new__(TokenOrder)  # what was just made need not be looked at
-    order.pairs, order.places, order.offsets = pairs, places.view(ids.shape), offsets
+    order.pairs, order.places, order.offsets = pairs, places, offsets
     return order
 
 
