@@ -234,11 +234,9 @@ bool few_rows(const FewArgs& a, int type, cudaStream_t s, int* rc) {
   return true;
 }
 
-// Neighbours that can move at once in rows of `cols` whose addresses and strides (in bytes) have these bits.
+// Neighbours (8, 2 or 1) that can move at once in rows of `cols` whose addresses and strides in bytes have these bits.
 int unit_of(int cols, unsigned long long bits) {
-  for (int u = 8; u > 1; u /= 2)
-    if (cols % u == 0 && bits % (2 * u) == 0) return u;
-  return 1;
+  return cols % 8 == 0 && bits % 16 == 0 ? 8 : cols % 2 == 0 && bits % 4 == 0 ? 2 : 1;
 }
 unsigned long long bits_of(const void* p, long long stride) {
   return reinterpret_cast<uintptr_t>(p) | (unsigned long long)stride * 2;
@@ -599,8 +597,8 @@ int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)rows, a.cols = n, a.depth = k, a.pairs = 1;
   a.type = p.type, a.act = p.activation, a.bias = p.bias, a.residual = p.residual, a.r_stride = p.r_row;
   a.y = p.y, a.z = p.z, a.u = p.z ? p.u : nullptr, a.low = static_cast<uint8_t*>(p.low), a.z_stride = p.z_row;
-  a.unit = unit_of(n, bits_of(p.y, n) | (p.z && !p.up ? bits_of(p.z, p.z_row) : 0) |
-                          (p.residual ? bits_of(p.residual, p.r_row) : 0));
+  a.wide = unit_of(n, bits_of(p.y, n) | (p.z && !p.up ? bits_of(p.z, p.z_row) : 0) |
+                          (p.residual ? bits_of(p.residual, p.r_row) : 0)) == 8;
   const int steps = (k + kTerms - 1) / kTerms;
   if (p.offsets) {
     const long long mean = rows / p.experts;
@@ -634,7 +632,7 @@ int input_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream_
   Args a = {};
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)p.rows, a.cols = k, a.depth = n, a.pairs = pairs;
   a.type = p.type, a.y = p.dx;
-  a.unit = unit_of(k, bits_of(p.dx, k));
+  a.wide = unit_of(k, bits_of(p.dx, k)) == 8;
   const int steps = (n + kTerms - 1) / kTerms * pairs;
   return start_rows<INPUT>(o, a, steps, s);
 }
@@ -644,7 +642,7 @@ int weight_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream
   Args a = {};
   a.offsets = p.offsets, a.groups = p.experts, a.rows = (int)p.rows, a.cols = k, a.depth = n, a.pairs = pairs;
   a.type = p.type, a.y = p.dw, a.u = p.dup;
-  a.unit = unit_of(k, bits_of(p.dw, k) | bits_of(p.dup, 0));
+  a.wide = unit_of(k, bits_of(p.dw, k) | bits_of(p.dup, 0)) == 8;
   if (p.offsets) {
     if (k > 128) return start<WEIGHT, 256, false, false>(o, a, 1, s);
     return start<WEIGHT, 128, false, false>(o, a, 1, s);
@@ -684,11 +682,11 @@ int backward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
     if (p.db) a.sums = static_cast<float*>(rooms.take((size_t)blocks * p.n * sizeof(float)));
     if (rooms.base) {
       const int unit = unit_of(p.n, bits_of(p.dy, p.dy_row) | (sloped ? bits_of(p.z, p.z_row) | bits_of(p.u, 0) : 0));
-      const int across = unit == 8 ? 256 : unit > 1 ? 64 : 32;
+      const int across = 32 * unit;
       const dim3 grid((p.n + across - 1) / across, blocks);
       if (unit == 8)
         start_slope<8>(a, grid, s);
-      else if (unit > 1)
+      else if (unit == 2)
         start_slope<2>(a, grid, s);
       else
         start_slope<1>(a, grid, s);

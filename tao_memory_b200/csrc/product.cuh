@@ -55,7 +55,7 @@ struct Args {
   void *y, *z, *u;     // z, u: act's argument and the gate's factor (FORWARD, FEW); u: the second matrix (WEIGHT)
   uint8_t* low;        // gated: the lower bits of both
   long long z_stride;
-  int unit;            // neighbours of y, z, u and the residual that move at once: 8, 4, 2 or 1
+  bool wide;           // rows of y, z and the residual start on 16 bytes, and cols is a multiple of 8
   int split;           // blocks of a cluster
 };
 
@@ -426,13 +426,11 @@ TAO_DEVI Tile tile_of(const Args& a, const int* first, const int* ends, int t, i
 // Through 2 KB of shared memory, 16-byte chunks of a row turned so that eight rows' meet all banks.
 TAO_DEVI int staged(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1 & 3)) << 4); }
 
-// `unit` neighbours at a time (8, 4, 2 or 1: what the rows' addresses allow), all rows on their way.
+// `U` neighbours at a time (8, or 1 where the rows' addresses do not allow it), all rows on their way.
 template <int U>
 struct Unit;
 template <>
 struct Unit<8> { using Type = uint4; };
-template <>
-struct Unit<4> { using Type = uint2; };
 template <>
 struct Unit<2> { using Type = uint32_t; };
 template <>
@@ -454,30 +452,28 @@ TAO_DEVI void move_rows(uint8_t* staging, uint16_t* memory, long long stride, in
     for (int i = 0; i < ACROSS; ++i)
       if (i * U + first < rows && c < cols) *at(i * U + first) = v[i];
   } else {
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < ACROSS; ++i)
       if (i * U + first < rows && c < cols) *reinterpret_cast<W*>(memory + i * U * stride) = *at(i * U + first);
   }
 }
-TAO_DEVI void move_rows(uint8_t* staging, void* memory, long long stride, int rows, int cols, int unit, bool in, int lane) {
+TAO_DEVI void move_rows(uint8_t* staging, void* memory, long long stride, int rows, int cols, bool wide, bool in, int lane) {
   uint16_t* const m = static_cast<uint16_t*>(memory);
-  switch (unit) {
-    case 8: return move_rows<8>(staging, m, stride, rows, cols, in, lane);
-    case 4: return move_rows<4>(staging, m, stride, rows, cols, in, lane);
-    case 2: return move_rows<2>(staging, m, stride, rows, cols, in, lane);
-  }
-  move_rows<1>(staging, m, stride, rows, cols, in, lane);
+  if (wide)
+    move_rows<8>(staging, m, stride, rows, cols, in, lane);
+  else
+    move_rows<1>(staging, m, stride, rows, cols, in, lane);
 }
 // This thread's row of v, rounded, to memory.  All lanes of the warp.
 TAO_DEVI void put_rows(uint8_t* staging, const float (&v)[32], bool is_bf16, void* to, long long stride, int rows,
-                       int cols, int unit, int lane) {
+                       int cols, bool wide, int lane) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     *reinterpret_cast<uint4*>(staging + staged(lane, c)) =
         make_uint4(pack(v[c * 8], v[c * 8 + 1], is_bf16), pack(v[c * 8 + 2], v[c * 8 + 3], is_bf16),
                    pack(v[c * 8 + 4], v[c * 8 + 5], is_bf16), pack(v[c * 8 + 6], v[c * 8 + 7], is_bf16));
   __syncwarp();
-  move_rows(staging, to, stride, rows, cols, unit, false, lane);
+  move_rows(staging, to, stride, rows, cols, wide, false, lane);
   __syncwarp();
 }
 
@@ -894,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 put_rows24(staging, u, static_cast<uint16_t*>(a.u) + at, a.low + a.rows * a.z_stride + at, a.z_stride, rows,
                            room, lane);
               } else {
-                put_rows(staging, v, is_bf16, static_cast<uint16_t*>(a.z) + at, a.z_stride, rows, cols, a.unit, lane);
+                put_rows(staging, v, is_bf16, static_cast<uint16_t*>(a.z) + at, a.z_stride, rows, cols, a.wide, lane);
               }
             }
             activate_all(v, a.act);
@@ -904,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (a.residual) {
               move_rows(staging, const_cast<uint16_t*>(static_cast<const uint16_t*>(a.residual)) + row0 * a.r_stride + col,
-                        a.r_stride, rows, cols, a.unit, true, lane);
+                        a.r_stride, rows, cols, a.wide, true, lane);
               __syncwarp();
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
@@ -920,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
             }
           }
-          put_rows(staging, v, is_bf16, y + row0 * a.cols + col, a.cols, rows, cols, a.unit, lane);
+          put_rows(staging, v, is_bf16, y + row0 * a.cols + col, a.cols, rows, cols, a.wide, lane);
         }
         if (blocks) {
           fence_before();
@@ -1013,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (col + j < a.cols) o[j] = finish<FORM>(a, o[j], row, col + j, is_bf16);
         }
         uint16_t* const out = y + row * a.cols + col;
-        if (a.unit >= 4) {
+        if (a.wide) {
           *reinterpret_cast<uint2*>(out) = make_uint2(pack(o[0], o[1], is_bf16), pack(o[2], o[3], is_bf16));
         } else {
 #pragma unroll
