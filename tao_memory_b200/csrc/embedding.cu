@@ -6,7 +6,7 @@
 // once; the sums of one that goes on in the next run are joined by a second kernel, in the runs' order, so a word
 // that comes 10000 times is added by 625 blocks and the result does not depend on when they ran.  Rows of no
 // token are zeros.  32768 tokens, 65536 x 768 in bf16: the sort 28 us (latency), zeros 18 (5.6 TB/s), the runs 17 (with
-// runs of 32 and of 64, eight rows on their way, 35 and 47), the joins 8; the forward pass 13 (5.2 TB/s).
+// runs of 32 and of 64, eight rows on their way, 35 and 47), the joins 12; the forward pass 13 (5.2 TB/s).
 #include <cuda_runtime.h>
 
 #include "rows.cuh"

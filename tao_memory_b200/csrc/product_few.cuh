@@ -5,8 +5,9 @@
 // bytes of a row of x for each eight rows, all of its loads of a round at once, and gives them to mma.m16n8k16 as they
 // are: the order of the terms inside a product is free, as long as both operands use the same (lane (g, t) has terms
 // 8t .. 8t + 7 of 32).  So there is no shared memory, no barrier and no copy engine between memory and the tensor
-// cores, and all of W is on its way at once.  With 128-row tcgen05 tiles, a ring and clusters that add their parts
-// 1x2048x6144 took 14.4 us.
+// cores, and all of W is on its way at once.  1x2048x6144 takes 5.9 us (its bytes 3.9), 1x8192x8192 24.9 (20.5),
+// 16x8192x2048 11.8 (5.1), 24x8192x2048 14.9; with 128-row tcgen05 tiles, a ring and clusters that add their parts the first
+// took 14.4 us.  Of long rows each warp's rounds of loads bound it, and from 17 rows on x, read from L2 by every block.
 #pragma once
 #include "product.cuh"
 

