@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (PAIR) {  // this block's 128 rows of A and its half of B; both blocks' copies arrive at the first one's
       if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
       const uint32_t bar = peer(smem_u32(&full[s]), 0);
-      const int each = tile.blocks / a.pairs;
+      const int each = FORM == INPUT ? tile.blocks / a.pairs : tile.blocks;
       const bool other = kb >= each;
       const int k = (kb - (other ? each : 0)) * kTerms;
       tma_3d_pair(sa, other ? &map_a2 : &map_a, k, tile.row0 + rank * 128, 0, bar);

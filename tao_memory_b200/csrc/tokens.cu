@@ -35,7 +35,10 @@ struct TokenArgs {
   void *out, *dw;
 };
 
-TAO_DEVI int kept_of(const TokenArgs& a) { return a.kept ? (int)min((long long)*a.kept, a.pairs) : (int)a.pairs; }
+// At most all pairs, whatever the number says.
+TAO_DEVI int kept_of(const TokenArgs& a) {
+  return a.kept ? (int)min((long long)max(*a.kept, 0), a.pairs) : (int)a.pairs;
+}
 
 // out[places[t][j]] = in[t], or, WEIGHTED, weights[t][j] in[t] (zeros for a pair that is not kept).
 template <class T, int N, bool WIDE, bool WEIGHTED>

@@ -142,6 +142,14 @@ def test_orders_made_elsewhere_and_what_is_refused():
     missed = made.places[[3, 4], [1, 0]].long()
     same[missed] = True
     assert same.all()
+    for kept in (-1, -2 ** 31, 0, 2 ** 31 - 1):  # the number of pairs that have an expert is held within them
+        offsets = made.offsets.clone()
+        offsets[-1] = kept
+        leaf = ys.clone().requires_grad_(True)
+        y = return_tokens(leaf, TokenOrder(made.pairs, made.places, offsets))
+        dys, = torch.autograd.grad(y.sum(), leaf)
+        assert torch.equal(y.detach(), full if kept > 0 else torch.zeros_like(full))
+        assert (dys == (1 if kept > 0 else 0)).all()
     w, offsets = torch.randn(7, 8, 40, device="cuda").bfloat16(), made.offsets
     rows = ys.bfloat16()
     for bad in (lambda: sort_tokens(ids.float(), 7), lambda: sort_tokens(ids[0], 7), lambda: sort_tokens(ids, 0),
