@@ -74,23 +74,23 @@ struct Operands {
   Operand2 a, b, a2, b2;
 };
 
-// Clusters of `split` blocks that the device runs at once (how many blocks of a cluster find room in one GPC).
-template <int FORM, int BN>
-int clusters_of(int split) {
+// Clusters of `blocks` blocks that the device runs at once (how many of them find room in one GPC).
+template <int FORM, int BN, bool PAIR>
+int clusters_of(int blocks) {
   static std::atomic<int> known[16][9];  // of the first 16 devices
   int device = 0;
-  if (split == 1 || cudaGetDevice(&device) != cudaSuccess) return sms();
+  if (cudaGetDevice(&device) != cudaSuccess) return 1;
   if (device < 16)
-    if (const int n = known[device][split].load(std::memory_order_relaxed)) return n;
-  using C = Cfg<FORM, BN, false, true>;
-  auto kernel = product_kernel<FORM, BN, false, true, false, true>;
+    if (const int n = known[device][blocks].load(std::memory_order_relaxed)) return n;
+  using C = Cfg<FORM, BN, false, true, PAIR>;
+  auto kernel = product_kernel<FORM, BN, false, true, PAIR, true>;
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(split);
+  c.gridDim = dim3(blocks);
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = C::SMEM;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.x = blocks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   c.attrs = attr;
   c.numAttrs = 1;
@@ -100,7 +100,7 @@ int clusters_of(int split) {
     cudaGetLastError();
     n = 1;
   }
-  if (device < 16) known[device][split].store(n, std::memory_order_relaxed);
+  if (device < 16) known[device][blocks].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -129,13 +129,13 @@ int start_typed(const Operands& o, Args a, int split, cudaStream_t stream) {
   const long long col_tiles = (a.cols + C::CT - 1) / C::CT;
   long long tiles;
   if (FORM == WEIGHT)
-    tiles = (long long)(a.depth + 127) / 128 * col_tiles * a.groups * a.pairs;
+    tiles = (long long)(a.depth + C::DOWN - 1) / C::DOWN * col_tiles * a.groups * a.pairs;
   else  // of experts: no more than this
     tiles = ((a.rows + C::TT - 1) / C::TT + (a.offsets ? a.groups : 0)) * col_tiles;
   if (tiles > (1 << 29)) return pfail(TAO_ERR_CAPACITY, "the product has too many tiles");
   a.split = split;
   cudaLaunchConfig_t c = {};
-  const int together = SPLIT ? split : PAIR ? 2 : 1;  // blocks of a cluster
+  const int together = (SPLIT ? split : 1) * (PAIR ? 2 : 1);  // blocks of a cluster
   c.gridDim = dim3((unsigned)(together * (SPLIT ? tiles : std::min<long long>(tiles, sms() / together))));
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = C::SMEM;
@@ -162,11 +162,13 @@ struct Split {
   int blocks;
   double cost;
 };
-template <int FORM, int BN>
+template <int FORM, int BN, bool PAIR = false>
 Split split_of(long long tiles, int steps, double join) {
-  Split best = {1, (double)((tiles + sms() - 1) / sms()) * (steps + 6)};
-  for (int s = 2; s <= 8 && s <= steps; ++s) {
-    const int fit = clusters_of<FORM, BN>(s);
+  constexpr int TOGETHER = PAIR ? 2 : 1;
+  const int at_once = sms() / TOGETHER;
+  Split best = {1, (double)((tiles + at_once - 1) / at_once) * (steps + 6)};
+  for (int s = 2; s * TOGETHER <= 8 && s <= steps; ++s) {
+    const int fit = clusters_of<FORM, BN, PAIR>(s * TOGETHER);
     const double cost = (double)((tiles + fit - 1) / fit) * ((steps + s - 1) / s + join);
     if (cost < best.cost) best = {s, cost};
   }
@@ -647,17 +649,24 @@ int weight_gradient(const TaoLinear& p, const Operands& o, int pairs, cudaStream
     if (k > 128) return start<WEIGHT, 256, false, false>(o, a, 1, s);
     return start<WEIGHT, 128, false, false>(o, a, 1, s);
   }
-  // in steps of a 128 tile, as start_rows; a split of 256 columns takes 26 steps of its own more
+  // In steps of a 128 tile, as start_rows: of 256 columns a step 1.6 and a split 26 steps of its own more, by pairs 1.42 and
+  // 33.  Measured (us), 256 columns / pairs / 128: 2304x768 of 32768 rows 110.2 (split over 2) / 93.6 (over 2) / 172; 768x768
+  // of them 48.9 (over 6) / 50.0 (over 4) / 67 (over 3); 4096x4096 of 4096 125.4 / 109.3; 1024x1024 of 2048 17.6 / 17.1 / 13.1.
   const long long down = (n + 127) / 128;
   const int steps = (int)((p.rows + kTerms - 1) / kTerms), all = sms();
-  const long long narrow = (down * ((k + 127) / 128) + all - 1) / all * steps;
-  const Split split = split_of<WEIGHT, 256>(down * ((k + 255) / 256), steps, 26);
-  if (k <= 128 || narrow < 1.6 * split.cost) {
+  const double narrow = (double)((down * ((k + 127) / 128) + all - 1) / all) * steps;
+  const Split wide = split_of<WEIGHT, 256>(down * ((k + 255) / 256), steps, 26);
+  const Split pair = split_of<WEIGHT, 256, true>((n + 255) / 256 * (long long)((k + 255) / 256), steps, 33);
+  if (k <= 128 || narrow < std::min(1.6 * wide.cost, 1.42 * pair.cost)) {
     const Split half = split_of<WEIGHT, 128>(down * ((k + 127) / 128), steps, 32);
     if (half.blocks > 1 && half.cost < narrow) return start<WEIGHT, 128, false, true>(o, a, half.blocks, s);
     return start<WEIGHT, 128, false, false>(o, a, 1, s);
   }
-  if (split.blocks > 1) return start<WEIGHT, 256, false, true>(o, a, split.blocks, s);
+  if (1.42 * pair.cost < 1.6 * wide.cost) {
+    if (pair.blocks > 1) return start<WEIGHT, 256, false, true, true>(o, a, pair.blocks, s);
+    return start<WEIGHT, 256, false, false, true>(o, a, 1, s);
+  }
+  if (wide.blocks > 1) return start<WEIGHT, 256, false, true>(o, a, wide.blocks, s);
   return start<WEIGHT, 256, false, false>(o, a, 1, s);
 }
 

@@ -69,6 +69,7 @@ template <int FORM, int BN, bool GATED, bool SPLIT, bool PAIR = false>
 struct Cfg {
   static constexpr bool A_MN = FORM == WEIGHT, B_MN = FORM == INPUT || FORM == WEIGHT;
   static constexpr int TT = FORM == FEW ? BN : PAIR ? 256 : 128;                 // token rows of a tile
+  static constexpr int DOWN = PAIR ? 256 : 128;                                  // rows of a tile of WEIGHT
   static constexpr int CT = FORM == FEW ? 128 : GATED ? BN / 2 : BN;             // output columns of a tile
   static constexpr int A = (FORM == FEW && GATED ? 2 : 1) * 128 * 128, B = (PAIR ? BN / 2 : BN) * 128, STAGE = A + B;
   static constexpr int STAGING = FORM == FEW || SPLIT ? 0 : kWorkers * 2048;
@@ -153,10 +154,10 @@ TAO_DEVI void multiply_pair(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(acc),
       "l"(a), "l"(b), "r"(idesc), "r"(more));
 }
-TAO_DEVI void commit_pair(uint64_t* bar) {
+TAO_DEVI void commit_pair(uint64_t* bar, int first) {  // `first`: the rank of the pair's first block
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)(3 << first))
       : "memory");
 }
 TAO_DEVI void arrive_at(uint32_t bar) {
@@ -394,13 +395,13 @@ TAO_DEVI Tile tile_of(const Args& a, const int* first, const int* ends, int t, i
   const int col_tiles = (a.cols + C::CT - 1) / C::CT;
   tile.second = tile.from = tile.upto = 0;
   if constexpr (FORM == WEIGHT) {
-    const int row_tiles = (a.depth + 127) / 128, per = row_tiles * col_tiles;
+    const int row_tiles = (a.depth + C::DOWN - 1) / C::DOWN, per = row_tiles * col_tiles;
     const int matrix = t / per, at = t - matrix * per;
     group = matrix / a.pairs;
     tile.second = matrix - group * a.pairs;
-    tile.row0 = at % row_tiles * 128;
+    tile.row0 = at % row_tiles * C::DOWN;
     tile.col0 = at / row_tiles * C::CT;
-    tile.rows = min(128, a.depth - tile.row0);
+    tile.rows = min(C::DOWN, a.depth - tile.row0);
     if (a.offsets) {
       tile.from = group ? ends[group - 1] : 0;
       tile.upto = ends[group];
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const Args a) {
   using namespace tc;
   using C = Cfg<FORM, BN, GATED, SPLIT, PAIR>;
-  static_assert(!PAIR || ((FORM == FORWARD || FORM == INPUT) && BN == 256 && !SPLIT), "");
+  static_assert(!PAIR || (BN == 256 && FORM != FEW && (!SPLIT || FORM == WEIGHT)), "");
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* const staging_all = sm + C::STAGES * C::STAGE;
   uint64_t* const full = reinterpret_cast<uint64_t*>(staging_all + C::STAGING);
@@ -557,34 +558,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   constexpr bool is_bf16 = BF16;
   const int rank = SPLIT || PAIR ? (int)cluster_rank() : 0;
-  const int start = SPLIT ? (int)blockIdx.x / a.split : (int)blockIdx.x / (PAIR ? 2 : 1);
-  const int step = SPLIT ? 1 << 30 : (int)gridDim.x / (PAIR ? 2 : 1);
+  constexpr int TOGETHER = PAIR ? 2 : 1;  // blocks of a tile, or of a part of its terms
+  const int half_of_pair = PAIR ? rank & 1 : 0, first_of_pair = rank - half_of_pair, part_of_split = rank / TOGETHER;
+  const int start = SPLIT ? (int)blockIdx.x / (a.split * TOGETHER) : (int)blockIdx.x / TOGETHER;
+  const int step = SPLIT ? 1 << 30 : (int)gridDim.x / TOGETHER;
   // this block's part of a tile's steps
   auto part = [&](const Tile& t, int& k0) {
     if constexpr (!SPLIT) return k0 = 0, t.blocks;
-    k0 = (int)((long long)t.blocks * rank / a.split);
-    return (int)((long long)t.blocks * (rank + 1) / a.split) - k0;
+    k0 = (int)((long long)t.blocks * part_of_split / a.split);
+    return (int)((long long)t.blocks * (part_of_split + 1) / a.split) - k0;
   };
   // 64 terms of a tile into slot s, by one thread
   auto fetch = [&](const Tile& tile, int kb, int s) {
     uint8_t* const sa = sm + s * C::STAGE;
     uint8_t* const sb = sa + C::A;
     if constexpr (PAIR) {  // this block's 128 rows of A and its half of B; both blocks' copies arrive at the first one's
-      if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
-      const uint32_t bar = peer(smem_u32(&full[s]), 0);
+      if (half_of_pair == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+      const uint32_t bar = peer(smem_u32(&full[s]), first_of_pair);
+      const int row0 = tile.row0 + half_of_pair * 128, col0 = tile.col0 + half_of_pair * 128;
+      if constexpr (FORM == WEIGHT) {
+        const int k = tile.from + kb * kTerms;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          tma_3d_pair(sa + j * 8192, tile.second ? &map_a2 : &map_a, row0 + j * 64, k, 0, bar);
+          tma_3d_pair(sb + j * 8192, &map_b, col0 + j * 64, k, 0, bar);
+        }
+        return;
+      }
       const int each = FORM == INPUT ? tile.blocks / a.pairs : tile.blocks;
       const bool other = kb >= each;
       const int k = (kb - (other ? each : 0)) * kTerms;
-      tma_3d_pair(sa, other ? &map_a2 : &map_a, k, tile.row0 + rank * 128, 0, bar);
+      tma_3d_pair(sa, other ? &map_a2 : &map_a, k, row0, 0, bar);
       if constexpr (FORM == FORWARD) {
         if constexpr (GATED)
-          tma_3d_pair(sb, rank ? &map_b2 : &map_b, k, tile.col0, tile.group, bar);
+          tma_3d_pair(sb, half_of_pair ? &map_b2 : &map_b, k, tile.col0, tile.group, bar);
         else
-          tma_3d_pair(sb, &map_b, k, tile.col0 + rank * 128, tile.group, bar);
+          tma_3d_pair(sb, &map_b, k, col0, tile.group, bar);
       } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          tma_3d_pair(sb + j * 8192, other ? &map_b2 : &map_b, tile.col0 + rank * 128 + j * 64, k, tile.group, bar);
+        for (int j = 0; j < 2; ++j) tma_3d_pair(sb + j * 8192, other ? &map_b2 : &map_b, col0 + j * 64, k, tile.group, bar);
       }
       return;
     }
@@ -658,11 +670,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if constexpr (PAIR) cluster_sync();  // both blocks' barriers and accumulators are there
   fence_after();
   const uint32_t tbase = *tmem_slot;
-  if constexpr (SPLIT) cluster_arrive();  // this block has begun: its shared memory can be written to
+  if constexpr (SPLIT && !PAIR) cluster_arrive();  // this block has begun: its shared memory can be written to
 
   int total;
   if (FORM == WEIGHT)
-    total = (a.depth + 127) / 128 * ((a.cols + C::CT - 1) / C::CT) * a.groups * a.pairs;
+    total = (a.depth + C::DOWN - 1) / C::DOWN * ((a.cols + C::CT - 1) / C::CT) * a.groups * a.pairs;
   else
     total = a.offsets ? first[a.groups + 1] : (a.rows + C::TT - 1) / C::TT * ((a.cols + C::CT - 1) / C::CT);
 
@@ -684,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++s == C::STAGES) s = 0, phase ^= 1;
       }
     }
-    if (!ok && !(PAIR && rank)) {  // copies in flight (PAIR: both blocks') have their time before the block ends
+    if (!ok && !half_of_pair) {  // copies in flight (PAIR: both blocks') have their time before the block ends
       fetched = max(fetched, early);
       for (int i = max(fetched - C::STAGES, 0); i < fetched; ++i) mbar_wait(&full[i % C::STAGES], i / C::STAGES & 1, nullptr);
     }
@@ -697,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t desc_b = sdesc(smem_u32(sm) + C::A, C::B_MN ? 8192 : 16, 1024);
     int s = 0, phase = 0, set = 0, set_phase = 0;
     bool ok = true;
-    for (int t = PAIR && rank ? total : start; ok && t < total; t += step) {  // PAIR: the first block's for both
+    for (int t = half_of_pair ? total : start; ok && t < total; t += step) {  // PAIR: the first block's for both
       const Tile tile = tile_of<FORM, C>(a, first, ends, t, group);
       int k0;
       const int blocks = part(tile, k0);
@@ -741,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               multiply(acc + BN, da + (C::A / 2 >> 4) + k * STEP_A, db + k * STEP_B, idesc, k > 0 ? 1 : kb);
           }
           if constexpr (PAIR)
-            commit_pair(&empty[s]);
+            commit_pair(&empty[s], first_of_pair);
           else
             commit(&empty[s]);
         }
@@ -751,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (elected()) {
         if constexpr (PAIR)
-          commit_pair(&acc_full[set]);
+          commit_pair(&acc_full[set], first_of_pair);
         else
           commit(&acc_full[set]);
       }
@@ -761,9 +773,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elected()) {  // nothing is in flight when the block ends
       if constexpr (!PAIR)
         commit(over);
-      else if (rank == 0)
-        commit_pair(over);
-      if (!PAIR || rank == 0) mbar_wait(over, 0, nullptr);
+      else if (half_of_pair == 0)
+        commit_pair(over, first_of_pair);
+      if (half_of_pair == 0) mbar_wait(over, 0, nullptr);
     }
     __syncwarp();
   } else {
@@ -850,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         constexpr int HALF = C::CT / 2;
-        const int down = PAIR ? rank * 128 + quarter * 32 : quarter * 32;
+        const int down = half_of_pair * 128 + quarter * 32;
         const long long row0 = tile.row0 + down;
         const int rows = tile.rows - down;
         uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
@@ -929,7 +941,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) {
             if constexpr (PAIR)
-              arrive_at(peer(smem_u32(&acc_empty[set]), 0));
+              arrive_at(peer(smem_u32(&acc_empty[set]), first_of_pair));
             else
               mbar_arrive(&acc_empty[set]);
           }
@@ -953,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int share = FORM == FEW ? (min(BN, tile.rows) + a.split - 1) / a.split : 0;  // rows of x of a block
     constexpr int ROW = FORM == FEW ? 128 : BN + 4;                                   // floats of a row of a part
     float* const sums = reinterpret_cast<float*>(FORM == FEW ? staging_all + 512 : sm);
-    cluster_wait();
+    if constexpr (!PAIR) cluster_wait();
     if (warp < kWorkers) {
       constexpr int W = BN / 2 < 32 ? BN / 2 : 32;
       const int r = (warp & 3) * 32 + lane, begin = (warp >> 2) * (BN / 2);
@@ -985,8 +997,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();
     uint16_t* y = static_cast<uint16_t*>(FORM == WEIGHT && tile.second ? a.u : a.y);
     constexpr int ACROSS = FORM == FEW ? 32 : BN / 4;
-    const int first_row = FORM == FEW ? rank * share : 0, rows = FORM == FEW ? min(share, tile.rows - first_row) : tile.rows;
-    const int begin = FORM == FEW ? tid : rank * kThreads + tid, stride = FORM == FEW ? kThreads : kThreads * a.split;
+    const int first_row = FORM == FEW ? rank * share : half_of_pair * 128;
+    const int rows = min(FORM == FEW ? share : 128, tile.rows - first_row);
+    const int begin = FORM == FEW ? tid : part_of_split * kThreads + tid, stride = FORM == FEW ? kThreads : kThreads * a.split;
     constexpr int AT_ONCE = 4;  // sums whose parts are on their way
     for (int i0 = begin; i0 < ACROSS * rows; i0 += stride * AT_ONCE) {
       float4 v[AT_ONCE];
@@ -998,7 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < AT_ONCE; ++e) {
           const int i = min(i0 + e * stride, ACROSS * rows - 1), r = i / ACROSS, c = i % ACROSS * 4;
           w[e] = FORM == FEW ? *reinterpret_cast<const float4*>(sums + (q * share + r) * ROW + c)
-                             : ld_cluster(smem_u32(sums + r * ROW + c), q);
+                             : ld_cluster(smem_u32(sums + r * ROW + c), q * TOGETHER + half_of_pair);
         }
 #pragma unroll
         for (int e = 0; e < AT_ONCE; ++e) v[e].x += w[e].x, v[e].y += w[e].y, v[e].z += w[e].z, v[e].w += w[e].w;
