@@ -17,11 +17,11 @@
 // What bounds it: operands.  A step of a 128 x 256 tile fetches 48 KB for 512 cycles of products, more than an SM gets from
 // L2 in that time while all ask (about 700 cycles); the tensor pipe is busy 63 to 75 % of the time.  PAIR: two blocks with
 // 128 rows each multiply one 256 x 256 tile from both blocks' shared memory (cta_group::2), each fetching half of B:
-// 32 KB a step.  16384x2048x8192 takes 353 us in pairs (1.56 PFLOP/s; 380 alone), with bias and gelu 371;
-// 32768x768x2304 93 us; 32768 rows of 64 experts, gated 2048 to 1024, 232 us.
+// 32 KB a step.  16384x2048x8192 takes 353 us in pairs (1.56 PFLOP/s; 380 alone), with bias and gelu 368;
+// 32768x768x2304 93 us, its gradients 90 and 94; 32768 rows of 64 experts, gated 2048 to 1024, 232 us.
 //
-// SPLIT: a product with fewer tiles than SMs deals the terms of a tile to the blocks of a cluster, which add
-// their parts through each other's shared memory in the order of their ranks.
+// SPLIT: a product with fewer tiles than SMs deals the terms of a tile to the blocks (WEIGHT: or the pairs) of a cluster,
+// which add their parts through each other's shared memory in the order of their ranks.
 //
 // Experts: rows of x are sorted by expert, offsets[e] .. offsets[e + 1] are those of expert e.  Every block
 // makes the list of tiles itself from the offsets, so the host never reads them.  A row tile never spans
