@@ -257,7 +257,7 @@ int tao_embed(const void* ids, int id_bytes, long long n, const void* table, lon
   return by_part(type, wide, [&](auto t, auto v, auto w) {
     const Mapping m = mapping(n, (width + decltype(v)::value - 1) / decltype(v)::value);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if ((long long)m.grid.x * m.grid.y < 148 * 8) {  // all at once, a token a thread
+    if ((long long)m.grid.x * m.grid.y < 148 * 8) {  // all at once, a token a thread (32768x768: 22 us, four a thread 13)
       embed_kernel<decltype(t), decltype(v)::value, decltype(w)::value, 1><<<m.grid, m.block, 0, s>>>(a);
     } else {
       const dim3 grid((m.grid.x + 3) / 4, m.grid.y);

@@ -218,7 +218,11 @@ int start_few(const FewArgs& a, int type, cudaStream_t s) {
   return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
 }
 
-// Up to 32 rows; `false`: the tcgen05 form is the faster one.
+// Up to 32 rows; `false`: the tcgen05 form is the faster one.  More warps where there are few blocks and long sums, fewer
+// where a warp would have no round.  Measured (us, warps x rounds ahead), one row: 6144 outputs of 2048 terms 8x4 7.0, 8x8 7.6,
+// 4x8 7.1; 2048 of 8192 16x4 9.9, 8x8 10.8; 8192 of 8192 8x8 25.3, 8x4 29.6; 640 of 2048 16x4 3.3, 8x4 4.0; 16384 of 512 4x4
+// 4.9, 8x4 9.2.  Sixteen rows: 6144 of 2048 8x2 8.4, 16x4 10.4; 2048 of 8192 16x4 11.7, 8x2 19.0.  32 rows: 2048 of 8192 16x2
+// 15.4, 8x1 28.7 (tcgen05 14.7); 6144 of 2048 8x1 11.4, 16x2 14.0 (13.5); 8192 of 8192 8x1 38.4 (28.7).
 bool few_rows(const FewArgs& a, int type, cudaStream_t s, int* rc) {
   const int outputs = (a.n + 15) / 16, rounds = (a.k + 31) / 32;
   const bool narrow = outputs <= 148 && rounds >= 48;
@@ -603,13 +607,18 @@ int forward(const TaoLinear& p, Rooms& rooms, cudaStream_t s) {
                           (p.residual ? bits_of(p.residual, p.r_row) : 0)) == 8;
   const int steps = (k + kTerms - 1) / kTerms;
   if (p.offsets) {
+    // By the experts' mean rows, columns of 32 or 64 rows or tiles of 128.  64 experts gated 2048 to 1024 (us): mean 4
+    // 63.3 / 63.5 / 66.9, 24 82.4 / 81.3 / 88.0, 32 78.2 / 70.0 / 78.1, 64 97.8 / 91.9 / 91.1, 96 120.4 / 107.2 / 100.8; 128
+    // experts 1024 to 512: mean 8 36.3 / 38.2 / 40.4, 48 53.1 / 50.2 / 50.1.
     const long long mean = rows / p.experts;
     const Operands few = {ow, ox, ou, none}, many = {ox, ow, none, ou};
     if (p.up) {
-      if (mean <= 32) return start<FEW, 32, true, false>(few, a, 1, s);
+      if (mean <= 24) return start<FEW, 32, true, false>(few, a, 1, s);
+      if (mean <= 64) return start<FEW, 64, true, false>(few, a, 1, s);
       return start_rows<FORWARD, true>(many, a, steps, s);
     }
-    if (mean <= 32) return start<FEW, 32, false, false>(few, a, 1, s);
+    if (mean <= 24) return start<FEW, 32, false, false>(few, a, 1, s);
+    if (mean <= 64) return start<FEW, 64, false, false>(few, a, 1, s);
     return start_rows<FORWARD>(many, a, steps, s);
   }
   if (rows <= 32) {

@@ -3,7 +3,7 @@
 // of many experts at once.  fp32 accumulators in TMEM, one rounding when a value is stored.
 //
 //   FORWARD  y[t][c] = act(sum_k x[t][k] W[c][k] + bias[c]) + residual[t][c], or act(x W^T) * (x U^T)
-//   FEW      the same for few rows: W is the operand of 128 rows, x the one of 16 to 64 columns, so that
+//   FEW      the same for few rows: W is the operand of 128 rows, x the one of 32 or 64 columns, so that
 //            a tile does not multiply rows that are not there
 //   INPUT    dx[t][k] = sum_c dz[t][c] W[c][k] (+ du U)
 //   WEIGHT   dW[c][k] = sum_t dz[t][c] x[t][k]
@@ -181,21 +181,16 @@ TAO_DEVI void multiply(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, uin
 // N consecutive fp32 columns of this thread's TMEM lane.
 template <int N>
 TAO_DEVI void load_columns(uint32_t at, float (&v)[N]) {
-  static_assert(N == 8 || N == 16 || N == 32, "");
+  static_assert(N == 16 || N == 32, "");
   if constexpr (N == 32) {
     tc::tmem_ld32(at, v);
   } else {
     uint32_t r[N];
-    if constexpr (N == 16)
-      asm volatile(
-          "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-            "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-          : "r"(at));
-    else
-      asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                   : "r"(at));
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);

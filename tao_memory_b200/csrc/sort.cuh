@@ -20,7 +20,7 @@ namespace tao {
 namespace sorting {
 
 constexpr int kMostBins = 513;  // 512 and one for what belongs to none
-constexpr int kSmallSort = 8192;
+constexpr int kSmallSort = 4096;  // one block and launch 8.4 us, two launches 7.6 and the host's second; 8192: 13.5, 7.6
 constexpr int kMostBlocks = 128;
 
 // A pass over n elements.  The key of element i is ids[value], value = values[i] or (values null) i: the whole id

@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(256) return_kernel(const TokenArgs a) {
 }
 
 // dw[t][j] = in[t] . other[places[t][j]], zero for a pair that is not kept.  WARPS a token (one, or where that leaves the
-// device empty eight, whose sums are added in their order), AT_ONCE experts' rows on their way at once.  (In one
+// device empty eight, whose sums are added in their order: 100 tokens of 3584 fp32 channels to 6 experts 6.3 us, by one
+// warp each 21.5), AT_ONCE experts' rows on their way at once.  (In one
 // kernel with the rows' gradient, which writes as much as this reads, the two took 115 to 156 us for 32768 tokens of 768
 // channels and 4 experts.)
 template <class T, int N, bool WIDE, int AT_ONCE, int WARPS>

@@ -30,7 +30,7 @@ def _order(ids, experts):
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("tokens,k,experts", [(1, 1, 1), (1, 8, 64), (5, 3, 7), (64, 8, 64), (1000, 2, 512), (1024, 8, 40),
+@pytest.mark.parametrize("tokens,k,experts", [(1, 1, 1), (1, 8, 64), (5, 3, 7), (64, 8, 64), (1000, 2, 512), (1024, 4, 40), (1025, 4, 5), (1024, 8, 40),
                                               (1025, 8, 5), (3001, 3, 512), (40000, 4, 129), (70000, 8, 64), (9000, 1, 1)])
 def test_order(tokens, k, experts, dtype):
     from tao_memory_b200 import sort_tokens
@@ -228,7 +228,7 @@ COUNTS = [([1], 0), ([0, 5, 0, 0], 0), ([3, 0, 200, 64, 1], 9), ([300, 129, 0, 1
 
 @pytest.mark.parametrize("dtype", TYPES[:2])
 @pytest.mark.parametrize("gated", [True, False])
-@pytest.mark.parametrize("counts,none", COUNTS)
+@pytest.mark.parametrize("counts,none", COUNTS + [([30, 50, 41, 0], 8), ([90, 33, 64, 1], 0), ([70] * 5, 0)])
 def test_experts(counts, none, gated, dtype):
     for k, n in ((64, 64), (136, 264), (1000, 130), (33, 7)):
         x, w, up, offsets, dy = _experts_case(counts, none, k, n, dtype, gated, seed=k)
