@@ -59,10 +59,11 @@ def _room(p, rows, gradient):
 
 
 def _point(p, kept, up):
-    p.z, p.z_row = kept.data_ptr(), kept.shape[-1]
+    at = kept.data_ptr()
+    p.z, p.z_row = at, kept.shape[-1]
     if up is not None:
         plane = 2 * kept.shape[1] * kept.shape[2]
-        p.u, p.low = p.z + plane, p.z + 2 * plane
+        p.u, p.low = at + plane, at + 2 * plane
 
 
 def _forward(p, rows, up, keep):

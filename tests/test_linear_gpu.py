@@ -55,6 +55,15 @@ def test_sizes(rows, k, n, dtype):
     _check(x, w, None, None, dy, None)
 
 
+# pairs of blocks: forward, the input's and the weight's gradient, the last one split or not; whole and ragged tiles
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k,n,name", [(5100, 2050, 2600, "silu"), (5120, 2048, 2560, None), (4737, 2056, 2497, "gelu"),
+                                           (20000, 770, 2300, None)])
+def test_pairs_of_blocks(rows, k, n, name, dtype):
+    x, w, b, res, dy = _inputs(rows, k, n, dtype, True, True, seed=rows)
+    _check(x, w, b, res, dy, name)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("rows,k,n", [(5, 72, 40), (64, 100, 129), (90, 256, 65), (1500, 64, 1200), (2500, 72, 2312)])

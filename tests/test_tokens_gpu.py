@@ -243,6 +243,14 @@ def test_experts_activations(name, gated):
                        _experts_case(counts, 5, 72, 136, torch.bfloat16, gated)[4])
 
 
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("dtype", TYPES[:2])
+def test_experts_by_pairs_of_blocks(dtype, gated):
+    """Experts of many rows, some whose last pair has one block's rows or fewer, one without any, rows of none."""
+    x, w, up, offsets, dy = _experts_case([2600, 0, 1300, 2501, 130, 1], 77, 1032, 2600, dtype, gated, seed=3)
+    _check_experts(x, w, up, offsets, "silu" if gated else None, dy)
+
+
 def test_512_experts():
     g = torch.Generator().manual_seed(1)
     counts = torch.randint(0, 9, (512,), generator=g).tolist()
