@@ -58,7 +58,8 @@ def test_sizes(rows, k, n, dtype):
 # pairs of blocks: forward, the input's and the weight's gradient, the last one split or not; whole and ragged tiles
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,k,n,name", [(5100, 2050, 2600, "silu"), (5120, 2048, 2560, None), (4737, 2056, 2497, "gelu"),
-                                           (20000, 770, 2300, None)])
+                                           (20000, 770, 2300, None), (20001, 762, 2297, None), (16500, 768, 2304, "relu"),
+                                           (1031, 3902, 4090, None), (1100, 4096, 4096, "gelu"), (3701, 4090, 4095, None)])
 def test_pairs_of_blocks(rows, k, n, name, dtype):
     x, w, b, res, dy = _inputs(rows, k, n, dtype, True, True, seed=rows)
     _check(x, w, b, res, dy, name)
