@@ -289,19 +289,20 @@ int tao_embed_gradient(const void* ids, int id_bytes, long long n, const void* d
   }
   if (overlaps(dtable, vocab * width * size, {extent(dy, n, dy_stride * size, width * size), extent(ids, 1, 0, n * id_bytes)}))
     return efail(TAO_ERR_ARG, "the table's gradient must not overlap the rows' or the ids");
-  cudaError_t e = cudaMemsetAsync(dtable, 0, (size_t)vocab * width * size, s);
-  if (e != cudaSuccess || n == 0) return launched(e);
+  if (n == 0) return launched(cudaMemsetAsync(dtable, 0, (size_t)vocab * width * size, s));
+  cudaError_t e = cudaSuccess;
   const Room r = room_of(n, vocab, width);
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   int passes;
   const int bits = bits_of(vocab, &passes);
   sorting::Pass p = {};
+  sorting::Clearing zeros = {static_cast<uint8_t*>(dtable), vocab * width * (long long)size, passes * sorting::launches_of(n)};
   p.ids = ids, p.limit = vocab, p.n = (int)n, p.bins = 1 << bits, p.wide = id_bytes == 8;
   for (int i = 0; i < passes; ++i) {
     p.shift = i * bits;
     p.sorted = reinterpret_cast<int*>(ws + r.values[i & 1]);
     p.keys = i + 1 == passes ? reinterpret_cast<int*>(ws + r.ids) : nullptr;
-    e = sorting::run(p, reinterpret_cast<int*>(ws + r.counts), s);
+    e = sorting::run(p, reinterpret_cast<int*>(ws + r.counts), s, &zeros);
     if (e != cudaSuccess) return launched(e);
     p.values = p.sorted;
   }

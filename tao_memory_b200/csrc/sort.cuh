@@ -37,7 +37,24 @@ struct Pass {
   int* places;              // where element i went, or null
   int* keys;                // whole ids in order, or null
   int* offsets;             // the first place of each bin, or null
+  uint8_t* zero;            // what the blocks behind the sort's own fill with zeros meanwhile: on 2 bytes
+  long long zero_bytes;
 };
+
+// Zeros of a range by blocks behind the sort's, by 16 bytes and what is left at its ends by two.
+TAO_DEVI void clear(const Pass& p) {
+  const int block = blockIdx.x - p.blocks, blocks = gridDim.x - p.blocks;
+  uint8_t* const end = p.zero + p.zero_bytes;
+  uint4* const from = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(p.zero) + 15) / 16 * 16);
+  uint4* const to = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(end) / 16 * 16);
+  for (uint4* at = from + (long long)block * blockDim.x + threadIdx.x; at < to; at += (long long)blocks * blockDim.x)
+    *at = make_uint4(0, 0, 0, 0);
+  if (block > 0 || threadIdx.x >= 8) return;
+  uint8_t* const head = p.zero + 2 * threadIdx.x;
+  if (head < end && head < reinterpret_cast<uint8_t*>(from)) *reinterpret_cast<uint16_t*>(head) = 0;
+  uint8_t* const tail = reinterpret_cast<uint8_t*>(to) + 2 * threadIdx.x;
+  if (tail >= p.zero && tail < end) *reinterpret_cast<uint16_t*>(tail) = 0;
+}
 
 TAO_DEVI int id_of(const Pass& p, int value) {
   const long long id = p.wide ? static_cast<const long long*>(p.ids)[value] : static_cast<const int*>(p.ids)[value];
@@ -73,6 +90,7 @@ TAO_DEVI void count_warps(const Pass& p, int* counts, int warps) {
 template <int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) count_kernel(const Pass p, int* out) {
   extern __shared__ int counts[];
+  if (blockIdx.x >= p.blocks) return clear(p);
   count_warps(p, counts, WARPS);
   for (int b = threadIdx.x; b < p.bins; b += 32 * WARPS) {
     int s = 0;
@@ -87,6 +105,7 @@ __global__ void __launch_bounds__(32 * WARPS) place_kernel(const Pass p) {
   extern __shared__ int counts[];
   __shared__ int first[kMostBins], before[kMostBins];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x >= p.blocks) return clear(p);
   count_warps(p, counts, WARPS);
   for (int b = threadIdx.x; b < p.bins; b += 32 * WARPS) {
     int all = 0;
@@ -172,8 +191,27 @@ __global__ void __launch_bounds__(32 * WARPS) place_kernel(const Pass p) {
 inline int blocks_of(long long n) { return n <= kSmallSort ? 1 : (int)std::min<long long>((n + 1023) / 1024, kMostBlocks); }
 inline size_t counts_bytes(long long n, int bins) { return n <= kSmallSort ? 0 : (size_t)blocks_of(n) * bins * sizeof(int); }
 
+inline int launches_of(long long n) { return blocks_of(n) == 1 ? 1 : 2; }
+
+// Bytes that become zeros while a sort runs, a share of them in each of its launches.
+struct Clearing {
+  uint8_t* at;
+  long long bytes;
+  int launches;  // of the sort, that are left
+  // The next launch's share, and the blocks of `threads` for it.
+  int next(Pass& p, int threads) {
+    if (!launches) return 0;
+    const long long share = launches == 1 ? bytes : bytes / launches / 16 * 16;
+    p.zero = at, p.zero_bytes = share;
+    at += share, bytes -= share, --launches;
+    return (int)std::min<long long>((share + threads * 16 - 1) / (threads * 16), 148ll * 1024 / threads);
+  }
+};
+
 // `counts`: counts_bytes of scratch.
-inline cudaError_t run(Pass p, int* counts, cudaStream_t s) {
+inline cudaError_t run(Pass p, int* counts, cudaStream_t s, Clearing* zeros = nullptr) {
+  Clearing none = {};
+  if (!zeros) zeros = &none;
   p.blocks = blocks_of(p.n);
   if (p.blocks == 1) {
     p.counts = nullptr;
@@ -189,14 +227,17 @@ inline cudaError_t run(Pass p, int* counts, cudaStream_t s) {
       if (e == cudaSuccess) ready |= mark;
     }
     if (e != cudaSuccess) return e;
-    place_kernel<32><<<1, 1024, 32 * p.bins * sizeof(int), s>>>(p);
+    const int more = zeros->next(p, 1024);
+    place_kernel<32><<<1 + more, 1024, 32 * p.bins * sizeof(int), s>>>(p);
     return cudaGetLastError();
   }
   const int warps = p.blocks * 8;
   p.per = (int)(((long long)p.n + warps - 1) / warps + 31) / 32 * 32;
   p.counts = counts;
-  count_kernel<8><<<p.blocks, 256, 8 * p.bins * sizeof(int), s>>>(p, counts);
-  place_kernel<8><<<p.blocks, 256, 8 * p.bins * sizeof(int), s>>>(p);
+  const int counting = zeros->next(p, 256);
+  count_kernel<8><<<p.blocks + counting, 256, 8 * p.bins * sizeof(int), s>>>(p, counts);
+  const int placing = zeros->next(p, 256);
+  place_kernel<8><<<p.blocks + placing, 256, 8 * p.bins * sizeof(int), s>>>(p);
   return cudaGetLastError();
 }
 

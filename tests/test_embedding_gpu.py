@@ -86,6 +86,28 @@ def test_ids_that_are_none():
     assert (y[[0, 1, 2, 3, 5]] == 0).all() and torch.equal(y[4], table[9])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [0, 1, 5, 8])
+@pytest.mark.parametrize("n,vocab,width", [(1, 1, 1), (1, 3, 5), (2, 700, 129), (4096, 600, 64), (4097, 33, 7), (40000, 300000, 24),
+                                           (9, 40001, 1031)])
+def test_gradient_fills_the_table_and_no_more(n, vocab, width, offset, dtype):
+    """Every row of a table that held NaN, from any element on, and nothing before or behind it."""
+    from tao_memory_b200 import _lib
+    from tao_memory_b200.norm import TYPES as CODES
+    g = torch.Generator(device="cuda").manual_seed(n)
+    ids = torch.randint(-1, vocab, (n,), device="cuda", generator=g)
+    dy = torch.ones(n, width, device="cuda", dtype=dtype)
+    held = torch.full((offset + vocab * width + 16,), float("nan"), device="cuda", dtype=dtype)
+    table = held[offset:offset + vocab * width]
+    size = _lib.lib().tao_embed_gradient_workspace_bytes(n, vocab, width)
+    room = torch.empty(size, dtype=torch.uint8, device="cuda")
+    _lib.on_device(0, _lib.lib().tao_embed_gradient, ids.data_ptr(), 8, n, dy.data_ptr(), width, vocab, width, CODES[dtype],
+                   1.0, table.data_ptr(), room.data_ptr(), size)
+    counts = torch.bincount(ids[ids >= 0], minlength=vocab).to(dtype)  # whole numbers up to 256: exact, or rounded once
+    assert torch.equal(table.view(vocab, width), counts.unsqueeze(1).expand(vocab, width))
+    assert held[:offset].isnan().all() and held[offset + vocab * width:].isnan().all()
+
+
 def test_refusals():
     from tao_memory_b200 import embed
     table, ids = torch.randn(10, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
