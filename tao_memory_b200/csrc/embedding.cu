@@ -147,19 +147,37 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
   }
 }
 
-// Ids that begin in one of the block's eight runs and go on behind it.  A warp looks at a run, then all join what was
-// found one by one: a warp has 32 threads' columns, the warps share out the id's runs, and their sums are added in order.
+// Ids that begin in one of the block's eight runs and go on behind it.  A warp looks at a run and joins up to eight that
+// follow it by itself; what goes on further all join, one by one: a warp has 32 threads' columns, the warps share out the
+// id's runs, and their sums are added in order.  (All of them by all warps: 200000 tokens of 50257 words 68 us.)
 template <class T, int N, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
   __shared__ float sums[8][N][33];
   __shared__ int found[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = (a.n + kRun - 1) / kRun;
+  const int c = first_of<N, WIDE>(blockIdx.y, 32, lane);
   {
     const int run = blockIdx.x * 8 + warp, begin = run * kRun, end = begin + kRun;
     int id = -1;
     if (end < a.n) {  // the last run goes on nowhere
       const int last = a.ids[end - 1], before = a.ids[max(begin - 1, 0)], first = a.ids[begin], next = a.ids[end];
       if (next == last && last < a.vocab && !(begin > 0 && first == last && before == last)) id = last;
+    }
+    const int later = run + 2 + lane;  // those of the runs behind the next that begin with the id
+    const bool more = id >= 0 && lane < 8 && later < runs && a.ids[min(later, runs - 1) * kRun] == id;
+    const int count = 1 + __popc(__ballot_sync(0xffffffffu, more));
+    if (id >= 0 && count <= 8) {
+      if (c < a.width) {
+        float sum[N] = {};
+        add_sums<N, WIDE>(a.parts + ((long long)run * 2 + 1) * a.width, c, 32, a.width, sum);
+#pragma unroll 4
+        for (int r = 0; r < count; ++r)
+          add_sums<N, WIDE>(a.parts + ((long long)run + 1 + r) * 2 * a.width, c, 32, a.width, sum);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] *= a.scale;
+        Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, 32, a.width);
+      }
+      id = -1;
     }
     if (lane == 0) found[warp] = id;
   }
@@ -174,7 +192,7 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
       more = __syncthreads_count(run < runs && a.ids[min(run, runs - 1) * kRun] == id);
       last += more;
     }
-    const int c = first_of<N, WIDE>(blockIdx.y, 32, lane), count = last - run0;
+    const int count = last - run0;
     float sum[N] = {};
     if (c < a.width) {
       if (warp == 0) add_sums<N, WIDE>(a.parts + ((long long)run0 * 2 + 1) * a.width, c, 32, a.width, sum);
