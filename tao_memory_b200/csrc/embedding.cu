@@ -3,10 +3,11 @@
 // Forward: bound by its bytes (and for a few tokens by the launch); a thread has 16 bytes of a row.
 // Gradient: the tokens are sorted by id (sort.cuh, stably), and a block adds the rows of a run of kRun sorted
 // tokens, in fp32 and in their order, a sum for each id.  An id whose tokens lie within the run is written at
-// once; the sums of one that goes on in the next run are joined by a second kernel, in the runs' order, so a word
-// that comes 10000 times is added by 625 blocks and the result does not depend on when they ran.  Rows of no
-// token are zeros.  32768 tokens, 65536 x 768 in bf16: the sort 28 us (latency), zeros 18 (5.6 TB/s), the runs 17 (with
-// runs of 32 and of 64, eight rows on their way, 35 and 47), the joins 12; the forward pass 13 (5.2 TB/s).
+// once; the sums of one that goes on in the next run are joined by a second kernel, in a fixed order of the runs, so a
+// word that comes 10000 times is added by 625 blocks and the result does not depend on when they ran.  Rows of no
+// token are zeros, written by blocks beside the sort's (bound by latency), before the sums.  32768 tokens, 65536 x 768 in
+// bf16: sort and zeros 37 us (one after the other 28 and 18), the runs 19 (with runs of 32 and of 64, eight rows on
+// their way, 35 and 47), the joins 5; the forward pass 18 after a flush, 13 in turn (5.2 TB/s).
 #include <cuda_runtime.h>
 
 #include "rows.cuh"
@@ -148,25 +149,32 @@ __global__ void __launch_bounds__(256) run_kernel(const SumArgs a) {
 }
 
 // Ids that begin in one of the block's eight runs and go on behind it.  A warp looks at a run and joins up to eight that
-// follow it by itself; what goes on further all join, one by one: a warp has 32 threads' columns, the warps share out the
-// id's runs, and their sums are added in order.  (All of them by all warps: 200000 tokens of 50257 words 68 us.)
+// follow it by itself.  An id that goes on further has the blocks whose runs have no other to help the one where it
+// begins: they share out its columns in fours (of the 32 threads' that gridDim.y parts have), and a block's threads the
+// runs, whose sums are added in order.  200000 tokens of 50257 words 24 us (each joined by all warps of a block: 68),
+// with a quarter of them one word's 60 (by its first block alone: 188).
 template <class T, int N, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
-  __shared__ float sums[8][N][33];
-  __shared__ int found[8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = (a.n + kRun - 1) / kRun;
-  const int c = first_of<N, WIDE>(blockIdx.y, 32, lane);
+  constexpr int SHARES = 32, LANES = 8;
+  __shared__ float sums[SHARES][N][LANES + 1];
+  __shared__ int head;  // the run where an id of more than nine runs begins: one in eight at most
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = (a.n + kRun - 1) / kRun, run8 = blockIdx.x * 8;
+  const auto begins = [&](int run, int id) { return run < runs && a.ids[min(run, runs - 1) * kRun] == id; };
+  if (threadIdx.x == 0) head = -1;
+  __syncthreads();
   {
-    const int run = blockIdx.x * 8 + warp, begin = run * kRun, end = begin + kRun;
+    const int run = run8 + warp, begin = run * kRun, end = begin + kRun;
     int id = -1;
     if (end < a.n) {  // the last run goes on nowhere
       const int last = a.ids[end - 1], before = a.ids[max(begin - 1, 0)], first = a.ids[begin], next = a.ids[end];
       if (next == last && last < a.vocab && !(begin > 0 && first == last && before == last)) id = last;
     }
-    const int later = run + 2 + lane;  // those of the runs behind the next that begin with the id
-    const bool more = id >= 0 && lane < 8 && later < runs && a.ids[min(later, runs - 1) * kRun] == id;
+    const bool more = id >= 0 && lane < 8 && begins(run + 2 + lane, id);
     const int count = 1 + __popc(__ballot_sync(0xffffffffu, more));
-    if (id >= 0 && count <= 8) {
+    if (id >= 0 && count > 8) {
+      if (lane == 0) head = run;
+    } else if (id >= 0) {
+      const int c = first_of<N, WIDE>(blockIdx.y, 32, lane);
       if (c < a.width) {
         float sum[N] = {};
         add_sums<N, WIDE>(a.parts + ((long long)run * 2 + 1) * a.width, c, 32, a.width, sum);
@@ -177,38 +185,55 @@ __global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
         for (int e = 0; e < N; ++e) sum[e] *= a.scale;
         Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, 32, a.width);
       }
-      id = -1;
     }
-    if (lane == 0) found[warp] = id;
   }
   __syncthreads();
-  for (int f = 0; f < 8; ++f) {
-    const int id = found[f];
-    if (id < 0) continue;
-    const int run0 = blockIdx.x * 8 + f;
-    int last = run0 + 1;  // the last run that begins with the id: sorted, those that do follow each other
+  // sorted: the runs that begin with an id follow each other
+  int run0 = head, id;
+  if (run0 >= 0) {
+    id = a.ids[min(run0 * kRun + kRun, a.n) - 1];
+  } else {
+    if (run8 == 0 || run8 + 8 >= runs) return;
+    id = a.ids[run8 * kRun];
+    if (id >= a.vocab || a.ids[run8 * kRun - 1] != id || a.ids[(run8 + 8) * kRun] != id) return;
+    run0 = run8;  // the first that begins with it
     for (int more = 256; more == 256;) {
-      const int run = last + 1 + threadIdx.x;
-      more = __syncthreads_count(run < runs && a.ids[min(run, runs - 1) * kRun] == id);
-      last += more;
+      const int run = run0 - 1 - (int)threadIdx.x;
+      more = __syncthreads_count(run >= 0 && begins(run, id));
+      run0 -= more;
     }
-    const int count = last - run0;
+    if (run0 > 0 && a.ids[run0 * kRun - 1] == id) --run0;
+  }
+  int last = head >= 0 ? run0 + 1 : run8 + 8;  // the last that does
+  for (int more = 256; more == 256;) {
+    more = __syncthreads_count(begins(last + 1 + threadIdx.x, id));
+    last += more;
+  }
+  const int count = last - run0, rank = blockIdx.x - run0 / 8, helpers = max(1, last / 8 - run0 / 8);
+  const int share = threadIdx.x / LANES, at = threadIdx.x % LANES;
+  for (int slice = rank; slice < 32 / LANES; slice += helpers) {
+    const int c = first_of<N, WIDE>(blockIdx.y, 32, slice * LANES + at);
     float sum[N] = {};
     if (c < a.width) {
-      if (warp == 0) add_sums<N, WIDE>(a.parts + ((long long)run0 * 2 + 1) * a.width, c, 32, a.width, sum);
+      if (share == 0) add_sums<N, WIDE>(a.parts + ((long long)run0 * 2 + 1) * a.width, c, 32, a.width, sum);
+      const int to = (int)((long long)count * (share + 1) / SHARES);
 #pragma unroll 8
-      for (int r = count * warp / 8; r < count * (warp + 1) / 8; ++r)
+      for (int r = (int)((long long)count * share / SHARES); r < to; ++r)
         add_sums<N, WIDE>(a.parts + ((long long)run0 + 1 + r) * 2 * a.width, c, 32, a.width, sum);
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) sums[warp][e][lane] = sum[e];
+    for (int e = 0; e < N; ++e) sums[share][e][at] = sum[e];
     __syncthreads();
-    if (warp == 0 && c < a.width) {
+    if (share < N) {
+      float s = sums[0][share][at];
+#pragma unroll 8
+      for (int w = 1; w < SHARES; ++w) s += sums[w][share][at];
+      sums[0][share][at] = s * a.scale;  // this thread's own
+    }
+    __syncthreads();
+    if (share == 0 && c < a.width) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        for (int w = 1; w < 8; ++w) sum[e] += sums[w][e][lane];
-        sum[e] *= a.scale;
-      }
+      for (int e = 0; e < N; ++e) sum[e] = sums[0][e][at];
       Part<T, N, WIDE>::of(sum).store(static_cast<T*>(a.out) + (long long)id * a.width, c, 32, a.width);
     }
     __syncthreads();

@@ -58,6 +58,21 @@ def test_one_word_many_times(share):
     _check(sorted_ids, table, 1.0, dy)
 
 
+@pytest.mark.parametrize("dtype,width", [(torch.bfloat16, 768), (torch.float16, 301), (torch.float32, 260)])
+@pytest.mark.parametrize("least,most", [(100, 200), (130, 400), (300, 900), (16, 5000)])
+def test_long_words_one_after_the_other(least, most, dtype, width):
+    """Words of many lengths, so that their first and last tokens lie anywhere among the runs that join them."""
+    g = torch.Generator(device="cuda").manual_seed(least)
+    vocab = 120
+    lengths = torch.randint(least, most + 1, (vocab,), device="cuda", generator=g)
+    lengths[::3] = lengths[::3] // 16 * 16  # and on their borders
+    ids = torch.repeat_interleave(torch.arange(vocab, device="cuda"), lengths)
+    ids = ids[torch.randperm(len(ids), device="cuda", generator=g)]
+    table, dy = (torch.randn(s, width, device="cuda", generator=g).to(dtype) for s in (vocab, len(ids)))
+    _check(ids, table, 1.0, dy)
+    _check(torch.cat([ids, ids.new_full((777,), vocab)]), table, 1.0, torch.cat([dy, dy[:777]]))
+
+
 def test_shapes_and_views():
     table = torch.randn(300, 200, device="cuda").bfloat16()
     ids = torch.randint(-2, 110, (6, 10), device="cuda")
