@@ -550,7 +550,8 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
  * by expert, offsets[e] .. offsets[e + 1] - 1 those of expert e:
  *   y = act(x W_e^T), or with `up` (like W) the gated act(x W_e^T) * (x U_e^T).
  * offsets[0] is taken as 0, values are held between the one before and `rows`, and rows from offsets[experts] on
- * give zeros.  z [rows][z_row]: what act is applied to, rounded to the type, for the gradient, or NULL.  Gated: z and u
+ * give zeros.  z [rows][z_row]: what act is applied to, rounded to the type, for the gradient (which takes an
+ * infinity there as a very large argument), or NULL.  Gated: z and u
  * are the upper 16 bits of act's argument and of its factor as fp32 numbers cut to 24 bits, and low [2][rows][z_row] bytes
  * has the lower 8 of both; the three start on 16 bytes, z_row is a multiple of 16, and all of a row may be written.
  *

@@ -293,22 +293,23 @@ TAO_DEVI float activate(float z, int act) {
   }
   return z;
 }
-// act(z) and act'(z).
+// act(z) and act'(z).  `near`: far out act' is 0 or 1, but as it is written 0 times z, which may be infinite (an argument
+// kept in fp16 is from 65520 on; NaN stays NaN by the other factors).
 TAO_DEVI float2 activate_slope(float z, int act) {
+  const float near = fminf(fmaxf(z, -128.f), 128.f);
   switch (act) {
     case TAO_ACT_RELU: return make_float2(z > 0.f || z != z ? z : 0.f, z > 0.f ? 1.f : 0.f);
     case TAO_ACT_SILU: {
       const float s = sigmoid(z);
-      return make_float2(z * s, s * (1.f + z * (1.f - s)));
+      return make_float2(z * s, s * (1.f + near * (1.f - s)));
     }
     case TAO_ACT_GELU: {
       float density;
       const float p = normal_integral(z, density);
-      return make_float2(z * p, p + z * 0.3989422804014327f * density);
+      return make_float2(z * p, p + near * 0.3989422804014327f * density);
     }
     case TAO_ACT_GELU_TANH: {
       const float s = sigmoid(2.f * kGeluRoot * (z + kGeluCube * z * z * z));
-      const float near = fminf(fmaxf(z, -32.f), 32.f);  // where s (1 - s) is 0 the square would be infinite
       return make_float2(z * s, s + near * s * (1.f - s) * 2.f * kGeluRoot * (1.f + 3.f * kGeluCube * near * near));
     }
   }
