@@ -558,7 +558,8 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
  * The gradient (tao_linear_gradient) of dy [rows][n] (neighbours next to each other), with dz = dy act'(z), or gated
  * dz = dy u act'(z) and du = dy act(z), rounded to the type for the products: dx [rows][k] = dz W (+ du U), zeros for
  * rows of no expert; dw [experts][n][k] = dz^T x, dup = du^T x over each expert's rows, zeros for an expert
- * without; db [n] = the sum of dz over the rows, in a fixed order.  Each may be NULL (dw and dup together); z (gated: u and
+ * without; db [n] = the sum of dz over all rows, in a fixed order.  Each may be NULL (dw and dup together), and all of them
+ * (nothing is launched); z (gated: u and
  * low too) are needed where there is an activation or a gate, x for dw, W and U for dx.
  *
  * x, W and U of any strides: what does not lie with neighbours next to each other and everything else on 16 bytes

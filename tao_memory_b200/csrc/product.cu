@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] += dy[i];
         if (a.dz) store(a.dz, r, dy);
-        if constexpr (GATED) store(a.du, r, z);
+        if constexpr (GATED)
+          if (a.du) store(a.du, r, z);
       }
     }
   }
@@ -785,6 +786,7 @@ int tao_linear_gradient(const TaoLinear* p, void* stream) {
   }
   if (missing(*p, true)) return pfail(TAO_ERR_ARG, "null pointer");
   if (!kept_ok(*p)) return pfail(TAO_ERR_ARG, "a gate's kept factors start on 16 bytes, in rows of a multiple of 16");
+  if (!p->dx && !p->dw && !p->db) return TAO_OK;  // dup comes with dw
   if (any_overlap(*p, true)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 1))) return rc;
   static uint8_t none[1];
