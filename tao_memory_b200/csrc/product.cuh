@@ -692,10 +692,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++s == C::STAGES) s = 0, phase ^= 1;
       }
     }
+    // the ends of the products that read the last slots arrive here too (PAIR: from the first block) before the block ends
+#pragma unroll 1
+    for (int i = 0; ok && i < C::STAGES; ++i) {
+      ok = warp_wait_for(&empty[s], phase ^ 1, abort);
+      if (++s == C::STAGES) s = 0, phase ^= 1;
+    }
     if (!ok && !half_of_pair) {  // copies in flight (PAIR: both blocks') have their time before the block ends
       fetched = max(fetched, early);
       for (int i = max(fetched - C::STAGES, 0); i < fetched; ++i) mbar_wait(&full[i % C::STAGES], i / C::STAGES & 1, nullptr);
     }
+    if (half_of_pair) mbar_wait(over, 0, nullptr);  // it arrives at both blocks: the first one's next warp waits for its own
   } else if (warp == kWorkers + 1) {
     // ---- issues the products
     const uint32_t type_bits = is_bf16 ? 1u << 7 | 1u << 10 : 0u;
@@ -1037,7 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (FORM != FEW) cluster_sync();  // the others' reads of this block's part are over
   }
   if constexpr (PAIR) {
-    cluster_sync();  // neither's products, copies or arrivals need the other any more
+    cluster_sync();  // neither's products, copies or arrivals need the other any more: each block has waited for those at its own
     if (warp == 0)
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(C::TMEM));
   } else if (warp == 0) {
