@@ -353,9 +353,10 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] += dy[i];
-        if (a.dz) store(a.dz, r, dy);
-        if constexpr (GATED)
-          if (a.du) store(a.du, r, z);
+        if (a.dz) {  // and du
+          store(a.dz, r, dy);
+          if constexpr (GATED) store(a.du, r, z);
+        }
       }
     }
   }
