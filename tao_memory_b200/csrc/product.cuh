@@ -95,8 +95,9 @@ TAO_DEVI bool arrived(uint64_t* bar, uint32_t phase) {
   return ok != 0;
 }
 
-// Waits at most about four seconds; a wait that runs out, or another's of this block, ends all of them.
-TAO_DEVI bool wait_for(uint64_t* bar, uint32_t phase, volatile int* abort) {
+// Waits at most about four seconds, and for the sums of a tile of WEIGHT two microseconds more for each of its steps (one
+// takes 0.3, and an expert of 2^30 rows has 2^24; other forms' sums have up to 2^24 terms, 0.2 s); a wait that runs out, or another's of this block, ends all of them.
+TAO_DEVI bool wait_for(uint64_t* bar, uint32_t phase, volatile int* abort, int steps = 0) {
   unsigned long long began = 0;
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, phase)) return true;
@@ -105,14 +106,14 @@ TAO_DEVI bool wait_for(uint64_t* bar, uint32_t phase, volatile int* abort) {
     unsigned long long now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (!began) began = now;
-    if (now - began > 4000000000ull) break;
+    if (now - began > 4000000000ull + steps * 2000ull) break;
   }
   *abort = 1;
   atomicOr(&g_error, kErrWaitTimeout);
   return false;
 }
-TAO_DEVI bool warp_wait_for(uint64_t* bar, uint32_t phase, volatile int* abort) {
-  return __all_sync(0xffffffffu, wait_for(bar, phase, abort));
+TAO_DEVI bool warp_wait_for(uint64_t* bar, uint32_t phase, volatile int* abort, int steps = 0) {
+  return __all_sync(0xffffffffu, wait_for(bar, phase, abort, steps));
 }
 
 TAO_DEVI void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -794,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int blocks = part(tile, k0);
       const uint32_t acc = tbase + set * C::ACC + lanes;
       if (blocks && (SPLIT || FORM == FEW)) {
-        if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort))) break;
+        if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort, FORM == WEIGHT ? blocks : 0))) break;
         fence_after();
       }
       if constexpr (SPLIT) {
@@ -876,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         float bias = bias_of(half * HALF);
         if (blocks) {  // all that is not the sums is on its way before them
-          if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort))) break;
+          if (!(ok = warp_wait_for(&acc_full[set], set_phase, abort, FORM == WEIGHT ? blocks : 0))) break;
           fence_after();
         }
 #pragma unroll 1
