@@ -150,13 +150,13 @@ def sorted_experts(x, ids, weights, gate, up, down):
 
 
 class TrainedBlock(nn.Module):
-    """One decoder block in training, its weights in bf16 or fp16 (the attention takes bf16):
+    """One decoder block in training, its weights in bf16 (the attention's type):
 
         h, stream = norm(x + stream);  x = W_out attention(split(W_qkv h))
         h, stream = norm(x + stream);  x = experts(h), or dense: W_2 gelu(W_1 h + b_1) + b_2 + stream, stream None
 
     ``experts`` 0: the dense form, whose sum with the stream is rounded once.  ``transform`` (q, k) -> (q, k) is the
-    caller's positional transform.  ``prefill`` and ``step`` take prompts and decode with the same weights."""
+    caller's positional transform; ``eps`` is the residual norms'.  ``prefill`` and ``step`` take prompts and decode with the same weights."""
 
     def __init__(self, heads, width, inner, experts=0, top_k=2, renormalize=True, alpha=0.5, transform=None, eps=RMS_EPS,
                  config=DEFAULT_CONFIG, device="cuda", dtype=_BF16):
@@ -164,6 +164,8 @@ class TrainedBlock(nn.Module):
         channels = heads * width
         if experts < 0 or (experts and not 1 <= top_k <= experts):
             raise ValueError("a token takes 1 to as many experts as there are")
+        if dtype != _BF16:
+            raise ValueError("the block's weights are bf16, as what the attention takes")
         self.heads, self.width, self.experts, self.top_k, self.renormalize = heads, width, experts, top_k, renormalize
         self.alpha, self.transform, self.eps, self.config = alpha, transform, eps, config
 
@@ -231,6 +233,8 @@ class TrainedDecoder(nn.Module):
     def __init__(self, vocab, blocks, device="cuda", dtype=_BF16):
         super().__init__()
         self.blocks = nn.ModuleList(blocks)
+        if dtype != _BF16:
+            raise ValueError("the decoder's weights are bf16, as its blocks'")
         channels = blocks[0].heads * blocks[0].width
         self.scale, self.eps = channels ** 0.5, blocks[0].eps
         self.table = nn.Parameter((torch.randn(vocab, channels, device=device) / self.scale).to(dtype))
