@@ -240,6 +240,10 @@ class TrainedDecoder(nn.Module):
         self.table = nn.Parameter((torch.randn(vocab, channels, device=device) / self.scale).to(dtype))
         self.norm = nn.Parameter(torch.ones(channels, device=device, dtype=dtype))
 
+    def _check(self, requests):
+        if any(len(states) != len(self.blocks) for states in requests):
+            raise ValueError(f"a request has a state for each of the {len(self.blocks)} blocks")
+
     def _head(self, x, stream):
         return linear(add_rms_norm(x, self.norm, stream, eps=self.eps)[0], self.table)
 
@@ -253,6 +257,7 @@ class TrainedDecoder(nn.Module):
     @torch.no_grad()
     def prefill(self, ids, states):
         """A prompt [tokens] of one request, a state for each block: the last token's logits [1, vocab]."""
+        self._check([states])
         x, stream = embed(ids[None], self.table, self.scale), None
         for block, state in zip(self.blocks, states):
             x, stream = block.prefill(x, stream, state)
@@ -261,6 +266,7 @@ class TrainedDecoder(nn.Module):
     @torch.no_grad()
     def step(self, ids, requests):
         """One token of each request, ids [requests], a sequence of states each: logits [requests, vocab]."""
+        self._check(requests)
         x, stream = embed(ids[:, None], self.table, self.scale), None
         for layer, block in enumerate(self.blocks):
             x, stream = block.step(x, stream, [states[layer] for states in requests])
