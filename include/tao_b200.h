@@ -551,16 +551,16 @@ int tao_expert_check(void* workspace, size_t workspace_bytes, int* flags, void* 
  *   y = act(x W_e^T), or with `up` (like W) the gated act(x W_e^T) * (x U_e^T).
  * offsets[0] is taken as 0, values are held between the one before and `rows`, and rows from offsets[experts] on
  * give zeros.  z [rows][z_row]: what act is applied to, rounded to the type, for the gradient (which takes an
- * infinity there as a very large argument), or NULL.  Gated: z and u
- * are the upper 16 bits of act's argument and of its factor as fp32 numbers cut to 24 bits, and low [2][rows][z_row] bytes
- * has the lower 8 of both; the three start on 16 bytes, z_row is a multiple of 16, and all of a row may be written.
+ * infinity there as a very large argument), or NULL.  Gated: z and u are the upper 16 bits of act's argument and of its
+ * factor as fp32 numbers cut to 24 bits, and low [2][rows][z_row] bytes has the lower 8 of both; the three start on
+ * 16 bytes, z_row is a multiple of 16, and all of a row may be written.
  *
  * The gradient (tao_linear_gradient) of dy [rows][n] (neighbours next to each other), with dz = dy act'(z), or gated
- * dz = dy u act'(z) and du = dy act(z), rounded to the type for the products: dx [rows][k] = dz W (+ du U), zeros for
- * rows of no expert; dw [experts][n][k] = dz^T x, dup = du^T x over each expert's rows, zeros for an expert
- * without; db [n] = the sum of dz over all rows, in a fixed order.  Each may be NULL (dw and dup together), and all of them
- * (nothing is launched); z (gated: u and
- * low too) are needed where there is an activation or a gate, x for dw, W and U for dx.
+ * dz = dy u act'(z) and du = dy act(z), rounded to the type for the products (beyond fp16's 65504 they are infinite):
+ * dx [rows][k] = dz W (+ du U), zeros for rows of no expert; dw [experts][n][k] = dz^T x, dup = du^T x over each expert's
+ * rows, zeros for an expert without; db [n] = the sum of dz over all rows, in a fixed order.  Each may be NULL (dw and
+ * dup together), and all of them (nothing is launched); z (gated: u and low too) are needed where there is an
+ * activation or a gate, x for dw, W and U for dx.
  *
  * x, W and U of any strides: what does not lie with neighbours next to each other and everything else on 16 bytes
  * is copied into the workspace first (tao_linear_workspace_bytes of the same structure, on 256 bytes; each

@@ -177,8 +177,11 @@ Split split_of(long long tiles, int steps, double join) {
 
 // FORWARD and INPUT of many rows, by what the rounds of all SMs cost in steps of a 128 tile (about 0.2 us): a step of a
 // tile of 256 columns 1.6 of them, of a pair's 256 x 256 1.48 (INPUT: 1.4) and 6 for its start, and for a split of 64
-// columns some 32.  Half of an expert's last tile is taken as empty.  A pair's two blocks share one round of outputs,
-// so with short sums and an activation to compute it loses (32768x768x2304 with gelu 162.5 us, alone 154.0).
+// columns some 32.  Half of an expert's last tile is taken as empty.  A pair's two blocks share one round of outputs, so
+// with sums of fewer than 16 steps and an activation to compute it may lose.  Alone / pair, us, gated 1536 channels of 16384
+// rows of 16 experts: 8 steps 48.7 / 58.3, 12 65.4 / 68.5, 14 75.5 / 74.4, 16 84.0 / 82.4; silu to 2304 channels with z kept,
+// 4096 rows: 12 steps 24.9 / 26.7, 15 28.1 / 28.9; 32768 rows: 8 steps 116.6 / 118.8, 12 129.1 / 128.5, 15 143.7 / 137.6.
+// (Many rows of one matrix would gain up to 5 % from 12 steps on.)
 // Measured (us), 256 columns / 128 / 64 and split: 2048x768x2304 9.2 / 9.9 / 46; 512x2048x2048 14.4 / 10.1 / 17.3;
 // 128x8192x2048 48.5 / 29.6 / 16.7.  256 columns / pair: 16384x2048x8192 379.8 / 353.3; 2048x2048x2048 22.0 / 23.3;
 // INPUT of 16384x8192x2048 523.6 / 364.0; gated 4096 tokens by 8 of 64 experts 240.5 / 249.2, 16384 by 2 of 16 208.6 / 195.2.
