@@ -583,11 +583,15 @@ bool any_overlap(const TaoLinear& p, bool gradient) {
          overlaps(p.db, n * 2, {x, weight, up, z, u, low, offsets, dy, dx, dw, dup});
 }
 
-// Gated: what is kept for the gradient goes by 16 bytes.
-bool kept_ok(const TaoLinear& p) {
-  return !p.up || !p.z || (p.z_row % 16 == 0 && p.z_row >= p.n &&
-                           (reinterpret_cast<uintptr_t>(p.z) | reinterpret_cast<uintptr_t>(p.u) |
-                            reinterpret_cast<uintptr_t>(p.low)) % 16 == 0);
+// What is kept for the gradient: rows that do not reach into each other; gated, on 16 bytes.
+int check_kept(const TaoLinear& p, bool gradient) {
+  const bool used = p.z && (!gradient || p.activation != TAO_ACT_NONE || p.up);
+  if (used && p.rows > 1 && p.z_row < p.n) return pfail(TAO_ERR_ARG, "a row of z has room for n values");
+  if (p.up && p.z && (p.z_row % 16 || p.z_row < p.n ||
+                      (reinterpret_cast<uintptr_t>(p.z) | reinterpret_cast<uintptr_t>(p.u) |
+                       reinterpret_cast<uintptr_t>(p.low)) % 16))
+    return pfail(TAO_ERR_ARG, "a gate's kept factors start on 16 bytes, in rows of a multiple of 16");
+  return TAO_OK;
 }
 
 int check_room(const TaoLinear& p, size_t need) {
@@ -768,7 +772,7 @@ int tao_linear(const TaoLinear* p, void* stream) {
   if (int rc = check(p)) return rc;
   if (p->rows == 0) return TAO_OK;
   if (missing(*p, false)) return pfail(TAO_ERR_ARG, "null pointer");
-  if (!kept_ok(*p)) return pfail(TAO_ERR_ARG, "a gate's kept factors start on 16 bytes, in rows of a multiple of 16");
+  if (int rc = check_kept(*p, false)) return rc;
   if (any_overlap(*p, false)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 0))) return rc;
   static uint8_t none[1];  // where no room is needed
@@ -789,7 +793,7 @@ int tao_linear_gradient(const TaoLinear* p, void* stream) {
     return e == cudaSuccess ? TAO_OK : pfail(TAO_ERR_CUDA, cudaGetErrorString(e));
   }
   if (missing(*p, true)) return pfail(TAO_ERR_ARG, "null pointer");
-  if (!kept_ok(*p)) return pfail(TAO_ERR_ARG, "a gate's kept factors start on 16 bytes, in rows of a multiple of 16");
+  if (int rc = check_kept(*p, true)) return rc;
   if (!p->dx && !p->dw && !p->db) return TAO_OK;  // dup comes with dw
   if (any_overlap(*p, true)) return pfail(TAO_ERR_ARG, "a product's output must not overlap its operands");
   if (int rc = check_room(*p, tao_linear_workspace_bytes(p, 1))) return rc;
